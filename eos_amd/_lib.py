@@ -212,6 +212,33 @@ class EosHipTQCodes(C.Structure):
     ]
 
 
+class EosHipKVDesc(C.Structure):
+    _fields_ = [
+        ("format", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("page_tokens", C.c_int32),
+        ("pages", C.c_int64),
+        ("d_k", C.c_void_p),
+        ("d_v", C.c_void_p),
+        ("d_k_scale", C.c_void_p),
+        ("d_v_scale", C.c_void_p),
+        ("codebook", C.c_void_p),
+        ("signs", C.c_void_p),
+    ]
+
+
+class EosHipKVBatch(C.Structure):
+    _fields_ = [
+        ("d_page_table", C.c_void_p),
+        ("table_stride", C.c_int32),
+        ("batch", C.c_int32),
+        ("d_lengths", C.c_void_p),
+        ("d_offsets", C.c_void_p),
+        ("rows", C.c_int64),
+    ]
+
+
 class EosHipHadamardSpec(C.Structure):
     _fields_ = [
         ("channels", C.c_int32),
@@ -380,6 +407,22 @@ _SIGNATURES = {
                                           C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                           C.c_void_p], C.c_int),
     "eoship_hadamard_tq_release": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_kv_bytes": ([C.POINTER(EosHipKVDesc), C.POINTER(C.c_int64), C.POINTER(C.c_int64),
+                         C.c_void_p], C.c_int),
+    "eoship_kv_check_batch": ([C.POINTER(EosHipKVDesc), C.c_void_p, C.c_int32, C.c_int32,
+                               C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p], C.c_int),
+    "eoship_kv_bind": ([C.c_void_p, C.POINTER(EosHipKVDesc), C.POINTER(C.c_void_p), C.c_void_p],
+                       C.c_int),
+    "eoship_kv_release": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_kv_append_device": ([C.c_void_p, C.c_void_p, C.POINTER(EosHipKVBatch), C.c_void_p,
+                                 C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p],
+                                C.c_int),
+    "eoship_kv_read_device": ([C.c_void_p, C.c_void_p, C.POINTER(EosHipKVBatch), C.c_void_p,
+                               C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p], C.c_int),
+    "eoship_kv_attention_device": ([C.c_void_p, C.c_void_p, C.POINTER(EosHipKVBatch), C.c_void_p,
+                                    C.c_int64, C.c_int32, C.c_int32, C.c_float, C.c_int32,
+                                    C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_kv_status": ([C.c_void_p, C.c_void_p, C.POINTER(C.c_int32), C.c_void_p], C.c_int),
     "eoship_tq_ip_encode_device": ([C.c_void_p, C.POINTER(EosHipTQIPSpec), C.c_void_p, C.c_int64,
                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
                                    C.c_int),

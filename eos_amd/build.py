@@ -35,6 +35,7 @@ DEVICE_SOURCES = [
     ("tqe", os.path.join(CSRC, "kernels", "tqe_kernels.hip")),
     ("enc", os.path.join(CSRC, "kernels", "enc_kernels.hip")),
     ("ret", os.path.join(CSRC, "kernels", "ret_kernels.hip")),
+    ("kv", os.path.join(CSRC, "kernels", "kv_kernels.hip")),
 ]
 # Extra flags per code object. The encoder kernels are built without the
 # mixed-precision FMA instructions (v_fma_mix*): the compiler folds some
@@ -62,6 +63,7 @@ HOST_SOURCES = [
     os.path.join(CSRC, "eoship_embed.cpp"),
     os.path.join(CSRC, "eoship_mll.cpp"),
     os.path.join(CSRC, "eoship_retrieval.cpp"),
+    os.path.join(CSRC, "eoship_kv.cpp"),
 ]
 
 # Packed-FP32 instructions are disabled for every device build.

@@ -1,0 +1,389 @@
+// Key-value cache half of the eoship C ABI: binds a caller's paged cache and
+// enqueues its writes, reads and attention. The counterpart of the kv_cache
+// capability that the reference's CUDA backend advertises
+// (runtime/backend/backend.go:1428-1431), with the Hadamard TurboQuant
+// quantizer (runtime/backends/cuda/native_linux.go:1812-2004) as one of its
+// storage formats.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+#include <vector>
+
+#include "eoship_internal.h"
+#include "kernels/kv_index.h"
+
+using eoship::hip_err;
+using eoship::set_err;
+
+struct EosHipKVCache {
+  EosHipRuntime* rt = nullptr;
+  EosHipKVDesc d{};
+  KvTables tables{};
+  int page_shift = 0;
+  void* mem = nullptr;  // status word, then the signs
+  ~EosHipKVCache() {
+    if (mem != nullptr) hipFree(mem);
+  }
+};
+
+namespace {
+
+const char* const kFormats[] = {"f16", "bf16", "q8", "tq4"};
+
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int bits_of(int format) { return format == kKvQ8 ? 8 : format == kKvTq4 ? 4 : 16; }
+
+// Makes a runtime's device current for the length of a call.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    if (hipGetDevice(&was_) != hipSuccess) was_ = device;
+    if (was_ != device) (void)hipSetDevice(device);
+    now_ = device;
+  }
+  ~OnDevice() {
+    if (was_ != now_) (void)hipSetDevice(was_);
+  }
+
+ private:
+  int was_ = 0, now_ = 0;
+};
+
+// The f16 bits of a float that f16 holds exactly and normally, or 0.
+uint16_t exact_f16(float f) {
+  uint32_t u;
+  std::memcpy(&u, &f, 4);
+  const int ex = (int)(u >> 23 & 255) - 127;
+  if ((u & 0x1fff) != 0 || ex < -14 || ex > 15) return 0;
+  return (uint16_t)((u >> 31) << 15 | (uint32_t)(ex + 15) << 10 | (u >> 13 & 0x3ff));
+}
+
+int check_desc(const EosHipKVDesc* d, const char* what, char** err) {
+  if (d == nullptr) return set_err(err, "%s: desc is NULL", what);
+  if (d->format < kKvF16 || d->format > kKvTq4)
+    return set_err(err, "%s: format must be 0 (f16), 1 (bf16), 2 (q8) or 3 (tq4), got %d", what,
+                   d->format);
+  if (d->kv_heads < 1 || d->kv_heads > 1024)
+    return set_err(err, "%s: kv_heads must be in 1..1024, got %d", what, d->kv_heads);
+  if (d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
+    return set_err(err, "%s: head_dim must be 32, 64, 128 or 256, got %d", what, d->head_dim);
+  const int p = d->page_tokens;
+  if (p < 16 || p > 256 || (p & (p - 1)) != 0)
+    return set_err(err, "%s: page_tokens must be 16, 32, 64, 128 or 256, got %d", what, p);
+  if (d->pages < 1 || d->pages > INT32_MAX)
+    return set_err(err, "%s: pages must be in 1..2^31-1, got %lld", what, (long long)d->pages);
+  return 0;
+}
+
+int check_tables(const EosHipKVDesc* d, const char* what, char** err) {
+  if (d->format != kKvTq4) return 0;
+  if (d->codebook == nullptr || d->signs == nullptr)
+    return set_err(err, "%s: tq4 needs a codebook and signs", what);
+  for (int i = 0; i < 8; ++i) {
+    if (!(d->codebook[i] > 0.0f) || exact_f16(d->codebook[i]) == 0)
+      return set_err(err, "%s: codebook[%d] must be a positive f16 number", what, i);
+    if (i > 0 && d->codebook[i] <= d->codebook[i - 1])
+      return set_err(err, "%s: codebook must be ascending", what);
+  }
+  for (int i = 0; i < d->head_dim; ++i)
+    if (d->signs[i] != 1.0f && d->signs[i] != -1.0f)
+      return set_err(err, "%s: signs must be 1 or -1", what);
+  return 0;
+}
+
+int check_batch(const EosHipRuntime* rt, const EosHipKVCache* kv, const EosHipKVBatch* b,
+                const char* what, char** err) {
+  if (rt == nullptr || kv == nullptr || b == nullptr)
+    return set_err(err, "%s: NULL argument", what);
+  if (kv->rt != rt) return set_err(err, "%s: the cache is bound to another runtime", what);
+  if (b->batch < 0 || b->rows < 0) return set_err(err, "%s: negative batch or rows", what);
+  if (b->rows > INT32_MAX) return set_err(err, "%s: more than 2^31-1 rows", what);
+  if (b->batch == 0 || b->rows == 0) return 0;
+  if (b->d_page_table == nullptr || b->d_lengths == nullptr)
+    return set_err(err, "%s: NULL page table or lengths", what);
+  if (b->table_stride < 1) return set_err(err, "%s: table_stride must be positive", what);
+  if (b->d_offsets == nullptr && b->rows != b->batch)
+    return set_err(err, "%s: without offsets every sequence has one row: rows %lld, batch %d",
+                   what, (long long)b->rows, b->batch);
+  return 0;
+}
+
+int check_rows(const void* p, int64_t stride, int64_t width, const char* name, const char* what,
+               char** err) {
+  if (p == nullptr) return set_err(err, "%s: %s is NULL", what, name);
+  if (!aligned(p)) return set_err(err, "%s: %s is not 16-byte aligned", what, name);
+  if (stride < width || stride % 8 != 0)
+    return set_err(err, "%s: the row stride of %s must be a multiple of 8 and at least %lld, got %lld",
+                   what, name, (long long)width, (long long)stride);
+  return 0;
+}
+
+KvCacheArgs cache_args(const EosHipKVCache* kv, const EosHipKVBatch* b) {
+  KvCacheArgs c{};
+  c.k = static_cast<uint8_t*>(kv->d.d_k);
+  c.v = static_cast<uint8_t*>(kv->d.d_v);
+  c.k_scale = kv->d.d_k_scale;
+  c.v_scale = kv->d.d_v_scale;
+  c.table = b->d_page_table;
+  c.lengths = b->d_lengths;
+  c.offsets = b->d_offsets;
+  c.status = static_cast<int32_t*>(kv->mem);
+  c.t = kv->tables;
+  c.rows = b->rows;
+  c.pages = (int)kv->d.pages;
+  c.kv_heads = kv->d.kv_heads;
+  c.page_shift = kv->page_shift;
+  c.table_stride = b->table_stride;
+  c.batch = b->batch;
+  return c;
+}
+
+int launch(EosHipRuntime* rt, const EosHipKVCache* kv, const char* op, long long gx, int gy,
+           int threads, void* args, const char* what, char** err) {
+  if (gx * threads > UINT32_MAX)
+    return set_err(err, "%s: too many rows for one call", what);
+  char name[64];
+  snprintf(name, sizeof(name), "eos_kv_%s_%s_%d", op, kFormats[kv->d.format], kv->d.head_dim);
+  return rt->launch(name, dim3((unsigned)gx, (unsigned)gy), dim3((unsigned)threads), 0, args, err);
+}
+
+int rows_call(EosHipRuntime* rt, const EosHipKVCache* kv, const EosHipKVBatch* b, const void* d_k,
+              int64_t k_stride, const void* d_v, int64_t v_stride, int32_t dtype, const char* op,
+              const char* what, char** err) {
+  const int64_t width = (int64_t)kv->d.kv_heads * kv->d.head_dim;
+  if (check_rows(d_k, k_stride, width, "k", what, err) != 0 ||
+      check_rows(d_v, v_stride, width, "v", what, err) != 0)
+    return 1;
+  OnDevice on(rt->device);
+  KvRowsArgs a{};
+  a.c = cache_args(kv, b);
+  a.k = static_cast<uint8_t*>(const_cast<void*>(d_k));
+  a.v = static_cast<uint8_t*>(const_cast<void*>(d_v));
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.dtype = dtype;
+  const long long units =
+      b->d_offsets == nullptr ? b->batch : kv_units(b->rows, b->batch, 1, kKvGroup, 2);
+  return launch(rt, kv, op, units, kv->d.kv_heads, 2 * kv->d.head_dim, &a, what, err);
+}
+
+}  // namespace
+
+extern "C" {
+
+int eoship_kv_bytes(const EosHipKVDesc* desc, int64_t* pool_bytes, int64_t* scale_bytes,
+                    char** err) {
+  const char* what = "eoship_kv_bytes";
+  if (check_desc(desc, what, err) != 0) return 1;
+  const int64_t tokens = desc->pages * desc->kv_heads * desc->page_tokens;
+  if (pool_bytes) *pool_bytes = tokens * (desc->head_dim * bits_of(desc->format) / 8);
+  if (scale_bytes) *scale_bytes = desc->format >= kKvQ8 ? tokens * 4 : 0;
+  return 0;
+}
+
+int eoship_kv_check_batch(const EosHipKVDesc* desc, const int32_t* page_table,
+                          int32_t table_stride, int32_t batch, const int32_t* lengths,
+                          const int32_t* offsets, int64_t rows, int32_t writes, char** err) {
+  const char* what = "eoship_kv_check_batch";
+  if (check_desc(desc, what, err) != 0) return 1;
+  if (batch < 0 || rows < 0 || rows > INT32_MAX)
+    return set_err(err, "%s: batch and rows must be in 0..2^31-1", what);
+  if (batch == 0 || rows == 0) return 0;
+  if (page_table == nullptr || lengths == nullptr || table_stride < 1)
+    return set_err(err, "%s: NULL page table or lengths, or no table columns", what);
+  if (offsets == nullptr && rows != batch)
+    return set_err(err, "%s: without offsets every sequence has one row: rows %lld, batch %d",
+                   what, (long long)rows, batch);
+  if (offsets != nullptr && offsets[0] != 0)
+    return set_err(err, "%s: offsets[0] must be 0, got %d", what, offsets[0]);
+  KvCacheArgs c{};
+  c.table = page_table;
+  c.lengths = lengths;
+  c.offsets = offsets;
+  c.rows = rows;
+  c.pages = (int)desc->pages;
+  c.table_stride = table_stride;
+  c.batch = batch;
+  while ((1 << c.page_shift) < desc->page_tokens) ++c.page_shift;
+  // Where a page is written: the sequence, and which of its pages.
+  std::vector<std::pair<int, std::pair<int, int>>> written;
+  for (int b = 0; b < batch; ++b) {
+    const KvSeq s = kv_seq(c, b);
+    if (s.bad & kKvBadOffset)
+      return set_err(err, "%s: sequence %d: offsets must ascend within 0..rows", what, b);
+    if (s.bad & kKvBadLength)
+      return set_err(err, "%s: sequence %d: length %d outside 0..%lld of its table row", what, b,
+                     lengths[b], (long long)table_stride * desc->page_tokens);
+    for (int i = 0; i << c.page_shift < s.keys; ++i)
+      if (kv_page(c, b, i << c.page_shift) < 0)
+        return set_err(err, "%s: sequence %d: page %d of its table row is %d, not in 0..%lld", what,
+                       b, i, page_table[(size_t)b * table_stride + i], (long long)desc->pages - 1);
+    if (writes != 0 && s.n > 0 && s.keys > 0)
+      for (int i = std::max(0, s.len - s.n) >> c.page_shift; i <= (s.keys - 1) >> c.page_shift; ++i)
+        written.push_back({page_table[(size_t)b * table_stride + i], {b, i}});
+  }
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first == written[i - 1].first)
+      return set_err(err, "%s: page %d is written twice, by sequences %d and %d", what,
+                     written[i].first, written[i - 1].second.first, written[i].second.first);
+  return 0;
+}
+
+int eoship_kv_bind(EosHipRuntime* rt, const EosHipKVDesc* desc, EosHipKVCache** out, char** err) {
+  const char* what = "eoship_kv_bind";
+  if (out != nullptr) *out = nullptr;
+  if (check_desc(desc, what, err) != 0 || check_tables(desc, what, err) != 0) return 1;
+  if (desc->d_k == nullptr || desc->d_v == nullptr)
+    return set_err(err, "%s: NULL pool", what);
+  if (!aligned(desc->d_k) || !aligned(desc->d_v))
+    return set_err(err, "%s: pools must be 16-byte aligned", what);
+  if (desc->format >= kKvQ8 &&
+      (desc->d_k_scale == nullptr || desc->d_v_scale == nullptr || !aligned(desc->d_k_scale) ||
+       !aligned(desc->d_v_scale)))
+    return set_err(err, "%s: %s needs 16-byte aligned scale pools", what, kFormats[desc->format]);
+  if (rt == nullptr || out == nullptr) return set_err(err, "%s: NULL argument", what);
+  OnDevice on(rt->device);
+  auto* kv = new EosHipKVCache();
+  kv->rt = rt;
+  kv->d = *desc;
+  while ((1 << kv->page_shift) < desc->page_tokens) ++kv->page_shift;
+  const size_t signs = desc->format == kKvTq4 ? (size_t)desc->head_dim * 4 : 0;
+  std::vector<char> host(16 + signs, 0);
+  if (rt->alloc(host.size(), &kv->mem, err) != 0) {
+    delete kv;
+    return 1;
+  }
+  if (desc->format == kKvTq4) {
+    std::memcpy(host.data() + 16, desc->signs, signs);
+    KvTables& t = kv->tables;
+    t.signs = reinterpret_cast<const float*>(static_cast<char*>(kv->mem) + 16);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = exact_f16(desc->codebook[i]);
+      t.mags[i] = desc->codebook[i];
+      t.hi[i / 4] |= (u >> 8) << (8 * (i % 4));
+      t.lo[i / 4] |= (u & 255) << (8 * (i % 4));
+      if (i > 0) t.edges[i - 1] = 0.5f * (desc->codebook[i] + desc->codebook[i - 1]);
+    }
+  }
+  kv->d.codebook = kv->d.signs = nullptr;  // the caller's host memory is not kept
+  const hipError_t e = rt->copy_sync(kv->mem, host.data(), host.size(), hipMemcpyHostToDevice);
+  if (e != hipSuccess) {
+    delete kv;
+    return hip_err(err, "hipMemcpy(cache tables)", e);
+  }
+  *out = kv;
+  return 0;
+}
+
+int eoship_kv_release(EosHipRuntime* rt, EosHipKVCache* kv, char** err) {
+  if (kv == nullptr) return 0;
+  if (rt == nullptr || kv->rt != rt) return set_err(err, "eoship_kv_release: wrong runtime");
+  OnDevice on(rt->device);
+  if (rt->sync(err) != 0) return 1;
+  delete kv;
+  return 0;
+}
+
+int eoship_kv_append_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
+                            const void* d_k, int64_t k_stride, const void* d_v, int64_t v_stride,
+                            int32_t dtype, char** err) {
+  const char* what = "eoship_kv_append_device";
+  if (check_batch(rt, kv, batch, what, err) != 0) return 1;
+  if (dtype != kKvRowF16 && dtype != kKvRowBf16)
+    return set_err(err, "%s: rows must be f16 (0) or bf16 (1), got %d", what, dtype);
+  if (kv->d.format <= kKvBf16 && dtype != kv->d.format)
+    return set_err(err, "%s: the cache holds %s, the rows are %s", what, kFormats[kv->d.format],
+                   kFormats[dtype]);
+  if (batch->batch == 0 || batch->rows == 0) return 0;
+  return rows_call(rt, kv, batch, d_k, k_stride, d_v, v_stride, dtype, "append", what, err);
+}
+
+int eoship_kv_read_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
+                          void* d_k, int64_t k_stride, void* d_v, int64_t v_stride, int32_t dtype,
+                          char** err) {
+  const char* what = "eoship_kv_read_device";
+  if (check_batch(rt, kv, batch, what, err) != 0) return 1;
+  if (dtype < kKvRowF16 || dtype > kKvRowF32)
+    return set_err(err, "%s: rows must be f16 (0), bf16 (1) or f32 (2), got %d", what, dtype);
+  if (batch->batch == 0 || batch->rows == 0) return 0;
+  return rows_call(rt, kv, batch, d_k, k_stride, d_v, v_stride, dtype, "read", what, err);
+}
+
+int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
+                               const void* d_q, int64_t q_stride, int32_t heads, int32_t dtype,
+                               float scale, int32_t window, void* d_out, int64_t out_stride,
+                               float* d_lse, char** err) {
+  const char* what = "eoship_kv_attention_device";
+  if (check_batch(rt, kv, batch, what, err) != 0) return 1;
+  if (dtype != kKvRowF16 && dtype != kKvRowBf16)
+    return set_err(err, "%s: rows must be f16 (0) or bf16 (1), got %d", what, dtype);
+  if (kv->d.format <= kKvBf16 && dtype != kv->d.format)
+    return set_err(err, "%s: the cache holds %s, the rows are %s", what, kFormats[kv->d.format],
+                   kFormats[dtype]);
+  if (heads < 1 || heads > 65535 || heads % kv->d.kv_heads != 0)
+    return set_err(err, "%s: heads must be a multiple of kv_heads (%d) up to 65535, got %d", what,
+                   kv->d.kv_heads, heads);
+  if (!std::isfinite(scale)) return set_err(err, "%s: scale must be finite", what);
+  if (window < 0) return set_err(err, "%s: window must not be negative, got %d", what, window);
+  if (batch->batch == 0 || batch->rows == 0) return 0;
+  if (batch->rows * (heads / kv->d.kv_heads) > 1 << 30)
+    return set_err(err, "%s: too many rows for one call", what);
+  const int64_t width = (int64_t)heads * kv->d.head_dim;
+  if (check_rows(d_q, q_stride, width, "q", what, err) != 0 ||
+      check_rows(d_out, out_stride, width, "out", what, err) != 0)
+    return 1;
+  OnDevice on(rt->device);
+  KvAttnArgs a{};
+  a.c = cache_args(kv, batch);
+  a.q = static_cast<const uint8_t*>(d_q);
+  a.out = static_cast<uint8_t*>(d_out);
+  a.lse = d_lse;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.scale = scale * 1.44269504089f;
+  a.heads = heads;
+  a.group = heads / kv->d.kv_heads;
+  a.window = window;
+  a.dtype = dtype;
+  const int kvh = kv->d.kv_heads, d = kv->d.head_dim;
+  const long long tiles =
+      batch->d_offsets == nullptr
+          ? (long long)batch->batch * ((a.group + kKvTileRows - 1) / kKvTileRows)
+          : kv_units(batch->rows, batch->batch, a.group, kKvTileRows, 1);
+  // Enough splits to give every CU four workgroups, none below 256 keys.
+  long long keys = (long long)batch->table_stride << kv->page_shift;
+  if (window > 0) keys = std::min(keys, (long long)window + batch->rows + 32);
+  const long long want = (4LL * rt->compute_units + tiles * kvh - 1) / (tiles * kvh);
+  a.splits = (int)std::max(1LL, std::min(want, (keys + 255) / 256));
+  if (a.splits > 1) {
+    const size_t parts = (size_t)tiles * kvh * a.splits * kKvTileRows;
+    void* ws = nullptr;
+    if (rt->workspace(parts * (size_t)(d + 2) * 4, &ws, err) != 0) return 1;
+    a.part = static_cast<float*>(ws);
+    a.part_ml = a.part + parts * (size_t)d;
+  }
+  if (launch(rt, kv, "split", tiles * a.splits, kvh, 256, &a, what, err) != 0) return 1;
+  if (a.splits == 1) return 0;
+  return launch(rt, kv, "join", batch->rows, heads, 256, &a, what, err);
+}
+
+int eoship_kv_status(EosHipRuntime* rt, EosHipKVCache* kv, int32_t* status, char** err) {
+  const char* what = "eoship_kv_status";
+  if (rt == nullptr || kv == nullptr || status == nullptr)
+    return set_err(err, "%s: NULL argument", what);
+  if (kv->rt != rt) return set_err(err, "%s: the cache is bound to another runtime", what);
+  OnDevice on(rt->device);
+  hipError_t e = rt->copy_async(status, kv->mem, 4, hipMemcpyDeviceToHost);
+  if (e != hipSuccess) return hip_err(err, what, e);
+  if (rt->sync(err) != 0) return 1;
+  if (*status == 0) return 0;
+  const int32_t zero = 0;
+  e = rt->copy_async(kv->mem, &zero, 4, hipMemcpyHostToDevice);
+  if (e != hipSuccess) return hip_err(err, what, e);
+  return rt->sync(err);
+}
+
+}  // extern "C"

@@ -29,6 +29,8 @@ extern const unsigned char eoship_enc_co_begin[];
 extern const unsigned char eoship_enc_co_end[];
 extern const unsigned char eoship_ret_co_begin[];
 extern const unsigned char eoship_ret_co_end[];
+extern const unsigned char eoship_kv_co_begin[];
+extern const unsigned char eoship_kv_co_end[];
 }
 
 namespace eoship {
@@ -228,10 +230,11 @@ int eoship_runtime_create(int device, EosHipRuntime** out, char** err) {
     delete rt;
     return hip_err(err, "hipStreamCreateWithFlags", e);
   }
-  const unsigned char* images[4][2] = {{eoship_tq_co_begin, eoship_tq_co_end},
+  const unsigned char* images[5][2] = {{eoship_tq_co_begin, eoship_tq_co_end},
                                        {eoship_tqe_co_begin, eoship_tqe_co_end},
                                        {eoship_enc_co_begin, eoship_enc_co_end},
-                                       {eoship_ret_co_begin, eoship_ret_co_end}};
+                                       {eoship_ret_co_begin, eoship_ret_co_end},
+                                       {eoship_kv_co_begin, eoship_kv_co_end}};
   for (auto& im : images) {
     hipModule_t m = nullptr;
     e = im[1] > im[0] ? hipModuleLoadData(&m, im[0]) : hipErrorInvalidImage;

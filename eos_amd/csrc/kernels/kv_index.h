@@ -1,0 +1,120 @@
+// Which rows, positions, pages and keys a workgroup of the key-value cache
+// kernels has: integer arithmetic only, compiled into the kernels and, for
+// tests, into host programs.
+#ifndef EOSHIP_KV_INDEX_H
+#define EOSHIP_KV_INDEX_H
+
+#include "kv_args.h"
+
+#ifdef __HIP_DEVICE_COMPILE__
+#define KV_HD __device__ __forceinline__
+#elif defined(__HIP__)
+#define KV_HD __device__ __host__ inline
+#else
+#define KV_HD inline
+#endif
+
+KV_HD int kv_min(int a, int b) { return a < b ? a : b; }
+KV_HD int kv_max(int a, int b) { return a > b ? a : b; }
+
+// The rows of sequence b in a call: rows row0 .. row0 + n - 1 stand at
+// positions len - n .. len - 1, of which the page table can hold the first
+// `keys`. What is out of range counts as empty and is reported in `bad`.
+struct KvSeq {
+  int b = 0;
+  long long row0 = 0;
+  int n = 0, len = 0, keys = 0, bad = 0;
+};
+
+KV_HD KvSeq kv_seq(const KvCacheArgs& c, int b) {
+  KvSeq s;
+  s.b = b;
+  long long lo = b, hi = (long long)b + 1;
+  if (c.offsets != nullptr) {
+    lo = c.offsets[b];
+    hi = c.offsets[b + 1];
+  }
+  if (lo < 0 || hi < lo || hi > c.rows) {
+    s.bad |= kKvBadOffset;
+    lo = hi = 0;
+  }
+  s.row0 = lo;
+  s.n = (int)(hi - lo);
+  s.len = c.lengths[b];
+  const long long cap = (long long)c.table_stride << c.page_shift;
+  if (s.len < 0 || s.len > cap) s.bad |= kKvBadLength;
+  if (s.len < 0) s.len = 0;
+  s.keys = s.len > cap ? (int)cap : s.len;
+  return s;
+}
+
+// Work units are numbered through a batch without knowing its row counts on
+// the host: sequence b's first unit is floor(offset * mul / per) + extra * b,
+// which leaves it floor(n * mul / per) + extra of them at least.
+KV_HD long long kv_unit_base(const KvCacheArgs& c, int b, int mul, int per, int extra) {
+  return (long long)c.offsets[b] * mul / per + (long long)extra * b;
+}
+// Units of the whole batch.
+KV_HD long long kv_units(long long rows, int batch, int mul, int per, int extra) {
+  return rows * mul / per + (long long)extra * batch;
+}
+
+// The page of a token, or -1 where it has none in range.
+KV_HD int kv_page(const KvCacheArgs& c, int b, int token) {
+  const int i = token >> c.page_shift;
+  if (token < 0 || i >= c.table_stride) return -1;
+  const int p = c.table[(long long)b * c.table_stride + i];
+  return p >= 0 && p < c.pages ? p : -1;
+}
+
+// Unit `within` of a sequence in append and read: 8 positions from pos0 on,
+// of which [from, upto) are rows of the call. False where it has none.
+struct KvGroup8 {
+  int pos0 = 0, from = 0, upto = 0;
+  long long row = 0;  // the call's row of position pos0 (before `from`: not one)
+};
+
+KV_HD bool kv_group8(const KvSeq& s, long long within, KvGroup8& g) {
+  const long long first = (long long)s.len - s.n;  // negative: padding rows before position 0
+  const long long pos0 = ((first > 0 ? first : 0) / kKvGroup + within) * kKvGroup;
+  if (s.n == 0 || within < 0 || pos0 >= s.keys) return false;
+  g.pos0 = (int)pos0;
+  g.from = first > pos0 ? (int)(first - pos0) : 0;
+  g.upto = s.keys - pos0 < kKvGroup ? (int)(s.keys - pos0) : kKvGroup;
+  g.row = s.row0 + (pos0 - first);
+  return true;
+}
+
+// 16 query rows of a sequence and a head group (row r: row r / group of the
+// sequence, head r % group), and the keys they attend.
+struct KvTile {
+  KvSeq s;
+  int r0 = 0;
+  int lo = 0, hi = 0;          // keys [lo, hi) that any row attends
+  int all_lo = 0, all_hi = 0;  // keys [all_lo, all_hi) that every row attends
+  int base = 0;                // lo, down to a whole 32
+  int chunk = 0, splits = 0;   // keys of a split (whole 128s), splits with any
+};
+
+KV_HD int kv_row_pos(const KvSeq& s, int row) { return s.len - s.n + row; }
+
+// Tile `within` of rows of sequence t.s; false where it has no rows.
+KV_HD bool kv_tile(KvTile& t, long long within, int tile_rows, int group, int window, int splits) {
+  if (within < 0 || within * tile_rows >= (long long)t.s.n * group) return false;
+  t.r0 = (int)within * tile_rows;
+  const int last = kv_min(t.r0 + tile_rows, t.s.n * group) - 1;
+  const int p0 = kv_row_pos(t.s, t.r0 / group), p1 = kv_row_pos(t.s, last / group);
+  t.hi = kv_min(t.s.keys, p1 + 1);
+  t.lo = window > 0 ? kv_max(0, p0 - window + 1) : 0;
+  if (t.hi <= t.lo) t.hi = t.lo = 0;
+  t.all_hi = kv_min(t.s.keys, p0 + 1);
+  t.all_lo = window > 0 ? p1 - window + 1 : 0;
+  t.base = t.lo & ~31;
+  const int steps = (t.hi - t.base + 127) / 128;
+  const int per = kv_max((steps + splits - 1) / splits, 1);
+  t.chunk = per * 128;
+  t.splits = (steps + per - 1) / per;
+  return true;
+}
+
+#endif

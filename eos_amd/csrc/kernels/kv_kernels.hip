@@ -1,0 +1,855 @@
+// Paged key-value cache on gfx950: rows written in a storage format, read
+// back, and attended.
+//
+// Pools, for pages of P tokens, H key-value heads of width D:
+//   K       [pages][H][P][D]        f16 / bf16 / int8 codes
+//           [pages][H][P][D / 8]    tq4: words, dimension 8 w + j at bits 4 j
+//   V       [pages][H][P / 8][D][8]  f16 / bf16 / int8 codes
+//           [pages][H][P / 8][D]    tq4: words, token 8 g + j at bits 4 j
+//   scales  [pages][H][P] f32 for K and for V (q8, tq4)
+// V keeps 8 tokens of a dimension side by side because the product with the
+// probabilities sums over tokens: an MFMA operand register holds consecutive
+// summands of one output, so a lane's load is its operand as it lies.
+//
+// q8:  s = max|x| / 127, code = rint(x * (127 / max|x|)), stands for code * s.
+// tq4: w = Hd (signs * x) (Walsh-Hadamard, unnormalised), s = sqrt(sum x^2 / D),
+//      index = number of edges below |w| / (s sqrt(D)), code = 8 [w < 0] + index,
+//      stands for signs * Hd (+-magnitude) * s / sqrt(D). Attention stays in
+//      the rotated space: q is rotated once, the output once.
+// A scale below 2^-60 is stored as zero, one above 2^40 or not finite as NaN.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kv_index.h"
+
+#define EOS_DEV __device__ __forceinline__
+
+namespace {
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+constexpr float kTiny = 0x1p-60f, kHuge = 0x1p40f;
+constexpr float kLowest = -1e30f;  // softmax reference before any key
+
+constexpr int bits_of(int fmt) { return fmt == kKvQ8 ? 8 : fmt == kKvTq4 ? 4 : 16; }
+constexpr int log2i(int x) { return x <= 1 ? 0 : 1 + log2i(x / 2); }
+
+EOS_DEV uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+  return __builtin_amdgcn_perm(hi, lo, sel);
+}
+
+EOS_DEV float bf16_to_f32(uint32_t u) { return __builtin_bit_cast(float, u << 16); }
+// Nearest, ties to even; NaN stays NaN.
+EOS_DEV uint32_t f32_to_bf16(float f) {
+  return __builtin_bit_cast(uint16_t, (__bf16)f);
+}
+EOS_DEV uint32_t f32_to_f16(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+EOS_DEV float f16_to_f32(uint32_t u) {
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+}
+
+// 8 consecutive elements of a caller's row, and back.
+EOS_DEV void load8(const uint8_t* p, int dtype, float (&x)[8]) {
+  const v4u u = *reinterpret_cast<const v4u*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = u[i] & 0xffffu, b = u[i] >> 16;
+    x[2 * i] = dtype == kKvRowF16 ? f16_to_f32(a) : bf16_to_f32(a);
+    x[2 * i + 1] = dtype == kKvRowF16 ? f16_to_f32(b) : bf16_to_f32(b);
+  }
+}
+EOS_DEV void store8(uint8_t* p, int dtype, const float (&x)[8]) {
+  if (dtype == kKvRowF32) {
+    reinterpret_cast<v4f*>(p)[0] = v4f{x[0], x[1], x[2], x[3]};
+    reinterpret_cast<v4f*>(p)[1] = v4f{x[4], x[5], x[6], x[7]};
+    return;
+  }
+  v4u u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    u[i] = dtype == kKvRowF16 ? f32_to_f16(x[2 * i]) | f32_to_f16(x[2 * i + 1]) << 16
+                              : f32_to_bf16(x[2 * i]) | f32_to_bf16(x[2 * i + 1]) << 16;
+  *reinterpret_cast<v4u*>(p) = u;
+}
+
+// Walsh-Hadamard transform of a row spread over LANES neighbouring lanes, 8
+// consecutive elements each.
+template <int LANES>
+EOS_DEV void hadamard8(float (&x)[8]) {
+#pragma unroll
+  for (int s = 1; s < 8; s *= 2)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((i & s) == 0) {
+        const float a = x[i], b = x[i + s];
+        x[i] = a + b;
+        x[i + s] = a - b;
+      }
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int s = 1; s < LANES; s *= 2)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float o = __shfl_xor(x[i], s);
+      x[i] = (lane & s) != 0 ? o - x[i] : x[i] + o;
+    }
+}
+
+// ------------------------------------------------------------- sequences
+
+EOS_DEV void flag(const KvCacheArgs& c, int bits) {
+  if (bits != 0 && threadIdx.x == 0) atomicOr(c.status, bits);
+}
+
+// The sequence that unit u belongs to and u's index within it; false where
+// no sequence has it. All threads of the workgroup call it.
+EOS_DEV bool find_seq(const KvCacheArgs& c, long long u, int mul, int per, int extra, KvSeq& s,
+                      long long& within) {
+  int count = 0;
+  for (int b0 = 0; b0 < c.batch; b0 += blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    count += __syncthreads_count(b < c.batch && kv_unit_base(c, b, mul, per, extra) <= u);
+  }
+  if (count == 0) return false;
+  s = kv_seq(c, count - 1);
+  flag(c, s.bad);
+  within = u - kv_unit_base(c, count - 1, mul, per, extra);
+  return true;
+}
+
+// --------------------------------------------------------- append and read
+
+// The workgroup's 8 positions and their page.
+EOS_DEV bool find_group(const KvCacheArgs& c, KvGroup8& g, int& page) {
+  KvSeq s;
+  long long within = 0;
+  if (c.offsets == nullptr) {
+    s = kv_seq(c, blockIdx.x);
+    flag(c, s.bad);
+  } else if (!find_seq(c, blockIdx.x, 1, kKvGroup, 2, s, within)) {
+    return false;
+  }
+  if (!kv_group8(s, within, g)) return false;
+  page = kv_page(c, s.b, g.pos0);
+  if (page < 0) flag(c, kKvBadPage);
+  return page >= 0;
+}
+
+// One workgroup of 2 D threads: 8 positions (one V group) of one head, the
+// first half of the threads K, the second V, D / 8 lanes a row of 8 elements.
+// The workgroup owns the group's words, so a partly filled 4-bit word is read
+// and merged without another writer.
+template <int FMT, int D>
+EOS_DEV void append_group(const KvRowsArgs& a) {
+  constexpr int LANES = D / 8;
+  __shared__ uint16_t vt[FMT == kKvTq4 ? 1 : D * 8];
+  __shared__ uint32_t vw[FMT == kKvTq4 ? 8 * LANES : 1];
+  const KvCacheArgs& c = a.c;
+  const int tid = threadIdx.x, h = blockIdx.y;
+  KvGroup8 g;
+  int page;
+  if (!find_group(c, g, page)) return;
+  const int slot0 = g.pos0 & ((1 << c.page_shift) - 1);
+  const size_t block = ((size_t)page * c.kv_heads + h) << c.page_shift;  // tokens before
+  const bool is_v = tid >= D;
+  const int r = (tid / LANES) & 7, l8 = tid % LANES;
+  const bool live = r >= g.from && r < g.upto;
+  float x[8] = {};
+  if (live) {
+    const long long row = g.row + r;
+    const uint8_t* src = is_v ? a.v : a.k;
+    const long long stride = is_v ? a.v_stride : a.k_stride;
+    const size_t at = ((size_t)row * stride + (size_t)h * D + l8 * 8) * 2;
+    if constexpr (FMT == kKvF16 || FMT == kKvBf16) {
+      const v4u u = *reinterpret_cast<const v4u*>(src + at);
+      if (!is_v) {
+        *reinterpret_cast<v4u*>(c.k + ((block + slot0 + r) * D + l8 * 8) * 2) = u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          vt[(l8 * 8 + 2 * i) * 8 + r] = (uint16_t)u[i];
+          vt[(l8 * 8 + 2 * i + 1) * 8 + r] = (uint16_t)(u[i] >> 16);
+        }
+      }
+    } else {
+      load8(src + at, a.dtype, x);
+    }
+  }
+  if constexpr (FMT == kKvQ8) {
+    float m = 0.0f;
+    bool odd = false;  // NaN or infinity
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      m = fmaxf(m, fabsf(x[i]));
+      odd |= !(fabsf(x[i]) <= 3.4028234e38f);
+    }
+    int bad = odd;
+#pragma unroll
+    for (int o = 1; o < LANES; o *= 2) {
+      m = fmaxf(m, __shfl_xor(m, o));
+      bad |= __shfl_xor(bad, o);
+    }
+    float scale = __fdiv_rn(m, 127.0f);
+    const bool none = scale < kTiny;
+    const bool nan = bad != 0 || scale > kHuge;
+    const float inv = none || nan ? 0.0f : __fdiv_rn(127.0f, m);
+    scale = nan ? __builtin_nanf("") : none ? 0.0f : scale;
+    uint32_t code[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q = nan ? 0.0f : fminf(fmaxf(rintf(x[i] * inv), -127.0f), 127.0f);
+      code[i] = (uint32_t)(int)q & 0xffu;
+    }
+    if (live) {
+      if (l8 == 0) (is_v ? c.v_scale : c.k_scale)[block + slot0 + r] = scale;
+      if (!is_v) {
+        *reinterpret_cast<v2u*>(c.k + (block + slot0 + r) * D + l8 * 8) =
+            v2u{code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
+                code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vt[(l8 * 8 + i) * 8 + r] = (uint16_t)code[i];
+      }
+    }
+  }
+  if constexpr (FMT == kKvTq4) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += (double)x[i] * (double)x[i];
+#pragma unroll
+    for (int o = 1; o < LANES; o *= 2) ss += __shfl_xor(ss, o);
+    float scale = (float)__builtin_sqrt(ss * (1.0 / D));
+    const bool none = scale < kTiny;
+    const bool nan = !(scale <= kHuge);
+    if (none || nan) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+    }
+    const v4f s0 = reinterpret_cast<const v4f*>(c.t.signs + l8 * 8)[0];
+    const v4f s1 = reinterpret_cast<const v4f*>(c.t.signs + l8 * 8)[1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= i < 4 ? s0[i & 3] : s1[i & 3];
+    hadamard8<LANES>(x);
+    // |w| / (s sqrt(D)) against the edges, the division moved to their side.
+    const float norm = none || nan ? 0.0f : scale * (float)__builtin_sqrt((double)D);
+    scale = nan ? __builtin_nanf("") : none ? 0.0f : scale;
+    float edge[7];
+#pragma unroll
+    for (int e = 0; e < 7; ++e) edge[e] = c.t.edges[e] * norm;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t idx = x[i] < 0.0f ? 8u : 0u;
+      const float w = fabsf(x[i]);
+#pragma unroll
+      for (int e = 0; e < 7; ++e) idx += w > edge[e] ? 1u : 0u;
+      word |= idx << (4 * i);
+    }
+    if (live && l8 == 0) (is_v ? c.v_scale : c.k_scale)[block + slot0 + r] = scale;
+    if (!is_v) {
+      if (live) reinterpret_cast<uint32_t*>(c.k)[(block + slot0 + r) * LANES + l8] = word;
+    } else {
+      vw[r * LANES + l8] = word;
+    }
+  }
+  __syncthreads();
+  // V: the group's 8 tokens of one dimension by one thread.
+  if (tid >= D) return;
+  const bool whole = g.from == 0 && g.upto == kKvGroup;
+  const size_t vrow = (block / kKvGroup + slot0 / kKvGroup) * D + tid;  // group-dimensions before
+  if constexpr (FMT == kKvF16 || FMT == kKvBf16) {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(c.v) + vrow * 8;
+    if (whole) {
+      *reinterpret_cast<v4u*>(dst) = *reinterpret_cast<const v4u*>(&vt[tid * 8]);
+    } else {
+      for (int t = g.from; t < g.upto; ++t) dst[t] = vt[tid * 8 + t];
+    }
+  } else if constexpr (FMT == kKvQ8) {
+    uint8_t* dst = c.v + vrow * 8;
+    if (whole) {
+      const v4u u = *reinterpret_cast<const v4u*>(&vt[tid * 8]);
+      *reinterpret_cast<v2u*>(dst) = v2u{perm(u[1], u[0], 0x06040200), perm(u[3], u[2], 0x06040200)};
+    } else {
+      for (int t = g.from; t < g.upto; ++t) dst[t] = (uint8_t)vt[tid * 8 + t];
+    }
+  } else {
+    uint32_t* dst = reinterpret_cast<uint32_t*>(c.v) + vrow;
+    uint32_t word = 0, mask = 0;
+    for (int t = g.from; t < g.upto; ++t) {
+      word |= (vw[t * LANES + tid / 8] >> (4 * (tid & 7)) & 15u) << (4 * t);
+      mask |= 15u << (4 * t);
+    }
+    *dst = whole ? word : (*dst & ~mask) | word;
+  }
+}
+
+// The values of 8 positions of one head, same shape of workgroup.
+template <int FMT, int D>
+EOS_DEV void read_group(const KvRowsArgs& a) {
+  constexpr int LANES = D / 8;
+  const KvCacheArgs& c = a.c;
+  const int tid = threadIdx.x, h = blockIdx.y;
+  KvGroup8 g;
+  int page;
+  if (!find_group(c, g, page)) return;
+  const int slot0 = g.pos0 & ((1 << c.page_shift) - 1);
+  const size_t block = ((size_t)page * c.kv_heads + h) << c.page_shift;
+  const bool is_v = tid >= D;
+  const int r = (tid / LANES) & 7, l8 = tid % LANES;
+  const bool live = r >= g.from && r < g.upto;
+  const size_t token = block + slot0 + r;
+  const size_t vrow = (block / kKvGroup + slot0 / kKvGroup) * D + l8 * 8;
+  float x[8] = {};
+  if (live) {
+    if constexpr (FMT == kKvF16 || FMT == kKvBf16) {
+      constexpr int kType = FMT == kKvF16 ? kKvRowF16 : kKvRowBf16;
+      if (!is_v) {
+        load8(c.k + (token * D + l8 * 8) * 2, kType, x);
+      } else {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(c.v) + vrow * 8 + r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[i] = kType == kKvRowF16 ? f16_to_f32(src[i * 8]) : bf16_to_f32(src[i * 8]);
+      }
+    } else if constexpr (FMT == kKvQ8) {
+      const int8_t* src = reinterpret_cast<const int8_t*>(is_v ? c.v + vrow * 8 + r
+                                                               : c.k + token * D + l8 * 8);
+      const int step = is_v ? 8 : 1;
+      const float scale = (is_v ? c.v_scale : c.k_scale)[token];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)src[i * step] * scale;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t code =
+            is_v ? reinterpret_cast<const uint32_t*>(c.v)[vrow + i] >> (4 * r) & 15u
+                 : reinterpret_cast<const uint32_t*>(c.k)[token * LANES + l8] >> (4 * i) & 15u;
+        float m = c.t.mags[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) m = (code & 7u) == (uint32_t)e ? c.t.mags[e] : m;
+        x[i] = (code & 8u) != 0 ? -m : m;
+      }
+    }
+  }
+  if constexpr (FMT == kKvTq4) {
+    hadamard8<LANES>(x);
+    if (live) {
+      const float scale = (is_v ? c.v_scale : c.k_scale)[token];
+      const float f = scale * (float)(1.0 / __builtin_sqrt((double)D));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= f * c.t.signs[l8 * 8 + i];
+    }
+  }
+  if (!live) return;
+  const long long row = g.row + r;
+  uint8_t* dst = is_v ? a.v : a.k;
+  const long long stride = is_v ? a.v_stride : a.k_stride;
+  const size_t at = (size_t)row * stride + (size_t)h * D + l8 * 8;
+  store8(dst + at * (a.dtype == kKvRowF32 ? 4 : 2), a.dtype, x);
+}
+
+// ---------------------------------------------------------------- attention
+
+EOS_DEV bool find_tile(const KvAttnArgs& a, long long u, KvTile& t) {
+  long long within = 0;
+  if (a.c.offsets == nullptr) {
+    const int per = (a.group + kKvTileRows - 1) / kKvTileRows;
+    t.s = kv_seq(a.c, (int)(u / per));
+    flag(a.c, t.s.bad);
+    within = u % per;
+  } else if (!find_seq(a.c, u, a.group, kKvTileRows, 1, t.s, within)) {
+    return false;
+  }
+  return kv_tile(t, within, kKvTileRows, a.group, a.window, a.splits);
+}
+
+// int8 codes -> f16, exact: 0x6400 | b is 1024 + b.
+EOS_DEV void codes_to_f16(uint32_t x, uint32_t (&out)[2]) {
+  const uint32_t b = x ^ 0x80808080u;
+  const v2h off = v2h{(_Float16)1152.0f, (_Float16)1152.0f};
+  out[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, perm(0x64646464u, b, 0x04010400u)) - off);
+  out[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, perm(0x64646464u, b, 0x04030402u)) - off);
+}
+
+// Eight 4-bit codes -> f16 magnitudes with their signs, in the order 0 2 4 6
+// 1 3 5 7: the magnitudes' bytes by two table lookups each over four codes.
+EOS_DEV void nibbles_to_f16(const KvTables& t, uint32_t x, uint32_t (&out)[4]) {
+  const uint32_t e = x & 0x07070707u, o = (x >> 4) & 0x07070707u;
+  const uint32_t eh = perm(t.hi[1], t.hi[0], e) | ((x << 4) & 0x80808080u);
+  const uint32_t el = perm(t.lo[1], t.lo[0], e);
+  const uint32_t oh = perm(t.hi[1], t.hi[0], o) | (x & 0x80808080u);
+  const uint32_t ol = perm(t.lo[1], t.lo[0], o);
+  out[0] = perm(eh, el, 0x05010400u);
+  out[1] = perm(eh, el, 0x07030602u);
+  out[2] = perm(oh, ol, 0x05010400u);
+  out[3] = perm(oh, ol, 0x07030602u);
+}
+
+template <int FMT>
+EOS_DEV v4f mfma16(v4u a, v4u b, v4f c) {
+  if constexpr (FMT == kKvBf16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a),
+                                                   __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
+                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+template <int FMT>
+EOS_DEV uint32_t pack2(float a, float b) {
+  if constexpr (FMT == kKvBf16)
+    return f32_to_bf16(a) | f32_to_bf16(b) << 16;
+  else
+    return f32_to_f16(a) | f32_to_f16(b) << 16;
+}
+
+// Place in a word of 8 codes of operand slot i.
+template <int FMT>
+constexpr int slot_of(int i) {
+  return FMT == kKvTq4 ? (i < 4 ? 2 * i : 2 * (i - 4) + 1) : i;
+}
+
+EOS_DEV float group_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+EOS_DEV float group_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// Eight outputs of one row: rotated back (tq4), divided, rounded and stored.
+template <int FMT, int D>
+EOS_DEV void finish_row(const KvAttnArgs& a, const KvSeq& s, int r, int h, int l8, bool live,
+                        float (&x)[8], float m, float l) {
+  if constexpr (FMT == kKvTq4) {
+    hadamard8<D / 8>(x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] *= a.c.t.signs[l8 * 8 + i] * (float)(1.0 / __builtin_sqrt((double)D));
+  }
+  if (!live) return;
+  const float inv = l != 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= inv;
+  const long long row = s.row0 + r / a.group;
+  const int head = h * a.group + r % a.group;
+  store8(a.out + ((size_t)row * a.out_stride + (size_t)head * D + l8 * 8) * 2, a.dtype, x);
+  if (a.lse != nullptr && l8 == 0)
+    a.lse[(size_t)row * a.heads + head] =
+        l != 0.0f ? (m + __log2f(l)) * 0.69314718056f : -__builtin_inff();
+}
+
+// One workgroup: 16 query rows of a head group against one split of their
+// keys, 32 keys a wavefront and step. Scores are computed as K q^T and the
+// outputs as V^T p^T, so a lane's 8 scores (keys 8 g .. 8 g + 7 of the step, g
+// = lane / 16, query lane % 16) are the 8 consecutive summands that its
+// operand of the second product holds: nothing crosses lanes between the two.
+// K's rows are taken in the order 8 (r / 4) + 4 j + r % 4 for that.
+template <int FMT, int D>
+EOS_DEV void attn_split(const KvAttnArgs& a) {
+  constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
+  constexpr int BITS = bits_of(FMT), KS = D / 32, NT = D / 16, LANES = D / 8;
+  // Dimensions of V in one load of a lane, loads a step, words of a load.
+  constexpr int VW = FMT == kKvTq4 ? (D >= 64 ? 4 : 2) : FMT == kKvQ8 ? 2 : 1;
+  constexpr int VL = NT / VW, VWORDS = VW * BITS * 8 / 32;
+  // Words of K a lane loads of each of its two keys.
+  constexpr int KWORDS = D * BITS / 4 / 32;
+  __shared__ float so[4][16 * D];
+  __shared__ float sm[4][16], sl[4][16];
+  const KvCacheArgs& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = blockIdx.x % a.splits, h = blockIdx.y;
+  const long long u = blockIdx.x / a.splits;
+  KvTile t;
+  if (!find_tile(a, u, t)) return;
+  if (split >= t.splits && (split > 0 || a.splits > 1)) return;
+  const int P = 1 << c.page_shift;
+  const int rr = t.r0 + r16;
+  const bool real = rr < t.s.n * a.group;
+  const int qrow = real ? rr / a.group : 0;
+  const int qpos = kv_row_pos(t.s, qrow);
+  const int hi_c = real ? kv_min(qpos + 1, t.s.keys) : t.hi;
+  const int lo_c = real && a.window > 0 ? qpos - a.window + 1 : 0;
+
+  // The query as the second operand; quantized formats take it in f16 with
+  // its largest element brought to [0.5, 1), tq4 rotated.
+  v4u q[KS];
+  float qs = a.scale;
+  {
+    const uint8_t* src = a.q + ((size_t)(t.s.row0 + qrow) * a.q_stride +
+                                (size_t)(h * a.group + (real ? rr % a.group : 0)) * D) * 2;
+    if constexpr (!kQuant) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        q[s] = real ? *reinterpret_cast<const v4u*>(src + (s * 32 + g * 8) * 2) : v4u{0, 0, 0, 0};
+    } else {
+      float x[KS][8];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if (real) load8(src + (g * (D / 4) + s * 8) * 2, a.dtype, x[s]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (!real) x[s][i] = 0.0f;
+          if (FMT == kKvTq4) x[s][i] *= c.t.signs[g * (D / 4) + s * 8 + i];
+        }
+      }
+      if constexpr (FMT == kKvTq4) {
+#pragma unroll
+        for (int st = 1; st < D / 4; st *= 2)
+#pragma unroll
+          for (int i = 0; i < D / 4; ++i)
+            if ((i & st) == 0) {
+              const float p = x[i / 8][i % 8], m = x[(i + st) / 8][(i + st) % 8];
+              x[i / 8][i % 8] = p + m;
+              x[(i + st) / 8][(i + st) % 8] = p - m;
+            }
+#pragma unroll
+        for (int st = 16; st < 64; st *= 2)
+#pragma unroll
+          for (int i = 0; i < D / 4; ++i) {
+            const float o = __shfl_xor(x[i / 8][i % 8], st);
+            x[i / 8][i % 8] = (lane & st) != 0 ? o - x[i / 8][i % 8] : x[i / 8][i % 8] + o;
+          }
+        qs *= (float)(1.0 / __builtin_sqrt((double)D));
+      }
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) most = fmaxf(most, fabsf(x[i / 8][i % 8]));
+      most = group_max(most);
+      // Powers of two only: exact but for elements 2^-14 below the largest.
+      int ex = most > 0.0f && most < __builtin_inff() ? __builtin_amdgcn_frexp_expf(most) : 0;
+      const float down = __builtin_amdgcn_ldexpf(1.0f, max(-ex, -126));
+      qs = __builtin_amdgcn_ldexpf(qs, ex);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          q[s][i] = pack2<FMT>(x[s][slot_of<FMT>(2 * i)] * down, x[s][slot_of<FMT>(2 * i + 1)] * down);
+    }
+  }
+
+  v4f acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = v4f{0, 0, 0, 0};
+  // Probabilities are 2^(score - m - e): m follows the scores, 2^e the scales
+  // of V, so that probability times scale stays below 2^8 in f16. Both move
+  // only when a score passes m + 8 or a scale 2^e.
+  float m = kLowest, l = 0.0f, e = kQuant ? -100.0f : 0.0f, elim = 0x1p-100f;
+  const int end = kv_min(t.hi, t.base + (split + 1) * t.chunk);
+  const size_t head_bytes = ((size_t)D * BITS / 8) << c.page_shift;
+  for (int tb = t.base + split * t.chunk + 32 * wave; tb < end; tb += 128) {
+    // The pages of this lane's keys of K and of V.
+    auto page = [&](int token16, bool& ok) {
+      int p = -1;
+      ok = token16 < t.hi && token16 + 16 > t.lo;
+      if (ok) {
+        p = kv_page(c, t.s.b, token16);
+        if (p < 0) {
+          atomicOr(c.status, kKvBadPage);
+          ok = false;
+        }
+      }
+      return ok ? p : 0;
+    };
+    bool kok, vok;
+    const int kp = page(tb + 16 * (r16 >> 3), kok), vp = page(tb + 16 * (g >> 1), vok);
+    const uint8_t* kb = c.k + ((size_t)kp * c.kv_heads + h) * head_bytes;
+    const uint8_t* vb = c.v + ((size_t)vp * c.kv_heads + h) * head_bytes;
+    const int vslot = (tb + 8 * g) & (P - 1);
+    uint32_t kr[2][KWORDS], vr[VL][VWORDS];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int slot = (tb + 8 * (r16 >> 2) + 4 * j + (r16 & 3)) & (P - 1);
+      const uint8_t* row = kb + (size_t)slot * (D * BITS / 8);
+      if constexpr (!kQuant) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const v4u x = *reinterpret_cast<const v4u*>(row + (s * 32 + g * 8) * 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) kr[j][4 * s + i] = x[i];
+        }
+      } else {
+        __builtin_memcpy(kr[j], __builtin_assume_aligned(row + g * (KWORDS * 4), KWORDS >= 4 ? 16 : KWORDS * 4),
+                         KWORDS * 4);
+      }
+    }
+    const uint8_t* vrow = vb + (size_t)(vslot / kKvGroup) * (D * BITS);
+#pragma unroll
+    for (int i = 0; i < VL; ++i)
+      __builtin_memcpy(vr[i], __builtin_assume_aligned(vrow + (i * 16 + r16) * (VWORDS * 4), VWORDS * 4),
+                       VWORDS * 4);
+    float ks[8], vs[8];
+    if constexpr (kQuant) {
+      const size_t at = (((size_t)vp * c.kv_heads + h) << c.page_shift) + vslot;
+      __builtin_memcpy(ks, __builtin_assume_aligned(c.k_scale + at, 16), 32);
+      __builtin_memcpy(vs, __builtin_assume_aligned(c.v_scale + at, 16), 32);
+    }
+    const bool masked = tb + 32 > t.all_hi || tb < t.all_lo || __any(!vok);
+
+    v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t f[4];
+        if constexpr (FMT == kKvTq4) {
+          nibbles_to_f16(c.t, kr[j][s], f);
+        } else if constexpr (FMT == kKvQ8) {
+          uint32_t lo2[2], hi2[2];
+          codes_to_f16(kr[j][2 * s], lo2);
+          codes_to_f16(kr[j][2 * s + 1], hi2);
+          f[0] = lo2[0], f[1] = lo2[1], f[2] = hi2[0], f[3] = hi2[1];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = kr[j][4 * s + i];
+        }
+        sc[j] = mfma16<FMT>(v4u{f[0], f[1], f[2], f[3]}, q[s], sc[j]);
+      }
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = sc[i >> 2][i & 3] * qs;
+      if (kQuant) x[i] *= ks[i];
+    }
+    uint32_t vmask[4] = {~0u, ~0u, ~0u, ~0u};
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = tb + 8 * g + i;
+        const bool there = vok && key >= t.lo && key < t.hi;
+        if (!(there && key >= lo_c && key < hi_c)) x[i] = -__builtin_inff();
+        if (kQuant && !there) vs[i] = 0.0f;
+        if (!there) vmask[i >> 1] &= (i & 1) != 0 ? 0x0000ffffu : 0xffff0000u;
+      }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+    if (__any(mx > m + 8.0f)) {
+      const float nm = fmaxf(m, group_max(mx));
+      const float f = __builtin_amdgcn_exp2f(m - nm);
+      m = nm;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[i] *= f;
+    }
+    if constexpr (kQuant) {
+      float mv = vs[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mv = fmaxf(mv, vs[i]);
+      if (__any(mv > elim)) {
+        mv = group_max(mv);
+        const float ne = fmaxf(e, (float)__builtin_amdgcn_frexp_expf(mv));
+        const float f = __builtin_amdgcn_exp2f(e - ne);
+        e = ne;
+        elim = __builtin_amdgcn_ldexpf(1.0f, (int)ne);
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] *= f;
+      }
+    }
+    const float ref = m + e;
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+      l += p[i];
+      // (a masked key's scale may be NaN: it must not reach the row)
+      if (kQuant) p[i] = masked && x[i] == -__builtin_inff() ? 0.0f : p[i] * vs[i];
+    }
+    v4u pf;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pf[i] = pack2<FMT>(p[slot_of<FMT>(2 * i)], p[slot_of<FMT>(2 * i + 1)]);
+    if constexpr (!kQuant) {
+      bool odd = false;  // a NaN or infinity that some row must not see
+      if (masked) {
+        constexpr uint32_t kExp = FMT == kKvF16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+        for (int i = 0; i < VL; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            vr[i][w] &= vmask[w];
+            odd |= (vr[i][w] & kExp) == kExp || (vr[i][w] >> 16 & kExp) == kExp;
+          }
+      }
+      if (__any(odd)) {
+        // Key by key without the matrix unit, rows that mask it left out.
+        for (int og = 0; og < 4; ++og)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int from = og * 16 + r16;
+            const float px = __shfl(p[i], from), sx = __shfl(x[i], from);
+            const int opage = __shfl(vp, og * 16);
+            const int slot = (tb + 8 * og + i) & (P - 1);
+            const uint16_t* ov = reinterpret_cast<const uint16_t*>(
+                c.v + ((size_t)opage * c.kv_heads + h) * head_bytes) + (size_t)(slot / 8) * D * 8 + i;
+            if (sx == -__builtin_inff()) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t w = ov[(16 * n + 4 * g + k) * 8];
+                acc[n][k] += px * (FMT == kKvF16 ? f16_to_f32(w) : bf16_to_f32(w));
+              }
+          }
+        continue;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i)
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        uint32_t f[4];
+        if constexpr (FMT == kKvTq4) {
+          nibbles_to_f16(c.t, vr[i][w], f);
+        } else if constexpr (FMT == kKvQ8) {
+          uint32_t lo2[2], hi2[2];
+          codes_to_f16(vr[i][2 * w], lo2);
+          codes_to_f16(vr[i][2 * w + 1], hi2);
+          f[0] = lo2[0], f[1] = lo2[1], f[2] = hi2[0], f[3] = hi2[1];
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f[k] = vr[i][k];
+        }
+        acc[i * VW + w] = mfma16<FMT>(v4u{f[0], f[1], f[2], f[3]}, pf, acc[i * VW + w]);
+      }
+  }
+
+  // The four wavefronts' parts, brought to one reference.
+  l = group_sum(l);
+  const float ref = m + e;
+  if (g == 0) {
+    sm[wave][r16] = ref;
+    sl[wave][r16] = l;
+  }
+  __syncthreads();
+  float top = sm[0][r16];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) top = fmaxf(top, sm[w][r16]);
+  const float f = __builtin_amdgcn_exp2f(ref - top);
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      so[wave][r16 * D + (i / VW) * 16 * VW + VW * (4 * g + k) + i % VW] = acc[i][k] * f;
+  __syncthreads();
+  for (int it = tid; it < 16 * LANES; it += 256) {
+    const int r = it / LANES, l8 = it % LANES;
+    float o[8], mt = sm[0][r], lt = 0.0f;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) mt = fmaxf(mt, sm[w][r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) lt += sl[w][r] * __builtin_amdgcn_exp2f(sm[w][r] - mt);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = r * D + l8 * 8 + i;
+      o[i] = so[0][at] + so[1][at] + so[2][at] + so[3][at];
+    }
+    const bool live = t.r0 + r < t.s.n * a.group;
+    if (a.splits == 1) {
+      finish_row<FMT, D>(a, t.s, t.r0 + r, h, l8, live, o, mt, lt);
+    } else if (live) {
+      const size_t at = (((size_t)u * c.kv_heads + h) * a.splits + split) * 16 + r;
+      reinterpret_cast<v4f*>(a.part + at * D + l8 * 8)[0] = v4f{o[0], o[1], o[2], o[3]};
+      reinterpret_cast<v4f*>(a.part + at * D + l8 * 8)[1] = v4f{o[4], o[5], o[6], o[7]};
+      if (l8 == 0) {
+        a.part_ml[at * 2] = mt;
+        a.part_ml[at * 2 + 1] = lt;
+      }
+    }
+  }
+}
+
+// Joins a row's splits: one workgroup a row and head, D / 8 lanes a split.
+template <int FMT, int D>
+EOS_DEV void attn_join(const KvAttnArgs& a) {
+  constexpr int LANES = D / 8, NG = 256 / LANES;
+  __shared__ float so[NG][D];
+  __shared__ float sl[NG];
+  __shared__ float smax[4];
+  const KvCacheArgs& c = a.c;
+  const int tid = threadIdx.x, l8 = tid % LANES, grp = tid / LANES;
+  const int head = blockIdx.y, h = head / a.group;
+  KvTile t;
+  long long within = 0, u;
+  if (c.offsets == nullptr) {
+    t.s = kv_seq(c, blockIdx.x);
+  } else if (!find_seq(c, blockIdx.x, 1, 1, 0, t.s, within)) {
+    return;
+  }
+  if (within < 0 || within >= t.s.n) return;
+  const int r = (int)within * a.group + head % a.group;
+  kv_tile(t, r / kKvTileRows, kKvTileRows, a.group, a.window, a.splits);
+  u = c.offsets == nullptr
+          ? (long long)t.s.b * ((a.group + kKvTileRows - 1) / kKvTileRows)
+          : kv_unit_base(c, t.s.b, a.group, kKvTileRows, 1);
+  u += r / kKvTileRows;
+  const size_t at = ((size_t)u * c.kv_heads + h) * a.splits * 16 + r % 16;
+  float top = kLowest;
+  for (int i = tid; i < t.splits; i += 256) top = fmaxf(top, a.part_ml[(at + (size_t)i * 16) * 2]);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+  if ((tid & 63) == 0) smax[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
+  float x[8] = {}, l = 0.0f;
+  for (int i = grp; i < t.splits; i += NG) {
+    const size_t p = at + (size_t)i * 16;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[p * 2] - top);
+    l += a.part_ml[p * 2 + 1] * f;
+    const v4f p0 = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[0];
+    const v4f p1 = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] += p0[k] * f;
+      x[4 + k] += p1[k] * f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) so[grp][l8 * 8 + k] = x[k];
+  if (l8 == 0) sl[grp] = l;
+  __syncthreads();
+  if (tid >= LANES) return;
+  l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+  for (int i = 0; i < NG; ++i) {
+    l += sl[i];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] += so[i][l8 * 8 + k];
+  }
+  finish_row<FMT, D>(a, t.s, r, h, l8, true, x, top, l);
+}
+
+}  // namespace
+
+#define KV_KERNELS(NAME, FMT, D)                                                             \
+  extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_append_##NAME##_##D(KvRowsArgs a) { \
+    append_group<FMT, D>(a);                                                                 \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_read_##NAME##_##D(KvRowsArgs a) {   \
+    read_group<FMT, D>(a);                                                                   \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void eos_kv_split_##NAME##_##D(KvAttnArgs a) {    \
+    attn_split<FMT, D>(a);                                                                   \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void eos_kv_join_##NAME##_##D(KvAttnArgs a) {     \
+    attn_join<FMT, D>(a);                                                                    \
+  }
+#define KV_FORMATS(D)           \
+  KV_KERNELS(f16, kKvF16, D)    \
+  KV_KERNELS(bf16, kKvBf16, D)  \
+  KV_KERNELS(q8, kKvQ8, D)      \
+  KV_KERNELS(tq4, kKvTq4, D)
+
+KV_FORMATS(32)
+KV_FORMATS(64)
+KV_FORMATS(128)
+KV_FORMATS(256)

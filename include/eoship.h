@@ -872,6 +872,103 @@ int eoship_hadamard_tq_decode_device(EosHipRuntime* rt, EosHipHadamardTQ* h,
                                      char** err);
 int eoship_hadamard_tq_release(EosHipRuntime* rt, EosHipHadamardTQ* h, char** err);
 
+/* ------------------------------------------------------------------------
+ * Paged key-value cache and attention over it: what a decoder-type embedder
+ * or reranker keeps between its calls (the kv_cache capability that the
+ * reference's CUDA backend advertises, runtime/backend/backend.go:1428-1431),
+ * stored plain, as 8-bit codes, or as 4-bit Hadamard TurboQuant codes.
+ *
+ * The cache is the caller's device memory, `pages` pages of P tokens for H
+ * key-value heads of width D:
+ *   K       [pages][H][P][D]         f16 / bf16 values, or int8 codes
+ *           [pages][H][P][D / 8]     tq4: u32, dimension 8 w + j at bits 4 j
+ *   V       [pages][H][P / 8][D][8]  f16 / bf16 values, or int8 codes: 8
+ *                                    consecutive tokens of a dimension
+ *           [pages][H][P / 8][D]     tq4: u32, token 8 g + j at bits 4 j
+ *   scales  [pages][H][P] f32        one array for K, one for V (q8, tq4)
+ * q8:  s = max|x| / 127, code = rint(x * (127 / max|x|)), stands for code * s.
+ * tq4: w = Hd (signs * x) with the Walsh-Hadamard matrix Hd, s = sqrt(mean
+ *      x^2), index = how many midpoints between codebook magnitudes lie below
+ *      |w| / (s sqrt(D)), code = index + 8 where w < 0, stands for
+ *      signs * Hd (+-codebook[index]) * s / sqrt(D).
+ * A scale below 2^-60 is stored as zero; a row with a NaN, an infinity or a
+ * scale above 2^40 is stored with a NaN scale and reads as NaN.
+ * ------------------------------------------------------------------------ */
+
+typedef struct {
+  int32_t format;         /* 0 f16, 1 bf16, 2 q8, 3 tq4 */
+  int32_t kv_heads;       /* H, 1..1024 */
+  int32_t head_dim;       /* D: 32, 64, 128 or 256 */
+  int32_t page_tokens;    /* P: 16, 32, 64, 128 or 256 */
+  int64_t pages;
+  void* d_k;              /* device, 16-byte aligned */
+  void* d_v;
+  float* d_k_scale;       /* device, 16-byte aligned; q8 and tq4 */
+  float* d_v_scale;
+  const float* codebook;  /* host [8], tq4: ascending magnitudes, positive normal f16 numbers */
+  const float* signs;     /* host [D], tq4: 1 or -1 */
+} EosHipKVDesc;
+
+typedef struct EosHipKVCache EosHipKVCache;
+
+/* A batch of sequences and the rows of a call. Sequence b's rows are
+ * offsets[b] .. offsets[b + 1] - 1 (offsets[0] = 0; d_offsets NULL: row b,
+ * one a sequence, the form for decoding), and stand at its last positions:
+ * row offsets[b + 1] - 1 at lengths[b] - 1. A row whose position would be
+ * negative is padding: not written, not read, attends nothing. Position p
+ * lies in page page_table[b][p / P]; entries past a sequence's length are not
+ * looked at, nor are pages wholly in front of every row's window. Rows from
+ * offsets[batch] on are left as they are. Device memory. */
+typedef struct {
+  const int32_t* d_page_table;  /* [batch][table_stride] */
+  int32_t table_stride;
+  int32_t batch;
+  const int32_t* d_lengths;     /* [batch], the call's rows included */
+  const int32_t* d_offsets;     /* [batch + 1] or NULL */
+  int64_t rows;                 /* rows the caller's arrays hold */
+} EosHipKVBatch;
+
+/* Bytes of the K pool (the V pool has as many) and of each scale pool. */
+int eoship_kv_bytes(const EosHipKVDesc* desc, int64_t* pool_bytes, int64_t* scale_bytes,
+                    char** err);
+/* Checks a batch in host memory before it is uploaded: offsets, lengths and
+ * page ids in range and, with writes nonzero, that no page is written by two
+ * sequences or twice by one (an append of such a batch leaves in the shared
+ * slots parts of either row). desc's device pointers are not looked at. */
+int eoship_kv_check_batch(const EosHipKVDesc* desc, const int32_t* page_table,
+                          int32_t table_stride, int32_t batch, const int32_t* lengths,
+                          const int32_t* offsets, int64_t rows, int32_t writes, char** err);
+/* Binds a cache for one runtime. The pools stay the caller's and have to
+ * outlive the handle; a second runtime binds them again. */
+int eoship_kv_bind(EosHipRuntime* rt, const EosHipKVDesc* desc, EosHipKVCache** out, char** err);
+int eoship_kv_release(EosHipRuntime* rt, EosHipKVCache* kv, char** err);
+/* Writes rows of K and V ([rows][H][D], dtype 0 f16 or 1 bf16, strides in
+ * elements between rows: multiples of 8) into their positions' slots. f16 and
+ * bf16 caches take rows of their own type. Enqueued (no wait). */
+int eoship_kv_append_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
+                            const void* d_k, int64_t k_stride, const void* d_v, int64_t v_stride,
+                            int32_t dtype, char** err);
+/* The values of the rows' positions (dtype 0 f16, 1 bf16, 2 f32): the last
+ * offsets[b + 1] - offsets[b] positions below lengths[b]. Enqueued. */
+int eoship_kv_read_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
+                          void* d_k, int64_t k_stride, void* d_v, int64_t v_stride, int32_t dtype,
+                          char** err);
+/* Attention of the rows' queries ([rows][heads][D]; head i reads key-value
+ * head i / (heads / H)) over the cache, the row's own position (appended
+ * before) included: out = softmax(scale q K^T) V over positions p' <= p, with
+ * window > 0 also p' > p - window. dtype as in append; out likewise. d_lse
+ * ([rows][heads], may be NULL): the logarithm of the weights' sum. A row with
+ * no key gives 0 and -inf. Uses the runtime's workspace. Enqueued. */
+int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
+                               const void* d_q, int64_t q_stride, int32_t heads, int32_t dtype,
+                               float scale, int32_t window, void* d_out, int64_t out_stride,
+                               float* d_lse, char** err);
+/* What the calls since the last status read found out of range on the device
+ * (bit 0 a page id, bit 1 a length, bit 2 an offset); synchronises and clears
+ * it. Positions without a valid page are not written or read and attend as
+ * if masked; nothing outside the pools and rows is touched. */
+int eoship_kv_status(EosHipRuntime* rt, EosHipKVCache* kv, int32_t* status, char** err);
+
 #ifdef __cplusplus
 }
 #endif

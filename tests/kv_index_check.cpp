@@ -1,0 +1,147 @@
+// Walks the work units of the key-value cache kernels on the host, with the
+// kernels' own index arithmetic (kv_index.h), over random batches: every row
+// is covered exactly once, every access stays inside pools, rows and
+// workspace, with sound batches and with damaged ones. Prints OK.
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <vector>
+
+#include "kv_index.h"
+
+namespace {
+
+std::mt19937_64 rng;
+int between(int a, int b) { return a + (int)(rng() % (uint64_t)(b - a + 1)); }
+
+#define CHECK(cond)                                                      \
+  do {                                                                   \
+    if (!(cond)) {                                                       \
+      std::printf("%s:%d: %s (case %d)\n", __FILE__, __LINE__, #cond, at); \
+      std::exit(1);                                                      \
+    }                                                                    \
+  } while (0)
+
+// find_seq of the kernels: how many sequences start at or before unit u.
+bool find(const KvCacheArgs& c, long long u, int mul, int per, int extra, KvSeq& s,
+          long long& within) {
+  int count = 0;
+  for (int b = 0; b < c.batch; ++b) count += kv_unit_base(c, b, mul, per, extra) <= u;
+  if (count == 0) return false;
+  s = kv_seq(c, count - 1);
+  within = u - kv_unit_base(c, count - 1, mul, per, extra);
+  return true;
+}
+
+void one(int at, bool sound) {
+  KvCacheArgs c{};
+  c.batch = between(1, 9);
+  c.page_shift = between(4, 8);
+  c.table_stride = between(1, 6);
+  c.pages = between(1, 40);
+  c.kv_heads = 1;
+  const int P = 1 << c.page_shift, cap = c.table_stride * P;
+  const bool one_each = between(0, 3) == 0;
+  std::vector<int32_t> table(c.batch * c.table_stride), lengths(c.batch), offsets(c.batch + 1);
+  for (auto& p : table) p = between(0, c.pages - 1);
+  for (int b = 0; b < c.batch; ++b) {
+    lengths[b] = between(0, cap);
+    offsets[b + 1] = offsets[b] + (one_each ? 1 : between(0, 2) == 0 ? between(0, 3) : between(0, cap + 5));
+  }
+  c.rows = offsets[c.batch] + (one_each ? 0 : between(0, 9));
+  if (!sound) {
+    const int many = between(1, 4);
+    for (int i = 0; i < many; ++i) {
+      const int32_t odd[] = {-1, INT32_MIN, INT32_MAX, between(-1000, 100000)};
+      const int32_t v = odd[between(0, 3)];
+      switch (between(0, 2)) {
+        case 0: table[between(0, (int)table.size() - 1)] = v; break;
+        case 1: lengths[between(0, c.batch - 1)] = v; break;
+        default: offsets[between(0, c.batch)] = v;
+      }
+    }
+  }
+  c.table = table.data();
+  c.lengths = lengths.data();
+  c.offsets = one_each ? nullptr : offsets.data();
+
+  // append / read
+  std::vector<int> seen(c.rows, 0);
+  const long long groups = one_each ? c.batch : kv_units(c.rows, c.batch, 1, kKvGroup, 2);
+  for (long long u = 0; u < groups; ++u) {
+    KvSeq s;
+    long long within = 0;
+    if (one_each) s = kv_seq(c, (int)u);
+    else if (!find(c, u, 1, kKvGroup, 2, s, within)) continue;
+    KvGroup8 g;
+    if (!kv_group8(s, within, g)) continue;
+    const int page = kv_page(c, s.b, g.pos0);
+    if (page < 0) continue;
+    CHECK(page < c.pages);
+    CHECK((g.pos0 & (P - 1)) + 8 <= P && g.pos0 % 8 == 0);
+    CHECK(g.from >= 0 && g.upto <= 8 && g.from < g.upto);
+    for (int r = g.from; r < g.upto; ++r) {
+      CHECK(g.row + r >= 0 && g.row + r < c.rows);
+      ++seen[g.row + r];
+      if (sound) CHECK(g.pos0 + r == s.len - s.n + (g.row + r - s.row0));
+    }
+  }
+  if (sound)
+    for (int b = 0; b < c.batch; ++b) {
+      const int lo = one_each ? b : offsets[b], n = one_each ? 1 : offsets[b + 1] - lo;
+      for (int i = 0; i < n; ++i) CHECK(seen[lo + i] == (lengths[b] - n + i >= 0 ? 1 : 0));
+    }
+
+  // attention
+  for (int tile_rows : {16, 64, 128}) {
+    const int group = between(1, 20), window = between(0, 1) ? 0 : between(1, cap + 3);
+    const int splits = between(1, 7);
+    const int per = (group + tile_rows - 1) / tile_rows;
+    const long long tiles = one_each ? (long long)c.batch * per
+                                     : kv_units(c.rows, c.batch, group, tile_rows, 1);
+    std::vector<int> rows(c.rows * group, 0);
+    for (long long u = 0; u < tiles; ++u) {
+      KvTile t;
+      long long within = u % per;
+      if (one_each) t.s = kv_seq(c, (int)(u / per));
+      else if (!find(c, u, group, tile_rows, 1, t.s, within)) continue;
+      if (!kv_tile(t, within, tile_rows, group, window, splits)) continue;
+      CHECK(t.splits <= splits && t.lo >= 0 && t.hi <= cap && t.base % 32 == 0);
+      CHECK(t.base <= t.lo && (t.splits > 0 || t.hi == 0));
+      CHECK((long long)t.base + (long long)t.splits * t.chunk >= t.hi);
+      CHECK(t.splits == 0 || t.base + (t.splits - 1) * t.chunk < t.hi);
+      for (int r = t.r0; r < t.r0 + tile_rows && r < t.s.n * group; ++r) {
+        const long long row = t.s.row0 + r / group;
+        CHECK(row >= 0 && row < c.rows);
+        ++rows[row * group + r % group];
+        if (!sound) continue;
+        // The row's own keys lie in [lo, hi), and [all_lo, all_hi) in them.
+        const int pos = kv_row_pos(t.s, r / group);
+        const int hi = kv_min(pos + 1, t.s.keys), lo = window > 0 ? kv_max(0, pos - window + 1) : 0;
+        if (hi > lo) CHECK(lo >= t.lo && hi <= t.hi);
+        CHECK(t.all_hi <= kv_max(hi, 0) && t.all_lo >= (window > 0 ? pos - window + 1 : 0));
+        // The unit that the join computes for this row.
+        const long long unit = (one_each ? (long long)t.s.b * per
+                                         : kv_unit_base(c, t.s.b, group, tile_rows, 1)) +
+                               r / tile_rows;
+        CHECK(unit == u && unit < tiles);
+      }
+    }
+    if (sound) {
+      const long long used = one_each ? c.batch : offsets[c.batch];
+      for (long long i = 0; i < c.rows * group; ++i) CHECK(rows[i] == (i < used * group ? 1 : 0));
+    }
+  }
+}
+
+}  // namespace
+
+int main(int argc, char** argv) {
+  const int cases = argc > 1 ? std::atoi(argv[1]) : 2000;
+  for (int i = 0; i < cases; ++i) {
+    rng.seed(1000 + i);
+    one(i, i % 2 == 0);
+  }
+  std::printf("OK\n");
+  return 0;
+}
