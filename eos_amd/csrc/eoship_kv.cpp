@@ -29,6 +29,8 @@ struct EosHipKVCache {
 
 namespace {
 
+constexpr int kPromptFrom = 48;
+
 const char* const kFormats[] = {"f16", "bf16", "q8", "tq4"};
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -349,23 +351,30 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
   a.window = window;
   a.dtype = dtype;
   const int kvh = kv->d.kv_heads, d = kv->d.head_dim;
-  const long long tiles =
-      batch->d_offsets == nullptr
-          ? (long long)batch->batch * ((a.group + kKvTileRows - 1) / kKvTileRows)
-          : kv_units(batch->rows, batch->batch, a.group, kKvTileRows, 1);
-  // Enough splits to give every CU four workgroups, none below 256 keys.
+  // Rows of a sequence on average, a group's heads counted: a few go 16 at a
+  // time, each wavefront with keys of its own, many 128 at a time.
+  const bool prompt = batch->d_offsets != nullptr &&
+                      batch->rows * a.group > (int64_t)kPromptFrom * batch->batch;
+  a.tile_rows = prompt ? kKvPromptRows : kKvTileRows;
+  a.tiles = batch->d_offsets == nullptr
+                ? (long long)batch->batch * ((a.group + kKvTileRows - 1) / kKvTileRows)
+                : kv_units(batch->rows, batch->batch, a.group, a.tile_rows, 1);
+  // Enough splits to give every CU four workgroups (two of the prompt kernel,
+  // whose registers hold no more), none below 256 keys.
   long long keys = (long long)batch->table_stride << kv->page_shift;
   if (window > 0) keys = std::min(keys, (long long)window + batch->rows + 32);
-  const long long want = (4LL * rt->compute_units + tiles * kvh - 1) / (tiles * kvh);
+  const long long units = a.tiles * kvh;
+  const long long want = ((prompt ? 2LL : 4LL) * rt->compute_units + units - 1) / units;
   a.splits = (int)std::max(1LL, std::min(want, (keys + 255) / 256));
   if (a.splits > 1) {
-    const size_t parts = (size_t)tiles * kvh * a.splits * kKvTileRows;
+    const size_t parts = (size_t)units * a.splits * a.tile_rows;
     void* ws = nullptr;
     if (rt->workspace(parts * (size_t)(d + 2) * 4, &ws, err) != 0) return 1;
     a.part = static_cast<float*>(ws);
     a.part_ml = a.part + parts * (size_t)d;
   }
-  if (launch(rt, kv, "split", tiles * a.splits, kvh, 256, &a, what, err) != 0) return 1;
+  if (launch(rt, kv, prompt ? "prompt" : "split", a.tiles * a.splits, kvh, 256, &a, what, err) != 0)
+    return 1;
   if (a.splits == 1) return 0;
   return launch(rt, kv, "join", batch->rows, heads, 256, &a, what, err);
 }

@@ -14,7 +14,8 @@ enum { kKvRowF16 = 0, kKvRowBf16 = 1, kKvRowF32 = 2 };
 enum { kKvBadPage = 1, kKvBadLength = 2, kKvBadOffset = 4 };
 
 constexpr int kKvGroup = 8;     // tokens of V stored side by side
-constexpr int kKvTileRows = 16;  // query rows of one MFMA column tile
+constexpr int kKvTileRows = 16;    // query rows of a workgroup of the split kernel
+constexpr int kKvPromptRows = 128;  // query rows of a workgroup of the prompt kernel
 
 struct KvTables {
   uint32_t hi[2], lo[2];  // tq4: high and low bytes of the 8 f16 magnitudes
@@ -48,11 +49,12 @@ struct KvAttnArgs {
   const uint8_t* q;
   uint8_t* out;
   float* lse;       // [rows][heads] or NULL
-  float* part;      // [tiles][kv_heads][splits][16][head_dim] unnormalised sums
-  float* part_ml;   // [tiles][kv_heads][splits][16][2] reference and weight sum
+  float* part;      // [tiles][kv_heads][splits][tile_rows][head_dim] unnormalised sums
+  float* part_ml;   // [tiles][kv_heads][splits][tile_rows][2] reference and weight sum
   long long q_stride, out_stride;
   float scale;      // of q . k, times log2(e)
-  int heads, group, window, splits, dtype;
+  long long tiles;
+  int heads, group, window, splits, dtype, tile_rows;
 };
 
 #endif

@@ -355,17 +355,18 @@ EOS_DEV void read_group(const KvRowsArgs& a) {
 
 // ---------------------------------------------------------------- attention
 
+template <int ROWS>
 EOS_DEV bool find_tile(const KvAttnArgs& a, long long u, KvTile& t) {
   long long within = 0;
   if (a.c.offsets == nullptr) {
-    const int per = (a.group + kKvTileRows - 1) / kKvTileRows;
+    const int per = (a.group + ROWS - 1) / ROWS;
     t.s = kv_seq(a.c, (int)(u / per));
     flag(a.c, t.s.bad);
     within = u % per;
-  } else if (!find_seq(a.c, u, a.group, kKvTileRows, 1, t.s, within)) {
+  } else if (!find_seq(a.c, u, a.group, ROWS, 1, t.s, within)) {
     return false;
   }
-  return kv_tile(t, within, kKvTileRows, a.group, a.window, a.splits);
+  return kv_tile(t, within, ROWS, a.group, a.window, a.splits);
 }
 
 // int8 codes -> f16, exact: 0x6400 | b is 1024 + b.
@@ -406,6 +407,44 @@ EOS_DEV uint32_t pack2(float a, float b) {
     return f32_to_bf16(a) | f32_to_bf16(b) << 16;
   else
     return f32_to_f16(a) | f32_to_f16(b) << 16;
+}
+
+// f16 / bf16 values with NaN and infinity apart: `x` keeps the finite ones, `pos`
+// is 1 where +infinity or NaN stood, `neg` where -infinity or NaN did. Returns
+// whether there was any.
+template <int FMT>
+EOS_DEV bool has_odd(v4u x) {
+  constexpr uint32_t kExp = FMT == kKvF16 ? 0x7c00u : 0x7f80u;
+  bool odd = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) odd |= (x[w] & kExp) == kExp || (x[w] >> 16 & kExp) == kExp;
+  return odd;
+}
+template <int FMT>
+EOS_DEV void split_odd(v4u& x, v4u& pos, v4u& neg) {
+  constexpr uint32_t kExp = FMT == kKvF16 ? 0x7c00u : 0x7f80u;
+  constexpr uint32_t kOne = FMT == kKvF16 ? 0x3c00u : 0x3f80u;
+  uint32_t keep[4], up[4], down[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    keep[w] = up[w] = down[w] = 0;
+#pragma unroll
+    for (int s = 0; s < 32; s += 16) {
+      const uint32_t u = x[w] >> s & 0xffffu;
+      const bool odd = (u & kExp) == kExp, nan = odd && (u & 0x7fffu) != kExp;
+      keep[w] |= (odd ? 0u : u) << s;
+      up[w] |= (odd && (nan || u < 0x8000u) ? kOne : 0u) << s;
+      down[w] |= (odd && (nan || u >= 0x8000u) ? kOne : 0u) << s;
+    }
+  }
+  x = v4u{keep[0], keep[1], keep[2], keep[3]};
+  pos = v4u{up[0], up[1], up[2], up[3]};
+  neg = v4u{down[0], down[1], down[2], down[3]};
+}
+// What the odd values that a row sees add to its sum.
+EOS_DEV float odd_sum(float up, float down) {
+  const float inf = __builtin_inff();
+  return (up > 0.0f ? inf : 0.0f) + (down > 0.0f ? -inf : 0.0f);
 }
 
 // Place in a word of 8 codes of operand slot i.
@@ -468,7 +507,7 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
   const int split = blockIdx.x % a.splits, h = blockIdx.y;
   const long long u = blockIdx.x / a.splits;
   KvTile t;
-  if (!find_tile(a, u, t)) return;
+  if (!find_tile<kKvTileRows>(a, u, t)) return;
   if (split >= t.splits && (split > 0 || a.splits > 1)) return;
   const int P = 1 << c.page_shift;
   const int rr = t.r0 + r16;
@@ -668,37 +707,34 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) pf[i] = pack2<FMT>(p[slot_of<FMT>(2 * i)], p[slot_of<FMT>(2 * i + 1)]);
     if constexpr (!kQuant) {
-      bool odd = false;  // a NaN or infinity that some row must not see
+      bool odd = false;
       if (masked) {
-        constexpr uint32_t kExp = FMT == kKvF16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
-        for (int i = 0; i < VL; ++i)
+        for (int i = 0; i < VL; ++i) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            vr[i][w] &= vmask[w];
-            odd |= (vr[i][w] & kExp) == kExp || (vr[i][w] >> 16 & kExp) == kExp;
-          }
+          for (int w = 0; w < 4; ++w) vr[i][w] &= vmask[w];
+          odd |= has_odd<FMT>(v4u{vr[i][0], vr[i][1], vr[i][2], vr[i][3]});
+        }
       }
       if (__any(odd)) {
-        // Key by key without the matrix unit, rows that mask it left out.
-        for (int og = 0; og < 4; ++og)
+        // A NaN or infinity beside rows that must not see it: weight 0 does
+        // not stop it. Finite values as ever, the odd ones counted for the
+        // rows that see them.
+        constexpr uint32_t kOne = FMT == kKvF16 ? 0x3c00u : 0x3f80u;
+        uint32_t see[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int from = og * 16 + r16;
-            const float px = __shfl(p[i], from), sx = __shfl(x[i], from);
-            const int opage = __shfl(vp, og * 16);
-            const int slot = (tb + 8 * og + i) & (P - 1);
-            const uint16_t* ov = reinterpret_cast<const uint16_t*>(
-                c.v + ((size_t)opage * c.kv_heads + h) * head_bytes) + (size_t)(slot / 8) * D * 8 + i;
-            if (sx == -__builtin_inff()) continue;
+        for (int i = 0; i < 8; ++i) see[i / 2] |= (x[i] == -__builtin_inff() ? 0u : kOne) << (16 * (i & 1));
+        const v4u sees = v4u{see[0], see[1], see[2], see[3]};
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < VL; ++i) {
+          v4u v = v4u{vr[i][0], vr[i][1], vr[i][2], vr[i][3]}, pos, neg;
+          split_odd<FMT>(v, pos, neg);
+          acc[i] = mfma16<FMT>(v, pf, acc[i]);
+          const v4f up = mfma16<FMT>(pos, sees, v4f{0, 0, 0, 0});
+          const v4f down = mfma16<FMT>(neg, sees, v4f{0, 0, 0, 0});
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t w = ov[(16 * n + 4 * g + k) * 8];
-                acc[n][k] += px * (FMT == kKvF16 ? f16_to_f32(w) : bf16_to_f32(w));
-              }
-          }
+          for (int k = 0; k < 4; ++k) acc[i][k] += odd_sum(up[k], down[k]);
+        }
         continue;
       }
     }
@@ -767,6 +803,452 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
   }
 }
 
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+template <int FMT>
+EOS_DEV v16f mfma32(v4u a, v4u b, v16f c) {
+  if constexpr (FMT == kKvBf16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a),
+                                                   __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a),
+                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// One 16-byte load of codes as 16-bit operands: BITS / 16 of 8 each.
+template <int FMT>
+EOS_DEV void expand(const KvTables& t, v4u x, v4u (&out)[16 / bits_of(FMT)]) {
+  if constexpr (FMT == kKvTq4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t f[4];
+      nibbles_to_f16(t, x[i], f);
+      out[i] = v4u{f[0], f[1], f[2], f[3]};
+    }
+  } else if constexpr (FMT == kKvQ8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t lo[2], hi[2];
+      codes_to_f16(x[2 * i], lo);
+      codes_to_f16(x[2 * i + 1], hi);
+      out[i] = v4u{lo[0], lo[1], hi[0], hi[1]};
+    }
+  } else {
+    out[0] = x;
+  }
+}
+
+// One workgroup: 128 query rows of a head group, 32 a wavefront, against a
+// split of their keys, 64 (D = 256: 32) at a time through two LDS stages that
+// hold K and V as 16-bit operands. Products as in attn_split, on 32 x 32
+// tiles: scores K q^T, outputs V^T p^T, so a lane (query lane % 32, half lane
+// / 32) holds the scores of keys 16 k + 8 half .. + 7, its operand of the
+// second product; K's rows are read with bits 2 and 3 exchanged for that.
+template <int FMT, int D>
+EOS_DEV void attn_prompt(const KvAttnArgs& a) {
+  constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
+  constexpr int BITS = bits_of(FMT), KS = D / 16, NT = D / 32;
+  constexpr int NK = D == 256 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
+  // 16-byte pieces of 16 tokens and of a stage (of K, and as many of V), a
+  // thread's loads, and the operand pieces of one.
+  constexpr int C16 = D * BITS / 8, CH = BLK * C16, PER = (CH + 255) / 256, EX = 16 / BITS;
+  constexpr int ROWC = D / 8;  // operand pieces of a K row
+  constexpr int RS = ROWC >= 16 ? 1 : 16 / ROWC;  // K rows that share 256 bytes
+  __shared__ v4u lk[2][NK * ROWC], lv[2][NK * ROWC];
+  __shared__ float lsc[2][2][kQuant ? NK : 1];
+  // The stage's first key + 1 where its V holds a NaN or infinity and it is
+  // one that some row masks.
+  __shared__ int lodd[2];
+  const KvCacheArgs& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = blockIdx.x % a.splits, h = blockIdx.y;
+  // The last tiles of a sequence attend the most keys: they go first.
+  const long long u = a.tiles - 1 - blockIdx.x / a.splits;
+  KvTile t;
+  if (!find_tile<kKvPromptRows>(a, u, t)) return;
+  if (split >= t.splits && (split > 0 || a.splits > 1)) return;
+  const int P = 1 << c.page_shift;
+  const int seq = __builtin_amdgcn_readfirstlane(t.s.b);
+  const int lo = __builtin_amdgcn_readfirstlane(t.lo), hi = __builtin_amdgcn_readfirstlane(t.hi);
+  const int begin = __builtin_amdgcn_readfirstlane(t.base + split * t.chunk);
+  const int end = __builtin_amdgcn_readfirstlane(kv_min(t.hi, t.base + (split + 1) * t.chunk));
+  const int all_lo = __builtin_amdgcn_readfirstlane(t.all_lo);
+  const int all_hi = __builtin_amdgcn_readfirstlane(t.all_hi);
+  const size_t head_bytes = ((size_t)D * BITS / 8) << c.page_shift;
+
+  const int nrows = t.s.n * a.group, w0 = t.r0 + 32 * wave, rr = w0 + r32;
+  const bool real = rr < nrows;
+  const int qrow = real ? rr / a.group : 0;
+  const int qpos = kv_row_pos(t.s, qrow);
+  const int hi_c = real ? kv_min(qpos + 1, t.s.keys) : 0;
+  const int lo_c = real && a.window > 0 ? qpos - a.window + 1 : 0;
+  // Keys that some row and that every row of the wavefront attends.
+  const bool busy = w0 < nrows;
+  const int wp0 = kv_row_pos(t.s, w0 / a.group);
+  const int wp1 = kv_row_pos(t.s, (kv_min(w0 + 32, nrows) - 1) / a.group);
+  const int w_hi = busy ? __builtin_amdgcn_readfirstlane(kv_min(t.s.keys, wp1 + 1)) : 0;
+  const int w_lo = __builtin_amdgcn_readfirstlane(a.window > 0 ? wp0 - a.window + 1 : 0);
+  const int w_all_hi = __builtin_amdgcn_readfirstlane(kv_min(t.s.keys, wp0 + 1));
+  const int w_all_lo = __builtin_amdgcn_readfirstlane(a.window > 0 ? wp1 - a.window + 1 : 0);
+
+  // Staging: this thread's pieces of the next stage, on their way.
+  v4u kr[PER], vr[PER];
+  float scr = 0.0f;
+  int okbits = 0, next_ok = 0;
+  bool next_edge = false;
+  auto fetch = [&](int tb) {
+    int pid[BLK];
+    next_ok = 0;
+#pragma unroll
+    for (int j = 0; j < BLK; ++j) {
+      const int t16 = tb + 16 * j;
+      pid[j] = -1;
+      if (t16 < hi && t16 + 16 > lo) {
+        pid[j] = kv_page(c, seq, t16);
+        if (pid[j] < 0) flag(c, kKvBadPage);
+      }
+      if (pid[j] >= 0) next_ok |= 1 << j;
+      pid[j] = kv_max(pid[j], 0);
+    }
+    next_edge = next_ok != (1 << BLK) - 1 || tb + NK > hi || tb < lo;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int id = tid + 256 * i;
+      if (CH % 256 != 0 && id >= CH) break;
+      // (a wavefront's pieces lie in one block of 16 tokens, or in several)
+      const int blk = C16 >= 64 ? __builtin_amdgcn_readfirstlane(id / C16) : id / C16;
+      const int rest = id - blk * C16;
+      int p = pid[0];
+#pragma unroll
+      for (int j = 1; j < BLK; ++j) p = blk == j ? pid[j] : p;
+      const size_t at = ((size_t)p * c.kv_heads + h) * head_bytes +
+                        (size_t)((tb + 16 * blk) & (P - 1)) * (D * BITS / 8) + rest * 16;
+      kr[i] = *reinterpret_cast<const v4u*>(c.k + at);
+      vr[i] = *reinterpret_cast<const v4u*>(c.v + at);
+    }
+    if constexpr (kQuant) {
+      if (tid < 2 * NK) {
+        const int tok = tb + tid % NK;
+        const int p = tok < hi && tok >= lo ? kv_page(c, seq, tok) : -1;
+        const float* sc = tid < NK ? c.k_scale : c.v_scale;
+        scr = p < 0 ? 0.0f
+                    : sc[(((size_t)p * c.kv_heads + h) << c.page_shift) + (tok & (P - 1))];
+      }
+    }
+  };
+  auto store = [&](int st, int tb) {
+    okbits = next_ok;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int id = tid + 256 * i;
+      if (CH % 256 != 0 && id >= CH) break;
+      const int blk = id / C16, rest = id % C16;
+      v4u x[EX];
+      expand<FMT>(c.t, kr[i], x);
+      const int row = blk * 16 + rest / (ROWC / EX), c0 = rest % (ROWC / EX) * EX;
+      const int sw = (row / RS) & (ROWC - 1);
+#pragma unroll
+      for (int e = 0; e < EX; ++e) lk[st][row * ROWC + ((c0 + e) ^ sw)] = x[e];
+      expand<FMT>(c.t, vr[i], x);
+      const int grp = rest / (D / EX);
+      if constexpr (!kQuant) {
+        if (next_edge) {
+          // Nothing may be read of slots that hold no token: they can be NaN.
+          const int t0 = tb + 16 * blk + 8 * grp;
+          const bool ok = (next_ok >> blk & 1) != 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int t2 = t0 + 2 * w;
+            x[0][w] &= (ok && t2 >= lo && t2 < hi ? 0xffffu : 0u) |
+                       (ok && t2 + 1 >= lo && t2 + 1 < hi ? 0xffff0000u : 0u);
+          }
+        }
+        if ((tb + NK > all_hi || tb < all_lo) && has_odd<FMT>(x[0])) lodd[st] = tb + 1;
+      }
+#pragma unroll
+      for (int e = 0; e < EX; ++e) lv[st][(blk * 2 + grp) * D + rest % (D / EX) * EX + e] = x[e];
+    }
+    if constexpr (kQuant)
+      if (tid < 2 * NK) lsc[st][tid / NK][tid % NK] = scr;
+  };
+
+  if (tid < 2) lodd[tid] = 0;
+  __syncthreads();
+  if (begin < end) fetch(begin);
+
+  // The query as the second operand (see attn_split).
+  v4u q[KS];
+  float qs = fabsf(a.scale);
+  {
+    const uint8_t* src = a.q + ((size_t)(t.s.row0 + qrow) * a.q_stride +
+                                (size_t)(h * a.group + (real ? rr % a.group : 0)) * D) * 2;
+    const uint32_t neg = a.scale < 0.0f ? 0x80008000u : 0u;
+    if constexpr (!kQuant) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        q[s] = real ? *reinterpret_cast<const v4u*>(src + (s * 16 + hh * 8) * 2) : v4u{0, 0, 0, 0};
+        q[s] ^= v4u{neg, neg, neg, neg};
+      }
+    } else {
+      float x[KS][8];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if (real) load8(src + (s * 16 + hh * 8) * 2, a.dtype, x[s]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (!real) x[s][i] = 0.0f;
+          if (FMT == kKvTq4) x[s][i] *= c.t.signs[s * 16 + hh * 8 + i];
+        }
+      }
+      if constexpr (FMT == kKvTq4) {
+#pragma unroll
+        for (int st = 1; st < D / 2; st *= 2)
+#pragma unroll
+          for (int i = 0; i < D / 2; ++i)
+            if ((i & st) == 0) {
+              const float p = x[i / 8][i % 8], m = x[(i + st) / 8][(i + st) % 8];
+              x[i / 8][i % 8] = p + m;
+              x[(i + st) / 8][(i + st) % 8] = p - m;
+            }
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) {
+          const float o = __shfl_xor(x[i / 8][i % 8], 32);
+          x[i / 8][i % 8] = hh != 0 ? o - x[i / 8][i % 8] : x[i / 8][i % 8] + o;
+        }
+        qs *= (float)(1.0 / __builtin_sqrt((double)D));
+      }
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) most = fmaxf(most, fabsf(x[i / 8][i % 8]));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      const int ex = most > 0.0f && most < __builtin_inff() ? __builtin_amdgcn_frexp_expf(most) : 0;
+      float down = __builtin_amdgcn_ldexpf(1.0f, kv_max(-ex, -126));
+      qs = __builtin_amdgcn_ldexpf(qs, ex);
+      if (neg != 0) down = -down;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          q[s][i] = pack2<FMT>(x[s][slot_of<FMT>(2 * i)] * down, x[s][slot_of<FMT>(2 * i + 1)] * down);
+    }
+  }
+  // Scores are compared before their factor, which must not be zero for it.
+  qs = fmaxf(qs, 0x1p-120f);
+  const float iqs = __fdiv_rn(1.0f, qs);
+
+  v16f acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = v16f{0};
+  float m = kLowest, l = 0.0f, e = kQuant ? -100.0f : 0.0f, elim = 0x1p-100f;
+  float lim = (m + 8.0f) * iqs;
+  // K row of lane r32: token bits 2 and 3 exchanged.
+  const int krow = (r32 & 19) | (r32 >> 1 & 4) | (r32 << 1 & 8);
+  if (begin < end) store(0, begin);
+  __syncthreads();
+  int st = 0;
+  for (int tb = begin; tb < end; tb += NK, st ^= 1) {
+    const int ok = okbits;
+    if (tb + NK < end) fetch(tb + NK);
+    if (tb < w_hi && tb + NK > w_lo) {
+      const bool masked = tb + NK > w_all_hi || tb < w_all_lo || ok != (1 << BLK) - 1;
+      v16f s[TT];
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        s[tt] = v16f{0};
+        const int row = tt * 32 + krow;
+        const int sw = (row / RS) & (ROWC - 1);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          s[tt] = mfma32<FMT>(lk[st][row * ROWC + ((2 * k + hh) ^ sw)], q[k], s[tt]);
+      }
+      float mv = 0.0f;
+      if constexpr (kQuant) {
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int tok = 32 * tt + 16 * (i / 8) + 8 * hh + i % 8;
+            s[tt][i] *= lsc[st][0][tok];
+            mv = fmaxf(mv, lsc[st][1][tok]);
+          }
+      }
+      if (masked) {
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int tok = 32 * tt + 16 * (i / 8) + 8 * hh + i % 8, key = tb + tok;
+            if (!(key >= lo_c && key < hi_c && (ok >> (2 * tt + i / 8) & 1) != 0))
+              s[tt][i] = -__builtin_inff();
+          }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
+      if (__any(mx > lim)) {
+        const float nm = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * qs);
+        const float f = __builtin_amdgcn_exp2f(m - nm);
+        m = nm;
+        lim = (m + 8.0f) * iqs;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] *= f;
+      }
+      if constexpr (kQuant) {
+        if (__any(mv > elim)) {
+          mv = fmaxf(mv, __shfl_xor(mv, 32));
+          const float ne = fmaxf(e, (float)__builtin_amdgcn_frexp_expf(mv));
+          const float f = __builtin_amdgcn_exp2f(e - ne);
+          e = ne;
+          elim = __builtin_amdgcn_ldexpf(1.0f, (int)ne);
+          l *= f;
+#pragma unroll
+          for (int i = 0; i < NT; ++i) acc[i] *= f;
+        }
+      }
+      const float ref = -(m + e);
+      v4u pf[2 * TT];
+#pragma unroll
+      for (int kk = 0; kk < 2 * TT; ++kk) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = s[kk / 2][8 * (kk % 2) + i];
+          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, qs, ref));
+          l += p[i];
+          if constexpr (kQuant) {
+            const float pv = p[i] * lsc[st][1][16 * kk + 8 * hh + i];
+            p[i] = masked && x == -__builtin_inff() ? 0.0f : pv;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          pf[kk][i] = pack2<FMT>(p[slot_of<FMT>(2 * i)], p[slot_of<FMT>(2 * i + 1)]);
+      }
+      if (!kQuant && masked && lodd[st] == tb + 1) {
+        // (see attn_split; one sum after the other to hold few registers)
+        constexpr uint32_t kOne = FMT == kKvF16 ? 0x3c00u : 0x3f80u;
+        v4u sees[2 * TT];
+#pragma unroll
+        for (int kk = 0; kk < 2 * TT; ++kk) {
+          uint32_t see[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = tb + 16 * kk + 8 * hh + i;
+            if (key >= lo_c && key < hi_c && (ok >> kk & 1) != 0) see[i / 2] |= kOne << (16 * (i & 1));
+          }
+          sees[kk] = v4u{see[0], see[1], see[2], see[3]};
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          v16f up = v16f{0};
+#pragma unroll
+          for (int kk = 0; kk < 2 * TT; ++kk) {
+            v4u v = lv[st][(2 * kk + hh) * D + 32 * n + r32], pos, neg;
+            split_odd<FMT>(v, pos, neg);
+            acc[n] = mfma32<FMT>(v, pf[kk], acc[n]);
+            up = mfma32<FMT>(pos, sees[kk], up);
+          }
+#pragma unroll
+          for (int k = 0; k < 16; ++k) acc[n][k] += odd_sum(up[k], 0.0f);
+          up = v16f{0};
+#pragma unroll
+          for (int kk = 0; kk < 2 * TT; ++kk) {
+            v4u v = lv[st][(2 * kk + hh) * D + 32 * n + r32], pos, neg;
+            split_odd<FMT>(v, pos, neg);
+            up = mfma32<FMT>(neg, sees[kk], up);
+          }
+#pragma unroll
+          for (int k = 0; k < 16; ++k) acc[n][k] += odd_sum(0.0f, up[k]);
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < 2 * TT; ++kk)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            acc[n] = mfma32<FMT>(lv[st][(2 * kk + hh) * D + 32 * n + r32], pf[kk], acc[n]);
+      }
+    }
+    if (tb + NK < end) store(st ^ 1, tb + NK);
+    __syncthreads();
+  }
+
+  l += __shfl_xor(l, 32);
+  const float ref = m + e;
+  if (a.splits > 1) {
+    if (!real) return;
+    const size_t at = (((size_t)u * c.kv_heads + h) * a.splits + split) * kKvPromptRows + 32 * wave + r32;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<v4f*>(a.part + at * D + 32 * n + 8 * k + 4 * hh) =
+            v4f{acc[n][4 * k], acc[n][4 * k + 1], acc[n][4 * k + 2], acc[n][4 * k + 3]};
+    if (hh == 0) {
+      a.part_ml[at * 2] = ref;
+      a.part_ml[at * 2 + 1] = l;
+    }
+    return;
+  }
+  float inv = l != 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
+  if constexpr (FMT == kKvTq4) {
+    // The rotation back, over the dimensions as a lane holds them: 32 n + 8
+    // (k / 4) + 4 half + k % 4.
+    auto both = [&](int n0, int k0, int n1, int k1) {
+      const float p = acc[n0][k0], o = acc[n1][k1];
+      acc[n0][k0] = p + o;
+      acc[n1][k1] = p - o;
+    };
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int b = 1; b < 16; b *= 2)
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if ((k & b) == 0) both(n, k, n, k + b);
+#pragma unroll
+    for (int b = 1; b < NT; b *= 2)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if ((n & b) == 0)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) both(n, k, n + b, k);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float o = __shfl_xor(acc[n][k], 32);
+        acc[n][k] = (hh != 0 ? o - acc[n][k] : acc[n][k] + o) *
+                    c.t.signs[32 * n + 8 * (k / 4) + 4 * hh + k % 4];
+      }
+    inv *= (float)(1.0 / __builtin_sqrt((double)D));
+  }
+  if (!real) return;
+  const long long row = t.s.row0 + qrow;
+  const int head = h * a.group + rr % a.group;
+  uint8_t* dst = a.out + ((size_t)row * a.out_stride + (size_t)head * D) * 2;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = acc[n][4 * k + i] * inv;
+      v2u w;
+      if (a.dtype == kKvRowF16)
+        w = v2u{f32_to_f16(o[0]) | f32_to_f16(o[1]) << 16, f32_to_f16(o[2]) | f32_to_f16(o[3]) << 16};
+      else
+        w = v2u{f32_to_bf16(o[0]) | f32_to_bf16(o[1]) << 16, f32_to_bf16(o[2]) | f32_to_bf16(o[3]) << 16};
+      *reinterpret_cast<v2u*>(dst + (32 * n + 8 * k + 4 * hh) * 2) = w;
+    }
+  if (a.lse != nullptr && hh == 0)
+    a.lse[(size_t)row * a.heads + head] =
+        l != 0.0f ? (ref + __log2f(l)) * 0.69314718056f : -__builtin_inff();
+}
+
 // Joins a row's splits: one workgroup a row and head, D / 8 lanes a split.
 template <int FMT, int D>
 EOS_DEV void attn_join(const KvAttnArgs& a) {
@@ -785,15 +1267,14 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
     return;
   }
   if (within < 0 || within >= t.s.n) return;
-  const int r = (int)within * a.group + head % a.group;
-  kv_tile(t, r / kKvTileRows, kKvTileRows, a.group, a.window, a.splits);
-  u = c.offsets == nullptr
-          ? (long long)t.s.b * ((a.group + kKvTileRows - 1) / kKvTileRows)
-          : kv_unit_base(c, t.s.b, a.group, kKvTileRows, 1);
-  u += r / kKvTileRows;
-  const size_t at = ((size_t)u * c.kv_heads + h) * a.splits * 16 + r % 16;
+  const int r = (int)within * a.group + head % a.group, rows = a.tile_rows;
+  kv_tile(t, r / rows, rows, a.group, a.window, a.splits);
+  u = (c.offsets == nullptr ? (long long)t.s.b * ((a.group + rows - 1) / rows)
+                            : kv_unit_base(c, t.s.b, a.group, rows, 1)) +
+      r / rows;
+  const size_t at = ((size_t)u * c.kv_heads + h) * a.splits * rows + r % rows;
   float top = kLowest;
-  for (int i = tid; i < t.splits; i += 256) top = fmaxf(top, a.part_ml[(at + (size_t)i * 16) * 2]);
+  for (int i = tid; i < t.splits; i += 256) top = fmaxf(top, a.part_ml[(at + (size_t)i * rows) * 2]);
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
   if ((tid & 63) == 0) smax[tid >> 6] = top;
@@ -801,7 +1282,7 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
   top = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
   float x[8] = {}, l = 0.0f;
   for (int i = grp; i < t.splits; i += NG) {
-    const size_t p = at + (size_t)i * 16;
+    const size_t p = at + (size_t)i * rows;
     const float f = __builtin_amdgcn_exp2f(a.part_ml[p * 2] - top);
     l += a.part_ml[p * 2 + 1] * f;
     const v4f p0 = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[0];
@@ -839,6 +1320,9 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(256) void eos_kv_split_##NAME##_##D(KvAttnArgs a) {    \
     attn_split<FMT, D>(a);                                                                   \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void eos_kv_prompt_##NAME##_##D(KvAttnArgs a) {   \
+    attn_prompt<FMT, D>(a);                                                                  \
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(256) void eos_kv_join_##NAME##_##D(KvAttnArgs a) {     \
     attn_join<FMT, D>(a);                                                                    \
