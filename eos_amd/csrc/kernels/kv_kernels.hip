@@ -848,7 +848,7 @@ template <int FMT, int D>
 EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
   constexpr int BITS = bits_of(FMT), KS = D / 16, NT = D / 32;
-  constexpr int NK = D == 256 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
+  constexpr int NK = D >= 128 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
   // 16-byte pieces of 16 tokens and of a stage (of K, and as many of V), a
   // thread's loads, and the operand pieces of one.
   constexpr int C16 = D * BITS / 8, CH = BLK * C16, PER = (CH + 255) / 256, EX = 16 / BITS;
@@ -897,20 +897,27 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   float scr = 0.0f;
   int okbits = 0, next_ok = 0;
   bool next_edge = false;
+  // Page ids of a stage's blocks of 16 tokens, one a lane, loaded a stage
+  // before their rows are.
+  int ids = 0;
+  auto pages = [&](int tb) {
+    const int t16 = tb + 16 * (lane & (BLK - 1));
+    ids = t16 < hi && t16 + 16 > lo
+              ? c.table[(size_t)seq * c.table_stride + (t16 >> c.page_shift)]
+              : -1;
+  };
   auto fetch = [&](int tb) {
     int pid[BLK];
     next_ok = 0;
 #pragma unroll
     for (int j = 0; j < BLK; ++j) {
-      const int t16 = tb + 16 * j;
-      pid[j] = -1;
-      if (t16 < hi && t16 + 16 > lo) {
-        pid[j] = kv_page(c, seq, t16);
-        if (pid[j] < 0) flag(c, kKvBadPage);
-      }
-      if (pid[j] >= 0) next_ok |= 1 << j;
-      pid[j] = kv_max(pid[j], 0);
+      const int p = __builtin_amdgcn_readlane(ids, j), t16 = tb + 16 * j;
+      const bool in = (unsigned)p < (unsigned)c.pages;
+      if (in) next_ok |= 1 << j;
+      else if (t16 < hi && t16 + 16 > lo) flag(c, kKvBadPage);
+      pid[j] = in ? p : 0;
     }
+    pages(tb + NK);
     next_edge = next_ok != (1 << BLK) - 1 || tb + NK > hi || tb < lo;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -929,11 +936,13 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
     }
     if constexpr (kQuant) {
       if (tid < 2 * NK) {
-        const int tok = tb + tid % NK;
-        const int p = tok < hi && tok >= lo ? kv_page(c, seq, tok) : -1;
+        const int tok = tb + tid % NK, blk = tid % NK / 16;
+        int p = pid[0];
+#pragma unroll
+        for (int j = 1; j < BLK; ++j) p = blk == j ? pid[j] : p;
         const float* sc = tid < NK ? c.k_scale : c.v_scale;
-        scr = p < 0 ? 0.0f
-                    : sc[(((size_t)p * c.kv_heads + h) << c.page_shift) + (tok & (P - 1))];
+        const bool there = tok < hi && tok >= lo && (next_ok >> blk & 1) != 0;
+        scr = there ? sc[(((size_t)p * c.kv_heads + h) << c.page_shift) + (tok & (P - 1))] : 0.0f;
       }
     }
   };
@@ -975,7 +984,10 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
 
   if (tid < 2) lodd[tid] = 0;
   __syncthreads();
-  if (begin < end) fetch(begin);
+  if (begin < end) {
+    pages(begin);
+    fetch(begin);
+  }
 
   // The query as the second operand (see attn_split).
   v4u q[KS];
