@@ -28,7 +28,9 @@ namespace {
 
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -404,9 +406,9 @@ EOS_DEV v4f mfma16(v4u a, v4u b, v4f c) {
 template <int FMT>
 EOS_DEV uint32_t pack2(float a, float b) {
   if constexpr (FMT == kKvBf16)
-    return f32_to_bf16(a) | f32_to_bf16(b) << 16;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2b));
   else
-    return f32_to_f16(a) | f32_to_f16(b) << 16;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2h));
 }
 
 // f16 / bf16 values with NaN and infinity apart: `x` keeps the finite ones, `pos`
@@ -848,7 +850,7 @@ template <int FMT, int D>
 EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
   constexpr int BITS = bits_of(FMT), KS = D / 16, NT = D / 32;
-  constexpr int NK = D >= 128 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
+  constexpr int NK = D == 256 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
   // 16-byte pieces of 16 tokens and of a stage (of K, and as many of V), a
   // thread's loads, and the operand pieces of one.
   constexpr int C16 = D * BITS / 8, CH = BLK * C16, PER = (CH + 255) / 256, EX = 16 / BITS;
@@ -856,9 +858,10 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   constexpr int RS = ROWC >= 16 ? 1 : 16 / ROWC;  // K rows that share 256 bytes
   __shared__ v4u lk[2][NK * ROWC], lv[2][NK * ROWC];
   __shared__ float lsc[2][2][kQuant ? NK : 1];
-  // The stage's first key + 1 where its V holds a NaN or infinity and it is
-  // one that some row masks.
-  __shared__ int lodd[2];
+  // Whether a stage that some row masks held a NaN or infinity in V: such
+  // values are staged as zero (weight 0 would not stop them) and added at the
+  // end to the rows that see them.
+  __shared__ int lodd;
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -887,7 +890,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   const bool busy = w0 < nrows;
   const int wp0 = kv_row_pos(t.s, w0 / a.group);
   const int wp1 = kv_row_pos(t.s, (kv_min(w0 + 32, nrows) - 1) / a.group);
-  const int w_hi = busy ? __builtin_amdgcn_readfirstlane(kv_min(t.s.keys, wp1 + 1)) : 0;
+  const int w_hi = __builtin_amdgcn_readfirstlane(busy ? kv_min(t.s.keys, wp1 + 1) : 0);
   const int w_lo = __builtin_amdgcn_readfirstlane(a.window > 0 ? wp0 - a.window + 1 : 0);
   const int w_all_hi = __builtin_amdgcn_readfirstlane(kv_min(t.s.keys, wp0 + 1));
   const int w_all_lo = __builtin_amdgcn_readfirstlane(a.window > 0 ? wp1 - a.window + 1 : 0);
@@ -973,7 +976,11 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
                        (ok && t2 + 1 >= lo && t2 + 1 < hi ? 0xffff0000u : 0u);
           }
         }
-        if ((tb + NK > all_hi || tb < all_lo) && has_odd<FMT>(x[0])) lodd[st] = tb + 1;
+        if ((tb + NK > all_hi || tb < all_lo) && has_odd<FMT>(x[0])) {
+          v4u pos, neg;
+          split_odd<FMT>(x[0], pos, neg);
+          lodd = 1;
+        }
       }
 #pragma unroll
       for (int e = 0; e < EX; ++e) lv[st][(blk * 2 + grp) * D + rest % (D / EX) * EX + e] = x[e];
@@ -982,7 +989,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
       if (tid < 2 * NK) lsc[st][tid / NK][tid % NK] = scr;
   };
 
-  if (tid < 2) lodd[tid] = 0;
+  if (tid == 0) lodd = 0;
   __syncthreads();
   if (begin < end) {
     pages(begin);
@@ -1140,54 +1147,41 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
         for (int i = 0; i < 4; ++i)
           pf[kk][i] = pack2<FMT>(p[slot_of<FMT>(2 * i)], p[slot_of<FMT>(2 * i + 1)]);
       }
-      if (!kQuant && masked && lodd[st] == tb + 1) {
-        // (see attn_split; one sum after the other to hold few registers)
-        constexpr uint32_t kOne = FMT == kKvF16 ? 0x3c00u : 0x3f80u;
-        v4u sees[2 * TT];
 #pragma unroll
-        for (int kk = 0; kk < 2 * TT; ++kk) {
-          uint32_t see[4] = {0, 0, 0, 0};
+      for (int kk = 0; kk < 2 * TT; ++kk)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = tb + 16 * kk + 8 * hh + i;
-            if (key >= lo_c && key < hi_c && (ok >> kk & 1) != 0) see[i / 2] |= kOne << (16 * (i & 1));
-          }
-          sees[kk] = v4u{see[0], see[1], see[2], see[3]};
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          v16f up = v16f{0};
-#pragma unroll
-          for (int kk = 0; kk < 2 * TT; ++kk) {
-            v4u v = lv[st][(2 * kk + hh) * D + 32 * n + r32], pos, neg;
-            split_odd<FMT>(v, pos, neg);
-            acc[n] = mfma32<FMT>(v, pf[kk], acc[n]);
-            up = mfma32<FMT>(pos, sees[kk], up);
-          }
-#pragma unroll
-          for (int k = 0; k < 16; ++k) acc[n][k] += odd_sum(up[k], 0.0f);
-          up = v16f{0};
-#pragma unroll
-          for (int kk = 0; kk < 2 * TT; ++kk) {
-            v4u v = lv[st][(2 * kk + hh) * D + 32 * n + r32], pos, neg;
-            split_odd<FMT>(v, pos, neg);
-            up = mfma32<FMT>(neg, sees[kk], up);
-          }
-#pragma unroll
-          for (int k = 0; k < 16; ++k) acc[n][k] += odd_sum(0.0f, up[k]);
-        }
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < 2 * TT; ++kk)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            acc[n] = mfma32<FMT>(lv[st][(2 * kk + hh) * D + 32 * n + r32], pf[kk], acc[n]);
-      }
+        for (int n = 0; n < NT; ++n)
+          acc[n] = mfma32<FMT>(lv[st][(2 * kk + hh) * D + 32 * n + r32], pf[kk], acc[n]);
     }
     if (tb + NK < end) store(st ^ 1, tb + NK);
     __syncthreads();
   }
 
+  if (!kQuant && lodd != 0) {
+    // The values of V that were left out, for the rows that see them.
+    constexpr uint32_t kOne = FMT == kKvF16 ? 0x3c00u : 0x3f80u;
+    for (int tb = begin; tb < end; tb += 16) {
+      const int stage = begin + (tb - begin) / NK * NK;
+      if (stage + NK <= all_hi && stage >= all_lo) continue;
+      const int page = kv_page(c, seq, tb), key = tb + 8 * hh;
+      uint32_t see[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (key + i >= lo_c && key + i < hi_c && page >= 0) see[i / 2] |= kOne << (16 * (i & 1));
+      const v4u sees = v4u{see[0], see[1], see[2], see[3]};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        v4u v = *reinterpret_cast<const v4u*>(
+            c.v + ((size_t)kv_max(page, 0) * c.kv_heads + h) * head_bytes +
+            ((size_t)((key & (P - 1)) / kKvGroup) * D + 32 * n + r32) * 16);
+        v4u pos, neg;
+        split_odd<FMT>(v, pos, neg);
+        const v16f up = mfma32<FMT>(pos, sees, v16f{0}), down = mfma32<FMT>(neg, sees, v16f{0});
+#pragma unroll
+        for (int k = 0; k < 16; ++k) acc[n][k] += odd_sum(up[k], down[k]);
+      }
+    }
+  }
   l += __shfl_xor(l, 32);
   const float ref = m + e;
   if (a.splits > 1) {
