@@ -23,6 +23,7 @@
 #include "kv_index.h"
 
 #define EOS_DEV __device__ __forceinline__
+#define KV_INLINE __attribute__((always_inline))
 
 namespace {
 
@@ -817,6 +818,24 @@ EOS_DEV v16f mfma32(v4u a, v4u b, v16f c) {
                                                   __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// 16 bytes a lane from base + off straight into LDS: lane i's at lds + 16 i. A
+// wait for the vector loads (lds_wait) and a barrier stand before their first
+// use. Written out because the compiler, which cannot tell the two stages of a
+// buffer apart, would wait for the builtin's before every read of the other.
+EOS_DEV void load_lds16(uint32_t lds, const void* base, uint32_t off) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(lds), "v"(off), "s"(base)
+      : "memory", "m0");
+}
+EOS_DEV void lds_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+EOS_DEV uint32_t lds_offset(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
 // One 16-byte load of codes as 16-bit operands: BITS / 16 of 8 each.
 template <int FMT>
 EOS_DEV void expand(const KvTables& t, v4u x, v4u (&out)[16 / bits_of(FMT)]) {
@@ -850,7 +869,7 @@ template <int FMT, int D>
 EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
   constexpr int BITS = bits_of(FMT), KS = D / 16, NT = D / 32;
-  constexpr int NK = D == 256 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
+  constexpr int NK = D >= 128 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
   // 16-byte pieces of 16 tokens and of a stage (of K, and as many of V), a
   // thread's loads, and the operand pieces of one.
   constexpr int C16 = D * BITS / 8, CH = BLK * C16, PER = (CH + 255) / 256, EX = 16 / BITS;
@@ -895,33 +914,31 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   const int w_all_hi = __builtin_amdgcn_readfirstlane(kv_min(t.s.keys, wp0 + 1));
   const int w_all_lo = __builtin_amdgcn_readfirstlane(a.window > 0 ? wp1 - a.window + 1 : 0);
 
-  // Staging: this thread's pieces of the next stage, on their way.
+  // Staging. K goes one stage ahead of V, so that a stage's scores can be
+  // computed beside the exponentials of the one before. This thread's pieces
+  // on their way, the page ids of the two stages ahead and, as bits, which of
+  // the stages' 16-token blocks have one.
   v4u kr[PER], vr[PER];
   float scr = 0.0f;
-  int okbits = 0, next_ok = 0;
-  bool next_edge = false;
-  // Page ids of a stage's blocks of 16 tokens, one a lane, loaded a stage
-  // before their rows are.
+  int pid1 = 0, pid2 = 0, ok0 = 0, ok1 = 0, ok2 = 0;
+  // Page ids of a stage's blocks, one a lane, loaded a stage before their rows.
   int ids = 0;
-  auto pages = [&](int tb) {
+  auto pages = [&](int tb) KV_INLINE {
     const int t16 = tb + 16 * (lane & (BLK - 1));
     ids = t16 < hi && t16 + 16 > lo
               ? c.table[(size_t)seq * c.table_stride + (t16 >> c.page_shift)]
               : -1;
   };
-  auto fetch = [&](int tb) {
-    int pid[BLK];
-    next_ok = 0;
-#pragma unroll
-    for (int j = 0; j < BLK; ++j) {
-      const int p = __builtin_amdgcn_readlane(ids, j), t16 = tb + 16 * j;
-      const bool in = (unsigned)p < (unsigned)c.pages;
-      if (in) next_ok |= 1 << j;
-      else if (t16 < hi && t16 + 16 > lo) flag(c, kKvBadPage);
-      pid[j] = in ? p : 0;
-    }
+  // Those ids made safe (lane j: block j's), and which of them were pages.
+  auto resolve = [&](int tb, int& pid) KV_INLINE {
+    const bool in = (unsigned)ids < (unsigned)c.pages;
+    const int t16 = tb + 16 * lane;
+    if (!in && tid < BLK && t16 < hi && t16 + 16 > lo) atomicOr(c.status, kKvBadPage);
+    pid = in ? ids : 0;
     pages(tb + NK);
-    next_edge = next_ok != (1 << BLK) - 1 || tb + NK > hi || tb < lo;
+    return (int)__ballot(in) & ((1 << BLK) - 1);
+  };
+  auto load = [&](const uint8_t* pool, int tb, int pid, v4u (&x)[PER]) KV_INLINE {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int id = tid + 256 * i;
@@ -929,28 +946,57 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
       // (a wavefront's pieces lie in one block of 16 tokens, or in several)
       const int blk = C16 >= 64 ? __builtin_amdgcn_readfirstlane(id / C16) : id / C16;
       const int rest = id - blk * C16;
-      int p = pid[0];
-#pragma unroll
-      for (int j = 1; j < BLK; ++j) p = blk == j ? pid[j] : p;
-      const size_t at = ((size_t)p * c.kv_heads + h) * head_bytes +
-                        (size_t)((tb + 16 * blk) & (P - 1)) * (D * BITS / 8) + rest * 16;
-      kr[i] = *reinterpret_cast<const v4u*>(c.k + at);
-      vr[i] = *reinterpret_cast<const v4u*>(c.v + at);
+      const int p = C16 >= 64 ? __builtin_amdgcn_readlane(pid, blk) : __shfl(pid, blk);
+      x[i] = *reinterpret_cast<const v4u*>(
+          pool + ((size_t)p * c.kv_heads + h) * head_bytes +
+          (size_t)((tb + 16 * blk) & (P - 1)) * (D * BITS / 8) + rest * 16);
     }
+  };
+  // 16-bit formats go to LDS without registers: the thread's piece of K is the
+  // one that its place in the swizzled stage holds.
+  auto direct = [&](const uint8_t* pool, const v4u* lds, int tb, int pid, bool is_k) KV_INLINE {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int id = tid + 256 * i;
+      const int blk = __builtin_amdgcn_readfirstlane(id / C16);
+      const int row = id / ROWC;
+      const uint32_t off = is_k ? (uint32_t)((row % 16) * ROWC + ((id % ROWC) ^ ((row / RS) & (ROWC - 1)))) * 16
+                                : (uint32_t)(id % C16) * 16;
+      const int p = __builtin_amdgcn_readlane(pid, blk);
+      load_lds16(lds_offset(lds) + (uint32_t)(wave * 64 + 256 * i) * 16,
+                 pool + ((size_t)p * c.kv_heads + h) * head_bytes +
+                     (size_t)((tb + 16 * blk) & (P - 1)) * (D * 2),
+                 off);
+    }
+  };
+  // Whether a stage's V may hold what must not be staged as it is.
+  auto odd_stage = [&](int tb, int ok) KV_INLINE {
+    return ok != (1 << BLK) - 1 || tb + NK > all_hi || tb < all_lo;
+  };
+  auto load_v = [&](int st, int tb, int pid, int ok) KV_INLINE {
+    if constexpr (!kQuant) {
+      if (!odd_stage(tb, ok)) direct(c.v, lv[st], tb, pid, false);
+      return;
+    }
+    load(c.v, tb, pid, vr);
     if constexpr (kQuant) {
       if (tid < 2 * NK) {
         const int tok = tb + tid % NK, blk = tid % NK / 16;
-        int p = pid[0];
-#pragma unroll
-        for (int j = 1; j < BLK; ++j) p = blk == j ? pid[j] : p;
+        const int p = __shfl(pid, blk);
         const float* sc = tid < NK ? c.k_scale : c.v_scale;
-        const bool there = tok < hi && tok >= lo && (next_ok >> blk & 1) != 0;
+        const bool there = tok < hi && tok >= lo && (ok >> blk & 1) != 0;
         scr = there ? sc[(((size_t)p * c.kv_heads + h) << c.page_shift) + (tok & (P - 1))] : 0.0f;
       }
     }
   };
-  auto store = [&](int st, int tb) {
-    okbits = next_ok;
+  auto load_k = [&](int st, int tb, int pid) KV_INLINE {
+    if constexpr (kQuant)
+      load(c.k, tb, pid, kr);
+    else
+      direct(c.k, lk[st], tb, pid, true);
+  };
+  auto store_k = [&](int st) KV_INLINE {
+    if constexpr (!kQuant) return;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int id = tid + 256 * i;
@@ -962,21 +1008,32 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
       const int sw = (row / RS) & (ROWC - 1);
 #pragma unroll
       for (int e = 0; e < EX; ++e) lk[st][row * ROWC + ((c0 + e) ^ sw)] = x[e];
+    }
+  };
+  auto store_v = [&](int st, int tb, int pid, int ok) KV_INLINE {
+    if constexpr (!kQuant) {
+      if (!odd_stage(tb, ok)) return;
+      load(c.v, tb, pid, vr);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int id = tid + 256 * i;
+      if (CH % 256 != 0 && id >= CH) break;
+      const int blk = id / C16, rest = id % C16;
+      v4u x[EX];
       expand<FMT>(c.t, vr[i], x);
       const int grp = rest / (D / EX);
       if constexpr (!kQuant) {
-        if (next_edge) {
-          // Nothing may be read of slots that hold no token: they can be NaN.
-          const int t0 = tb + 16 * blk + 8 * grp;
-          const bool ok = (next_ok >> blk & 1) != 0;
+        // Slots that hold no token may hold anything: zeros instead.
+        const int t0 = tb + 16 * blk + 8 * grp;
+        const bool there = (ok >> blk & 1) != 0;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int t2 = t0 + 2 * w;
-            x[0][w] &= (ok && t2 >= lo && t2 < hi ? 0xffffu : 0u) |
-                       (ok && t2 + 1 >= lo && t2 + 1 < hi ? 0xffff0000u : 0u);
-          }
+        for (int w = 0; w < 4; ++w) {
+          const int t2 = t0 + 2 * w;
+          x[0][w] &= (there && t2 >= lo && t2 < hi ? 0xffffu : 0u) |
+                     (there && t2 + 1 >= lo && t2 + 1 < hi ? 0xffff0000u : 0u);
         }
-        if ((tb + NK > all_hi || tb < all_lo) && has_odd<FMT>(x[0])) {
+        if (has_odd<FMT>(x[0])) {
           v4u pos, neg;
           split_odd<FMT>(x[0], pos, neg);
           lodd = 1;
@@ -993,7 +1050,9 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   __syncthreads();
   if (begin < end) {
     pages(begin);
-    fetch(begin);
+    ok0 = resolve(begin, pid2);
+    load_k(0, begin, pid2);
+    load_v(0, begin, pid2, ok0);
   }
 
   // The query as the second operand (see attn_split).
@@ -1063,24 +1122,27 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   float lim = (m + 8.0f) * iqs;
   // K row of lane r32: token bits 2 and 3 exchanged.
   const int krow = (r32 & 19) | (r32 >> 1 & 4) | (r32 << 1 & 8);
-  if (begin < end) store(0, begin);
-  __syncthreads();
-  int st = 0;
-  for (int tb = begin; tb < end; tb += NK, st ^= 1) {
-    const int ok = okbits;
-    if (tb + NK < end) fetch(tb + NK);
+  auto scores = [&](int st, v16f (&s)[TT]) KV_INLINE {
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      s[tt] = v16f{0};
+      const int row = tt * 32 + krow;
+      const int sw = (row / RS) & (ROWC - 1);
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        s[tt] = mfma32<FMT>(lk[st][row * ROWC + ((2 * k + hh) ^ sw)], q[k], s[tt]);
+    }
+  };
+  // One stage: `s` are its scores, `next` becomes those of the following one.
+  auto step = [&](int st, int tb, v16f (&s)[TT], v16f (&next)[TT]) KV_INLINE {
+    const bool has1 = tb + NK < end, has2 = tb + 2 * NK < end;
+    if (has1) load_v(st ^ 1, tb + NK, pid1, ok1);
+    if (has2) {
+      ok2 = resolve(tb + 2 * NK, pid2);
+      load_k(st, tb + 2 * NK, pid2);
+    }
     if (tb < w_hi && tb + NK > w_lo) {
-      const bool masked = tb + NK > w_all_hi || tb < w_all_lo || ok != (1 << BLK) - 1;
-      v16f s[TT];
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt) {
-        s[tt] = v16f{0};
-        const int row = tt * 32 + krow;
-        const int sw = (row / RS) & (ROWC - 1);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-          s[tt] = mfma32<FMT>(lk[st][row * ROWC + ((2 * k + hh) ^ sw)], q[k], s[tt]);
-      }
+      const bool masked = tb + NK > w_all_hi || tb < w_all_lo || ok0 != (1 << BLK) - 1;
       float mv = 0.0f;
       if constexpr (kQuant) {
 #pragma unroll
@@ -1097,8 +1159,8 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int tok = 32 * tt + 16 * (i / 8) + 8 * hh + i % 8, key = tb + tok;
-            if (!(key >= lo_c && key < hi_c && (ok >> (2 * tt + i / 8) & 1) != 0))
+            const int key = tb + 32 * tt + 16 * (i / 8) + 8 * hh + i % 8;
+            if (!(key >= lo_c && key < hi_c && (ok0 >> (2 * tt + i / 8) & 1) != 0))
               s[tt][i] = -__builtin_inff();
           }
       }
@@ -1129,6 +1191,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
         }
       }
       const float ref = -(m + e);
+      scores(st ^ 1, next);
       v4u pf[2 * TT];
 #pragma unroll
       for (int kk = 0; kk < 2 * TT; ++kk) {
@@ -1138,10 +1201,9 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
           const float x = s[kk / 2][8 * (kk % 2) + i];
           p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, qs, ref));
           l += p[i];
-          if constexpr (kQuant) {
-            const float pv = p[i] * lsc[st][1][16 * kk + 8 * hh + i];
-            p[i] = masked && x == -__builtin_inff() ? 0.0f : pv;
-          }
+          // (a masked key's scale may be NaN: it must not reach the row)
+          if constexpr (kQuant)
+            p[i] = x == -__builtin_inff() ? 0.0f : p[i] * lsc[st][1][16 * kk + 8 * hh + i];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -1152,9 +1214,37 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
           acc[n] = mfma32<FMT>(lv[st][(2 * kk + hh) * D + 32 * n + r32], pf[kk], acc[n]);
+    } else {
+      scores(st ^ 1, next);
     }
-    if (tb + NK < end) store(st ^ 1, tb + NK);
+    if (has1) store_v(st ^ 1, tb + NK, pid1, ok1);
+    if (has2) store_k(st);
+    if constexpr (!kQuant) lds_wait();
     __syncthreads();
+    ok0 = ok1;
+    ok1 = ok2;
+    pid1 = pid2;
+  };
+  if (begin < end) {
+    store_k(0);
+    store_v(0, begin, pid2, ok0);
+    if (begin + NK < end) {
+      ok1 = resolve(begin + NK, pid1);
+      load_k(1, begin + NK, pid1);
+      store_k(1);
+    }
+    if constexpr (!kQuant) lds_wait();
+  }
+  __syncthreads();
+  if (begin < end) {
+    v16f sa[TT], sb[TT];
+    scores(0, sa);
+    for (int tb = begin;;) {
+      step(0, tb, sa, sb);
+      if ((tb += NK) >= end) break;
+      step(1, tb, sb, sa);
+      if ((tb += NK) >= end) break;
+    }
   }
 
   if (!kQuant && lodd != 0) {
