@@ -373,7 +373,9 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
     a.part = static_cast<float*>(ws);
     a.part_ml = a.part + parts * (size_t)d;
   }
-  if (launch(rt, kv, prompt ? "prompt" : "split", a.tiles * a.splits, kvh, 256, &a, what, err) != 0)
+  const long long items = a.tiles * a.splits;
+  if (prompt ? launch(rt, kv, "prompt", kv_place_blocks(kvh, items), 1, 256, &a, what, err) != 0
+             : launch(rt, kv, "split", items, kvh, 256, &a, what, err) != 0)
     return 1;
   if (a.splits == 1) return 0;
   return launch(rt, kv, "join", batch->rows, heads, 256, &a, what, err);

@@ -85,6 +85,30 @@ KV_HD bool kv_group8(const KvSeq& s, long long within, KvGroup8& g) {
   return true;
 }
 
+// Where workgroup `block` works when consecutive ones go to the 8 XCDs in
+// turn and each of `heads` heads has `items` pieces: heads are dealt to as
+// many groups of XCDs as divide both, a group's XCDs take its heads' items in
+// turn. The item may lie past the last one.
+struct KvPlace {
+  int head = 0;
+  long long item = 0;
+};
+KV_HD int kv_xcd_groups(int heads) { return heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1; }
+KV_HD KvPlace kv_place(unsigned block, int heads, long long items) {
+  const int groups = kv_xcd_groups(heads), share = 8 / groups;
+  const unsigned xcd = block % 8, turn = block / 8;
+  const unsigned per = (unsigned)((items + share - 1) / share);  // of a head, an XCD
+  KvPlace p;
+  p.head = (int)(xcd % groups + groups * (turn / per));
+  p.item = (long long)(turn % per) * share + xcd / groups;
+  return p;
+}
+// Workgroups of such a launch.
+KV_HD long long kv_place_blocks(int heads, long long items) {
+  const int share = 8 / kv_xcd_groups(heads);
+  return heads * ((items + share - 1) / share * share);
+}
+
 // 16 query rows of a sequence and a head group (row r: row r / group of the
 // sequence, head r % group), and the keys they attend.
 struct KvTile {

@@ -884,9 +884,14 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.x % a.splits, h = blockIdx.y;
-  // The last tiles of a sequence attend the most keys: they go first.
-  const long long u = a.tiles - 1 - blockIdx.x / a.splits;
+  // Workgroups go to the 8 XCDs in turn. An XCD takes whole heads, or shares
+  // them with as few others as it can, so that the keys and values of few
+  // heads pass through its L2; the last tiles of a sequence, which attend the
+  // most keys, go first.
+  const KvPlace at0 = kv_place(blockIdx.x, c.kv_heads, a.tiles * a.splits);
+  if (at0.item >= a.tiles * a.splits) return;
+  const int split = (int)(at0.item % a.splits), h = at0.head;
+  const long long u = a.tiles - 1 - at0.item / a.splits;
   KvTile t;
   if (!find_tile<kKvPromptRows>(a, u, t)) return;
   if (split >= t.splits && (split > 0 || a.splits > 1)) return;

@@ -65,6 +65,19 @@ void one(int at, bool sound) {
   c.lengths = lengths.data();
   c.offsets = one_each ? nullptr : offsets.data();
 
+  // workgroups dealt to the XCDs: every item of every head once
+  {
+    const int heads = between(1, 20);
+    const long long items = between(1, 40), blocks = kv_place_blocks(heads, items);
+    std::vector<int> got(heads * items, 0);
+    for (long long i = 0; i < blocks; ++i) {
+      const KvPlace p = kv_place((unsigned)i, heads, items);
+      CHECK(p.head >= 0 && p.head < heads && p.item >= 0);
+      if (p.item < items) ++got[p.head * items + p.item];
+    }
+    for (int n : got) CHECK(n == 1);
+  }
+
   // append / read
   std::vector<int> seen(c.rows, 0);
   const long long groups = one_each ? c.batch : kv_units(c.rows, c.batch, 1, kKvGroup, 2);
