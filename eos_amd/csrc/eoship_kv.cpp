@@ -29,7 +29,10 @@ struct EosHipKVCache {
 
 namespace {
 
-constexpr int kPromptFrom = 48;
+#ifndef X_FROM
+#define X_FROM 48
+#endif
+constexpr int kPromptFrom = X_FROM;
 
 const char* const kFormats[] = {"f16", "bf16", "q8", "tq4"};
 
@@ -364,7 +367,8 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
   long long keys = (long long)batch->table_stride << kv->page_shift;
   if (window > 0) keys = std::min(keys, (long long)window + batch->rows + 32);
   const long long units = a.tiles * kvh;
-  const long long want = ((prompt ? 2LL : 4LL) * rt->compute_units + units - 1) / units;
+  const long long want = prompt ? 2LL * rt->compute_units / units
+                                : (4LL * rt->compute_units + units - 1) / units;
   a.splits = (int)std::max(1LL, std::min(want, (keys + 255) / 256));
   if (a.splits > 1) {
     const size_t parts = (size_t)units * a.splits * a.tile_rows;

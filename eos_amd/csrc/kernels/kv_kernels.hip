@@ -869,7 +869,7 @@ template <int FMT, int D>
 EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
   constexpr int BITS = bits_of(FMT), KS = D / 16, NT = D / 32;
-  constexpr int NK = D >= 128 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
+  constexpr int NK = D == 256 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
   // 16-byte pieces of 16 tokens and of a stage (of K, and as many of V), a
   // thread's loads, and the operand pieces of one.
   constexpr int C16 = D * BITS / 8, CH = BLK * C16, PER = (CH + 255) / 256, EX = 16 / BITS;
@@ -1422,8 +1422,9 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
   extern "C" __global__ __launch_bounds__(256) void eos_kv_split_##NAME##_##D(KvAttnArgs a) {    \
     attn_split<FMT, D>(a);                                                                   \
   }                                                                                          \
-  extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void eos_kv_prompt_##NAME##_##D(KvAttnArgs a) {   \
-    attn_prompt<FMT, D>(a);                                                                  \
+  extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void eos_kv_prompt_##NAME##_##D(  \
+      KvAttnArgs a) {                                                                        \
+    attn_prompt<FMT, D>(a);                                                               \
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(256) void eos_kv_join_##NAME##_##D(KvAttnArgs a) {     \
     attn_join<FMT, D>(a);                                                                    \
