@@ -511,6 +511,19 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
   const long long u = blockIdx.x / a.splits;
   KvTile t;
   if (!find_tile<kKvTileRows>(a, u, t)) return;
+  // The same in every lane, as the compiler cannot see.
+  t.s.b = __builtin_amdgcn_readfirstlane(t.s.b);
+  t.s.n = __builtin_amdgcn_readfirstlane(t.s.n);
+  t.s.len = __builtin_amdgcn_readfirstlane(t.s.len);
+  t.s.keys = __builtin_amdgcn_readfirstlane(t.s.keys);
+  t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
+  t.lo = __builtin_amdgcn_readfirstlane(t.lo);
+  t.hi = __builtin_amdgcn_readfirstlane(t.hi);
+  t.all_lo = __builtin_amdgcn_readfirstlane(t.all_lo);
+  t.all_hi = __builtin_amdgcn_readfirstlane(t.all_hi);
+  t.base = __builtin_amdgcn_readfirstlane(t.base);
+  t.chunk = __builtin_amdgcn_readfirstlane(t.chunk);
+  t.splits = __builtin_amdgcn_readfirstlane(t.splits);
   if (split >= t.splits && (split > 0 || a.splits > 1)) return;
   const int P = 1 << c.page_shift;
   const int rr = t.r0 + r16;
@@ -586,26 +599,31 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
   float m = kLowest, l = 0.0f, e = kQuant ? -100.0f : 0.0f, elim = 0x1p-100f;
   const int end = kv_min(t.hi, t.base + (split + 1) * t.chunk);
   const size_t head_bytes = ((size_t)D * BITS / 8) << c.page_shift;
-  for (int tb = t.base + split * t.chunk + 32 * wave; tb < end; tb += 128) {
-    // The pages of this lane's keys of K and of V.
-    auto page = [&](int token16, bool& ok) {
-      int p = -1;
-      ok = token16 < t.hi && token16 + 16 > t.lo;
-      if (ok) {
-        p = kv_page(c, t.s.b, token16);
-        if (p < 0) {
-          atomicOr(c.status, kKvBadPage);
-          ok = false;
-        }
-      }
-      return ok ? p : 0;
-    };
-    bool kok, vok;
-    const int kp = page(tb + 16 * (r16 >> 3), kok), vp = page(tb + 16 * (g >> 1), vok);
+  bool odd_seen = false;  // a value of V that is NaN or infinite in a masked step
+  // A step's codes and scales as loaded: the next step's are on their way
+  // while one is computed, and the page ids of the step after it.
+  struct Raw {
+    uint32_t k[2][KWORDS] = {}, v[VL][VWORDS] = {};
+    float ks[kQuant ? 8 : 1] = {}, vs[kQuant ? 8 : 1] = {};
+    bool vok = false;
+  };
+  // The page ids of this lane's keys of K and of V (-1: none there).
+  int kid = -1, vid = -1;
+  auto ids = [&](int tb) KV_INLINE {
+    const int kt = tb + 16 * (r16 >> 3), vt = tb + 16 * (g >> 1);
+    const int32_t* row = c.table + (size_t)t.s.b * c.table_stride;
+    kid = kt < t.hi && kt + 16 > t.lo ? row[kt >> c.page_shift] : -1;
+    vid = vt < t.hi && vt + 16 > t.lo ? row[vt >> c.page_shift] : -1;
+  };
+  auto fetch = [&](int tb, Raw& x) KV_INLINE {
+    const int vt = tb + 16 * (g >> 1);
+    const int kp = (unsigned)kid < (unsigned)c.pages ? kid : 0;
+    x.vok = (unsigned)vid < (unsigned)c.pages;
+    const int vp = x.vok ? vid : 0;
+    if (!x.vok && vt < t.hi && vt + 16 > t.lo) atomicOr(c.status, kKvBadPage);
     const uint8_t* kb = c.k + ((size_t)kp * c.kv_heads + h) * head_bytes;
     const uint8_t* vb = c.v + ((size_t)vp * c.kv_heads + h) * head_bytes;
     const int vslot = (tb + 8 * g) & (P - 1);
-    uint32_t kr[2][KWORDS], vr[VL][VWORDS];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int slot = (tb + 8 * (r16 >> 2) + 4 * j + (r16 & 3)) & (P - 1);
@@ -613,26 +631,32 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
       if constexpr (!kQuant) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const v4u x = *reinterpret_cast<const v4u*>(row + (s * 32 + g * 8) * 2);
+          const v4u w = *reinterpret_cast<const v4u*>(row + (s * 32 + g * 8) * 2);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) kr[j][4 * s + i] = x[i];
+          for (int i = 0; i < 4; ++i) x.k[j][4 * s + i] = w[i];
         }
       } else {
-        __builtin_memcpy(kr[j], __builtin_assume_aligned(row + g * (KWORDS * 4), KWORDS >= 4 ? 16 : KWORDS * 4),
+        __builtin_memcpy(x.k[j], __builtin_assume_aligned(row + g * (KWORDS * 4), KWORDS >= 4 ? 16 : KWORDS * 4),
                          KWORDS * 4);
       }
     }
     const uint8_t* vrow = vb + (size_t)(vslot / kKvGroup) * (D * BITS);
 #pragma unroll
     for (int i = 0; i < VL; ++i)
-      __builtin_memcpy(vr[i], __builtin_assume_aligned(vrow + (i * 16 + r16) * (VWORDS * 4), VWORDS * 4),
+      __builtin_memcpy(x.v[i], __builtin_assume_aligned(vrow + (i * 16 + r16) * (VWORDS * 4), VWORDS * 4),
                        VWORDS * 4);
-    float ks[8], vs[8];
     if constexpr (kQuant) {
       const size_t at = (((size_t)vp * c.kv_heads + h) << c.page_shift) + vslot;
-      __builtin_memcpy(ks, __builtin_assume_aligned(c.k_scale + at, 16), 32);
-      __builtin_memcpy(vs, __builtin_assume_aligned(c.v_scale + at, 16), 32);
+      __builtin_memcpy(x.ks, __builtin_assume_aligned(c.k_scale + at, 16), 32);
+      __builtin_memcpy(x.vs, __builtin_assume_aligned(c.v_scale + at, 16), 32);
     }
+  };
+  auto step = [&](int tb, Raw& raw) KV_INLINE {
+    auto& kr = raw.k;
+    auto& vr = raw.v;
+    auto& ks = raw.ks;
+    auto& vs = raw.vs;
+    const bool vok = raw.vok;
     const bool masked = tb + 32 > t.all_hi || tb < t.all_lo || __any(!vok);
 
     v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
@@ -710,35 +734,22 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) pf[i] = pack2<FMT>(p[slot_of<FMT>(2 * i)], p[slot_of<FMT>(2 * i + 1)]);
     if constexpr (!kQuant) {
-      bool odd = false;
       if (masked) {
+        // Weight 0 does not stop a NaN or infinity: slots that hold no token
+        // count as zero, and so do odd values until the loop is over.
+        bool odd = false;
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
+          v4u v = v4u{vr[i][0] & vmask[0], vr[i][1] & vmask[1], vr[i][2] & vmask[2], vr[i][3] & vmask[3]};
+          if (__any(has_odd<FMT>(v))) {
+            v4u pos, neg;
+            split_odd<FMT>(v, pos, neg);
+            odd = true;
+          }
 #pragma unroll
-          for (int w = 0; w < 4; ++w) vr[i][w] &= vmask[w];
-          odd |= has_odd<FMT>(v4u{vr[i][0], vr[i][1], vr[i][2], vr[i][3]});
+          for (int w = 0; w < 4; ++w) vr[i][w] = v[w];
         }
-      }
-      if (__any(odd)) {
-        // A NaN or infinity beside rows that must not see it: weight 0 does
-        // not stop it. Finite values as ever, the odd ones counted for the
-        // rows that see them.
-        constexpr uint32_t kOne = FMT == kKvF16 ? 0x3c00u : 0x3f80u;
-        uint32_t see[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) see[i / 2] |= (x[i] == -__builtin_inff() ? 0u : kOne) << (16 * (i & 1));
-        const v4u sees = v4u{see[0], see[1], see[2], see[3]};
-#pragma unroll
-        for (int i = 0; i < VL; ++i) {
-          v4u v = v4u{vr[i][0], vr[i][1], vr[i][2], vr[i][3]}, pos, neg;
-          split_odd<FMT>(v, pos, neg);
-          acc[i] = mfma16<FMT>(v, pf, acc[i]);
-          const v4f up = mfma16<FMT>(pos, sees, v4f{0, 0, 0, 0});
-          const v4f down = mfma16<FMT>(neg, sees, v4f{0, 0, 0, 0});
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[i][k] += odd_sum(up[k], down[k]);
-        }
-        continue;
+        odd_seen |= odd;
       }
     }
 #pragma unroll
@@ -759,6 +770,58 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
         }
         acc[i * VW + w] = mfma16<FMT>(v4u{f[0], f[1], f[2], f[3]}, pf, acc[i * VW + w]);
       }
+  };
+  // (from 1024 bits of width on there are no registers for a second step)
+  constexpr bool kAhead = D * BITS <= 1024;
+  const int first = t.base + split * t.chunk + 32 * wave;
+  Raw ra, rb;
+  if (first < end) {
+    ids(first);
+    fetch(first, ra);
+    ids(first + 128);
+  }
+  for (int tb = first; tb < end;) {
+    if constexpr (kAhead) {
+      if (tb + 128 < end) fetch(tb + 128, rb);
+      ids(tb + 256);
+      step(tb, ra);
+      if ((tb += 128) >= end) break;
+      if (tb + 128 < end) fetch(tb + 128, ra);
+      ids(tb + 256);
+      step(tb, rb);
+      tb += 128;
+    } else {
+      step(tb, ra);
+      if ((tb += 128) >= end) break;
+      fetch(tb, ra);
+      ids(tb + 128);
+    }
+  }
+
+  if (!kQuant && odd_seen) {
+    // The values left out, for the rows that see them.
+    constexpr uint32_t kOne = FMT == kKvF16 ? 0x3c00u : 0x3f80u;
+    for (int tb = first; tb < end; tb += 128) {
+      const int key = tb + 8 * g, vp = kv_page(c, t.s.b, tb + 16 * (g >> 1));
+      if (!(tb + 32 > t.all_hi || tb < t.all_lo || __any(vp < 0))) continue;
+      uint32_t see[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (vp >= 0 && key + i >= t.lo && key + i < t.hi && key + i >= lo_c && key + i < hi_c)
+          see[i / 2] |= kOne << (16 * (i & 1));
+      const v4u sees = v4u{see[0], see[1], see[2], see[3]};
+      const uint8_t* vb = c.v + ((size_t)kv_max(vp, 0) * c.kv_heads + h) * head_bytes +
+                          (size_t)((key & (P - 1)) / kKvGroup) * (D * BITS);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        v4u v = *reinterpret_cast<const v4u*>(vb + (n * 16 + r16) * 16), pos, neg;
+        split_odd<FMT>(v, pos, neg);
+        const v4f up = mfma16<FMT>(pos, sees, v4f{0, 0, 0, 0});
+        const v4f down = mfma16<FMT>(neg, sees, v4f{0, 0, 0, 0});
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[n][k] += odd_sum(up[k], down[k]);
+      }
+    }
   }
 
   // The four wavefronts' parts, brought to one reference.
@@ -1419,7 +1482,7 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
   extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_read_##NAME##_##D(KvRowsArgs a) {   \
     read_group<FMT, D>(a);                                                                   \
   }                                                                                          \
-  extern "C" __global__ __launch_bounds__(256) void eos_kv_split_##NAME##_##D(KvAttnArgs a) {    \
+  extern "C" __global__ __launch_bounds__(256, D * bits_of(FMT) > 2048 ? 1 : 2) void eos_kv_split_##NAME##_##D(KvAttnArgs a) {    \
     attn_split<FMT, D>(a);                                                                   \
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void eos_kv_prompt_##NAME##_##D(  \
