@@ -169,9 +169,12 @@ int rows_call(EosHipRuntime* rt, const EosHipKVCache* kv, const EosHipKVBatch* b
   a.k_stride = k_stride;
   a.v_stride = v_stride;
   a.dtype = dtype;
-  const long long units =
-      b->d_offsets == nullptr ? b->batch : kv_units(b->rows, b->batch, 1, kKvGroup, 2);
-  return launch(rt, kv, op, units, kv->d.kv_heads, 2 * kv->d.head_dim, &a, what, err);
+  if (b->d_offsets == nullptr) {
+    const std::string one = std::string(op) + "1";
+    return launch(rt, kv, one.c_str(), b->batch, kv->d.kv_heads, 2 * kv->d.head_dim, &a, what, err);
+  }
+  return launch(rt, kv, op, kv_units(b->rows, b->batch, 1, kKvRun, 2), kv->d.kv_heads,
+                2 * kv->d.head_dim, &a, what, err);
 }
 
 }  // namespace
@@ -362,13 +365,14 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
   a.tiles = batch->d_offsets == nullptr
                 ? (long long)batch->batch * ((a.group + kKvTileRows - 1) / kKvTileRows)
                 : kv_units(batch->rows, batch->batch, a.group, a.tile_rows, 1);
-  // Enough splits to give every CU four workgroups (two of the prompt kernel,
-  // whose registers hold no more), none below 256 keys.
+  // Splits while all workgroups are on the CUs at once (two each, by their
+  // registers), none below 256 keys: further ones cost more in prologues and
+  // joining than their balance gains (64 x 2,000 tokens of tq4: 39 us at two
+  // workgroups a CU, 53 at four, 68 at eight).
   long long keys = (long long)batch->table_stride << kv->page_shift;
   if (window > 0) keys = std::min(keys, (long long)window + batch->rows + 32);
   const long long units = a.tiles * kvh;
-  const long long want = prompt ? 2LL * rt->compute_units / units
-                                : (4LL * rt->compute_units + units - 1) / units;
+  const long long want = 2LL * rt->compute_units / units;
   a.splits = (int)std::max(1LL, std::min(want, (keys + 255) / 256));
   if (a.splits > 1) {
     const size_t parts = (size_t)units * a.splits * a.tile_rows;

@@ -13,7 +13,8 @@ enum { kKvRowF16 = 0, kKvRowBf16 = 1, kKvRowF32 = 2 };
 // range (nothing outside the pool and the rows is touched).
 enum { kKvBadPage = 1, kKvBadLength = 2, kKvBadOffset = 4 };
 
-constexpr int kKvGroup = 8;     // tokens of V stored side by side
+constexpr int kKvGroup = 8;       // tokens of V stored side by side
+constexpr int kKvRun = 32;         // positions of a workgroup of append and read
 constexpr int kKvTileRows = 16;    // query rows of a workgroup of the split kernel
 constexpr int kKvPromptRows = 128;  // query rows of a workgroup of the prompt kernel
 

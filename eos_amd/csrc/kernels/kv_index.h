@@ -67,20 +67,21 @@ KV_HD int kv_page(const KvCacheArgs& c, int b, int token) {
   return p >= 0 && p < c.pages ? p : -1;
 }
 
-// Unit `within` of a sequence in append and read: 8 positions from pos0 on,
-// of which [from, upto) are rows of the call. False where it has none.
-struct KvGroup8 {
+// Unit `within` of a sequence in append and read: `run` positions (whole
+// groups) from pos0 on, of which [from, upto) are rows of the call. False
+// where it has none.
+struct KvRun {
   int pos0 = 0, from = 0, upto = 0;
   long long row = 0;  // the call's row of position pos0 (before `from`: not one)
 };
 
-KV_HD bool kv_group8(const KvSeq& s, long long within, KvGroup8& g) {
+KV_HD bool kv_run(const KvSeq& s, long long within, int run, KvRun& g) {
   const long long first = (long long)s.len - s.n;  // negative: padding rows before position 0
-  const long long pos0 = ((first > 0 ? first : 0) / kKvGroup + within) * kKvGroup;
+  const long long pos0 = ((first > 0 ? first : 0) / run + within) * run;
   if (s.n == 0 || within < 0 || pos0 >= s.keys) return false;
   g.pos0 = (int)pos0;
   g.from = first > pos0 ? (int)(first - pos0) : 0;
-  g.upto = s.keys - pos0 < kKvGroup ? (int)(s.keys - pos0) : kKvGroup;
+  g.upto = s.keys - pos0 < run ? (int)(s.keys - pos0) : run;
   g.row = s.row0 + (pos0 - first);
   return true;
 }

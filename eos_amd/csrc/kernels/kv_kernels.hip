@@ -57,14 +57,16 @@ EOS_DEV float f16_to_f32(uint32_t u) {
 }
 
 // 8 consecutive elements of a caller's row, and back.
-EOS_DEV void load8(const uint8_t* p, int dtype, float (&x)[8]) {
-  const v4u u = *reinterpret_cast<const v4u*>(p);
+EOS_DEV void unpack8(v4u u, int dtype, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t a = u[i] & 0xffffu, b = u[i] >> 16;
     x[2 * i] = dtype == kKvRowF16 ? f16_to_f32(a) : bf16_to_f32(a);
     x[2 * i + 1] = dtype == kKvRowF16 ? f16_to_f32(b) : bf16_to_f32(b);
   }
+}
+EOS_DEV void load8(const uint8_t* p, int dtype, float (&x)[8]) {
+  unpack8(*reinterpret_cast<const v4u*>(p), dtype, x);
 }
 EOS_DEV void store8(uint8_t* p, int dtype, const float (&x)[8]) {
   if (dtype == kKvRowF32) {
@@ -127,233 +129,324 @@ EOS_DEV bool find_seq(const KvCacheArgs& c, long long u, int mul, int per, int e
 
 // --------------------------------------------------------- append and read
 
-// The workgroup's 8 positions and their page.
-EOS_DEV bool find_group(const KvCacheArgs& c, KvGroup8& g, int& page) {
+// The positions of a workgroup of append or read and their sequence.
+template <int RUN>
+EOS_DEV bool find_run(const KvCacheArgs& c, KvRun& g, int& b) {
   KvSeq s;
   long long within = 0;
-  if (c.offsets == nullptr) {
+  if (RUN == kKvGroup) {
     s = kv_seq(c, blockIdx.x);
     flag(c, s.bad);
-  } else if (!find_seq(c, blockIdx.x, 1, kKvGroup, 2, s, within)) {
+  } else if (!find_seq(c, blockIdx.x, 1, RUN, 2, s, within)) {
     return false;
   }
-  if (!kv_group8(s, within, g)) return false;
-  page = kv_page(c, s.b, g.pos0);
-  if (page < 0) flag(c, kKvBadPage);
-  return page >= 0;
+  b = __builtin_amdgcn_readfirstlane(s.b);
+  if (!kv_run(s, within, RUN, g)) return false;
+  g.pos0 = __builtin_amdgcn_readfirstlane(g.pos0);
+  return true;
 }
 
-// One workgroup of 2 D threads: 8 positions (one V group) of one head, the
-// first half of the threads K, the second V, D / 8 lanes a row of 8 elements.
-// The workgroup owns the group's words, so a partly filled 4-bit word is read
-// and merged without another writer.
-template <int FMT, int D>
-EOS_DEV void append_group(const KvRowsArgs& a) {
-  constexpr int LANES = D / 8;
-  __shared__ uint16_t vt[FMT == kKvTq4 ? 1 : D * 8];
-  __shared__ uint32_t vw[FMT == kKvTq4 ? 8 * LANES : 1];
+// Tokens of the pools in front of the run's groups, or -1 where the group has
+// no row of the call or no page.
+template <int NG>
+EOS_DEV void find_blocks(const KvCacheArgs& c, const KvRun& g, int b, int h, long long (&at)[NG]) {
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    at[j] = -1;
+    if (8 * j >= g.upto || 8 * j + 8 <= g.from) continue;
+    const int pos = g.pos0 + 8 * j, page = kv_page(c, b, pos);
+    if (page < 0)
+      flag(c, kKvBadPage);
+    else
+      at[j] = ((((long long)page * c.kv_heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1)));
+  }
+}
+
+// One workgroup of 2 D threads: RUN positions of one head, in groups of 8 (the
+// tokens that V stores side by side); the first half of the threads has K, the
+// second V, D / 8 lanes a row of 8 elements. A group's words are one
+// workgroup's, so a partly filled 4-bit word is read and merged without
+// another writer. Bound by the rows' bytes and the latency of four dependent
+// loads, which runs of 32 positions spread over four groups.
+template <int FMT, int D, int RUN>
+EOS_DEV void append_run(const KvRowsArgs& a) {
+  constexpr int LANES = D / 8, NG = RUN / 8;
+  constexpr bool kPlain = FMT == kKvF16 || FMT == kKvBf16;
+  __shared__ uint16_t vt[FMT == kKvTq4 ? 1 : NG * D * 8];
+  __shared__ uint32_t vw[FMT == kKvTq4 ? NG * 8 * LANES : 1];
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, h = blockIdx.y;
-  KvGroup8 g;
-  int page;
-  if (!find_group(c, g, page)) return;
-  const int slot0 = g.pos0 & ((1 << c.page_shift) - 1);
-  const size_t block = ((size_t)page * c.kv_heads + h) << c.page_shift;  // tokens before
+  KvRun g;
+  int b;
+  if (!find_run<RUN>(c, g, b)) return;
+  long long at[NG];
+  find_blocks<NG>(c, g, b, h, at);
   const bool is_v = tid >= D;
   const int r = (tid / LANES) & 7, l8 = tid % LANES;
-  const bool live = r >= g.from && r < g.upto;
-  float x[8] = {};
-  if (live) {
-    const long long row = g.row + r;
-    const uint8_t* src = is_v ? a.v : a.k;
-    const long long stride = is_v ? a.v_stride : a.k_stride;
-    const size_t at = ((size_t)row * stride + (size_t)h * D + l8 * 8) * 2;
-    if constexpr (FMT == kKvF16 || FMT == kKvBf16) {
-      const v4u u = *reinterpret_cast<const v4u*>(src + at);
-      if (!is_v) {
-        *reinterpret_cast<v4u*>(c.k + ((block + slot0 + r) * D + l8 * 8) * 2) = u;
-      } else {
+  const uint8_t* src = (is_v ? a.v : a.k) + ((size_t)h * D + l8 * 8) * 2;
+  const size_t stride = (size_t)(is_v ? a.v_stride : a.k_stride) * 2;
+  v4u raw[NG];
+  bool live[NG];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          vt[(l8 * 8 + 2 * i) * 8 + r] = (uint16_t)u[i];
-          vt[(l8 * 8 + 2 * i + 1) * 8 + r] = (uint16_t)(u[i] >> 16);
-        }
-      }
-    } else {
-      load8(src + at, a.dtype, x);
-    }
+  for (int j = 0; j < NG; ++j) {
+    const int p = 8 * j + r;
+    live[j] = at[j] >= 0 && p >= g.from && p < g.upto;
+    raw[j] = v4u{0, 0, 0, 0};
+    if (live[j]) raw[j] = *reinterpret_cast<const v4u*>(src + (size_t)(g.row + p) * stride);
   }
-  if constexpr (FMT == kKvQ8) {
-    float m = 0.0f;
-    bool odd = false;  // NaN or infinity
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m = fmaxf(m, fabsf(x[i]));
-      odd |= !(fabsf(x[i]) <= 3.4028234e38f);
-    }
-    int bad = odd;
-#pragma unroll
-    for (int o = 1; o < LANES; o *= 2) {
-      m = fmaxf(m, __shfl_xor(m, o));
-      bad |= __shfl_xor(bad, o);
-    }
-    float scale = __fdiv_rn(m, 127.0f);
-    const bool none = scale < kTiny;
-    const bool nan = bad != 0 || scale > kHuge;
-    const float inv = none || nan ? 0.0f : __fdiv_rn(127.0f, m);
-    scale = nan ? __builtin_nanf("") : none ? 0.0f : scale;
-    uint32_t code[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q = nan ? 0.0f : fminf(fmaxf(rintf(x[i] * inv), -127.0f), 127.0f);
-      code[i] = (uint32_t)(int)q & 0xffu;
-    }
-    if (live) {
-      if (l8 == 0) (is_v ? c.v_scale : c.k_scale)[block + slot0 + r] = scale;
-      if (!is_v) {
-        *reinterpret_cast<v2u*>(c.k + (block + slot0 + r) * D + l8 * 8) =
-            v2u{code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
-                code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vt[(l8 * 8 + i) * 8 + r] = (uint16_t)code[i];
-      }
-    }
-  }
+  float sgn[8];
   if constexpr (FMT == kKvTq4) {
-    double ss = 0.0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss += (double)x[i] * (double)x[i];
-#pragma unroll
-    for (int o = 1; o < LANES; o *= 2) ss += __shfl_xor(ss, o);
-    float scale = (float)__builtin_sqrt(ss * (1.0 / D));
-    const bool none = scale < kTiny;
-    const bool nan = !(scale <= kHuge);
-    if (none || nan) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    }
     const v4f s0 = reinterpret_cast<const v4f*>(c.t.signs + l8 * 8)[0];
     const v4f s1 = reinterpret_cast<const v4f*>(c.t.signs + l8 * 8)[1];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= i < 4 ? s0[i & 3] : s1[i & 3];
-    hadamard8<LANES>(x);
-    // |w| / (s sqrt(D)) against the edges, the division moved to their side.
-    const float norm = none || nan ? 0.0f : scale * (float)__builtin_sqrt((double)D);
-    scale = nan ? __builtin_nanf("") : none ? 0.0f : scale;
-    float edge[7];
+    for (int i = 0; i < 8; ++i) sgn[i] = i < 4 ? s0[i & 3] : s1[i & 3];
+  }
 #pragma unroll
-    for (int e = 0; e < 7; ++e) edge[e] = c.t.edges[e] * norm;
-    uint32_t word = 0;
+  for (int j = 0; j < NG; ++j) {
+    if (at[j] < 0) continue;
+    if constexpr (kPlain) {
+      if (!is_v) {
+        if (live[j]) *reinterpret_cast<v4u*>(c.k + ((size_t)(at[j] + r) * D + l8 * 8) * 2) = raw[j];
+      } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t idx = x[i] < 0.0f ? 8u : 0u;
-      const float w = fabsf(x[i]);
-#pragma unroll
-      for (int e = 0; e < 7; ++e) idx += w > edge[e] ? 1u : 0u;
-      word |= idx << (4 * i);
+        for (int i = 0; i < 4; ++i) {
+          vt[(j * D + l8 * 8 + 2 * i) * 8 + r] = (uint16_t)raw[j][i];
+          vt[(j * D + l8 * 8 + 2 * i + 1) * 8 + r] = (uint16_t)(raw[j][i] >> 16);
+        }
+      }
+      continue;
     }
-    if (live && l8 == 0) (is_v ? c.v_scale : c.k_scale)[block + slot0 + r] = scale;
-    if (!is_v) {
-      if (live) reinterpret_cast<uint32_t*>(c.k)[(block + slot0 + r) * LANES + l8] = word;
-    } else {
-      vw[r * LANES + l8] = word;
+    float x[8];
+    unpack8(raw[j], a.dtype, x);
+    if constexpr (FMT == kKvQ8) {
+      float m = 0.0f;
+      int bad = 0;  // NaN or infinity
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        m = fmaxf(m, fabsf(x[i]));
+        bad |= !(fabsf(x[i]) <= 3.4028234e38f);
+      }
+#pragma unroll
+      for (int o = 1; o < LANES; o *= 2) {
+        m = fmaxf(m, __shfl_xor(m, o));
+        bad |= __shfl_xor(bad, o);
+      }
+      float scale = __fdiv_rn(m, 127.0f);
+      const bool none = scale < kTiny;
+      const bool nan = bad != 0 || scale > kHuge;
+      const float inv = none || nan ? 0.0f : __fdiv_rn(127.0f, m);
+      scale = nan ? __builtin_nanf("") : none ? 0.0f : scale;
+      uint32_t code[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float q = nan ? 0.0f : fminf(fmaxf(rintf(x[i] * inv), -127.0f), 127.0f);
+        code[i] = (uint32_t)(int)q & 0xffu;
+      }
+      if (live[j] && l8 == 0) (is_v ? c.v_scale : c.k_scale)[at[j] + r] = scale;
+      if (!is_v) {
+        if (live[j])
+          *reinterpret_cast<v2u*>(c.k + (size_t)(at[j] + r) * D + l8 * 8) =
+              v2u{code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
+                  code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vt[(j * D + l8 * 8 + i) * 8 + r] = (uint16_t)code[i];
+      }
+    }
+    if constexpr (FMT == kKvTq4) {
+      double ss = 0.0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += (double)x[i] * (double)x[i];
+#pragma unroll
+      for (int o = 1; o < LANES; o *= 2) ss += __shfl_xor(ss, o);
+      float scale = (float)__builtin_sqrt(ss * (1.0 / D));
+      const bool none = scale < kTiny;
+      const bool nan = !(scale <= kHuge);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = none || nan ? 0.0f : x[i] * sgn[i];
+      hadamard8<LANES>(x);
+      // |w| / (s sqrt(D)) against the edges, the division moved to their side;
+      // they ascend, so three comparisons place a value among the seven.
+      const float norm = none || nan ? 0.0f : scale * (float)__builtin_sqrt((double)D);
+      scale = nan ? __builtin_nanf("") : none ? 0.0f : scale;
+      float e[7];
+#pragma unroll
+      for (int i = 0; i < 7; ++i) e[i] = c.t.edges[i] * norm;
+      uint32_t word = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = fabsf(x[i]);
+        const bool b2 = w > e[3];
+        const bool b1 = w > (b2 ? e[5] : e[1]);
+        const bool b0 = w > (b2 ? (b1 ? e[6] : e[4]) : (b1 ? e[2] : e[0]));
+        const uint32_t code = (x[i] < 0.0f ? 8u : 0u) | (b2 ? 4u : 0u) | (b1 ? 2u : 0u) | (b0 ? 1u : 0u);
+        word |= code << (4 * i);
+      }
+      if (live[j] && l8 == 0) (is_v ? c.v_scale : c.k_scale)[at[j] + r] = scale;
+      if (!is_v) {
+        if (live[j]) reinterpret_cast<uint32_t*>(c.k)[(size_t)(at[j] + r) * LANES + l8] = word;
+      } else {
+        vw[(j * 8 + r) * LANES + l8] = word;
+      }
     }
   }
   __syncthreads();
-  // V: the group's 8 tokens of one dimension by one thread.
-  if (tid >= D) return;
-  const bool whole = g.from == 0 && g.upto == kKvGroup;
-  const size_t vrow = (block / kKvGroup + slot0 / kKvGroup) * D + tid;  // group-dimensions before
-  if constexpr (FMT == kKvF16 || FMT == kKvBf16) {
-    uint16_t* dst = reinterpret_cast<uint16_t*>(c.v) + vrow * 8;
-    if (whole) {
-      *reinterpret_cast<v4u*>(dst) = *reinterpret_cast<const v4u*>(&vt[tid * 8]);
+  // V: a group's 8 tokens of one dimension by one thread.
+#pragma unroll
+  for (int it = 0; it < (NG + 1) / 2; ++it) {
+    const int j = 2 * it + (NG > 1 ? tid / D : 0), dim = tid % D;
+    if (NG == 1 && tid >= D) break;
+    long long base = at[2 * it];
+    if (NG > 1 && j != 2 * it) base = at[(2 * it + 1) % NG];
+    if (base < 0) continue;
+    const int from = g.from > 8 * j ? g.from - 8 * j : 0;
+    const int upto = g.upto - 8 * j < 8 ? g.upto - 8 * j : 8;
+    const bool whole = from == 0 && upto == 8;
+    const size_t vrow = (size_t)(base / kKvGroup) * D + dim;  // group-dimensions before
+    if constexpr (kPlain) {
+      uint16_t* dst = reinterpret_cast<uint16_t*>(c.v) + vrow * 8;
+      if (whole) {
+        *reinterpret_cast<v4u*>(dst) = *reinterpret_cast<const v4u*>(&vt[(j * D + dim) * 8]);
+      } else {
+        for (int t = from; t < upto; ++t) dst[t] = vt[(j * D + dim) * 8 + t];
+      }
+    } else if constexpr (FMT == kKvQ8) {
+      uint8_t* dst = c.v + vrow * 8;
+      if (whole) {
+        const v4u u = *reinterpret_cast<const v4u*>(&vt[(j * D + dim) * 8]);
+        *reinterpret_cast<v2u*>(dst) = v2u{perm(u[1], u[0], 0x06040200), perm(u[3], u[2], 0x06040200)};
+      } else {
+        for (int t = from; t < upto; ++t) dst[t] = (uint8_t)vt[(j * D + dim) * 8 + t];
+      }
     } else {
-      for (int t = g.from; t < g.upto; ++t) dst[t] = vt[tid * 8 + t];
+      uint32_t* dst = reinterpret_cast<uint32_t*>(c.v) + vrow;
+      uint32_t word = 0, mask = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const bool in = t >= from && t < upto;
+        word |= in ? (vw[(j * 8 + t) * LANES + dim / 8] >> (4 * (dim & 7)) & 15u) << (4 * t) : 0u;
+        mask |= in ? 15u << (4 * t) : 0u;
+      }
+      *dst = whole ? word : (*dst & ~mask) | word;
     }
-  } else if constexpr (FMT == kKvQ8) {
-    uint8_t* dst = c.v + vrow * 8;
-    if (whole) {
-      const v4u u = *reinterpret_cast<const v4u*>(&vt[tid * 8]);
-      *reinterpret_cast<v2u*>(dst) = v2u{perm(u[1], u[0], 0x06040200), perm(u[3], u[2], 0x06040200)};
-    } else {
-      for (int t = g.from; t < g.upto; ++t) dst[t] = (uint8_t)vt[tid * 8 + t];
-    }
-  } else {
-    uint32_t* dst = reinterpret_cast<uint32_t*>(c.v) + vrow;
-    uint32_t word = 0, mask = 0;
-    for (int t = g.from; t < g.upto; ++t) {
-      word |= (vw[t * LANES + tid / 8] >> (4 * (tid & 7)) & 15u) << (4 * t);
-      mask |= 15u << (4 * t);
-    }
-    *dst = whole ? word : (*dst & ~mask) | word;
   }
 }
 
-// The values of 8 positions of one head, same shape of workgroup.
-template <int FMT, int D>
-EOS_DEV void read_group(const KvRowsArgs& a) {
-  constexpr int LANES = D / 8;
+// The values of RUN positions of one head, same shape of workgroup; V passes
+// through LDS from its groups of 8 tokens into rows.
+template <int FMT, int D, int RUN>
+EOS_DEV void read_run(const KvRowsArgs& a) {
+  constexpr int LANES = D / 8, NG = RUN / 8;
+  constexpr bool kPlain = FMT == kKvF16 || FMT == kKvBf16;
+  constexpr int kType = FMT == kKvF16 ? kKvRowF16 : kKvRowBf16;
+  __shared__ __align__(16) uint16_t vh[kPlain ? NG * 8 * D : 8];
+  __shared__ __align__(16) uint8_t vb[kPlain ? 16 : NG * 8 * D];
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, h = blockIdx.y;
-  KvGroup8 g;
-  int page;
-  if (!find_group(c, g, page)) return;
-  const int slot0 = g.pos0 & ((1 << c.page_shift) - 1);
-  const size_t block = ((size_t)page * c.kv_heads + h) << c.page_shift;
+  KvRun g;
+  int b;
+  if (!find_run<RUN>(c, g, b)) return;
+  long long at[NG];
+  find_blocks<NG>(c, g, b, h, at);
   const bool is_v = tid >= D;
   const int r = (tid / LANES) & 7, l8 = tid % LANES;
-  const bool live = r >= g.from && r < g.upto;
-  const size_t token = block + slot0 + r;
-  const size_t vrow = (block / kKvGroup + slot0 / kKvGroup) * D + l8 * 8;
-  float x[8] = {};
-  if (live) {
-    if constexpr (FMT == kKvF16 || FMT == kKvBf16) {
-      constexpr int kType = FMT == kKvF16 ? kKvRowF16 : kKvRowBf16;
-      if (!is_v) {
-        load8(c.k + (token * D + l8 * 8) * 2, kType, x);
-      } else {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(c.v) + vrow * 8 + r;
+  // V's groups, one dimension a thread.
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          x[i] = kType == kKvRowF16 ? f16_to_f32(src[i * 8]) : bf16_to_f32(src[i * 8]);
-      }
+  for (int it = 0; it < (NG + 1) / 2; ++it) {
+    const int j = 2 * it + (NG > 1 ? tid / D : 0), dim = tid % D;
+    if (NG == 1 && tid >= D) break;
+    long long base = at[2 * it];
+    if (NG > 1 && j != 2 * it) base = at[(2 * it + 1) % NG];
+    if (base < 0) continue;
+    const size_t vrow = (size_t)(base / kKvGroup) * D + dim;
+    if constexpr (kPlain) {
+      const v4u u = *reinterpret_cast<const v4u*>(c.v + vrow * 16);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) vh[(j * 8 + t) * D + dim] = (uint16_t)(u[t / 2] >> (16 * (t & 1)));
     } else if constexpr (FMT == kKvQ8) {
-      const int8_t* src = reinterpret_cast<const int8_t*>(is_v ? c.v + vrow * 8 + r
-                                                               : c.k + token * D + l8 * 8);
-      const int step = is_v ? 8 : 1;
-      const float scale = (is_v ? c.v_scale : c.k_scale)[token];
+      const v2u u = *reinterpret_cast<const v2u*>(c.v + vrow * 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)src[i * step] * scale;
+      for (int t = 0; t < 8; ++t) vb[(j * 8 + t) * D + dim] = (uint8_t)(u[t / 4] >> (8 * (t & 3)));
     } else {
+      const uint32_t u = reinterpret_cast<const uint32_t*>(c.v)[vrow];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t code =
-            is_v ? reinterpret_cast<const uint32_t*>(c.v)[vrow + i] >> (4 * r) & 15u
-                 : reinterpret_cast<const uint32_t*>(c.k)[token * LANES + l8] >> (4 * i) & 15u;
-        float m = c.t.mags[0];
+      for (int t = 0; t < 8; ++t) vb[(j * 8 + t) * D + dim] = (uint8_t)(u >> (4 * t) & 15u);
+    }
+  }
+  // K rows and scales; the values a thread has no row for are not stored.
+  v4u raw[NG];
+  float scale[NG];
+  bool live[NG];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) m = (code & 7u) == (uint32_t)e ? c.t.mags[e] : m;
-        x[i] = (code & 8u) != 0 ? -m : m;
+  for (int j = 0; j < NG; ++j) {
+    const int p = 8 * j + r;
+    live[j] = at[j] >= 0 && p >= g.from && p < g.upto;
+    raw[j] = v4u{0, 0, 0, 0};
+    scale[j] = 0.0f;
+    if (!live[j]) continue;
+    const size_t token = (size_t)(at[j] + r);
+    if constexpr (!kPlain) scale[j] = (is_v ? c.v_scale : c.k_scale)[token];
+    if (is_v) continue;
+    if constexpr (kPlain) {
+      raw[j] = *reinterpret_cast<const v4u*>(c.k + (token * D + l8 * 8) * 2);
+    } else if constexpr (FMT == kKvQ8) {
+      const v2u u = *reinterpret_cast<const v2u*>(c.k + token * D + l8 * 8);
+      raw[j][0] = u[0], raw[j][1] = u[1];
+    } else {
+      raw[j][0] = reinterpret_cast<const uint32_t*>(c.k)[token * LANES + l8];
+    }
+  }
+  float sgn[8];
+  if constexpr (FMT == kKvTq4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sgn[i] = c.t.signs[l8 * 8 + i] * (float)(1.0 / __builtin_sqrt((double)D));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    if (at[j] < 0) continue;
+    float x[8];
+    if (is_v) {
+      if constexpr (kPlain) {
+        raw[j] = *reinterpret_cast<const v4u*>(&vh[(j * 8 + r) * D + l8 * 8]);
+      } else {
+        const v2u u = *reinterpret_cast<const v2u*>(&vb[(j * 8 + r) * D + l8 * 8]);
+        raw[j][0] = u[0], raw[j][1] = u[1];
       }
     }
-  }
-  if constexpr (FMT == kKvTq4) {
-    hadamard8<LANES>(x);
-    if (live) {
-      const float scale = (is_v ? c.v_scale : c.k_scale)[token];
-      const float f = scale * (float)(1.0 / __builtin_sqrt((double)D));
+    if constexpr (kPlain) {
+      unpack8(raw[j], kType, x);
+    } else if constexpr (FMT == kKvQ8) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= f * c.t.signs[l8 * 8 + i];
+      for (int i = 0; i < 8; ++i) x[i] = (float)(int8_t)(raw[j][i / 4] >> (8 * (i & 3))) * scale[j];
+    } else {
+      // Codes as bytes: K's nibbles spread, V's already are.
+      uint32_t lo = raw[j][0], hi = raw[j][1];
+      if (!is_v) {
+        const uint32_t ev = lo & 0x0f0f0f0fu, od = lo >> 4 & 0x0f0f0f0fu;
+        lo = perm(od, ev, 0x05010400u);
+        hi = perm(od, ev, 0x07030602u);
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t k = w == 0 ? lo : hi, idx = k & 0x07070707u;
+        const uint32_t fh = perm(c.t.hi[1], c.t.hi[0], idx) | (k << 4 & 0x80808080u);
+        const uint32_t fl = perm(c.t.lo[1], c.t.lo[0], idx);
+        const uint32_t p0 = perm(fh, fl, 0x05010400u), p1 = perm(fh, fl, 0x07030602u);
+        x[4 * w] = f16_to_f32(p0 & 0xffffu);
+        x[4 * w + 1] = f16_to_f32(p0 >> 16);
+        x[4 * w + 2] = f16_to_f32(p1 & 0xffffu);
+        x[4 * w + 3] = f16_to_f32(p1 >> 16);
+      }
+      hadamard8<LANES>(x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= scale[j] * sgn[i];
     }
+    if (!live[j]) continue;
+    const size_t row = (size_t)(g.row + 8 * j + r);
+    const size_t to = row * (is_v ? a.v_stride : a.k_stride) + (size_t)h * D + l8 * 8;
+    store8((is_v ? a.v : a.k) + to * (a.dtype == kKvRowF32 ? 4 : 2), a.dtype, x);
   }
-  if (!live) return;
-  const long long row = g.row + r;
-  uint8_t* dst = is_v ? a.v : a.k;
-  const long long stride = is_v ? a.v_stride : a.k_stride;
-  const size_t at = (size_t)row * stride + (size_t)h * D + l8 * 8;
-  store8(dst + at * (a.dtype == kKvRowF32 ? 4 : 2), a.dtype, x);
 }
 
 // ---------------------------------------------------------------- attention
@@ -1477,10 +1570,16 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
 
 #define KV_KERNELS(NAME, FMT, D)                                                             \
   extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_append_##NAME##_##D(KvRowsArgs a) { \
-    append_group<FMT, D>(a);                                                                 \
+    append_run<FMT, D, kKvRun>(a);                                                           \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_append1_##NAME##_##D(KvRowsArgs a) { \
+    append_run<FMT, D, kKvGroup>(a);                                                         \
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_read_##NAME##_##D(KvRowsArgs a) {   \
-    read_group<FMT, D>(a);                                                                   \
+    read_run<FMT, D, kKvRun>(a);                                                             \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_read1_##NAME##_##D(KvRowsArgs a) {  \
+    read_run<FMT, D, kKvGroup>(a);                                                           \
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(256, D * bits_of(FMT) > 2048 ? 1 : 2) void eos_kv_split_##NAME##_##D(KvAttnArgs a) {    \
     attn_split<FMT, D>(a);                                                                   \

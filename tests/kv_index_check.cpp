@@ -79,22 +79,21 @@ void one(int at, bool sound) {
   }
 
   // append / read
+  const int run = one_each ? kKvGroup : kKvRun;
   std::vector<int> seen(c.rows, 0);
-  const long long groups = one_each ? c.batch : kv_units(c.rows, c.batch, 1, kKvGroup, 2);
-  for (long long u = 0; u < groups; ++u) {
+  const long long runs = one_each ? c.batch : kv_units(c.rows, c.batch, 1, run, 2);
+  for (long long u = 0; u < runs; ++u) {
     KvSeq s;
     long long within = 0;
     if (one_each) s = kv_seq(c, (int)u);
-    else if (!find(c, u, 1, kKvGroup, 2, s, within)) continue;
-    KvGroup8 g;
-    if (!kv_group8(s, within, g)) continue;
-    const int page = kv_page(c, s.b, g.pos0);
-    if (page < 0) continue;
-    CHECK(page < c.pages);
-    CHECK((g.pos0 & (P - 1)) + 8 <= P && g.pos0 % 8 == 0);
-    CHECK(g.from >= 0 && g.upto <= 8 && g.from < g.upto);
+    else if (!find(c, u, 1, run, 2, s, within)) continue;
+    KvRun g;
+    if (!kv_run(s, within, run, g)) continue;
+    CHECK(g.pos0 % 8 == 0 && g.from >= 0 && g.upto <= run && g.from < g.upto);
     for (int r = g.from; r < g.upto; ++r) {
       CHECK(g.row + r >= 0 && g.row + r < c.rows);
+      const int page = kv_page(c, s.b, g.pos0 + r / 8 * 8);
+      CHECK(page < c.pages && page == kv_page(c, s.b, g.pos0 + r));
       ++seen[g.row + r];
       if (sound) CHECK(g.pos0 + r == s.len - s.n + (g.row + r - s.row0));
     }
