@@ -82,8 +82,61 @@ EOS_DEV void store8(uint8_t* p, int dtype, const float (&x)[8]) {
   *reinterpret_cast<v4u*>(p) = u;
 }
 
+// The value of lane ^ S, by the vector unit's own lane moves where it has them
+// (a shuffle goes through LDS: of 67 M values read back from tq4, 66 us with
+// shuffles).
+template <int CTRL>
+EOS_DEV uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+template <int S>
+EOS_DEV uint32_t lane_xor(uint32_t x) {
+  if constexpr (S == 1) return dpp<0xb1>(x);                // quad_perm 1 0 3 2
+  else if constexpr (S == 2) return dpp<0x4e>(x);           // quad_perm 2 3 0 1
+  else if constexpr (S == 4) return dpp<0x1b>(dpp<0x141>(x));  // half mirror, quad reversed
+  else if constexpr (S == 8) return dpp<0x128>(x);          // row rotated by 8
+  else return (uint32_t)__shfl_xor((int)x, S);
+}
+template <int S>
+EOS_DEV float lane_xor(float x) {
+  return __builtin_bit_cast(float, lane_xor<S>(__builtin_bit_cast(uint32_t, x)));
+}
+template <int S>
+EOS_DEV double lane_xor(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, (uint64_t)lane_xor<S>((uint32_t)(u >> 32)) << 32 |
+                                        lane_xor<S>((uint32_t)u));
+}
+template <int LANES, int S = 1>
+EOS_DEV double row_sum(double x) {
+  if constexpr (S < LANES) return row_sum<LANES, 2 * S>(x + lane_xor<S>(x));
+  else return x;
+}
+template <int LANES, int S = 1>
+EOS_DEV float row_max(float x) {
+  if constexpr (S < LANES) return row_max<LANES, 2 * S>(fmaxf(x, lane_xor<S>(x)));
+  else return x;
+}
+template <int LANES, int S = 1>
+EOS_DEV uint32_t row_or(uint32_t x) {
+  if constexpr (S < LANES) return row_or<LANES, 2 * S>(x | lane_xor<S>(x));
+  else return x;
+}
+
 // Walsh-Hadamard transform of a row spread over LANES neighbouring lanes, 8
 // consecutive elements each.
+template <int LANES, int S = 1>
+EOS_DEV void hadamard_lanes(float (&x)[8]) {
+  if constexpr (S < LANES) {
+    const uint32_t flip = (threadIdx.x & S) != 0 ? 0x80000000u : 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float o = lane_xor<S>(x[i]);
+      x[i] = o + __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[i]) ^ flip);
+    }
+    hadamard_lanes<LANES, 2 * S>(x);
+  }
+}
 template <int LANES>
 EOS_DEV void hadamard8(float (&x)[8]) {
 #pragma unroll
@@ -95,14 +148,7 @@ EOS_DEV void hadamard8(float (&x)[8]) {
         x[i] = a + b;
         x[i + s] = a - b;
       }
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int s = 1; s < LANES; s *= 2)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float o = __shfl_xor(x[i], s);
-      x[i] = (lane & s) != 0 ? o - x[i] : x[i] + o;
-    }
+  hadamard_lanes<LANES>(x);
 }
 
 // ------------------------------------------------------------- sequences
@@ -220,17 +266,14 @@ EOS_DEV void append_run(const KvRowsArgs& a) {
     unpack8(raw[j], a.dtype, x);
     if constexpr (FMT == kKvQ8) {
       float m = 0.0f;
-      int bad = 0;  // NaN or infinity
+      uint32_t bad = 0;  // NaN or infinity
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         m = fmaxf(m, fabsf(x[i]));
         bad |= !(fabsf(x[i]) <= 3.4028234e38f);
       }
-#pragma unroll
-      for (int o = 1; o < LANES; o *= 2) {
-        m = fmaxf(m, __shfl_xor(m, o));
-        bad |= __shfl_xor(bad, o);
-      }
+      m = row_max<LANES>(m);
+      bad = row_or<LANES>(bad);
       float scale = __fdiv_rn(m, 127.0f);
       const bool none = scale < kTiny;
       const bool nan = bad != 0 || scale > kHuge;
@@ -257,8 +300,7 @@ EOS_DEV void append_run(const KvRowsArgs& a) {
       double ss = 0.0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += (double)x[i] * (double)x[i];
-#pragma unroll
-      for (int o = 1; o < LANES; o *= 2) ss += __shfl_xor(ss, o);
+      ss = row_sum<LANES>(ss);
       float scale = (float)__builtin_sqrt(ss * (1.0 / D));
       const bool none = scale < kTiny;
       const bool nan = !(scale <= kHuge);
