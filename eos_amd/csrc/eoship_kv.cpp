@@ -174,7 +174,7 @@ int rows_call(EosHipRuntime* rt, const EosHipKVCache* kv, const EosHipKVBatch* b
     return launch(rt, kv, one.c_str(), b->batch, kv->d.kv_heads, 2 * kv->d.head_dim, &a, what, err);
   }
   return launch(rt, kv, op, kv_units(b->rows, b->batch, 1, kKvRun, 2), kv->d.kv_heads,
-                2 * kv->d.head_dim, &a, what, err);
+                kv->d.format == kKvTq4 ? 256 : 2 * kv->d.head_dim, &a, what, err);
 }
 
 }  // namespace

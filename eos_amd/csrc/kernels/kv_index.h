@@ -26,33 +26,36 @@ struct KvSeq {
   int n = 0, len = 0, keys = 0, bad = 0;
 };
 
-KV_HD KvSeq kv_seq(const KvCacheArgs& c, int b) {
+// From its row range [lo, hi) and length as they stand in memory.
+KV_HD KvSeq kv_seq_of(const KvCacheArgs& c, int b, long long lo, long long hi, int len) {
   KvSeq s;
   s.b = b;
-  long long lo = b, hi = (long long)b + 1;
-  if (c.offsets != nullptr) {
-    lo = c.offsets[b];
-    hi = c.offsets[b + 1];
-  }
   if (lo < 0 || hi < lo || hi > c.rows) {
     s.bad |= kKvBadOffset;
     lo = hi = 0;
   }
   s.row0 = lo;
   s.n = (int)(hi - lo);
-  s.len = c.lengths[b];
+  s.len = len;
   const long long cap = (long long)c.table_stride << c.page_shift;
   if (s.len < 0 || s.len > cap) s.bad |= kKvBadLength;
   if (s.len < 0) s.len = 0;
   s.keys = s.len > cap ? (int)cap : s.len;
   return s;
 }
+KV_HD KvSeq kv_seq(const KvCacheArgs& c, int b) {
+  return c.offsets != nullptr ? kv_seq_of(c, b, c.offsets[b], c.offsets[b + 1], c.lengths[b])
+                              : kv_seq_of(c, b, b, (long long)b + 1, c.lengths[b]);
+}
 
 // Work units are numbered through a batch without knowing its row counts on
 // the host: sequence b's first unit is floor(offset * mul / per) + extra * b,
 // which leaves it floor(n * mul / per) + extra of them at least.
+KV_HD long long kv_unit_base_of(long long offset, int b, int mul, int per, int extra) {
+  return offset * mul / per + (long long)extra * b;
+}
 KV_HD long long kv_unit_base(const KvCacheArgs& c, int b, int mul, int per, int extra) {
-  return (long long)c.offsets[b] * mul / per + (long long)extra * b;
+  return kv_unit_base_of(c.offsets[b], b, mul, per, extra);
 }
 // Units of the whole batch.
 KV_HD long long kv_units(long long rows, int batch, int mul, int per, int extra) {

@@ -158,22 +158,102 @@ EOS_DEV void flag(const KvCacheArgs& c, int bits) {
 }
 
 // The sequence that unit u belongs to and u's index within it; false where
-// no sequence has it. All threads of the workgroup call it.
+// no sequence has it. All threads of the workgroup call it; each looks at one
+// sequence of 256 (of 64, 128, 512), so that its numbers come with one load's
+// latency.
 EOS_DEV bool find_seq(const KvCacheArgs& c, long long u, int mul, int per, int extra, KvSeq& s,
                       long long& within) {
+  __shared__ int found[4];
   int count = 0;
   for (int b0 = 0; b0 < c.batch; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
-    count += __syncthreads_count(b < c.batch && kv_unit_base(c, b, mul, per, extra) <= u);
+    const bool in = b < c.batch;
+    const int lo = in ? c.offsets[b] : 0, hi = in ? c.offsets[b + 1] : 0, len = in ? c.lengths[b] : 0;
+    const int n = __syncthreads_count(in && kv_unit_base_of(lo, b, mul, per, extra) <= u);
+    if ((int)threadIdx.x == n - 1) {
+      found[0] = b;
+      found[1] = lo;
+      found[2] = hi;
+      found[3] = len;
+    }
+    count += n;
   }
   if (count == 0) return false;
-  s = kv_seq(c, count - 1);
+  __syncthreads();
+  s = kv_seq_of(c, found[0], found[1], found[2], found[3]);
   flag(c, s.bad);
-  within = u - kv_unit_base(c, count - 1, mul, per, extra);
+  within = u - kv_unit_base_of(found[1], s.b, mul, per, extra);
   return true;
 }
 
 // --------------------------------------------------------- append and read
+
+template <int FMT>
+EOS_DEV v4f mfma16(v4u a, v4u b, v4f c) {
+  if constexpr (FMT == kKvBf16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a),
+                                                   __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
+                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// The rotation of tq4 on the matrix cores. A wavefront has 16 rows; lane (row r
+// = lane % 16, part g = lane / 16) holds elements 32 s + 8 g + j of its row as
+// 16-bit operands x[s][j] and receives elements 32 (t / 2) + 8 g + 4 (t % 2) + i
+// of the transform as y[t][i]. The other operand is the Walsh-Hadamard matrix,
+// whose entries are signs: the parity of i & j % 4, t % 2 & j / 4, g' & g and
+// t / 2 & s for output (t, g', i) and input (s, g, j). So there are two fragments,
+// for even and odd t, and the rest is a sign of x. Products by +-1 are exact,
+// sums f32. (By butterflies between lanes the vector unit bound both kernels:
+// 32,768 tokens x 8 heads x 128 took 106 us to append, 59 to read.)
+template <int FMT, int D>
+EOS_DEV void rotate16(const v4u (&x)[D / 32], v4f (&y)[D / 16]) {
+  constexpr uint32_t kOne = FMT == kKvBf16 ? 0x3f80u : 0x3c00u;
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  v4u f[2];
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t u = kOne | kOne << 16;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int j = 2 * w + b;
+        const int par = __builtin_popcount(r & 3 & j & 3) ^ __builtin_popcount((r >> 2) & g) ^ (odd & j >> 2);
+        u |= (uint32_t)(par & 1) << (15 + 16 * b);
+      }
+      f[odd][w] = u;
+    }
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) {
+    y[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      const uint32_t flip = (__builtin_popcount((t >> 1) & s) & 1) != 0 ? 0x80008000u : 0u;
+      y[t] = mfma16<FMT>(f[t & 1], x[s] ^ v4u{flip, flip, flip, flip}, y[t]);
+    }
+  }
+}
+
+// Codes (a byte each) -> f16 magnitudes with their signs, four of them.
+EOS_DEV void bytes_to_f16(const KvTables& t, uint32_t k, uint32_t& p0, uint32_t& p1) {
+  const uint32_t idx = k & 0x07070707u;
+  const uint32_t fh = perm(t.hi[1], t.hi[0], idx) | (k << 4 & 0x80808080u);
+  const uint32_t fl = perm(t.lo[1], t.lo[0], idx);
+  p0 = perm(fh, fl, 0x05010400u);
+  p1 = perm(fh, fl, 0x07030602u);
+}
+
+// The 4-bit code of a rotated value: the edges ascend, so three comparisons
+// place it among the seven.
+EOS_DEV uint32_t code_of(float x, const float (&e)[7]) {
+  const float w = fabsf(x);
+  const bool b2 = w > e[3];
+  const bool b1 = w > (b2 ? e[5] : e[1]);
+  const bool b0 = w > (b2 ? (b1 ? e[6] : e[4]) : (b1 ? e[2] : e[0]));
+  return (x < 0.0f ? 8u : 0u) | (b2 ? 4u : 0u) | (b1 ? 2u : 0u) | (b0 ? 1u : 0u);
+}
 
 // The positions of a workgroup of append or read and their sequence.
 template <int RUN>
@@ -193,19 +273,25 @@ EOS_DEV bool find_run(const KvCacheArgs& c, KvRun& g, int& b) {
 }
 
 // Tokens of the pools in front of the run's groups, or -1 where the group has
-// no row of the call or no page.
+// no row of the call or no page. The page ids are loaded together.
 template <int NG>
 EOS_DEV void find_blocks(const KvCacheArgs& c, const KvRun& g, int b, int h, long long (&at)[NG]) {
+  const int32_t* row = c.table + (size_t)b * c.table_stride;
+  int page[NG];
+#pragma unroll
+  for (int j = 0; j < NG; ++j)
+    page[j] = row[kv_min((g.pos0 + 8 * j) >> c.page_shift, c.table_stride - 1)];
+  bool bad = false;
 #pragma unroll
   for (int j = 0; j < NG; ++j) {
-    at[j] = -1;
-    if (8 * j >= g.upto || 8 * j + 8 <= g.from) continue;
-    const int pos = g.pos0 + 8 * j, page = kv_page(c, b, pos);
-    if (page < 0)
-      flag(c, kKvBadPage);
-    else
-      at[j] = ((((long long)page * c.kv_heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1)));
+    const bool need = 8 * j < g.upto && 8 * j + 8 > g.from;
+    const bool in = (unsigned)page[j] < (unsigned)c.pages;
+    bad |= need && !in;
+    at[j] = need && in ? ((((long long)page[j] * c.kv_heads + h) << c.page_shift) +
+                          ((g.pos0 + 8 * j) & ((1 << c.page_shift) - 1)))
+                       : -1;
   }
+  if (bad) flag(c, kKvBadPage);
 }
 
 // One workgroup of 2 D threads: RUN positions of one head, in groups of 8 (the
@@ -307,8 +393,7 @@ EOS_DEV void append_run(const KvRowsArgs& a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = none || nan ? 0.0f : x[i] * sgn[i];
       hadamard8<LANES>(x);
-      // |w| / (s sqrt(D)) against the edges, the division moved to their side;
-      // they ascend, so three comparisons place a value among the seven.
+      // |w| / (s sqrt(D)) against the edges, the division moved to their side.
       const float norm = none || nan ? 0.0f : scale * (float)__builtin_sqrt((double)D);
       scale = nan ? __builtin_nanf("") : none ? 0.0f : scale;
       float e[7];
@@ -316,14 +401,7 @@ EOS_DEV void append_run(const KvRowsArgs& a) {
       for (int i = 0; i < 7; ++i) e[i] = c.t.edges[i] * norm;
       uint32_t word = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = fabsf(x[i]);
-        const bool b2 = w > e[3];
-        const bool b1 = w > (b2 ? e[5] : e[1]);
-        const bool b0 = w > (b2 ? (b1 ? e[6] : e[4]) : (b1 ? e[2] : e[0]));
-        const uint32_t code = (x[i] < 0.0f ? 8u : 0u) | (b2 ? 4u : 0u) | (b1 ? 2u : 0u) | (b0 ? 1u : 0u);
-        word |= code << (4 * i);
-      }
+      for (int i = 0; i < 8; ++i) word |= code_of(x[i], e) << (4 * i);
       if (live[j] && l8 == 0) (is_v ? c.v_scale : c.k_scale)[at[j] + r] = scale;
       if (!is_v) {
         if (live[j]) reinterpret_cast<uint32_t*>(c.k)[(size_t)(at[j] + r) * LANES + l8] = word;
@@ -471,10 +549,8 @@ EOS_DEV void read_run(const KvRowsArgs& a) {
       }
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        const uint32_t k = w == 0 ? lo : hi, idx = k & 0x07070707u;
-        const uint32_t fh = perm(c.t.hi[1], c.t.hi[0], idx) | (k << 4 & 0x80808080u);
-        const uint32_t fl = perm(c.t.lo[1], c.t.lo[0], idx);
-        const uint32_t p0 = perm(fh, fl, 0x05010400u), p1 = perm(fh, fl, 0x07030602u);
+        uint32_t p0, p1;
+        bytes_to_f16(c.t, w == 0 ? lo : hi, p0, p1);
         x[4 * w] = f16_to_f32(p0 & 0xffffu);
         x[4 * w + 1] = f16_to_f32(p0 >> 16);
         x[4 * w + 2] = f16_to_f32(p1 & 0xffffu);
@@ -488,6 +564,182 @@ EOS_DEV void read_run(const KvRowsArgs& a) {
     const size_t row = (size_t)(g.row + 8 * j + r);
     const size_t to = row * (is_v ? a.v_stride : a.k_stride) + (size_t)h * D + l8 * 8;
     store8((is_v ? a.v : a.k) + to * (a.dtype == kKvRowF32 ? 4 : 2), a.dtype, x);
+  }
+}
+
+// tq4 rows by the run, on the matrix cores: 4 wavefronts, 16 rows each, two of
+// K and two of V.
+template <int IO, int D>
+EOS_DEV void append_tq4(const KvRowsArgs& a, const KvRun& g, long long at0, long long at1, long long at2,
+                        long long at3, uint32_t* vw) {
+  constexpr int KS = D / 32, NT = D / 16, LANES = D / 8;
+  const KvCacheArgs& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, part = lane >> 4, h = blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool is_v = wave >= 2;
+  const int half = wave & 1, p = 16 * half + r16;
+  const long long base = r16 < 8 ? (half != 0 ? at2 : at0) : (half != 0 ? at3 : at1);
+  const bool live = base >= 0 && p >= g.from && p < g.upto;
+  v4u x[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) x[s] = v4u{0, 0, 0, 0};
+  if (live) {
+    const uint8_t* src = (is_v ? a.v : a.k) +
+                         ((size_t)(g.row + p) * (is_v ? a.v_stride : a.k_stride) + (size_t)h * D + part * 8) * 2;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) x[s] = *reinterpret_cast<const v4u*>(src + 64 * s);
+  }
+  double ss = 0.0;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    float f[8];
+    unpack8(x[s], IO, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += (double)f[i] * (double)f[i];
+  }
+  ss += __shfl_xor(ss, 16);
+  ss += __shfl_xor(ss, 32);
+  float scale = (float)__builtin_sqrt(ss * (1.0 / D));
+  const bool none = scale < kTiny;
+  const bool nan = !(scale <= kHuge);
+  const float norm = none || nan ? 0.0f : scale * (float)__builtin_sqrt((double)D);
+  scale = nan ? __builtin_nanf("") : none ? 0.0f : scale;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const uint32_t* sg = reinterpret_cast<const uint32_t*>(c.t.signs) + 32 * s + 8 * part;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      x[s][w] = none || nan ? 0u : x[s][w] ^ ((sg[2 * w] >> 16 & 0x8000u) | (sg[2 * w + 1] & 0x80000000u));
+  }
+  v4f y[NT];
+  rotate16<IO == kKvRowBf16 ? kKvBf16 : kKvF16, D>(x, y);
+  float e[7];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) e[i] = c.t.edges[i] * norm;
+  uint32_t word[KS];
+#pragma unroll
+  for (int w = 0; w < KS; ++w) {
+    word[w] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word[w] |= code_of(y[2 * w + i / 4][i & 3], e) << (4 * i);
+  }
+  if (live && part == 0) (is_v ? c.v_scale : c.k_scale)[base + r16 % 8] = scale;
+  if (!is_v) {
+    if (live) {
+      uint32_t* dst = reinterpret_cast<uint32_t*>(c.k) + (size_t)(base + r16 % 8) * LANES + part;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) dst[4 * w] = word[w];
+    }
+  } else {
+#pragma unroll
+    for (int w = 0; w < KS; ++w) vw[p * LANES + 4 * w + part] = word[w];
+  }
+}
+
+template <int D>
+EOS_DEV void append_tq4_run(const KvRowsArgs& a) {
+  constexpr int LANES = D / 8, NG = kKvRun / 8;
+  __shared__ __align__(16) uint32_t vw[kKvRun * LANES];
+  const KvCacheArgs& c = a.c;
+  KvRun g;
+  int b;
+  if (!find_run<kKvRun>(c, g, b)) return;
+  long long at[NG];
+  find_blocks<NG>(c, g, b, blockIdx.y, at);
+  if (a.dtype == kKvRowF16)
+    append_tq4<kKvRowF16, D>(a, g, at[0], at[1], at[2], at[3], vw);
+  else
+    append_tq4<kKvRowBf16, D>(a, g, at[0], at[1], at[2], at[3], vw);
+  __syncthreads();
+  // V: a group's 8 tokens of one dimension by one thread.
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    if (at[j] < 0) continue;
+    const int from = g.from > 8 * j ? g.from - 8 * j : 0;
+    const int upto = g.upto - 8 * j < 8 ? g.upto - 8 * j : 8;
+    // (D of the 256 threads, for the next group others)
+    for (int dim = (threadIdx.x + 256 - j * D % 256) % 256; dim < D; dim += 256) {
+      uint32_t* dst = reinterpret_cast<uint32_t*>(c.v) + (size_t)(at[j] / kKvGroup) * D + dim;
+      uint32_t word = 0, mask = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const bool in = t >= from && t < upto;
+        word |= in ? (vw[(j * 8 + t) * LANES + dim / 8] >> (4 * (dim & 7)) & 15u) << (4 * t) : 0u;
+        mask |= in ? 15u << (4 * t) : 0u;
+      }
+      *dst = mask == ~0u ? word : (*dst & ~mask) | word;
+    }
+  }
+}
+
+template <int D>
+EOS_DEV void read_tq4_run(const KvRowsArgs& a) {
+  constexpr int KS = D / 32, NT = D / 16, LANES = D / 8, NG = kKvRun / 8;
+  constexpr int VS = D + 16;  // bytes between V's rows in LDS: 8 rows on different banks
+  __shared__ __align__(16) uint8_t vb[kKvRun * VS];
+  const KvCacheArgs& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, part = lane >> 4, h = blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  KvRun g;
+  int b;
+  if (!find_run<kKvRun>(c, g, b)) return;
+  long long at[NG];
+  find_blocks<NG>(c, g, b, h, at);
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    if (at[j] < 0) continue;
+    for (int dim = (tid + 256 - j * D % 256) % 256; dim < D; dim += 256) {
+      const uint32_t u = reinterpret_cast<const uint32_t*>(c.v)[(size_t)(at[j] / kKvGroup) * D + dim];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) vb[(j * 8 + t) * VS + dim] = (uint8_t)(u >> (4 * t) & 15u);
+    }
+  }
+  const bool is_v = wave >= 2;
+  const int half = wave & 1, p = 16 * half + r16;
+  const long long base = r16 < 8 ? (half != 0 ? at[2] : at[0]) : (half != 0 ? at[3] : at[1]);
+  const bool live = base >= 0 && p >= g.from && p < g.upto;
+  uint32_t word[KS] = {};
+  float scale = 0.0f;
+  if (live) {
+    scale = (is_v ? c.v_scale : c.k_scale)[base + r16 % 8];
+    if (!is_v) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(c.k) + (size_t)(base + r16 % 8) * LANES + part;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) word[w] = src[4 * w];
+    }
+  }
+  __syncthreads();
+  v4u x[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    uint32_t lo, hi;
+    if (is_v) {
+      const v2u u = *reinterpret_cast<const v2u*>(&vb[p * VS + 32 * s + 8 * part]);
+      lo = live ? u[0] : 0u;
+      hi = live ? u[1] : 0u;
+    } else {
+      const uint32_t ev = word[s] & 0x0f0f0f0fu, od = word[s] >> 4 & 0x0f0f0f0fu;
+      lo = perm(od, ev, 0x05010400u);
+      hi = perm(od, ev, 0x07030602u);
+    }
+    uint32_t f[4];
+    bytes_to_f16(c.t, lo, f[0], f[1]);
+    bytes_to_f16(c.t, hi, f[2], f[3]);
+    x[s] = v4u{f[0], f[1], f[2], f[3]};
+  }
+  v4f y[NT];
+  rotate16<kKvF16, D>(x, y);
+  if (!live) return;
+  scale *= (float)(1.0 / __builtin_sqrt((double)D));
+  const float* sg = c.t.signs + 8 * part;
+  const size_t to = (size_t)(g.row + p) * (is_v ? a.v_stride : a.k_stride) + (size_t)h * D + 8 * part;
+  uint8_t* dst = (is_v ? a.v : a.k) + to * (a.dtype == kKvRowF32 ? 4 : 2);
+#pragma unroll
+  for (int w = 0; w < KS; ++w) {
+    float o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = y[2 * w + i / 4][i & 3] * (scale * sg[32 * w + i]);
+    store8(dst + 32 * w * (a.dtype == kKvRowF32 ? 4 : 2), a.dtype, o);
   }
 }
 
@@ -527,16 +779,6 @@ EOS_DEV void nibbles_to_f16(const KvTables& t, uint32_t x, uint32_t (&out)[4]) {
   out[1] = perm(eh, el, 0x07030602u);
   out[2] = perm(oh, ol, 0x05010400u);
   out[3] = perm(oh, ol, 0x07030602u);
-}
-
-template <int FMT>
-EOS_DEV v4f mfma16(v4u a, v4u b, v4f c) {
-  if constexpr (FMT == kKvBf16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a),
-                                                   __builtin_bit_cast(v8b, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
-                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
 template <int FMT>
@@ -1548,62 +1790,81 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
         l != 0.0f ? (ref + __log2f(l)) * 0.69314718056f : -__builtin_inff();
 }
 
-// Joins a row's splits: one workgroup a row and head, D / 8 lanes a split.
+// Joins a row's splits: one workgroup a row and head, D / 8 lanes a split. The
+// first splits' parts are loaded before it is known how many there are, so
+// that they do not wait for the sequence's numbers.
 template <int FMT, int D>
 EOS_DEV void attn_join(const KvAttnArgs& a) {
   constexpr int LANES = D / 8, NG = 256 / LANES;
-  __shared__ float so[NG][D];
-  __shared__ float sl[NG];
-  __shared__ float smax[4];
+  __shared__ __align__(16) float so[NG][D];
+  __shared__ float sl[NG], sm[NG];
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, l8 = tid % LANES, grp = tid / LANES;
-  const int head = blockIdx.y, h = head / a.group;
-  KvTile t;
-  long long within = 0, u;
-  if (c.offsets == nullptr) {
-    t.s = kv_seq(c, blockIdx.x);
-  } else if (!find_seq(c, blockIdx.x, 1, 1, 0, t.s, within)) {
-    return;
-  }
-  if (within < 0 || within >= t.s.n) return;
-  const int r = (int)within * a.group + head % a.group, rows = a.tile_rows;
-  kv_tile(t, r / rows, rows, a.group, a.window, a.splits);
-  u = (c.offsets == nullptr ? (long long)t.s.b * ((a.group + rows - 1) / rows)
-                            : kv_unit_base(c, t.s.b, a.group, rows, 1)) +
-      r / rows;
-  const size_t at = ((size_t)u * c.kv_heads + h) * a.splits * rows + r % rows;
-  float top = kLowest;
-  for (int i = tid; i < t.splits; i += 256) top = fmaxf(top, a.part_ml[(at + (size_t)i * rows) * 2]);
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
-  if ((tid & 63) == 0) smax[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
-  float x[8] = {}, l = 0.0f;
-  for (int i = grp; i < t.splits; i += NG) {
+  const int head = blockIdx.y, h = head / a.group, rows = a.tile_rows;
+  struct Part {
+    v4f lo, hi;
+    float m, l;
+  };
+  auto load = [&](size_t at, int i) KV_INLINE {
     const size_t p = at + (size_t)i * rows;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[p * 2] - top);
-    l += a.part_ml[p * 2 + 1] * f;
-    const v4f p0 = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[0];
-    const v4f p1 = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[1];
+    Part x;
+    x.lo = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[0];
+    x.hi = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[1];
+    x.m = a.part_ml[p * 2];
+    x.l = a.part_ml[p * 2 + 1];
+    return x;
+  };
+  KvTile t;
+  size_t at;
+  int r;
+  Part first = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}, kLowest, 0.0f};
+  if (c.offsets == nullptr) {
+    r = head % a.group;
+    at = (((size_t)blockIdx.x * ((a.group + rows - 1) / rows) + r / rows) * c.kv_heads + h) * a.splits * rows + r % rows;
+    if (grp < a.splits) first = load(at, grp);
+    t.s = kv_seq(c, blockIdx.x);
+  } else {
+    long long within = 0;
+    if (!find_seq(c, blockIdx.x, 1, 1, 0, t.s, within)) return;
+    if (within < 0 || within >= t.s.n) return;
+    r = (int)within * a.group + head % a.group;
+    const long long u = kv_unit_base(c, t.s.b, a.group, rows, 1) + r / rows;
+    at = ((size_t)u * c.kv_heads + h) * a.splits * rows + r % rows;
+    if (grp < a.splits) first = load(at, grp);
+  }
+  kv_tile(t, r / rows, rows, a.group, a.window, a.splits);
+  // This lane group's splits, with the running reference of attn_split.
+  float x[8] = {}, m = kLowest, l = 0.0f;
+  for (int i = grp; i < t.splits; i += NG) {
+    const Part p = i == grp ? first : load(at, i);
+    const float nm = fmaxf(m, p.m), fo = __builtin_amdgcn_exp2f(m - nm), fn = __builtin_amdgcn_exp2f(p.m - nm);
+    m = nm;
+    l = l * fo + p.l * fn;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      x[k] += p0[k] * f;
-      x[4 + k] += p1[k] * f;
+      x[k] = x[k] * fo + p.lo[k] * fn;
+      x[4 + k] = x[4 + k] * fo + p.hi[k] * fn;
     }
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) so[grp][l8 * 8 + k] = x[k];
-  if (l8 == 0) sl[grp] = l;
+  if (l8 == 0) {
+    sl[grp] = l;
+    sm[grp] = m;
+  }
   __syncthreads();
   if (tid >= LANES) return;
+  const int used = kv_min(t.splits, NG);
+  float top = kLowest;
+  for (int i = 0; i < used; ++i) top = fmaxf(top, sm[i]);
   l = 0.0f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-  for (int i = 0; i < NG; ++i) {
-    l += sl[i];
+  for (int i = 0; i < used; ++i) {
+    const float f = __builtin_amdgcn_exp2f(sm[i] - top);
+    l += sl[i] * f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] += so[i][l8 * 8 + k];
+    for (int k = 0; k < 8; ++k) x[k] += so[i][l8 * 8 + k] * f;
   }
   finish_row<FMT, D>(a, t.s, r, h, l8, true, x, top, l);
 }
@@ -1611,14 +1872,22 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
 }  // namespace
 
 #define KV_KERNELS(NAME, FMT, D)                                                             \
-  extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_append_##NAME##_##D(KvRowsArgs a) { \
-    append_run<FMT, D, kKvRun>(a);                                                           \
+  extern "C" __global__ __launch_bounds__(FMT == kKvTq4 ? 256 : 2 * D, D == 256 ? 2 : 4) void eos_kv_append_##NAME##_##D( \
+      KvRowsArgs a) {                                                                        \
+    if constexpr (FMT == kKvTq4)                                                             \
+      append_tq4_run<D>(a);                                                                  \
+    else                                                                                     \
+      append_run<FMT, D, kKvRun>(a);                                                         \
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_append1_##NAME##_##D(KvRowsArgs a) { \
     append_run<FMT, D, kKvGroup>(a);                                                         \
   }                                                                                          \
-  extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_read_##NAME##_##D(KvRowsArgs a) {   \
-    read_run<FMT, D, kKvRun>(a);                                                             \
+  extern "C" __global__ __launch_bounds__(FMT == kKvTq4 ? 256 : 2 * D) void eos_kv_read_##NAME##_##D( \
+      KvRowsArgs a) {                                                                        \
+    if constexpr (FMT == kKvTq4)                                                             \
+      read_tq4_run<D>(a);                                                                    \
+    else                                                                                     \
+      read_run<FMT, D, kKvRun>(a);                                                           \
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(2 * D) void eos_kv_read1_##NAME##_##D(KvRowsArgs a) {  \
     read_run<FMT, D, kKvGroup>(a);                                                           \
