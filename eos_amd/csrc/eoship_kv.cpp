@@ -372,8 +372,31 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
   long long keys = (long long)batch->table_stride << kv->page_shift;
   if (window > 0) keys = std::min(keys, (long long)window + batch->rows + 32);
   const long long units = a.tiles * kvh;
-  const long long want = 2LL * rt->compute_units / units;
+  const long long slots = 2LL * rt->compute_units;
+#ifdef X_CEIL
+  const long long want = prompt ? (slots + units - 1) / units : slots / units;
+#else
+  const long long want = slots / units;
+#endif
   a.splits = (int)std::max(1LL, std::min(want, (keys + 255) / 256));
+  // Several sequences with room for enough keys: equal shares of all of them
+  // instead, whatever the lengths. 64 sequences of 1,024 to 16,384 tokens in
+  // tq4: 164 us, in splits 230; of 2,000 tokens each 46 and 39; 32 of 64 to
+  // 4,096 in bf16: 66 and 79. Many workgroups balance by themselves (256
+  // sequences of 1,000: 206 in shares, 185 in splits), few keys do not pay for
+  // the prefix sum (4 of up to 3,000: 21 and 16).
+  const long long steps = ((long long)batch->table_stride << kv->page_shift) / 128;
+  if (batch->d_offsets == nullptr && batch->batch > 1 && batch->batch <= kKvStreamBatch &&
+      units < 4 * slots && steps * units >= 4 * slots) {
+    a.workgroups = (int)slots;
+    const size_t parts = (size_t)a.workgroups * 2 * kKvTileRows;
+    void* ws = nullptr;
+    if (rt->workspace(parts * (size_t)(d + 2) * 4, &ws, err) != 0) return 1;
+    a.part = static_cast<float*>(ws);
+    a.part_ml = a.part + parts * (size_t)d;
+    if (launch(rt, kv, "stream", a.workgroups, 1, 256, &a, what, err) != 0) return 1;
+    return launch(rt, kv, "stream_join", batch->batch, heads, 256, &a, what, err);
+  }
   if (a.splits > 1) {
     const size_t parts = (size_t)units * a.splits * a.tile_rows;
     void* ws = nullptr;

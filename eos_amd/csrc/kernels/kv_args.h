@@ -9,6 +9,8 @@
 enum { kKvF16 = 0, kKvBf16 = 1, kKvQ8 = 2, kKvTq4 = 3 };
 enum { kKvRowF16 = 0, kKvRowBf16 = 1, kKvRowF32 = 2 };
 
+constexpr int kKvStreamBatch = 1024;  // sequences whose steps a workgroup keeps in LDS
+
 // Status bits a kernel sets when what it read from the device was out of
 // range (nothing outside the pool and the rows is touched).
 enum { kKvBadPage = 1, kKvBadLength = 2, kKvBadOffset = 4 };
@@ -52,10 +54,11 @@ struct KvAttnArgs {
   float* lse;       // [rows][heads] or NULL
   float* part;      // [tiles][kv_heads][splits][tile_rows][head_dim] unnormalised sums
   float* part_ml;   // [tiles][kv_heads][splits][tile_rows][2] reference and weight sum
+                    // (stream kernels: both [workgroups][2][16]...)
   long long q_stride, out_stride;
   float scale;      // of q . k, times log2(e)
   long long tiles;
-  int heads, group, window, splits, dtype, tile_rows;
+  int heads, group, window, splits, dtype, tile_rows, workgroups;
 };
 
 #endif

@@ -145,4 +145,38 @@ KV_HD bool kv_tile(KvTile& t, long long within, int tile_rows, int group, int wi
   return true;
 }
 
+// The stream kernels' order of work, one row a sequence: head by head, in it
+// sequence by sequence, in it 16-row tile by tile, in it 128-key step by step.
+// Every workgroup takes `share` consecutive steps, so that long and short
+// sequences keep all of them busy alike.
+KV_HD int kv_steps(const KvCacheArgs& c, int b, int group, int window) {
+  KvTile t;
+  t.s = kv_seq(c, b);
+  if (!kv_tile(t, 0, kKvTileRows, group, window, 1)) return 0;
+  return (t.hi - t.base + 127) / 128;
+}
+KV_HD long long kv_share(long long steps, int workgroups) {
+  const long long q = (steps + workgroups - 1) / workgroups;
+  return q < 2 ? 2 : q;
+}
+// The step at `pos` of a head whose sequence b has `steps` of them a tile from
+// `first` on: the tile, and the steps [from, upto) of it that end at `end`.
+struct KvSegment {
+  int tile = 0, from = 0, upto = 0;
+};
+KV_HD KvSegment kv_segment(long long pos, long long end, long long first, int steps) {
+  KvSegment g;
+  const long long in = pos - first;
+  g.tile = (int)(in / steps);
+  g.from = (int)(in % steps);
+  const long long left = end - pos;
+  g.upto = left < steps - g.from ? g.from + (int)left : steps;
+  return g;
+}
+// Where a workgroup that starts at step `start` leaves the part of a tile that
+// begins at step `tile`: its first segment's place or its last one's.
+KV_HD long long kv_part(long long workgroup, long long start, long long tile) {
+  return (workgroup * 2 + (tile > start ? 1 : 0)) * kKvTileRows;
+}
+
 #endif

@@ -864,14 +864,16 @@ EOS_DEV void finish_row(const KvAttnArgs& a, const KvSeq& s, int r, int h, int l
         l != 0.0f ? (m + __log2f(l)) * 0.69314718056f : -__builtin_inff();
 }
 
-// One workgroup: 16 query rows of a head group against one split of their
-// keys, 32 keys a wavefront and step. Scores are computed as K q^T and the
+// One workgroup: 16 query rows of a head group against keys [begin, end) of
+// theirs, 32 keys a wavefront and step. Scores are computed as K q^T and the
 // outputs as V^T p^T, so a lane's 8 scores (keys 8 g .. 8 g + 7 of the step, g
 // = lane / 16, query lane % 16) are the 8 consecutive summands that its
 // operand of the second product holds: nothing crosses lanes between the two.
 // K's rows are taken in the order 8 (r / 4) + 4 j + r % 4 for that.
+// The whole of the rows' keys goes to the output, else the sums go to place
+// `at` of the parts.
 template <int FMT, int D>
-EOS_DEV void attn_split(const KvAttnArgs& a) {
+EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int end, bool whole, size_t at) {
   constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
   constexpr int BITS = bits_of(FMT), KS = D / 32, NT = D / 16, LANES = D / 8;
   // Dimensions of V in one load of a lane, loads a step, words of a load.
@@ -884,11 +886,10 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.x % a.splits, h = blockIdx.y;
-  const long long u = blockIdx.x / a.splits;
-  KvTile t;
-  if (!find_tile<kKvTileRows>(a, u, t)) return;
   // The same in every lane, as the compiler cannot see.
+  h = __builtin_amdgcn_readfirstlane(h);
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  end = __builtin_amdgcn_readfirstlane(end);
   t.s.b = __builtin_amdgcn_readfirstlane(t.s.b);
   t.s.n = __builtin_amdgcn_readfirstlane(t.s.n);
   t.s.len = __builtin_amdgcn_readfirstlane(t.s.len);
@@ -898,10 +899,6 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
   t.hi = __builtin_amdgcn_readfirstlane(t.hi);
   t.all_lo = __builtin_amdgcn_readfirstlane(t.all_lo);
   t.all_hi = __builtin_amdgcn_readfirstlane(t.all_hi);
-  t.base = __builtin_amdgcn_readfirstlane(t.base);
-  t.chunk = __builtin_amdgcn_readfirstlane(t.chunk);
-  t.splits = __builtin_amdgcn_readfirstlane(t.splits);
-  if (split >= t.splits && (split > 0 || a.splits > 1)) return;
   const int P = 1 << c.page_shift;
   const int rr = t.r0 + r16;
   const bool real = rr < t.s.n * a.group;
@@ -974,7 +971,6 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
   // of V, so that probability times scale stays below 2^8 in f16. Both move
   // only when a score passes m + 8 or a scale 2^e.
   float m = kLowest, l = 0.0f, e = kQuant ? -100.0f : 0.0f, elim = 0x1p-100f;
-  const int end = kv_min(t.hi, t.base + (split + 1) * t.chunk);
   const size_t head_bytes = ((size_t)D * BITS / 8) << c.page_shift;
   bool odd_seen = false;  // a value of V that is NaN or infinite in a masked step
   // A step's codes and scales as loaded: the next step's are on their way
@@ -1150,7 +1146,7 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
   };
   // (from 1024 bits of width on there are no registers for a second step)
   constexpr bool kAhead = D * BITS <= 1024;
-  const int first = t.base + split * t.chunk + 32 * wave;
+  const int first = begin + 32 * wave;
   Raw ra, rb;
   if (first < end) {
     ids(first);
@@ -1232,17 +1228,96 @@ EOS_DEV void attn_split(const KvAttnArgs& a) {
       o[i] = so[0][at] + so[1][at] + so[2][at] + so[3][at];
     }
     const bool live = t.r0 + r < t.s.n * a.group;
-    if (a.splits == 1) {
+    if (whole) {
       finish_row<FMT, D>(a, t.s, t.r0 + r, h, l8, live, o, mt, lt);
     } else if (live) {
-      const size_t at = (((size_t)u * c.kv_heads + h) * a.splits + split) * 16 + r;
-      reinterpret_cast<v4f*>(a.part + at * D + l8 * 8)[0] = v4f{o[0], o[1], o[2], o[3]};
-      reinterpret_cast<v4f*>(a.part + at * D + l8 * 8)[1] = v4f{o[4], o[5], o[6], o[7]};
+      reinterpret_cast<v4f*>(a.part + (at + r) * D + l8 * 8)[0] = v4f{o[0], o[1], o[2], o[3]};
+      reinterpret_cast<v4f*>(a.part + (at + r) * D + l8 * 8)[1] = v4f{o[4], o[5], o[6], o[7]};
       if (l8 == 0) {
-        a.part_ml[at * 2] = mt;
-        a.part_ml[at * 2 + 1] = lt;
+        a.part_ml[(at + r) * 2] = mt;
+        a.part_ml[(at + r) * 2 + 1] = lt;
       }
     }
+  }
+}
+
+// One split of one tile.
+template <int FMT, int D>
+EOS_DEV void attn_split(const KvAttnArgs& a) {
+  const int split = blockIdx.x % a.splits, h = blockIdx.y;
+  const long long u = blockIdx.x / a.splits;
+  KvTile t;
+  if (!find_tile<kKvTileRows>(a, u, t)) return;
+  if (split >= t.splits && (split > 0 || a.splits > 1)) return;
+  attn_segment<FMT, D>(a, t, h, t.base + split * t.chunk, kv_min(t.hi, t.base + (split + 1) * t.chunk),
+                       a.splits == 1, (((size_t)u * a.c.kv_heads + h) * a.splits + split) * kKvTileRows);
+}
+
+// Steps of the sequences before each one, of a head: pre[b], and of all:
+// pre[batch]. 256 threads, each with neighbouring sequences.
+EOS_DEV void stream_steps(const KvAttnArgs& a, long long* pre) {
+  __shared__ long long part[4];
+  const KvCacheArgs& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, per = (c.batch + 255) / 256;
+  const int tiles = (a.group + kKvTileRows - 1) / kKvTileRows;
+  long long sum = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b < c.batch) {
+      const int n = kv_steps(c, b, a.group, a.window) * tiles;
+      pre[b] = n;
+      sum += n;
+    }
+  }
+  long long upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const long long x = __shfl_up(upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 63) part[tid >> 6] = upto;
+  __syncthreads();
+  long long at = upto - sum;
+  for (int w = 0; w < tid >> 6; ++w) at += part[w];
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b < c.batch) {
+      const long long n = pre[b];
+      pre[b] = at;
+      at += n;
+    }
+  }
+  if (tid == 0) pre[c.batch] = part[0] + part[1] + part[2] + part[3];
+  __syncthreads();
+}
+
+// One row a sequence, any lengths: equal shares of all steps (see kv_index.h).
+template <int FMT, int D>
+EOS_DEV void attn_stream(const KvAttnArgs& a) {
+  __shared__ long long pre[kKvStreamBatch + 1];
+  const KvCacheArgs& c = a.c;
+  stream_steps(a, pre);
+  const int tiles = (a.group + kKvTileRows - 1) / kKvTileRows;
+  const long long total = pre[c.batch], all = total * c.kv_heads;
+  const long long share = kv_share(all, a.workgroups), start = share * blockIdx.x;
+  const long long end = start + share < all ? start + share : all;
+  for (long long pos = start; pos < end;) {
+    const int h = (int)(pos / total);
+    const long long rel = pos - h * total;
+    int b = 0;  // the last sequence that starts at or before rel
+    for (int o = kKvStreamBatch; o > 0; o /= 2)
+      if (b + o < c.batch && pre[b + o] <= rel) b += o;
+    const int steps = (int)((pre[b + 1] - pre[b]) / tiles);
+    const KvSegment g = kv_segment(rel, rel + (end - pos), pre[b], steps);
+    KvTile t;
+    t.s = kv_seq(c, b);
+    flag(c, t.s.bad);
+    kv_tile(t, g.tile, kKvTileRows, a.group, a.window, 1);
+    attn_segment<FMT, D>(a, t, h, t.base + 128 * g.from, kv_min(t.hi, t.base + 128 * g.upto),
+                         g.from == 0 && g.upto == steps,
+                         kv_part(blockIdx.x, start, pos - g.from));
+    pos += g.upto - g.from;
+    __syncthreads();
   }
 }
 
@@ -1790,53 +1865,34 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
         l != 0.0f ? (ref + __log2f(l)) * 0.69314718056f : -__builtin_inff();
 }
 
-// Joins a row's splits: one workgroup a row and head, D / 8 lanes a split. The
-// first splits' parts are loaded before it is known how many there are, so
-// that they do not wait for the sequence's numbers.
-template <int FMT, int D>
-EOS_DEV void attn_join(const KvAttnArgs& a) {
+// One split's part of a row, D / 8 lanes.
+struct Part {
+  v4f lo, hi;
+  float m, l;
+};
+template <int D>
+EOS_DEV Part load_part(const KvAttnArgs& a, size_t p) {
+  const int l8 = threadIdx.x % (D / 8);
+  Part x;
+  x.lo = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[0];
+  x.hi = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[1];
+  x.m = a.part_ml[p * 2];
+  x.l = a.part_ml[p * 2 + 1];
+  return x;
+}
+
+// A row from its n parts, part(i) loading the i-th and `first` holding a lane
+// group's first one: each lane group its own parts with a running reference
+// as in attn_segment, then the groups.
+template <int FMT, int D, class F>
+EOS_DEV void join_parts(const KvAttnArgs& a, const KvSeq& s, int r, int h, int n, Part first, F part) {
   constexpr int LANES = D / 8, NG = 256 / LANES;
   __shared__ __align__(16) float so[NG][D];
   __shared__ float sl[NG], sm[NG];
-  const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, l8 = tid % LANES, grp = tid / LANES;
-  const int head = blockIdx.y, h = head / a.group, rows = a.tile_rows;
-  struct Part {
-    v4f lo, hi;
-    float m, l;
-  };
-  auto load = [&](size_t at, int i) KV_INLINE {
-    const size_t p = at + (size_t)i * rows;
-    Part x;
-    x.lo = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[0];
-    x.hi = reinterpret_cast<const v4f*>(a.part + p * D + l8 * 8)[1];
-    x.m = a.part_ml[p * 2];
-    x.l = a.part_ml[p * 2 + 1];
-    return x;
-  };
-  KvTile t;
-  size_t at;
-  int r;
-  Part first = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}, kLowest, 0.0f};
-  if (c.offsets == nullptr) {
-    r = head % a.group;
-    at = (((size_t)blockIdx.x * ((a.group + rows - 1) / rows) + r / rows) * c.kv_heads + h) * a.splits * rows + r % rows;
-    if (grp < a.splits) first = load(at, grp);
-    t.s = kv_seq(c, blockIdx.x);
-  } else {
-    long long within = 0;
-    if (!find_seq(c, blockIdx.x, 1, 1, 0, t.s, within)) return;
-    if (within < 0 || within >= t.s.n) return;
-    r = (int)within * a.group + head % a.group;
-    const long long u = kv_unit_base(c, t.s.b, a.group, rows, 1) + r / rows;
-    at = ((size_t)u * c.kv_heads + h) * a.splits * rows + r % rows;
-    if (grp < a.splits) first = load(at, grp);
-  }
-  kv_tile(t, r / rows, rows, a.group, a.window, a.splits);
-  // This lane group's splits, with the running reference of attn_split.
   float x[8] = {}, m = kLowest, l = 0.0f;
-  for (int i = grp; i < t.splits; i += NG) {
-    const Part p = i == grp ? first : load(at, i);
+  for (int i = grp; i < n; i += NG) {
+    const Part p = i == grp ? first : part(i);
     const float nm = fmaxf(m, p.m), fo = __builtin_amdgcn_exp2f(m - nm), fn = __builtin_amdgcn_exp2f(p.m - nm);
     m = nm;
     l = l * fo + p.l * fn;
@@ -1854,7 +1910,7 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
   }
   __syncthreads();
   if (tid >= LANES) return;
-  const int used = kv_min(t.splits, NG);
+  const int used = kv_min(n, NG);
   float top = kLowest;
   for (int i = 0; i < used; ++i) top = fmaxf(top, sm[i]);
   l = 0.0f;
@@ -1866,7 +1922,62 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] += so[i][l8 * 8 + k] * f;
   }
-  finish_row<FMT, D>(a, t.s, r, h, l8, true, x, top, l);
+  finish_row<FMT, D>(a, s, r, h, l8, true, x, top, l);
+}
+
+// Joins a row's splits: one workgroup a row and head, D / 8 lanes a split. The
+// first splits' parts are loaded before it is known how many there are, so
+// that they do not wait for the sequence's numbers.
+template <int FMT, int D>
+EOS_DEV void attn_join(const KvAttnArgs& a) {
+  const KvCacheArgs& c = a.c;
+  const int grp = threadIdx.x / (D / 8), head = blockIdx.y, h = head / a.group, rows = a.tile_rows;
+  KvTile t;
+  size_t at;
+  int r;
+  Part first = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}, kLowest, 0.0f};
+  if (c.offsets == nullptr) {
+    r = head % a.group;
+    at = (((size_t)blockIdx.x * ((a.group + rows - 1) / rows) + r / rows) * c.kv_heads + h) * a.splits * rows + r % rows;
+    if (grp < a.splits) first = load_part<D>(a, at + (size_t)grp * rows);
+    t.s = kv_seq(c, blockIdx.x);
+  } else {
+    long long within = 0;
+    if (!find_seq(c, blockIdx.x, 1, 1, 0, t.s, within)) return;
+    if (within < 0 || within >= t.s.n) return;
+    r = (int)within * a.group + head % a.group;
+    const long long u = kv_unit_base(c, t.s.b, a.group, rows, 1) + r / rows;
+    at = ((size_t)u * c.kv_heads + h) * a.splits * rows + r % rows;
+    if (grp < a.splits) first = load_part<D>(a, at + (size_t)grp * rows);
+  }
+  kv_tile(t, r / rows, rows, a.group, a.window, a.splits);
+  join_parts<FMT, D>(a, t.s, r, h, t.splits, first,
+                     [&](int i) KV_INLINE { return load_part<D>(a, at + (size_t)i * rows); });
+}
+
+// Joins what the stream's workgroups left of a row, where more than one had
+// it, and writes the rows that have no key.
+template <int FMT, int D>
+EOS_DEV void attn_stream_join(const KvAttnArgs& a) {
+  __shared__ long long pre[kKvStreamBatch + 1];
+  const KvCacheArgs& c = a.c;
+  const int grp = threadIdx.x / (D / 8), b = blockIdx.x, head = blockIdx.y, h = head / a.group;
+  const int tiles = (a.group + kKvTileRows - 1) / kKvTileRows, r = head % a.group;
+  const KvSeq s = kv_seq(c, b);
+  flag(c, s.bad);
+  stream_steps(a, pre);
+  const long long total = pre[c.batch], share = kv_share(total * c.kv_heads, a.workgroups);
+  const int steps = (int)((pre[b + 1] - pre[b]) / tiles);
+  const long long tile = h * total + pre[b] + (long long)(r / kKvTileRows) * steps;
+  const long long w0 = tile / share, w1 = steps > 0 ? (tile + steps - 1) / share : w0 - 1;
+  if (w0 == w1) return;
+  auto part = [&](int i) KV_INLINE {
+    return load_part<D>(a, (size_t)kv_part(w0 + i, (w0 + i) * share, tile) + r % kKvTileRows);
+  };
+  const int n = (int)(w1 - w0 + 1);
+  Part first = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}, kLowest, 0.0f};
+  if (grp < n) first = part(grp);
+  join_parts<FMT, D>(a, s, r, h, n, first, part);
 }
 
 }  // namespace
@@ -1898,6 +2009,13 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
   extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void eos_kv_prompt_##NAME##_##D(  \
       KvAttnArgs a) {                                                                        \
     attn_prompt<FMT, D>(a);                                                               \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(256, D * bits_of(FMT) > 2048 ? 1 : 2) void eos_kv_stream_##NAME##_##D( \
+      KvAttnArgs a) {                                                                        \
+    attn_stream<FMT, D>(a);                                                                  \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void eos_kv_stream_join_##NAME##_##D(KvAttnArgs a) { \
+    attn_stream_join<FMT, D>(a);                                                             \
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(256) void eos_kv_join_##NAME##_##D(KvAttnArgs a) {     \
     attn_join<FMT, D>(a);                                                                    \

@@ -104,6 +104,57 @@ void one(int at, bool sound) {
       for (int i = 0; i < n; ++i) CHECK(seen[lo + i] == (lengths[b] - n + i >= 0 ? 1 : 0));
     }
 
+  // the stream's shares: every step of every tile of every head once, and the
+  // parts that a join looks for are those that were written
+  if (one_each) {
+    const int group = between(1, 40), window = between(0, 1) ? 0 : between(1, cap + 3);
+    const int heads = between(1, 5), workgroups = between(1, 30);
+    const int tiles = (group + kKvTileRows - 1) / kKvTileRows;
+    std::vector<long long> pre(c.batch + 1, 0);
+    for (int b = 0; b < c.batch; ++b) pre[b + 1] = pre[b] + (long long)kv_steps(c, b, group, window) * tiles;
+    const long long total = pre[c.batch], all = total * heads, share = kv_share(all, workgroups);
+    std::vector<int> done(all, 0);
+    std::vector<long long> left(workgroups * 2 * kKvTileRows, -1);  // the tile whose part lies there
+    for (int w = 0; w < workgroups; ++w) {
+      const long long start = w * share, end = start + share < all ? start + share : all;
+      for (long long pos = start; pos < end;) {
+        const int h = (int)(pos / total);
+        const long long rel = pos - h * total;
+        int b = 0;
+        for (int o = kKvStreamBatch; o > 0; o /= 2)
+          if (b + o < c.batch && pre[b + o] <= rel) b += o;
+        const int steps = (int)((pre[b + 1] - pre[b]) / tiles);
+        CHECK(steps > 0 && rel >= pre[b] && rel < pre[b + 1]);
+        const KvSegment g = kv_segment(rel, rel + (end - pos), pre[b], steps);
+        KvTile t;
+        t.s = kv_seq(c, b);
+        CHECK(kv_tile(t, g.tile, kKvTileRows, group, window, 1));
+        CHECK(g.from < g.upto && g.upto <= steps && t.base + 128 * g.from < t.hi);
+        CHECK(t.base + 128 * steps >= t.hi);
+        for (int i = g.from; i < g.upto; ++i) ++done[pos - g.from + i];
+        if (!(g.from == 0 && g.upto == steps)) {
+          const long long at_part = kv_part(w, start, pos - g.from);
+          CHECK(at_part >= 0 && at_part + kKvTileRows <= (long long)left.size() && left[at_part] == -1);
+          left[at_part] = pos - g.from;
+        }
+        pos += g.upto - g.from;
+      }
+    }
+    CHECK(all <= share * workgroups);
+    for (int n : done) CHECK(n == 1);
+    for (int h = 0; h < heads; ++h)
+      for (int b = 0; b < c.batch; ++b)
+        for (int tile = 0; tile < tiles; ++tile) {
+          const int steps = (int)((pre[b + 1] - pre[b]) / tiles);
+          const long long first = h * total + pre[b] + (long long)tile * steps;
+          const long long w0 = first / share, w1 = steps > 0 ? (first + steps - 1) / share : w0 - 1;
+          if (w0 < w1)
+            for (long long w = w0; w <= w1; ++w) {
+              CHECK(w < workgroups && left[kv_part(w, w * share, first)] == first);
+            }
+        }
+  }
+
   // attention
   for (int tile_rows : {16, 64, 128}) {
     const int group = between(1, 20), window = between(0, 1) ? 0 : between(1, cap + 3);

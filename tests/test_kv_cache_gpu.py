@@ -272,6 +272,30 @@ def test_single_token_split_over_the_length(rt, fmt, length, stride):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("d,kvh,group,p,window", [(32, 2, 3, 16, 0), (64, 3, 1, 32, 0),
+                                                  (128, 2, 4, 64, 700), (128, 1, 35, 16, 0),
+                                                  (256, 1, 7, 128, 0)])
+def test_single_token_rows_of_many_lengths(rt, fmt, d, kvh, group, p, window):
+    """A wide page table: the workgroups take equal shares of all keys, which
+    begin and end inside sequences."""
+    _case(f"decode shares {fmt} d={d} kvh={kvh} group={group} p={p} window={window}")
+    lengths = np.array([0, 3000, 1, 129, 0, 4096, 2, 511, 128, 1500, 0])
+    w = World(rt, fmt, kvh, d, p, lengths, np.ones_like(lengths), seed=d + group, stride=200000 // p)
+    w.fill()
+    _check(w, kvh * group, _io(fmt, group), window=window, pad=8)
+
+
+@pytest.mark.parametrize("batch", [2, 300, 1024, 1025])
+def test_single_token_rows_of_many_sequences(rt, batch):
+    _case(f"decode batch {batch}")
+    lengths = np.random.default_rng(batch).integers(0, 40, batch)
+    lengths[-1] = 300
+    w = World(rt, "q8", 1, 32, 16, lengths, np.ones_like(lengths), seed=batch, stride=40000 // batch)
+    w.fill()
+    _check(w, 2, "f16")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("d,kvh,group,p,window", [(64, 2, 1, 16, 0), (128, 1, 5, 32, 0),
                                                   (32, 1, 16, 16, 19), (256, 1, 3, 64, 70),
                                                   (128, 2, 4, 16, 1)])
@@ -491,6 +515,28 @@ def test_out_of_range_is_reported_and_masked(rt):
                 assert touched <= {int(plan.table[b, 2]) for b in range(3)} - {-1}
             for name, b in w.dev.items():
                 b.upload(before[name])
+
+
+def test_out_of_range_single_tokens(rt):
+    """The same for one row a sequence, with and without equal shares."""
+    _case("bad batches, single tokens")
+    for stride in (3, 20000):
+        lengths = np.array([40, 40, 40])
+        w = World(rt, "q8", 1, 64, 16, lengths, np.ones(3, int), seed=2, stride=stride)
+        w.fill()
+        q = w.rng.normal(size=(3, 2, 64)).astype(np.float32)
+        clean = _attend(w, 2, "f16", q=q)[1]
+        for what, bit in (("page", 1), ("length", 2), ("negative length", 2)):
+            plan = ref.Plan(w.pool, lengths, np.ones(3, int), 2, stride=stride)
+            if what == "page":
+                plan.table[1, 1] = w.pool.pages
+            else:
+                plan.lengths[1] = 10 ** 9 if what == "length" else -3
+            got = _attend(w, 2, "f16", q=q, plan=plan, batch=w.on_device(plan))[1]
+            assert w.cache.status() & bit, (stride, what)
+            np.testing.assert_array_equal(got[[0, 2]], clean[[0, 2]])
+            if what == "negative length":
+                assert (got[1] == 0).all()
 
 
 def test_call_refusals(rt):
