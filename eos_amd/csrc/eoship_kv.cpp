@@ -29,10 +29,17 @@ struct EosHipKVCache {
 
 namespace {
 
-#ifndef X_FROM
-#define X_FROM 48
-#endif
-constexpr int kPromptFrom = X_FROM;
+// Query rows a sequence (heads of a group counted) from which the prompt
+// kernel takes a call, for 16-bit and for quantized caches. Below, 16 rows at
+// a time, each wavefront with keys of its own, are faster: the prompt kernel's
+// stage has a latency of its own, and quantized stages are expanded by few
+// wavefronts. 8 sequences behind 8,000 keys, heads 32 to 8 of 128, us (16 rows
+// / 128 rows at a time): bf16 2 rows each 65 / 59, 8 rows 116 / 66; q8 8 rows
+// 65 / 96, 16 rows 107 / 119, 32 rows behind 2,000 58 / 56, 128 rows 124 / 104.
+constexpr int kPromptFrom = 8, kPromptFromQuantized = 96;
+// ... and not while the 16-row workgroups are on the CUs at once over so few
+// keys (4 prompts of 256, 8 heads of 64: 10 / 17).
+constexpr int kPromptKeys = 1024;
 
 const char* const kFormats[] = {"f16", "bf16", "q8", "tq4"};
 
@@ -357,27 +364,25 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
   a.window = window;
   a.dtype = dtype;
   const int kvh = kv->d.kv_heads, d = kv->d.head_dim;
-  // Rows of a sequence on average, a group's heads counted: a few go 16 at a
-  // time, each wavefront with keys of its own, many 128 at a time.
-  const bool prompt = batch->d_offsets != nullptr &&
-                      batch->rows * a.group > (int64_t)kPromptFrom * batch->batch;
-  a.tile_rows = prompt ? kKvPromptRows : kKvTileRows;
-  a.tiles = batch->d_offsets == nullptr
-                ? (long long)batch->batch * ((a.group + kKvTileRows - 1) / kKvTileRows)
-                : kv_units(batch->rows, batch->batch, a.group, a.tile_rows, 1);
-  // Splits while all workgroups are on the CUs at once (two each, by their
-  // registers), none below 256 keys: further ones cost more in prologues and
-  // joining than their balance gains (64 x 2,000 tokens of tq4: 39 us at two
-  // workgroups a CU, 53 at four, 68 at eight).
+  const long long slots = 2LL * rt->compute_units;  // two workgroups a CU, by their registers
   long long keys = (long long)batch->table_stride << kv->page_shift;
   if (window > 0) keys = std::min(keys, (long long)window + batch->rows + 32);
+  const auto tiles = [&](int rows) {
+    return batch->d_offsets == nullptr ? (long long)batch->batch * ((a.group + rows - 1) / rows)
+                                       : kv_units(batch->rows, batch->batch, a.group, rows, 1);
+  };
+  const int64_t from = kv->d.format >= kKvQ8 ? kPromptFromQuantized : kPromptFrom;
+  const bool prompt = batch->d_offsets != nullptr && batch->rows * a.group >= from * batch->batch &&
+                      (tiles(kKvTileRows) * kvh > slots || keys > kPromptKeys);
+  a.tile_rows = prompt ? kKvPromptRows : kKvTileRows;
+  a.tiles = tiles(a.tile_rows);
+  // Splits while the workgroups are on the CUs at once, none below 256 keys:
+  // further ones cost more in prologues and joining than their balance gains
+  // (64 x 2,000 tokens of tq4: 39 us at two workgroups a CU, 53 at four, 68 at
+  // eight). Prompts, whose joins are few, fill the last slots too (8 x 128 rows
+  // behind 2,000 keys in q8: 104 us, 156 without).
   const long long units = a.tiles * kvh;
-  const long long slots = 2LL * rt->compute_units;
-#ifdef X_CEIL
   const long long want = prompt ? (slots + units - 1) / units : slots / units;
-#else
-  const long long want = slots / units;
-#endif
   a.splits = (int)std::max(1LL, std::min(want, (keys + 255) / 256));
   // Several sequences with room for enough keys: equal shares of all of them
   // instead, whatever the lengths. 64 sequences of 1,024 to 16,384 tokens in
@@ -409,6 +414,10 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
              : launch(rt, kv, "split", items, kvh, 256, &a, what, err) != 0)
     return 1;
   if (a.splits == 1) return 0;
+  if (a.splits <= kKvFewSplits) {
+    const int each = 256 / (d / 8);
+    return launch(rt, kv, "join_few", batch->rows, (heads + each - 1) / each, 256, &a, what, err);
+  }
   return launch(rt, kv, "join", batch->rows, heads, 256, &a, what, err);
 }
 

@@ -9,6 +9,7 @@
 enum { kKvF16 = 0, kKvBf16 = 1, kKvQ8 = 2, kKvTq4 = 3 };
 enum { kKvRowF16 = 0, kKvRowBf16 = 1, kKvRowF32 = 2 };
 
+constexpr int kKvFewSplits = 8;        // splits that one lane group joins by itself
 constexpr int kKvStreamBatch = 1024;  // sequences whose steps a workgroup keeps in LDS
 
 // Status bits a kernel sets when what it read from the device was out of
@@ -54,7 +55,7 @@ struct KvAttnArgs {
   float* lse;       // [rows][heads] or NULL
   float* part;      // [tiles][kv_heads][splits][tile_rows][head_dim] unnormalised sums
   float* part_ml;   // [tiles][kv_heads][splits][tile_rows][2] reference and weight sum
-                    // (stream kernels: both [workgroups][2][16]...)
+                    // (stream kernels: [workgroups][2][16] of both)
   long long q_stride, out_stride;
   float scale;      // of q . k, times log2(e)
   long long tiles;

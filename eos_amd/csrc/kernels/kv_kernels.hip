@@ -1955,6 +1955,52 @@ EOS_DEV void attn_join(const KvAttnArgs& a) {
                      [&](int i) KV_INLINE { return load_part<D>(a, at + (size_t)i * rows); });
 }
 
+// The same for few splits: a workgroup has as many heads of a row as it has
+// lane groups, each of which goes through its head's splits (1,024 rows x 8
+// heads in two splits: 5 us, by one workgroup a row and head 20).
+template <int FMT, int D>
+EOS_DEV void attn_join_few(const KvAttnArgs& a) {
+  constexpr int LANES = D / 8, NG = 256 / LANES;
+  const KvCacheArgs& c = a.c;
+  const int l8 = threadIdx.x % LANES, rows = a.tile_rows;
+  const int head = blockIdx.y * NG + threadIdx.x / LANES, h = head / a.group;
+  KvTile t;
+  long long within = 0;
+  if (c.offsets == nullptr) {
+    t.s = kv_seq(c, blockIdx.x);
+  } else if (!find_seq(c, blockIdx.x, 1, 1, 0, t.s, within)) {
+    return;
+  }
+  if (within < 0 || within >= t.s.n) return;
+  const bool live = head < a.heads;
+  const int r = (int)within * a.group + head % a.group;
+  kv_tile(t, r / rows, rows, a.group, a.window, a.splits);
+  const long long u = (c.offsets == nullptr ? (long long)t.s.b * ((a.group + rows - 1) / rows)
+                                            : kv_unit_base(c, t.s.b, a.group, rows, 1)) +
+                      r / rows;
+  const size_t at = ((size_t)u * c.kv_heads + h) * a.splits * rows + r % rows;
+  float x[8] = {}, m = kLowest, l = 0.0f;
+  const int n = live ? t.splits : 0;
+  Part p[kKvFewSplits];
+#pragma unroll
+  for (int i = 0; i < kKvFewSplits; ++i)
+    if (i < n) p[i] = load_part<D>(a, at + (size_t)i * rows);
+#pragma unroll
+  for (int i = 0; i < kKvFewSplits; ++i)
+    if (i < n) {
+      const float nm = fmaxf(m, p[i].m);
+      const float fo = __builtin_amdgcn_exp2f(m - nm), fn = __builtin_amdgcn_exp2f(p[i].m - nm);
+      m = nm;
+      l = l * fo + p[i].l * fn;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = x[k] * fo + p[i].lo[k] * fn;
+        x[4 + k] = x[4 + k] * fo + p[i].hi[k] * fn;
+      }
+    }
+  finish_row<FMT, D>(a, t.s, r, h, l8, live, x, m, l);
+}
+
 // Joins what the stream's workgroups left of a row, where more than one had
 // it, and writes the rows that have no key.
 template <int FMT, int D>
@@ -2019,6 +2065,9 @@ EOS_DEV void attn_stream_join(const KvAttnArgs& a) {
   }                                                                                          \
   extern "C" __global__ __launch_bounds__(256) void eos_kv_join_##NAME##_##D(KvAttnArgs a) {     \
     attn_join<FMT, D>(a);                                                                    \
+  }                                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void eos_kv_join_few_##NAME##_##D(KvAttnArgs a) { \
+    attn_join_few<FMT, D>(a);                                                                \
   }
 #define KV_FORMATS(D)           \
   KV_KERNELS(f16, kKvF16, D)    \

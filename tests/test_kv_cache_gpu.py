@@ -298,12 +298,18 @@ def test_single_token_rows_of_many_sequences(rt, batch):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("d,kvh,group,p,window", [(64, 2, 1, 16, 0), (128, 1, 5, 32, 0),
                                                   (32, 1, 16, 16, 19), (256, 1, 3, 64, 70),
-                                                  (128, 2, 4, 16, 1)])
-def test_prompt_rows(rt, fmt, d, kvh, group, p, window):
-    _case(f"prompt {fmt} d={d} group={group} p={p} window={window}")
+                                                  (128, 2, 4, 16, 1), (64, 1, 20, 16, 0)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_prompt_rows(rt, fmt, d, kvh, group, p, window, wide):
+    """Few keys in the page table, and (wide) room for many: the second goes by
+    128 query rows a workgroup where a sequence has rows enough, the first by 16."""
+    _case(f"prompt {fmt} d={d} group={group} p={p} window={window} wide={wide}")
     lengths = np.array([37, 1, 150, 64, 3, 0, 131])
     n = np.array([37, 1, 5, 33, 4, 0, 20])      # whole prompts, behind a prefix, a padding row
-    w = World(rt, fmt, kvh, d, p, lengths, n, seed=d, extra_rows=3)
+    if wide:
+        lengths, n = lengths * 3, n * 3
+        lengths[1], n[1] = 1, 2
+    w = World(rt, fmt, kvh, d, p, lengths, n, seed=d, extra_rows=3, stride=4096 // p if wide else None)
     w.fill()
     _check(w, kvh * group, _io(fmt, group), window=window, pad=16)
 
@@ -380,9 +386,15 @@ def test_what_lies_behind_a_sequence_does_not_reach_it(rt, fmt):
     _case(f"NaN slots {fmt}")
     lengths = np.array([37, 3, 130])
     n = np.array([5, 3, 2])
-    w = World(rt, fmt, 1, 64, 16, lengths, n, seed=6)
+    for stride in (None, 200):                  # 16 and 128 query rows a workgroup
+        _nan_slots(rt, fmt, lengths, n, stride)
+
+
+def _nan_slots(rt, fmt, lengths, n, stride):
+    heads = 2 if stride is None else 64
+    w = World(rt, fmt, 1, 64, 16, lengths, n, seed=6, stride=stride)
     w.fill()
-    clean = [_attend(w, 2, _io(fmt), window, q=np.ones((10, 2, 64), np.float32))[1:] for window in (0, 9)]
+    clean = [_attend(w, heads, _io(fmt), window, q=np.ones((10, heads, 64), np.float32))[1:] for window in (0, 9)]
     used = set()
     for b, t in enumerate(lengths):
         used |= {(int(w.plan.table[b, i // 16]), i % 16) for i in range(t)}
@@ -392,9 +404,9 @@ def test_what_lies_behind_a_sequence_does_not_reach_it(rt, fmt):
         bad[::2] = np.inf
         put_rows(w.pool, name, bad, free)
     w.upload()
-    q = np.ones((10, 2, 64), np.float32)
+    q = np.ones((10, heads, 64), np.float32)
     for window, want in zip((0, 9), clean):
-        got = _attend(w, 2, _io(fmt), window, q=q)[1:]
+        got = _attend(w, heads, _io(fmt), window, q=q)[1:]
         np.testing.assert_array_equal(got[0], want[0])
         np.testing.assert_array_equal(got[1], want[1])
     # ... and what a window has passed
@@ -402,7 +414,7 @@ def test_what_lies_behind_a_sequence_does_not_reach_it(rt, fmt):
     for name in "kv":
         put_rows(w.pool, name, np.full((len(passed), 1, 64), np.nan, np.float32), passed)
     w.upload()
-    got = _attend(w, 2, _io(fmt), 9, q=q)[1:]
+    got = _attend(w, heads, _io(fmt), 9, q=q)[1:]
     np.testing.assert_array_equal(got[0], clean[1][0])
 
 
@@ -411,22 +423,28 @@ def test_a_later_token_does_not_reach_earlier_rows(rt, fmt):
     """NaN and infinities in a token of the prompt: rows before it are as
     without it, rows from it on are NaN or follow the infinity."""
     _case(f"NaN token {fmt}")
+    for stride, heads in ((None, 2), (200, 2), (200, 7)):   # 16 and 128 query rows a workgroup
+        _nan_token(rt, fmt, stride, heads)
+
+
+def _nan_token(rt, fmt, stride, heads):
     n = 40
-    w = World(rt, fmt, 1, 64, 16, np.array([n]), np.array([n]), seed=6, shuffle=False, spare=0)
+    w = World(rt, fmt, 1, 64, 16, np.array([n]), np.array([n]), seed=6, shuffle=False, spare=0,
+              stride=stride)
     w.fill()
-    q = w.rng.normal(size=(n, 2, 64)).astype(np.float32)
-    clean = _attend(w, 2, _io(fmt), q=q)[1]
+    q = w.rng.normal(size=(n, heads, 64)).astype(np.float32)
+    clean = _attend(w, heads, _io(fmt), q=q)[1]
     bad = np.ones((1, 1, 64), np.float32)
     bad[0, 0, 7] = np.nan
     put_rows(w.pool, "v", bad, [(1, 4)])          # token 20
     bad[0, 0, 7] = np.inf
     put_rows(w.pool, "v", bad, [(1, 14)])         # token 30
     w.upload()
-    got = _attend(w, 2, _io(fmt), q=q)[1]
+    got = _attend(w, heads, _io(fmt), q=q)[1]
     vals = w.pool.values()
     q64 = ref.from_rows(ref.to_rows(q, _io(fmt)), _io(fmt)).astype(np.float64)
     with np.errstate(all="ignore"):
-        want, _, tol, _ = ref.attention(w.plan, vals, q64, 2, _io(fmt), 64 ** -0.5)
+        want, _, tol, _ = ref.attention(w.plan, vals, q64, heads, _io(fmt), 64 ** -0.5)
     assert (np.abs(got[:20] - want[:20]) <= tol[:20]).all()
     assert (np.abs(got[:20] - clean[:20]) <= 2 * tol[:20]).all()
     np.testing.assert_array_equal(np.isnan(got[20:]), np.isnan(want[20:]))
