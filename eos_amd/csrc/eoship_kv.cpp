@@ -8,6 +8,8 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <exception>
+#include <string>
 #include <vector>
 
 #include "eoship_internal.h"
@@ -30,13 +32,14 @@ struct EosHipKVCache {
 namespace {
 
 // Query rows a sequence (heads of a group counted) from which the prompt
-// kernel takes a call, for 16-bit and for quantized caches. Below, 16 rows at
-// a time, each wavefront with keys of its own, are faster: the prompt kernel's
-// stage has a latency of its own, and quantized stages are expanded by few
-// wavefronts. 8 sequences behind 8,000 keys, heads 32 to 8 of 128, us (16 rows
-// / 128 rows at a time): bf16 2 rows each 65 / 59, 8 rows 116 / 66; q8 8 rows
-// 65 / 96, 16 rows 107 / 119, 32 rows behind 2,000 58 / 56, 128 rows 124 / 104.
-constexpr int kPromptFrom = 8, kPromptFromQuantized = 96;
+// kernel takes a call, by format. Below, 16 rows at a time, each wavefront with
+// keys of its own, are faster: the prompt kernel's stage has a latency of its
+// own, and quantized stages are expanded by few wavefronts. 8 sequences, heads
+// 32 to 8 of 128, us (16 rows / 128 rows at a time): behind 8,000 keys bf16 2
+// rows each 65 / 59, 8 rows 116 / 66; q8 8 rows 65 / 96, 16 rows 107 / 119;
+// behind 2,000 keys q8 32 rows 58 / 56, 128 rows 124 / 104; tq4 32 rows 52 /
+// 71, 128 rows 133 / 128.
+constexpr int kPromptFrom[] = {8, 8, 96, 384};
 // ... and not while the 16-row workgroups are on the CUs at once over so few
 // keys (4 prompts of 256, 8 heads of 64: 10 / 17).
 constexpr int kPromptKeys = 1024;
@@ -62,6 +65,16 @@ class OnDevice {
  private:
   int was_ = 0, now_ = 0;
 };
+
+// Runs a call's body: no exception (host memory may run out) leaves a C entry.
+template <class F>
+int guarded(const char* what, char** err, F body) {
+  try {
+    return body();
+  } catch (const std::exception& e) {
+    return set_err(err, "%s: %s", what, e.what());
+  }
+}
 
 // The f16 bits of a float that f16 holds exactly and normally, or 0.
 uint16_t exact_f16(float f) {
@@ -202,95 +215,99 @@ int eoship_kv_check_batch(const EosHipKVDesc* desc, const int32_t* page_table,
                           int32_t table_stride, int32_t batch, const int32_t* lengths,
                           const int32_t* offsets, int64_t rows, int32_t writes, char** err) {
   const char* what = "eoship_kv_check_batch";
-  if (check_desc(desc, what, err) != 0) return 1;
-  if (batch < 0 || rows < 0 || rows > INT32_MAX)
-    return set_err(err, "%s: batch and rows must be in 0..2^31-1", what);
-  if (batch == 0 || rows == 0) return 0;
-  if (page_table == nullptr || lengths == nullptr || table_stride < 1)
-    return set_err(err, "%s: NULL page table or lengths, or no table columns", what);
-  if (offsets == nullptr && rows != batch)
-    return set_err(err, "%s: without offsets every sequence has one row: rows %lld, batch %d",
-                   what, (long long)rows, batch);
-  if (offsets != nullptr && offsets[0] != 0)
-    return set_err(err, "%s: offsets[0] must be 0, got %d", what, offsets[0]);
-  KvCacheArgs c{};
-  c.table = page_table;
-  c.lengths = lengths;
-  c.offsets = offsets;
-  c.rows = rows;
-  c.pages = (int)desc->pages;
-  c.table_stride = table_stride;
-  c.batch = batch;
-  while ((1 << c.page_shift) < desc->page_tokens) ++c.page_shift;
-  // Where a page is written: the sequence, and which of its pages.
-  std::vector<std::pair<int, std::pair<int, int>>> written;
-  for (int b = 0; b < batch; ++b) {
-    const KvSeq s = kv_seq(c, b);
-    if (s.bad & kKvBadOffset)
-      return set_err(err, "%s: sequence %d: offsets must ascend within 0..rows", what, b);
-    if (s.bad & kKvBadLength)
-      return set_err(err, "%s: sequence %d: length %d outside 0..%lld of its table row", what, b,
-                     lengths[b], (long long)table_stride * desc->page_tokens);
-    for (int i = 0; i << c.page_shift < s.keys; ++i)
-      if (kv_page(c, b, i << c.page_shift) < 0)
-        return set_err(err, "%s: sequence %d: page %d of its table row is %d, not in 0..%lld", what,
-                       b, i, page_table[(size_t)b * table_stride + i], (long long)desc->pages - 1);
-    if (writes != 0 && s.n > 0 && s.keys > 0)
-      for (int i = std::max(0, s.len - s.n) >> c.page_shift; i <= (s.keys - 1) >> c.page_shift; ++i)
-        written.push_back({page_table[(size_t)b * table_stride + i], {b, i}});
-  }
-  std::sort(written.begin(), written.end());
-  for (size_t i = 1; i < written.size(); ++i)
-    if (written[i].first == written[i - 1].first)
-      return set_err(err, "%s: page %d is written twice, by sequences %d and %d", what,
-                     written[i].first, written[i - 1].second.first, written[i].second.first);
-  return 0;
+  return guarded(what, err, [&]() -> int {
+    if (check_desc(desc, what, err) != 0) return 1;
+    if (batch < 0 || rows < 0 || rows > INT32_MAX)
+      return set_err(err, "%s: batch and rows must be in 0..2^31-1", what);
+    if (batch == 0 || rows == 0) return 0;
+    if (page_table == nullptr || lengths == nullptr || table_stride < 1)
+      return set_err(err, "%s: NULL page table or lengths, or no table columns", what);
+    if (offsets == nullptr && rows != batch)
+      return set_err(err, "%s: without offsets every sequence has one row: rows %lld, batch %d",
+                     what, (long long)rows, batch);
+    if (offsets != nullptr && offsets[0] != 0)
+      return set_err(err, "%s: offsets[0] must be 0, got %d", what, offsets[0]);
+    KvCacheArgs c{};
+    c.table = page_table;
+    c.lengths = lengths;
+    c.offsets = offsets;
+    c.rows = rows;
+    c.pages = (int)desc->pages;
+    c.table_stride = table_stride;
+    c.batch = batch;
+    while ((1 << c.page_shift) < desc->page_tokens) ++c.page_shift;
+    // Where a page is written: the sequence, and which of its pages.
+    std::vector<std::pair<int, std::pair<int, int>>> written;
+    for (int b = 0; b < batch; ++b) {
+      const KvSeq s = kv_seq(c, b);
+      if (s.bad & kKvBadOffset)
+        return set_err(err, "%s: sequence %d: offsets must ascend within 0..rows", what, b);
+      if (s.bad & kKvBadLength)
+        return set_err(err, "%s: sequence %d: length %d outside 0..%lld of its table row", what, b,
+                       lengths[b], (long long)table_stride * desc->page_tokens);
+      for (int i = 0; i << c.page_shift < s.keys; ++i)
+        if (kv_page(c, b, i << c.page_shift) < 0)
+          return set_err(err, "%s: sequence %d: page %d of its table row is %d, not in 0..%lld", what,
+                         b, i, page_table[(size_t)b * table_stride + i], (long long)desc->pages - 1);
+      if (writes != 0 && s.n > 0 && s.keys > 0)
+        for (int i = std::max(0, s.len - s.n) >> c.page_shift; i <= (s.keys - 1) >> c.page_shift; ++i)
+          written.push_back({page_table[(size_t)b * table_stride + i], {b, i}});
+    }
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+      if (written[i].first == written[i - 1].first)
+        return set_err(err, "%s: page %d is written twice, by sequences %d and %d", what,
+                       written[i].first, written[i - 1].second.first, written[i].second.first);
+    return 0;
+  });
 }
 
 int eoship_kv_bind(EosHipRuntime* rt, const EosHipKVDesc* desc, EosHipKVCache** out, char** err) {
   const char* what = "eoship_kv_bind";
-  if (out != nullptr) *out = nullptr;
-  if (check_desc(desc, what, err) != 0 || check_tables(desc, what, err) != 0) return 1;
-  if (desc->d_k == nullptr || desc->d_v == nullptr)
-    return set_err(err, "%s: NULL pool", what);
-  if (!aligned(desc->d_k) || !aligned(desc->d_v))
-    return set_err(err, "%s: pools must be 16-byte aligned", what);
-  if (desc->format >= kKvQ8 &&
-      (desc->d_k_scale == nullptr || desc->d_v_scale == nullptr || !aligned(desc->d_k_scale) ||
-       !aligned(desc->d_v_scale)))
-    return set_err(err, "%s: %s needs 16-byte aligned scale pools", what, kFormats[desc->format]);
-  if (rt == nullptr || out == nullptr) return set_err(err, "%s: NULL argument", what);
-  OnDevice on(rt->device);
-  auto* kv = new EosHipKVCache();
-  kv->rt = rt;
-  kv->d = *desc;
-  while ((1 << kv->page_shift) < desc->page_tokens) ++kv->page_shift;
-  const size_t signs = desc->format == kKvTq4 ? (size_t)desc->head_dim * 4 : 0;
-  std::vector<char> host(16 + signs, 0);
-  if (rt->alloc(host.size(), &kv->mem, err) != 0) {
-    delete kv;
-    return 1;
-  }
-  if (desc->format == kKvTq4) {
-    std::memcpy(host.data() + 16, desc->signs, signs);
-    KvTables& t = kv->tables;
-    t.signs = reinterpret_cast<const float*>(static_cast<char*>(kv->mem) + 16);
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = exact_f16(desc->codebook[i]);
-      t.mags[i] = desc->codebook[i];
-      t.hi[i / 4] |= (u >> 8) << (8 * (i % 4));
-      t.lo[i / 4] |= (u & 255) << (8 * (i % 4));
-      if (i > 0) t.edges[i - 1] = 0.5f * (desc->codebook[i] + desc->codebook[i - 1]);
+  return guarded(what, err, [&]() -> int {
+    if (out != nullptr) *out = nullptr;
+    if (check_desc(desc, what, err) != 0 || check_tables(desc, what, err) != 0) return 1;
+    if (desc->d_k == nullptr || desc->d_v == nullptr)
+      return set_err(err, "%s: NULL pool", what);
+    if (!aligned(desc->d_k) || !aligned(desc->d_v))
+      return set_err(err, "%s: pools must be 16-byte aligned", what);
+    if (desc->format >= kKvQ8 &&
+        (desc->d_k_scale == nullptr || desc->d_v_scale == nullptr || !aligned(desc->d_k_scale) ||
+         !aligned(desc->d_v_scale)))
+      return set_err(err, "%s: %s needs 16-byte aligned scale pools", what, kFormats[desc->format]);
+    if (rt == nullptr || out == nullptr) return set_err(err, "%s: NULL argument", what);
+    OnDevice on(rt->device);
+    auto* kv = new EosHipKVCache();
+    kv->rt = rt;
+    kv->d = *desc;
+    while ((1 << kv->page_shift) < desc->page_tokens) ++kv->page_shift;
+    const size_t signs = desc->format == kKvTq4 ? (size_t)desc->head_dim * 4 : 0;
+    std::vector<char> host(16 + signs, 0);
+    if (rt->alloc(host.size(), &kv->mem, err) != 0) {
+      delete kv;
+      return 1;
     }
-  }
-  kv->d.codebook = kv->d.signs = nullptr;  // the caller's host memory is not kept
-  const hipError_t e = rt->copy_sync(kv->mem, host.data(), host.size(), hipMemcpyHostToDevice);
-  if (e != hipSuccess) {
-    delete kv;
-    return hip_err(err, "hipMemcpy(cache tables)", e);
-  }
-  *out = kv;
-  return 0;
+    if (desc->format == kKvTq4) {
+      std::memcpy(host.data() + 16, desc->signs, signs);
+      KvTables& t = kv->tables;
+      t.signs = reinterpret_cast<const float*>(static_cast<char*>(kv->mem) + 16);
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t u = exact_f16(desc->codebook[i]);
+        t.mags[i] = desc->codebook[i];
+        t.hi[i / 4] |= (u >> 8) << (8 * (i % 4));
+        t.lo[i / 4] |= (u & 255) << (8 * (i % 4));
+        if (i > 0) t.edges[i - 1] = 0.5f * (desc->codebook[i] + desc->codebook[i - 1]);
+      }
+    }
+    kv->d.codebook = kv->d.signs = nullptr;  // the caller's host memory is not kept
+    const hipError_t e = rt->copy_sync(kv->mem, host.data(), host.size(), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+      delete kv;
+      return hip_err(err, "hipMemcpy(cache tables)", e);
+    }
+    *out = kv;
+    return 0;
+  });
 }
 
 int eoship_kv_release(EosHipRuntime* rt, EosHipKVCache* kv, char** err) {
@@ -306,25 +323,29 @@ int eoship_kv_append_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKV
                             const void* d_k, int64_t k_stride, const void* d_v, int64_t v_stride,
                             int32_t dtype, char** err) {
   const char* what = "eoship_kv_append_device";
-  if (check_batch(rt, kv, batch, what, err) != 0) return 1;
-  if (dtype != kKvRowF16 && dtype != kKvRowBf16)
-    return set_err(err, "%s: rows must be f16 (0) or bf16 (1), got %d", what, dtype);
-  if (kv->d.format <= kKvBf16 && dtype != kv->d.format)
-    return set_err(err, "%s: the cache holds %s, the rows are %s", what, kFormats[kv->d.format],
-                   kFormats[dtype]);
-  if (batch->batch == 0 || batch->rows == 0) return 0;
-  return rows_call(rt, kv, batch, d_k, k_stride, d_v, v_stride, dtype, "append", what, err);
+  return guarded(what, err, [&]() -> int {
+    if (check_batch(rt, kv, batch, what, err) != 0) return 1;
+    if (dtype != kKvRowF16 && dtype != kKvRowBf16)
+      return set_err(err, "%s: rows must be f16 (0) or bf16 (1), got %d", what, dtype);
+    if (kv->d.format <= kKvBf16 && dtype != kv->d.format)
+      return set_err(err, "%s: the cache holds %s, the rows are %s", what, kFormats[kv->d.format],
+                     kFormats[dtype]);
+    if (batch->batch == 0 || batch->rows == 0) return 0;
+    return rows_call(rt, kv, batch, d_k, k_stride, d_v, v_stride, dtype, "append", what, err);
+  });
 }
 
 int eoship_kv_read_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
                           void* d_k, int64_t k_stride, void* d_v, int64_t v_stride, int32_t dtype,
                           char** err) {
   const char* what = "eoship_kv_read_device";
-  if (check_batch(rt, kv, batch, what, err) != 0) return 1;
-  if (dtype < kKvRowF16 || dtype > kKvRowF32)
-    return set_err(err, "%s: rows must be f16 (0), bf16 (1) or f32 (2), got %d", what, dtype);
-  if (batch->batch == 0 || batch->rows == 0) return 0;
-  return rows_call(rt, kv, batch, d_k, k_stride, d_v, v_stride, dtype, "read", what, err);
+  return guarded(what, err, [&]() -> int {
+    if (check_batch(rt, kv, batch, what, err) != 0) return 1;
+    if (dtype < kKvRowF16 || dtype > kKvRowF32)
+      return set_err(err, "%s: rows must be f16 (0), bf16 (1) or f32 (2), got %d", what, dtype);
+    if (batch->batch == 0 || batch->rows == 0) return 0;
+    return rows_call(rt, kv, batch, d_k, k_stride, d_v, v_stride, dtype, "read", what, err);
+  });
 }
 
 int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
@@ -332,93 +353,98 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
                                float scale, int32_t window, void* d_out, int64_t out_stride,
                                float* d_lse, char** err) {
   const char* what = "eoship_kv_attention_device";
-  if (check_batch(rt, kv, batch, what, err) != 0) return 1;
-  if (dtype != kKvRowF16 && dtype != kKvRowBf16)
-    return set_err(err, "%s: rows must be f16 (0) or bf16 (1), got %d", what, dtype);
-  if (kv->d.format <= kKvBf16 && dtype != kv->d.format)
-    return set_err(err, "%s: the cache holds %s, the rows are %s", what, kFormats[kv->d.format],
-                   kFormats[dtype]);
-  if (heads < 1 || heads > 65535 || heads % kv->d.kv_heads != 0)
-    return set_err(err, "%s: heads must be a multiple of kv_heads (%d) up to 65535, got %d", what,
-                   kv->d.kv_heads, heads);
-  if (!std::isfinite(scale)) return set_err(err, "%s: scale must be finite", what);
-  if (window < 0) return set_err(err, "%s: window must not be negative, got %d", what, window);
-  if (batch->batch == 0 || batch->rows == 0) return 0;
-  if (batch->rows * (heads / kv->d.kv_heads) > 1 << 30)
-    return set_err(err, "%s: too many rows for one call", what);
-  const int64_t width = (int64_t)heads * kv->d.head_dim;
-  if (check_rows(d_q, q_stride, width, "q", what, err) != 0 ||
-      check_rows(d_out, out_stride, width, "out", what, err) != 0)
-    return 1;
-  OnDevice on(rt->device);
-  KvAttnArgs a{};
-  a.c = cache_args(kv, batch);
-  a.q = static_cast<const uint8_t*>(d_q);
-  a.out = static_cast<uint8_t*>(d_out);
-  a.lse = d_lse;
-  a.q_stride = q_stride;
-  a.out_stride = out_stride;
-  a.scale = scale * 1.44269504089f;
-  a.heads = heads;
-  a.group = heads / kv->d.kv_heads;
-  a.window = window;
-  a.dtype = dtype;
-  const int kvh = kv->d.kv_heads, d = kv->d.head_dim;
-  const long long slots = 2LL * rt->compute_units;  // two workgroups a CU, by their registers
-  long long keys = (long long)batch->table_stride << kv->page_shift;
-  if (window > 0) keys = std::min(keys, (long long)window + batch->rows + 32);
-  const auto tiles = [&](int rows) {
-    return batch->d_offsets == nullptr ? (long long)batch->batch * ((a.group + rows - 1) / rows)
-                                       : kv_units(batch->rows, batch->batch, a.group, rows, 1);
-  };
-  const int64_t from = kv->d.format >= kKvQ8 ? kPromptFromQuantized : kPromptFrom;
-  const bool prompt = batch->d_offsets != nullptr && batch->rows * a.group >= from * batch->batch &&
-                      (tiles(kKvTileRows) * kvh > slots || keys > kPromptKeys);
-  a.tile_rows = prompt ? kKvPromptRows : kKvTileRows;
-  a.tiles = tiles(a.tile_rows);
-  // Splits while the workgroups are on the CUs at once, none below 256 keys:
-  // further ones cost more in prologues and joining than their balance gains
-  // (64 x 2,000 tokens of tq4: 39 us at two workgroups a CU, 53 at four, 68 at
-  // eight). Prompts, whose joins are few, fill the last slots too (8 x 128 rows
-  // behind 2,000 keys in q8: 104 us, 156 without).
-  const long long units = a.tiles * kvh;
-  const long long want = prompt ? (slots + units - 1) / units : slots / units;
-  a.splits = (int)std::max(1LL, std::min(want, (keys + 255) / 256));
-  // Several sequences with room for enough keys: equal shares of all of them
-  // instead, whatever the lengths. 64 sequences of 1,024 to 16,384 tokens in
-  // tq4: 164 us, in splits 230; of 2,000 tokens each 46 and 39; 32 of 64 to
-  // 4,096 in bf16: 66 and 79. Many workgroups balance by themselves (256
-  // sequences of 1,000: 206 in shares, 185 in splits), few keys do not pay for
-  // the prefix sum (4 of up to 3,000: 21 and 16).
-  const long long steps = ((long long)batch->table_stride << kv->page_shift) / 128;
-  if (batch->d_offsets == nullptr && batch->batch > 1 && batch->batch <= kKvStreamBatch &&
-      units < 4 * slots && steps * units >= 4 * slots) {
-    a.workgroups = (int)slots;
-    const size_t parts = (size_t)a.workgroups * 2 * kKvTileRows;
-    void* ws = nullptr;
-    if (rt->workspace(parts * (size_t)(d + 2) * 4, &ws, err) != 0) return 1;
-    a.part = static_cast<float*>(ws);
-    a.part_ml = a.part + parts * (size_t)d;
-    if (launch(rt, kv, "stream", a.workgroups, 1, 256, &a, what, err) != 0) return 1;
-    return launch(rt, kv, "stream_join", batch->batch, heads, 256, &a, what, err);
-  }
-  if (a.splits > 1) {
-    const size_t parts = (size_t)units * a.splits * a.tile_rows;
-    void* ws = nullptr;
-    if (rt->workspace(parts * (size_t)(d + 2) * 4, &ws, err) != 0) return 1;
-    a.part = static_cast<float*>(ws);
-    a.part_ml = a.part + parts * (size_t)d;
-  }
-  const long long items = a.tiles * a.splits;
-  if (prompt ? launch(rt, kv, "prompt", kv_place_blocks(kvh, items), 1, 256, &a, what, err) != 0
-             : launch(rt, kv, "split", items, kvh, 256, &a, what, err) != 0)
-    return 1;
-  if (a.splits == 1) return 0;
-  if (a.splits <= kKvFewSplits) {
-    const int each = 256 / (d / 8);
-    return launch(rt, kv, "join_few", batch->rows, (heads + each - 1) / each, 256, &a, what, err);
-  }
-  return launch(rt, kv, "join", batch->rows, heads, 256, &a, what, err);
+  return guarded(what, err, [&]() -> int {
+    if (check_batch(rt, kv, batch, what, err) != 0) return 1;
+    if (dtype != kKvRowF16 && dtype != kKvRowBf16)
+      return set_err(err, "%s: rows must be f16 (0) or bf16 (1), got %d", what, dtype);
+    if (kv->d.format <= kKvBf16 && dtype != kv->d.format)
+      return set_err(err, "%s: the cache holds %s, the rows are %s", what, kFormats[kv->d.format],
+                     kFormats[dtype]);
+    if (heads < 1 || heads > 65535 || heads % kv->d.kv_heads != 0)
+      return set_err(err, "%s: heads must be a multiple of kv_heads (%d) up to 65535, got %d", what,
+                     kv->d.kv_heads, heads);
+    if (!std::isfinite(scale)) return set_err(err, "%s: scale must be finite", what);
+    if (window < 0) return set_err(err, "%s: window must not be negative, got %d", what, window);
+    if (batch->batch == 0 || batch->rows == 0) return 0;
+    if (batch->rows * (heads / kv->d.kv_heads) > 1 << 30)
+      return set_err(err, "%s: too many rows for one call", what);
+    const int64_t width = (int64_t)heads * kv->d.head_dim;
+    if (check_rows(d_q, q_stride, width, "q", what, err) != 0 ||
+        check_rows(d_out, out_stride, width, "out", what, err) != 0)
+      return 1;
+    OnDevice on(rt->device);
+    KvAttnArgs a{};
+    a.c = cache_args(kv, batch);
+    a.q = static_cast<const uint8_t*>(d_q);
+    a.out = static_cast<uint8_t*>(d_out);
+    a.lse = d_lse;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.scale = scale * 1.44269504089f;
+    a.heads = heads;
+    a.group = heads / kv->d.kv_heads;
+    a.window = window;
+    a.dtype = dtype;
+    const int kvh = kv->d.kv_heads, d = kv->d.head_dim;
+    // A window that holds the whole table restricts nothing.
+    if (window >= std::min<long long>((long long)batch->table_stride << kv->page_shift, kKvMostKeys))
+      a.window = window = 0;
+    const long long slots = 2LL * rt->compute_units;  // two workgroups a CU, by their registers
+    long long keys = (long long)batch->table_stride << kv->page_shift;
+    if (window > 0) keys = std::min(keys, (long long)window + batch->rows + 32);
+    const auto tiles = [&](int rows) {
+      return batch->d_offsets == nullptr ? (long long)batch->batch * ((a.group + rows - 1) / rows)
+                                         : kv_units(batch->rows, batch->batch, a.group, rows, 1);
+    };
+    const int64_t from = kPromptFrom[kv->d.format];
+    const bool prompt = batch->d_offsets != nullptr && batch->rows * a.group >= from * batch->batch &&
+                        (tiles(kKvTileRows) * kvh > slots || keys > kPromptKeys);
+    a.tile_rows = prompt ? kKvPromptRows : kKvTileRows;
+    a.tiles = tiles(a.tile_rows);
+    // Splits while the workgroups are on the CUs at once, none below 256 keys:
+    // further ones cost more in prologues and joining than their balance gains
+    // (64 x 2,000 tokens of tq4: 39 us at two workgroups a CU, 53 at four, 68 at
+    // eight). Prompts, whose joins are few, fill the last slots too (8 x 128 rows
+    // behind 2,000 keys in q8: 104 us, 156 without).
+    const long long units = a.tiles * kvh;
+    const long long want = prompt ? (slots + units - 1) / units : slots / units;
+    a.splits = (int)std::max(1LL, std::min(want, (keys + 255) / 256));
+    // Several sequences with room for enough keys: equal shares of all of them
+    // instead, whatever the lengths. 64 sequences of 1,024 to 16,384 tokens in
+    // tq4: 164 us, in splits 230; of 2,000 tokens each 46 and 39; 32 of 64 to
+    // 4,096 in bf16: 66 and 79. Many workgroups balance by themselves (256
+    // sequences of 1,000: 206 in shares, 185 in splits), few keys do not pay for
+    // the prefix sum (4 of up to 3,000: 21 and 16).
+    const long long steps = ((long long)batch->table_stride << kv->page_shift) / 128;
+    if (batch->d_offsets == nullptr && batch->batch > 1 && batch->batch <= kKvStreamBatch &&
+        units < 4 * slots && steps * units >= 4 * slots) {
+      a.workgroups = (int)slots;
+      const size_t parts = (size_t)a.workgroups * 2 * kKvTileRows;
+      void* ws = nullptr;
+      if (rt->workspace(parts * (size_t)(d + 2) * 4, &ws, err) != 0) return 1;
+      a.part = static_cast<float*>(ws);
+      a.part_ml = a.part + parts * (size_t)d;
+      if (launch(rt, kv, "stream", a.workgroups, 1, 256, &a, what, err) != 0) return 1;
+      return launch(rt, kv, "stream_join", batch->batch, heads, 256, &a, what, err);
+    }
+    if (a.splits > 1) {
+      const size_t parts = (size_t)units * a.splits * a.tile_rows;
+      void* ws = nullptr;
+      if (rt->workspace(parts * (size_t)(d + 2) * 4, &ws, err) != 0) return 1;
+      a.part = static_cast<float*>(ws);
+      a.part_ml = a.part + parts * (size_t)d;
+    }
+    const long long items = a.tiles * a.splits;
+    if (prompt ? launch(rt, kv, "prompt", kv_place_blocks(kvh, items), 1, 256, &a, what, err) != 0
+               : launch(rt, kv, "split", items, kvh, 256, &a, what, err) != 0)
+      return 1;
+    if (a.splits == 1) return 0;
+    if (a.splits <= kKvFewSplits) {
+      const int each = 256 / (d / 8);
+      return launch(rt, kv, "join_few", batch->rows, (heads + each - 1) / each, 256, &a, what, err);
+    }
+    return launch(rt, kv, "join", batch->rows, heads, 256, &a, what, err);
+  });
 }
 
 int eoship_kv_status(EosHipRuntime* rt, EosHipKVCache* kv, int32_t* status, char** err) {

@@ -16,6 +16,7 @@ constexpr int kKvStreamBatch = 1024;  // sequences whose steps a workgroup keeps
 // range (nothing outside the pool and the rows is touched).
 enum { kKvBadPage = 1, kKvBadLength = 2, kKvBadOffset = 4 };
 
+constexpr int kKvMostKeys = 1 << 30;  // tokens of a sequence: positions and steps stay in 32 bits
 constexpr int kKvGroup = 8;       // tokens of V stored side by side
 constexpr int kKvRun = 32;         // positions of a workgroup of append and read
 constexpr int kKvTileRows = 16;    // query rows of a workgroup of the split kernel

@@ -37,7 +37,8 @@ KV_HD KvSeq kv_seq_of(const KvCacheArgs& c, int b, long long lo, long long hi, i
   s.row0 = lo;
   s.n = (int)(hi - lo);
   s.len = len;
-  const long long cap = (long long)c.table_stride << c.page_shift;
+  const long long room = (long long)c.table_stride << c.page_shift;
+  const long long cap = room < kKvMostKeys ? room : kKvMostKeys;
   if (s.len < 0 || s.len > cap) s.bad |= kKvBadLength;
   if (s.len < 0) s.len = 0;
   s.keys = s.len > cap ? (int)cap : s.len;

@@ -827,6 +827,15 @@ EOS_DEV float odd_sum(float up, float down) {
   return (up > 0.0f ? inf : 0.0f) + (down > 0.0f ? -inf : 0.0f);
 }
 
+// Two elements of a query whose largest is below 2^kQUp: f16, and what f16
+// leaves of them (not below 2^-14 before 2^-26 of the largest).
+constexpr int kQUp = 12;
+template <int FMT>
+EOS_DEV v2u query2(float a, float b) {
+  const uint32_t hi = pack2<FMT>(a, b);
+  return v2u{hi, FMT == kKvTq4 ? pack2<FMT>(a - f16_to_f32(hi & 0xffffu), b - f16_to_f32(hi >> 16)) : 0u};
+}
+
 // Place in a word of 8 codes of operand slot i.
 template <int FMT>
 constexpr int slot_of(int i) {
@@ -874,7 +883,7 @@ EOS_DEV void finish_row(const KvAttnArgs& a, const KvSeq& s, int r, int h, int l
 // `at` of the parts.
 template <int FMT, int D>
 EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int end, bool whole, size_t at) {
-  constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
+  constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4, kTwo = FMT == kKvTq4;
   constexpr int BITS = bits_of(FMT), KS = D / 32, NT = D / 16, LANES = D / 8;
   // Dimensions of V in one load of a lane, loads a step, words of a load.
   constexpr int VW = FMT == kKvTq4 ? (D >= 64 ? 4 : 2) : FMT == kKvQ8 ? 2 : 1;
@@ -907,9 +916,11 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
   const int hi_c = real ? kv_min(qpos + 1, t.s.keys) : t.hi;
   const int lo_c = real && a.window > 0 ? qpos - a.window + 1 : 0;
 
-  // The query as the second operand; quantized formats take it in f16 with
-  // its largest element brought to [0.5, 1), tq4 rotated.
-  v4u q[KS];
+  // The query as the second operand. Quantized formats take it in f16, its
+  // largest element brought to [2^11, 2^12) by a power of two, tq4 rotated and,
+  // since that has more bits than f16, in two terms (one would move the weights
+  // by 2^-12 of a score).
+  v4u q[KS], q2[kTwo ? KS : 1];
   float qs = a.scale;
   {
     const uint8_t* src = a.q + ((size_t)(t.s.row0 + qrow) * a.q_stride +
@@ -952,15 +963,18 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
 #pragma unroll
       for (int i = 0; i < D / 4; ++i) most = fmaxf(most, fabsf(x[i / 8][i % 8]));
       most = group_max(most);
-      // Powers of two only: exact but for elements 2^-14 below the largest.
       int ex = most > 0.0f && most < __builtin_inff() ? __builtin_amdgcn_frexp_expf(most) : 0;
-      const float down = __builtin_amdgcn_ldexpf(1.0f, max(-ex, -126));
+      ex = kv_max(ex, -100) - kQUp;
+      const float down = __builtin_amdgcn_ldexpf(1.0f, -ex);
       qs = __builtin_amdgcn_ldexpf(qs, ex);
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          q[s][i] = pack2<FMT>(x[s][slot_of<FMT>(2 * i)] * down, x[s][slot_of<FMT>(2 * i + 1)] * down);
+        for (int i = 0; i < 4; ++i) {
+          const v2u w = query2<FMT>(x[s][slot_of<FMT>(2 * i)] * down, x[s][slot_of<FMT>(2 * i + 1)] * down);
+          q[s][i] = w[0];
+          if (kTwo) q2[kTwo ? s : 0][i] = w[1];
+        }
     }
   }
 
@@ -1050,6 +1064,7 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
           for (int i = 0; i < 4; ++i) f[i] = kr[j][4 * s + i];
         }
         sc[j] = mfma16<FMT>(v4u{f[0], f[1], f[2], f[3]}, q[s], sc[j]);
+        if constexpr (kTwo) sc[j] = mfma16<FMT>(v4u{f[0], f[1], f[2], f[3]}, q2[s], sc[j]);
       }
     float x[8];
 #pragma unroll
@@ -1144,8 +1159,9 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
         acc[i * VW + w] = mfma16<FMT>(v4u{f[0], f[1], f[2], f[3]}, pf, acc[i * VW + w]);
       }
   };
-  // (from 1024 bits of width on there are no registers for a second step)
-  constexpr bool kAhead = D * BITS <= 1024;
+  // (where registers hold a second step: 32 sequences of 4,000 tokens, width 256
+  // in tq4, 46 us without it, 111 with what it spills)
+  constexpr bool kAhead = D * BITS <= 1024 && D < 256;
   const int first = begin + 32 * wave;
   Raw ra, rb;
   if (first < end) {
@@ -1375,16 +1391,16 @@ EOS_DEV void expand(const KvTables& t, v4u x, v4u (&out)[16 / bits_of(FMT)]) {
 }
 
 // One workgroup: 128 query rows of a head group, 32 a wavefront, against a
-// split of their keys, 64 (D = 256: 32) at a time through two LDS stages that
+// split of their keys, 64 (as registers allow, else 32) at a time through two LDS stages that
 // hold K and V as 16-bit operands. Products as in attn_split, on 32 x 32
 // tiles: scores K q^T, outputs V^T p^T, so a lane (query lane % 32, half lane
 // / 32) holds the scores of keys 16 k + 8 half .. + 7, its operand of the
 // second product; K's rows are read with bits 2 and 3 exchanged for that.
 template <int FMT, int D>
 EOS_DEV void attn_prompt(const KvAttnArgs& a) {
-  constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4;
+  constexpr bool kQuant = FMT == kKvQ8 || FMT == kKvTq4, kTwo = FMT == kKvTq4;
   constexpr int BITS = bits_of(FMT), KS = D / 16, NT = D / 32;
-  constexpr int NK = D == 256 ? 32 : 64, TT = NK / 32, BLK = NK / 16;
+  constexpr int NK = D == 256 || (D == 128 && kTwo) ? 32 : 64, TT = NK / 32, BLK = NK / 16;
   // 16-byte pieces of 16 tokens and of a stage (of K, and as many of V), a
   // thread's loads, and the operand pieces of one.
   constexpr int C16 = D * BITS / 8, CH = BLK * C16, PER = (CH + 255) / 256, EX = 16 / BITS;
@@ -1576,7 +1592,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   }
 
   // The query as the second operand (see attn_split).
-  v4u q[KS];
+  v4u q[KS], q2[kTwo ? KS : 1];
   float qs = fabsf(a.scale);
   {
     const uint8_t* src = a.q + ((size_t)(t.s.row0 + qrow) * a.q_stride +
@@ -1620,15 +1636,19 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
 #pragma unroll
       for (int i = 0; i < D / 2; ++i) most = fmaxf(most, fabsf(x[i / 8][i % 8]));
       most = fmaxf(most, __shfl_xor(most, 32));
-      const int ex = most > 0.0f && most < __builtin_inff() ? __builtin_amdgcn_frexp_expf(most) : 0;
-      float down = __builtin_amdgcn_ldexpf(1.0f, kv_max(-ex, -126));
+      int ex = most > 0.0f && most < __builtin_inff() ? __builtin_amdgcn_frexp_expf(most) : 0;
+      ex = kv_max(ex, -100) - kQUp;
+      float down = __builtin_amdgcn_ldexpf(1.0f, -ex);
       qs = __builtin_amdgcn_ldexpf(qs, ex);
       if (neg != 0) down = -down;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          q[s][i] = pack2<FMT>(x[s][slot_of<FMT>(2 * i)] * down, x[s][slot_of<FMT>(2 * i + 1)] * down);
+        for (int i = 0; i < 4; ++i) {
+          const v2u w = query2<FMT>(x[s][slot_of<FMT>(2 * i)] * down, x[s][slot_of<FMT>(2 * i + 1)] * down);
+          q[s][i] = w[0];
+          if (kTwo) q2[kTwo ? s : 0][i] = w[1];
+        }
     }
   }
   // Scores are compared before their factor, which must not be zero for it.
@@ -1649,8 +1669,11 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
       const int row = tt * 32 + krow;
       const int sw = (row / RS) & (ROWC - 1);
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
-        s[tt] = mfma32<FMT>(lk[st][row * ROWC + ((2 * k + hh) ^ sw)], q[k], s[tt]);
+      for (int k = 0; k < KS; ++k) {
+        const v4u x = lk[st][row * ROWC + ((2 * k + hh) ^ sw)];
+        s[tt] = mfma32<FMT>(x, q[k], s[tt]);
+        if constexpr (kTwo) s[tt] = mfma32<FMT>(x, q2[k], s[tt]);
+      }
     }
   };
   // One stage: `s` are its scores, `next` becomes those of the following one.

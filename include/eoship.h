@@ -918,7 +918,8 @@ typedef struct EosHipKVCache EosHipKVCache;
  * negative is padding: not written, not read, attends nothing. Position p
  * lies in page page_table[b][p / P]; entries past a sequence's length are not
  * looked at, nor are pages wholly in front of every row's window. Rows from
- * offsets[batch] on are left as they are. Device memory. */
+ * offsets[batch] on are left as they are. A sequence has at most 2^30 tokens.
+ * Device memory. */
 typedef struct {
   const int32_t* d_page_table;  /* [batch][table_stride] */
   int32_t table_stride;

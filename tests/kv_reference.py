@@ -173,8 +173,9 @@ def attention(plan, values, q, heads, dtype, scale, window=0):
     lse = np.full((plan.rows, heads), -np.inf)
     tol, ltol = np.zeros_like(out), np.zeros_like(lse)
     up = U["bf16" if pool.fmt == "bf16" else "f16"]
-    # Rounding of the query: a rotated one goes to f16; any other is exact.
-    uq = U["f16"] if pool.fmt == "tq4" else 0.0
+    # Rounding of the query: a rotated one (log2(d) f32 additions) goes to two f16
+    # terms, 2^-22; any other is exact.
+    uq = U["f16"] ** 2 + (np.log2(d) + 2) * U["f32"] if pool.fmt == "tq4" else 0.0
     back = hadamard(d) * (1 / np.sqrt(d)) if pool.fmt == "tq4" else np.eye(d)
     sg = pool.signs if pool.fmt == "tq4" else np.ones(d)
     for b in range(len(plan.n)):
@@ -197,10 +198,11 @@ def attention(plan, values, q, heads, dtype, scale, window=0):
                 lse[row, j] = top + np.log(tot)
                 qa = np.abs((q[row, j] * sg) @ back)
                 mag = (ka[h, lo:pos + 1] @ qa) * abs(scale)
-                # Score: the query's rounding (what f16 keeps below 2^-14 of its largest: 2^-25
-                # of that), d f32 additions, a few f32 factors; exponential and its argument.
-                small = 2.0 ** -25 * 2 * qa.max() * ka[h, lo:pos + 1].sum(-1) * abs(scale) if uq else 0.0
-                ds = (uq + (d + 8) * U["f32"]) * mag + small + 8 * U["f32"] * (np.abs(s).max() + 2)
+                # Score: the query's rounding (its second term is not below f16's normal range
+                # before 2^-25 of its largest), d f32 additions of two terms, a few f32 factors;
+                # exponential and its argument.
+                small = 2.0 ** -25 * qa.max() * ka[h, lo:pos + 1].sum(-1) * abs(scale) if uq else 0.0
+                ds = (uq + (2 * d + 8) * U["f32"]) * mag + small + 8 * U["f32"] * (np.abs(s).max() + 2)
                 dmax = float(np.max(ds))
                 n = pos + 1 - lo
                 # Weights: rounded to the operand's type (f16 below 2^-14: 2^-25 absolute, of a

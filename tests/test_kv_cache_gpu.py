@@ -391,7 +391,7 @@ def test_what_lies_behind_a_sequence_does_not_reach_it(rt, fmt):
 
 
 def _nan_slots(rt, fmt, lengths, n, stride):
-    heads = 2 if stride is None else 64
+    heads = 2 if stride is None else 128
     w = World(rt, fmt, 1, 64, 16, lengths, n, seed=6, stride=stride)
     w.fill()
     clean = [_attend(w, heads, _io(fmt), window, q=np.ones((10, heads, 64), np.float32))[1:] for window in (0, 9)]
@@ -423,7 +423,7 @@ def test_a_later_token_does_not_reach_earlier_rows(rt, fmt):
     """NaN and infinities in a token of the prompt: rows before it are as
     without it, rows from it on are NaN or follow the infinity."""
     _case(f"NaN token {fmt}")
-    for stride, heads in ((None, 2), (200, 2), (200, 7)):   # 16 and 128 query rows a workgroup
+    for stride, heads in ((None, 2), (200, 2), (200, 11)):   # 16 and 128 query rows a workgroup
         _nan_token(rt, fmt, stride, heads)
 
 
