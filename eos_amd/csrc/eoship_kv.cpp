@@ -414,9 +414,14 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
     // tq4: 164 us, in splits 230; of 2,000 tokens each 46 and 39; 32 of 64 to
     // 4,096 in bf16: 66 and 79. Many workgroups balance by themselves (256
     // sequences of 1,000: 206 in shares, 185 in splits), few keys do not pay for
-    // the prefix sum (4 of up to 3,000: 21 and 16).
+    // the prefix sum (4 of up to 3,000: 21 and 16), and more sequences lose to it
+    // what balance gains, in the smaller formats sooner (one head, 64 to 4,096
+    // tokens: 300 of bf16 77 and 116, 500 of bf16 114 and 135, 900 of f16 190 and
+    // 202, but of 2,000 each 185 and 170; 300 of q8 51 and 54, 500 of q8 74 and
+    // 63; 300 of tq4 51 and 60, 400 of tq4 65 and 58, 300 of 2,000 each 43 and 37).
     const long long steps = ((long long)batch->table_stride << kv->page_shift) / 128;
-    if (batch->d_offsets == nullptr && batch->batch > 1 && batch->batch <= kKvStreamBatch &&
+    const int most = kv->d.format <= kKvBf16 ? kKvStreamBatch : kKvStreamBatch / 2;
+    if (batch->d_offsets == nullptr && batch->batch > 1 && batch->batch <= most &&
         units < 4 * slots && steps * units >= 4 * slots) {
       a.workgroups = (int)slots;
       const size_t parts = (size_t)a.workgroups * 2 * kKvTileRows;

@@ -10,7 +10,7 @@ enum { kKvF16 = 0, kKvBf16 = 1, kKvQ8 = 2, kKvTq4 = 3 };
 enum { kKvRowF16 = 0, kKvRowBf16 = 1, kKvRowF32 = 2 };
 
 constexpr int kKvFewSplits = 8;        // splits that one lane group joins by itself
-constexpr int kKvStreamBatch = 1024;  // sequences whose steps a workgroup keeps in LDS
+constexpr int kKvStreamBatch = 512;   // sequences whose steps every workgroup sums up
 
 // Status bits a kernel sets when what it read from the device was out of
 // range (nothing outside the pool and the rows is touched).

@@ -285,14 +285,15 @@ def test_single_token_rows_of_many_lengths(rt, fmt, d, kvh, group, p, window):
     _check(w, kvh * group, _io(fmt, group), window=window, pad=8)
 
 
-@pytest.mark.parametrize("batch", [2, 300, 1024, 1025])
-def test_single_token_rows_of_many_sequences(rt, batch):
-    _case(f"decode batch {batch}")
+@pytest.mark.parametrize("fmt", ["q8", "bf16"])
+@pytest.mark.parametrize("batch", [2, 65, 256, 257, 300, 512, 513, 1024, 1025])
+def test_single_token_rows_of_many_sequences(rt, fmt, batch):
+    _case(f"decode batch {batch} {fmt}")
     lengths = np.random.default_rng(batch).integers(0, 40, batch)
     lengths[-1] = 300
-    w = World(rt, "q8", 1, 32, 16, lengths, np.ones_like(lengths), seed=batch, stride=40000 // batch)
+    w = World(rt, fmt, 1, 32, 16, lengths, np.ones_like(lengths), seed=batch, stride=40000 // batch)
     w.fill()
-    _check(w, 2, "f16")
+    _check(w, 2, _io(fmt))
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -331,6 +332,24 @@ def test_windows_on_single_tokens(rt, fmt):
         w.plan.table[w.plan.table < 0] = 0
         want, wl, tol, ltol = ref.attention(w.plan, vals, q64, 4, _io(fmt), 64 ** -0.5, window)
         assert (np.abs(out - want) <= tol).all() and (np.abs(lse - wl) <= ltol).all()
+
+
+@pytest.mark.parametrize("rows", [False, True])
+def test_widest_windows(rt, rows):
+    """Windows of any width up to the type's largest, also beside padding rows
+    whose positions are negative, as without one."""
+    _case(f"widest windows rows={rows}")
+    lengths = np.array([3, 40, 90])
+    n = np.array([5, 40, 7]) if rows else np.ones(3, int)
+    w = World(rt, "bf16", 1, 64, 16, lengths, n, seed=1)
+    w.fill()
+    q = w.rng.normal(size=(w.plan.rows, 3, 64)).astype(np.float32)
+    want = _attend(w, 3, "bf16", q=q)[1:]
+    for window in (96, 2 ** 30, 2 ** 31 - 1):
+        got = _attend(w, 3, "bf16", window, q=q)[1:]
+        np.testing.assert_array_equal(got[0], want[0])
+        np.testing.assert_array_equal(got[1], want[1])
+    w.cache.status()
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
