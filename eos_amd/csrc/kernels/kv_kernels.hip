@@ -822,6 +822,23 @@ EOS_DEV void split_odd(v4u& x, v4u& pos, v4u& neg) {
   pos = v4u{up[0], up[1], up[2], up[3]};
   neg = v4u{down[0], down[1], down[2], down[3]};
 }
+// Quantized formats: a row's weights are 2^(score - m) for its weights' sum and
+// times the V scale for the products. One reference m follows the score plus
+// the scale's exponent, over the keys that the row attends and no others, so that
+// what it does not see or hardly weighs takes no bits from what it does. An
+// exponent counts as -64 at least (a scale of zero): the sum of the weights stays
+// below 2^(64 + 8) a key, and above 2^-41 as scales end at 2^40.
+constexpr float kMostProduct = 0x1p8f, kMostWeight = 0x1p72f;
+EOS_DEV float scale_exp(float vs) {
+  return vs > 0.0f ? fmaxf((float)__builtin_amdgcn_frexp_expf(vs), -64.0f) : -64.0f;
+}
+// x 2^d for d <= 0, by halves: a sum of weights may be far above 1 where 2^d
+// alone is below f32's range.
+EOS_DEV float decay(float x, float d) {
+  const float h = __builtin_amdgcn_exp2f(0.5f * d);
+  return x * h * h;
+}
+
 // What the odd values that a row sees add to its sum.
 EOS_DEV float odd_sum(float up, float down) {
   const float inf = __builtin_inff();
@@ -987,10 +1004,9 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
   v4f acc[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = v4f{0, 0, 0, 0};
-  // Probabilities are 2^(score - m - e): m follows the scores, 2^e the scales
-  // of V, so that probability times scale stays below 2^8 in f16. Both move
-  // only when a score passes m + 8 or a scale 2^e.
-  float m = kLowest, l = 0.0f, e = kQuant ? -100.0f : 0.0f, elim = 0x1p-100f;
+  // Weights are 2^(score - m): m moves only when one (in quantized formats one
+  // times its scale) passes 2^8.
+  float m = kLowest, l = 0.0f;
   const size_t head_bytes = ((size_t)D * BITS / 8) << c.page_shift;
   bool odd_seen = false;  // a value of V that is NaN or infinite in a masked step
   // A step's codes and scales as loaded: the next step's are on their way
@@ -1089,40 +1105,58 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
         if (!there) vmask[i >> 1] &= (i & 1) != 0 ? 0x0000ffffu : 0xffff0000u;
       }
     }
-    float mx = x[0];
+    float p[8];
+    if constexpr (!kQuant) {
+      float mx = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-    if (__any(mx > m + 8.0f)) {
-      const float nm = fmaxf(m, group_max(mx));
-      const float f = __builtin_amdgcn_exp2f(m - nm);
-      m = nm;
-      l *= f;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) acc[i] *= f;
-    }
-    if constexpr (kQuant) {
-      float mv = vs[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) mv = fmaxf(mv, vs[i]);
-      if (__any(mv > elim)) {
-        mv = group_max(mv);
-        const float ne = fmaxf(e, (float)__builtin_amdgcn_frexp_expf(mv));
-        const float f = __builtin_amdgcn_exp2f(e - ne);
-        e = ne;
-        elim = __builtin_amdgcn_ldexpf(1.0f, (int)ne);
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+      if (__any(mx > m + 8.0f)) {
+        const float nm = fmaxf(m, group_max(mx));
+        const float f = __builtin_amdgcn_exp2f(m - nm);
+        m = nm;
         l *= f;
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] *= f;
       }
-    }
-    const float ref = m + e;
-    float p[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(x[i] - ref);
-      l += p[i];
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(x[i] - m);
+        l += p[i];
+      }
+    } else {
+      float w[8];
       // (a masked key's scale may be NaN: it must not reach the row)
-      if (kQuant) p[i] = masked && x[i] == -__builtin_inff() ? 0.0f : p[i] * vs[i];
+      auto weigh = [&]() KV_INLINE {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(x[i] - m);
+          w[i] = masked && x[i] == -__builtin_inff() ? 0.0f : p[i] * vs[i];
+        }
+      };
+      weigh();
+      float mw = w[0], mp = p[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        mw = fmaxf(mw, w[i]);
+        mp = fmaxf(mp, p[i]);
+      }
+      if (__any(mw > kMostProduct || mp > kMostWeight)) {
+        float y = x[0] + scale_exp(vs[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) y = fmaxf(y, x[i] + scale_exp(vs[i]));
+        const float nm = fmaxf(m, group_max(y));
+        const float f = __builtin_amdgcn_exp2f(m - nm);
+        l = decay(l, m - nm);
+        m = nm;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] *= f;
+        weigh();
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        l += p[i];
+        p[i] = w[i];
+      }
     }
     v4u pf;
 #pragma unroll
@@ -1221,16 +1255,15 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
 
   // The four wavefronts' parts, brought to one reference.
   l = group_sum(l);
-  const float ref = m + e;
   if (g == 0) {
-    sm[wave][r16] = ref;
+    sm[wave][r16] = m;
     sl[wave][r16] = l;
   }
   __syncthreads();
   float top = sm[0][r16];
 #pragma unroll
   for (int w = 1; w < 4; ++w) top = fmaxf(top, sm[w][r16]);
-  const float f = __builtin_amdgcn_exp2f(ref - top);
+  const float f = __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -1243,7 +1276,7 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
 #pragma unroll
     for (int w = 1; w < 4; ++w) mt = fmaxf(mt, sm[w][r]);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) lt += sl[w][r] * __builtin_amdgcn_exp2f(sm[w][r] - mt);
+    for (int w = 0; w < 4; ++w) lt += decay(sl[w][r], sm[w][r] - mt);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int at = r * D + l8 * 8 + i;
@@ -1417,7 +1450,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   constexpr int ROWC = D / 8;  // operand pieces of a K row
   constexpr int RS = ROWC >= 16 ? 1 : 16 / ROWC;  // K rows that share 256 bytes
   __shared__ v4u lk[2][NK * ROWC], lv[2][NK * ROWC];
-  __shared__ float lsc[2][2][kQuant ? NK : 1];
+  __shared__ float lsc[2][3][kQuant ? NK : 1];  // scales of K and of V, exponents of V's
   // Whether a stage that some row masks held a NaN or infinity in V: such
   // values are staged as zero (weight 0 would not stop them) and added at the
   // end to the rows that see them.
@@ -1589,7 +1622,10 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
       for (int e = 0; e < EX; ++e) lv[st][(blk * 2 + grp) * D + rest % (D / EX) * EX + e] = x[e];
     }
     if constexpr (kQuant)
-      if (tid < 2 * NK) lsc[st][tid / NK][tid % NK] = scr;
+      if (tid < 2 * NK) {
+        lsc[st][tid / NK][tid % NK] = scr;
+        if (tid >= NK) lsc[st][2][tid % NK] = scale_exp(scr);
+      }
   };
 
   if (tid == 0) lodd = 0;
@@ -1668,8 +1704,10 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   v16f acc[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = v16f{0};
-  float m = kLowest, l = 0.0f, e = kQuant ? -100.0f : 0.0f, elim = 0x1p-100f;
-  float lim = (m + 8.0f) * iqs;
+  float m = kLowest, l = 0.0f;
+  // What a score (quantized: a score times its factor, plus its scale's
+  // exponent) may be before m moves.
+  float lim = (m + 8.0f) * (kQuant ? 1.0f : iqs);
   // K row of lane r32: token bits 2 and 3 exchanged.
   const int krow = (r32 & 19) | (r32 >> 1 & 4) | (r32 << 1 & 8);
   auto scores = [&](int st, v16f (&s)[TT]) KV_INLINE {
@@ -1696,16 +1734,11 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
     }
     if (tb < w_hi && tb + NK > w_lo) {
       const bool masked = tb + NK > w_all_hi || tb < w_all_lo || ok0 != (1 << BLK) - 1;
-      float mv = 0.0f;
       if constexpr (kQuant) {
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int tok = 32 * tt + 16 * (i / 8) + 8 * hh + i % 8;
-            s[tt][i] *= lsc[st][0][tok];
-            mv = fmaxf(mv, lsc[st][1][tok]);
-          }
+          for (int i = 0; i < 16; ++i) s[tt][i] *= lsc[st][0][32 * tt + 16 * (i / 8) + 8 * hh + i % 8];
       }
       if (masked) {
 #pragma unroll
@@ -1717,33 +1750,24 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
               s[tt][i] = -__builtin_inff();
           }
       }
-      float mx = s[0][0];
+      float mx = -__builtin_inff();
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tt][i]);
+        for (int i = 0; i < 16; ++i) {
+          float y = s[tt][i];
+          if constexpr (kQuant) y = __builtin_fmaf(y, qs, lsc[st][2][32 * tt + 16 * (i / 8) + 8 * hh + i % 8]);
+          mx = fmaxf(mx, y);
+        }
       if (__any(mx > lim)) {
-        const float nm = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * qs);
+        const float nm = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * (kQuant ? 1.0f : qs));
         const float f = __builtin_amdgcn_exp2f(m - nm);
+        l = kQuant ? decay(l, m - nm) : l * f;
         m = nm;
-        lim = (m + 8.0f) * iqs;
-        l *= f;
+        lim = (m + 8.0f) * (kQuant ? 1.0f : iqs);
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] *= f;
       }
-      if constexpr (kQuant) {
-        if (__any(mv > elim)) {
-          mv = fmaxf(mv, __shfl_xor(mv, 32));
-          const float ne = fmaxf(e, (float)__builtin_amdgcn_frexp_expf(mv));
-          const float f = __builtin_amdgcn_exp2f(e - ne);
-          e = ne;
-          elim = __builtin_amdgcn_ldexpf(1.0f, (int)ne);
-          l *= f;
-#pragma unroll
-          for (int i = 0; i < NT; ++i) acc[i] *= f;
-        }
-      }
-      const float ref = -(m + e);
       scores(st ^ 1, next);
       v4u pf[2 * TT];
 #pragma unroll
@@ -1752,7 +1776,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float x = s[kk / 2][8 * (kk % 2) + i];
-          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, qs, ref));
+          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, qs, -m));
           l += p[i];
           // (a masked key's scale may be NaN: it must not reach the row)
           if constexpr (kQuant)
@@ -1826,7 +1850,6 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
     }
   }
   l += __shfl_xor(l, 32);
-  const float ref = m + e;
   if (a.splits > 1) {
     if (!real) return;
     const size_t at = (((size_t)u * c.kv_heads + h) * a.splits + split) * kKvPromptRows + 32 * wave + r32;
@@ -1837,7 +1860,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
         *reinterpret_cast<v4f*>(a.part + at * D + 32 * n + 8 * k + 4 * hh) =
             v4f{acc[n][4 * k], acc[n][4 * k + 1], acc[n][4 * k + 2], acc[n][4 * k + 3]};
     if (hh == 0) {
-      a.part_ml[at * 2] = ref;
+      a.part_ml[at * 2] = m;
       a.part_ml[at * 2 + 1] = l;
     }
     return;
@@ -1895,7 +1918,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
     }
   if (a.lse != nullptr && hh == 0)
     a.lse[(size_t)row * a.heads + head] =
-        l != 0.0f ? (ref + __log2f(l)) * 0.69314718056f : -__builtin_inff();
+        l != 0.0f ? (m + __log2f(l)) * 0.69314718056f : -__builtin_inff();
 }
 
 // One split's part of a row, D / 8 lanes.
@@ -1927,8 +1950,8 @@ EOS_DEV void join_parts(const KvAttnArgs& a, const KvSeq& s, int r, int h, int n
   for (int i = grp; i < n; i += NG) {
     const Part p = i == grp ? first : part(i);
     const float nm = fmaxf(m, p.m), fo = __builtin_amdgcn_exp2f(m - nm), fn = __builtin_amdgcn_exp2f(p.m - nm);
+    l = decay(l, m - nm) + decay(p.l, p.m - nm);
     m = nm;
-    l = l * fo + p.l * fn;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       x[k] = x[k] * fo + p.lo[k] * fn;
@@ -1951,7 +1974,7 @@ EOS_DEV void join_parts(const KvAttnArgs& a, const KvSeq& s, int r, int h, int n
   for (int k = 0; k < 8; ++k) x[k] = 0.0f;
   for (int i = 0; i < used; ++i) {
     const float f = __builtin_amdgcn_exp2f(sm[i] - top);
-    l += sl[i] * f;
+    l += decay(sl[i], sm[i] - top);
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] += so[i][l8 * 8 + k] * f;
   }
@@ -2023,8 +2046,8 @@ EOS_DEV void attn_join_few(const KvAttnArgs& a) {
     if (i < n) {
       const float nm = fmaxf(m, p[i].m);
       const float fo = __builtin_amdgcn_exp2f(m - nm), fn = __builtin_amdgcn_exp2f(p[i].m - nm);
+      l = decay(l, m - nm) + decay(p[i].l, p[i].m - nm);
       m = nm;
-      l = l * fo + p[i].l * fn;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[k] = x[k] * fo + p[i].lo[k] * fn;
