@@ -1126,14 +1126,20 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
     } else {
       float w[8];
       // (a masked key's scale may be NaN: it must not reach the row)
-      auto weigh = [&]() KV_INLINE {
+      auto weigh = [&](bool limit) KV_INLINE {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(x[i] - m);
+          float d = x[i] - m;
+          // (a score beyond 2^24 absorbs an exponent: nothing passes its limit)
+          if (limit) {
+            const float most = 8.0f - scale_exp(vs[i]);
+            d = d > most ? most : d;
+          }
+          p[i] = __builtin_amdgcn_exp2f(d);
           w[i] = masked && x[i] == -__builtin_inff() ? 0.0f : p[i] * vs[i];
         }
       };
-      weigh();
+      weigh(false);
       float mw = w[0], mp = p[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) {
@@ -1150,7 +1156,7 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
         m = nm;
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] *= f;
-        weigh();
+        weigh(true);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -1705,6 +1711,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = v16f{0};
   float m = kLowest, l = 0.0f;
+  constexpr float kFar = 0x1p20f;
   // What a score (quantized: a score times its factor, plus its scale's
   // exponent) may be before m moves.
   float lim = (m + 8.0f) * (kQuant ? 1.0f : iqs);
@@ -1759,14 +1766,32 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
           if constexpr (kQuant) y = __builtin_fmaf(y, qs, lsc[st][2][32 * tt + 16 * (i / 8) + 8 * hh + i % 8]);
           mx = fmaxf(mx, y);
         }
+      float from = m;
       if (__any(mx > lim)) {
         const float nm = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * (kQuant ? 1.0f : qs));
         const float f = __builtin_amdgcn_exp2f(m - nm);
         l = kQuant ? decay(l, m - nm) : l * f;
-        m = nm;
+        m = from = nm;
         lim = (m + 8.0f) * (kQuant ? 1.0f : iqs);
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] *= f;
+        // Scores so large that a product's rounding is no longer small beside 1:
+        // they are rounded before they are compared with m, as m was, stage by
+        // stage (any score passes this limit).
+        const bool far = fabsf(m) > kFar && m > kLowest;
+        if (far) lim = -__builtin_inff();
+        if (__any(far)) {
+#pragma unroll
+          for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float most = 8.0f;
+              if constexpr (kQuant) most -= lsc[st][2][32 * tt + 16 * (i / 8) + 8 * hh + i % 8];
+              const float d = s[tt][i] * qs - m;
+              s[tt][i] = (d > most ? most : d) * iqs;
+            }
+          from = 0.0f;
+        }
       }
       scores(st ^ 1, next);
       v4u pf[2 * TT];
@@ -1776,7 +1801,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float x = s[kk / 2][8 * (kk % 2) + i];
-          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, qs, -m));
+          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, qs, -from));
           l += p[i];
           // (a masked key's scale may be NaN: it must not reach the row)
           if constexpr (kQuant)

@@ -1,0 +1,51 @@
+"""Attention where scores, weights and values span wide ranges."""
+import numpy as np
+import pytest
+
+from test_kv_cache_gpu import World, _attend, _case
+
+pytestmark = pytest.mark.gpu
+
+# One row a sequence (splits of the length, and equal shares of a wide table),
+# 16 and 128 query rows a workgroup: batch, rows, heads, table columns.
+FORMS = {"split": (1, 1, 2, None), "shares": (3, 1, 2, 40000), "rows16": (2, 5, 2, None),
+         "rows128": (1, 64, 6, 200)}
+
+
+def _world(rt, fmt, form, n, seed, rows, d=64):
+    batch, r, heads, stride = FORMS[form]
+    w = World(rt, fmt, 1, d, 16, np.full(batch, n), np.full(batch, r), seed=seed, shuffle=False,
+              stride=stride, spare=0)
+    each = -(-n // 16) * 16
+
+    def values(x):
+        for b in range(batch):
+            rows(x[:, each * b:each * b + n])
+        return x
+    w.fill(values)
+    return w, heads
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "q8", "tq4"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_equal_scores_of_any_size(rt, fmt, form, sign):
+    """Equal keys whose score is far beyond f32's whole numbers (and no power of
+    two, so that its products are rounded): weights as equal as ever."""
+    _case(f"far scores {fmt} {form} {sign}")
+    size = 2.0 ** (14 if fmt == "f16" else 30)
+
+    def rows(x):
+        x[0] = 1.37 * size
+        x[1] = 1.5
+    w, heads = _world(rt, fmt, form, 90, 1, rows)
+    io = "f16" if fmt == "f16" else "bf16"
+    q = np.full((w.plan.rows, heads, 64), sign * 1.7 * size, np.float32)
+    q64, out, lse = _attend(w, heads, io, q=q)
+    k, v = (x[w.plan.table[0, 0], 0, 0] for x in w.pool.values())
+    # equal weights of equal values: the output's rounding and the weights' (one
+    # 16-bit value, in a bf16 cache 2^-8 off), sums in f32
+    tol = (2.0 ** -8 + 2.0 ** -8 + 200 * 2.0 ** -24) * np.abs(v).max()
+    assert (np.abs(out - v) <= tol).all(), (float(out.min()), float(out.max()))
+    s = float(k @ q64[0, 0]) / 8
+    assert (np.abs(lse - s) <= 2.0 ** -14 * abs(s)).all()
