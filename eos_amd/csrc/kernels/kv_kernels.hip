@@ -37,7 +37,7 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr float kTiny = 0x1p-60f, kHuge = 0x1p40f;
-constexpr float kLowest = -1e30f;  // softmax reference before any key
+constexpr float kLowest = -0x1.fffffep127f;  // softmax reference before any key: below every score
 
 constexpr int bits_of(int fmt) { return fmt == kKvQ8 ? 8 : fmt == kKvTq4 ? 4 : 16; }
 constexpr int log2i(int x) { return x <= 1 ? 0 : 1 + log2i(x / 2); }

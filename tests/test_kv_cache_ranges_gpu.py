@@ -49,3 +49,24 @@ def test_equal_scores_of_any_size(rt, fmt, form, sign):
     assert (np.abs(out - v) <= tol).all(), (float(out.min()), float(out.max()))
     s = float(k @ q64[0, 0]) / 8
     assert (np.abs(lse - s) <= 2.0 ** -14 * abs(s)).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("fmt", ["bf16", "q8", "tq4"])
+def test_scores_of_any_size_below_zero(rt, fmt, form):
+    """Every key's score is -2^108 and less: the weights are as equal as ever."""
+    _case(f"low scores {fmt} {form}")
+
+    def rows(x):
+        x[0] = -2.0 ** 39                   # (scales of tq4 end at 2^40)
+        x[1] = 1.5
+    w, heads = _world(rt, fmt, form, 90, 1, rows)
+    q = np.full((w.plan.rows, heads, 64), 2.0 ** 66, np.float32)
+    q64, out, lse = _attend(w, heads, "bf16", q=q)
+    k, v = (x[w.plan.table[0, 0], 0, 0] for x in w.pool.values())
+    # equal weights of equal values: the output's rounding, some f32 sums and the
+    # weights' roundings (one 16-bit value each, its sum exact in f32)
+    tol = (2.0 ** -8 + 2.0 ** -8 + 200 * 2.0 ** -24) * np.abs(v).max()
+    assert (np.abs(out - v) <= tol).all(), (float(out.min()), float(out.max()))
+    s = float(k @ q64[0, 0]) / 8
+    assert np.isfinite(lse).all() and (np.abs(lse - s) <= 2.0 ** -14 * abs(s)).all()
