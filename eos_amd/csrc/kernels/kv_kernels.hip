@@ -822,13 +822,22 @@ EOS_DEV void split_odd(v4u& x, v4u& pos, v4u& neg) {
   pos = v4u{up[0], up[1], up[2], up[3]};
   neg = v4u{down[0], down[1], down[2], down[3]};
 }
+// Where a row's largest weight is put when its reference moves, as a power of
+// two: f16 holds weights from 2^-24 to 2^16, so the more of them lie above its
+// steps the higher the largest does; bf16 has f32's range. A weight (with its V
+// scale) may grow by 2^8 before the reference moves again.
+template <int FMT>
+constexpr float kTop = FMT == kKvBf16 ? 0.0f : 7.0f;
+template <int FMT>
+constexpr float kMost = kTop<FMT> + 8.0f;
+
 // Quantized formats: a row's weights are 2^(score - m) for its weights' sum and
 // times the V scale for the products. One reference m follows the score plus
 // the scale's exponent, over the keys that the row attends and no others, so that
 // what it does not see or hardly weighs takes no bits from what it does. An
-// exponent counts as -64 at least (a scale of zero): the sum of the weights stays
-// below 2^(64 + 8) a key, and above 2^-41 as scales end at 2^40.
-constexpr float kMostProduct = 0x1p8f, kMostWeight = 0x1p72f;
+// exponent counts as -64 at least (a scale of zero): a weight stays below 2^(64
+// + 15), and their sum above 2^(6 - 41) as scales end at 2^40.
+constexpr float kMostProduct = 0x1p15f, kMostWeight = 0x1p79f;
 EOS_DEV float scale_exp(float vs) {
   return vs > 0.0f ? fmaxf((float)__builtin_amdgcn_frexp_expf(vs), -64.0f) : -64.0f;
 }
@@ -1005,7 +1014,7 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = v4f{0, 0, 0, 0};
   // Weights are 2^(score - m): m moves only when one (in quantized formats one
-  // times its scale) passes 2^8.
+  // times its scale) passes its limit.
   float m = kLowest, l = 0.0f;
   const size_t head_bytes = ((size_t)D * BITS / 8) << c.page_shift;
   bool odd_seen = false;  // a value of V that is NaN or infinite in a masked step
@@ -1110,8 +1119,8 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
       float mx = x[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-      if (__any(mx > m + 8.0f)) {
-        const float nm = fmaxf(m, group_max(mx));
+      if (__any(mx > m + kMost<FMT>)) {
+        const float nm = fmaxf(m, group_max(mx) - kTop<FMT>);
         const float f = __builtin_amdgcn_exp2f(m - nm);
         m = nm;
         l *= f;
@@ -1132,7 +1141,7 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
           float d = x[i] - m;
           // (a score beyond 2^24 absorbs an exponent: nothing passes its limit)
           if (limit) {
-            const float most = 8.0f - scale_exp(vs[i]);
+            const float most = kMost<FMT> - scale_exp(vs[i]);
             d = d > most ? most : d;
           }
           p[i] = __builtin_amdgcn_exp2f(d);
@@ -1150,7 +1159,7 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
         float y = x[0] + scale_exp(vs[0]);
 #pragma unroll
         for (int i = 1; i < 8; ++i) y = fmaxf(y, x[i] + scale_exp(vs[i]));
-        const float nm = fmaxf(m, group_max(y));
+        const float nm = fmaxf(m, group_max(y) - kTop<FMT>);
         const float f = __builtin_amdgcn_exp2f(m - nm);
         l = decay(l, m - nm);
         m = nm;
@@ -1714,7 +1723,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   constexpr float kFar = 0x1p20f;
   // What a score (quantized: a score times its factor, plus its scale's
   // exponent) may be before m moves.
-  float lim = (m + 8.0f) * (kQuant ? 1.0f : iqs);
+  float lim = (m + kMost<FMT>) * (kQuant ? 1.0f : iqs);
   // K row of lane r32: token bits 2 and 3 exchanged.
   const int krow = (r32 & 19) | (r32 >> 1 & 4) | (r32 << 1 & 8);
   auto scores = [&](int st, v16f (&s)[TT]) KV_INLINE {
@@ -1768,11 +1777,11 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
         }
       float from = m;
       if (__any(mx > lim)) {
-        const float nm = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * (kQuant ? 1.0f : qs));
+        const float nm = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * (kQuant ? 1.0f : qs) - kTop<FMT>);
         const float f = __builtin_amdgcn_exp2f(m - nm);
         l = kQuant ? decay(l, m - nm) : l * f;
         m = from = nm;
-        lim = (m + 8.0f) * (kQuant ? 1.0f : iqs);
+        lim = (m + kMost<FMT>) * (kQuant ? 1.0f : iqs);
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] *= f;
         // Scores so large that a product's rounding is no longer small beside 1:
@@ -1785,7 +1794,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
           for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              float most = 8.0f;
+              float most = kMost<FMT>;
               if constexpr (kQuant) most -= lsc[st][2][32 * tt + 16 * (i / 8) + 8 * hh + i % 8];
               const float d = s[tt][i] * qs - m;
               s[tt][i] = (d > most ? most : d) * iqs;

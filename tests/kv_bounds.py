@@ -4,7 +4,7 @@ weights give: what a row does not attend, or hardly weighs, allows it nothing.
 A weight times its V scale (the weight alone in a cache without scales) is
 rounded to the matrix operand's 16 bits: by u = 2^-11 (f16) or 2^-8 (bf16) of
 itself, in f16 at least by half the smallest step, 2^-25, where the largest
-product of the row that a reference was taken from is at least 2^-1."""
+product of the row that a reference was taken from is at least 2^6."""
 import numpy as np
 
 import kv_reference as ref
@@ -62,9 +62,9 @@ def attention(plan, q, heads, dtype, scale, window=0):
                         one = p * vah.max(-1)
                         if tq4:  # (a row may lack the largest magnitude)
                             one = p * np.sqrt((vah ** 2).mean(-1)) * 4.0
-                        e = e + 2.0 ** -24 * n * one.max() / tot
+                        e = e + 2.0 ** -31 * n * one.max() / tot
                     else:
-                        e = e + 2.0 ** -24 * vah.sum(0) * p.max() / tot
+                        e = e + 2.0 ** -31 * vah.sum(0) * p.max() / tot
                 if tq4:  # rotated back: every coordinate has a share of each error
                     e = np.full(d, np.sqrt((e * e).sum()))
                 tol[row, j] = U[dtype] * (np.abs(out[row, j]) + e) + e + (2.0 ** -25 if dtype == "f16" else 0)

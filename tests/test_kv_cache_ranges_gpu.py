@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import kv_bounds
 from test_kv_cache_gpu import World, _attend, _case
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +71,25 @@ def test_scores_of_any_size_below_zero(rt, fmt, form):
     assert (np.abs(out - v) <= tol).all(), (float(out.min()), float(out.max()))
     s = float(k @ q64[0, 0]) / 8
     assert np.isfinite(lse).all() and (np.abs(lse - s) <= 2.0 ** -14 * abs(s)).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_small_weights_of_large_values(rt, form):
+    """f16: 16 keys of weight 2^-26 and value 2^15 beside one of weight 1 and
+    value 0: what they give is the whole of the row."""
+    _case(f"small weights {form}")
+
+    def rows(x):
+        x[0] = 0.0
+        x[0, 3] = 26 * np.log(2) / 8
+        x[1] = 0.0
+        x[1, 4:20] = 2.0 ** 15
+    w, heads = _world(rt, "f16", form, 90, 2, rows)
+    q = np.ones((w.plan.rows, heads, 64), np.float32)
+    q64, out, lse = _attend(w, heads, "f16", q=q)
+    want, wl, tol, ltol = kv_bounds.attention(w.plan, q64, heads, "f16", 64 ** -0.5)
+    # (16 weights' smallest steps are 16 * 2^15 * 2^-31 = 2^-12, every rounding to 11
+    # bits 2^-7 * 2^-11 and so little beside it; nothing summed would be 2^-7 off)
+    assert want.min() > 2.0 ** -8 and tol.max() < 2.0 ** -11, (want.min(), tol.max())
+    assert (np.abs(out - want) <= tol).all(), (float(out.min()), float(want.min()))
+    assert (np.abs(lse - wl) <= ltol).all()
