@@ -1466,9 +1466,9 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
   constexpr int RS = ROWC >= 16 ? 1 : 16 / ROWC;  // K rows that share 256 bytes
   __shared__ v4u lk[2][NK * ROWC], lv[2][NK * ROWC];
   __shared__ float lsc[2][3][kQuant ? NK : 1];  // scales of K and of V, exponents of V's
-  // Whether a stage that some row masks held a NaN or infinity in V: such
-  // values are staged as zero (weight 0 would not stop them) and added at the
-  // end to the rows that see them.
+  // Whether a stage that some row masks, or that lacks a page, held a NaN or
+  // infinity in V: such values are staged as zero (weight 0 would not stop them)
+  // and added at the end to the rows that see them.
   __shared__ int lodd;
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, hh = lane >> 5;
@@ -1863,7 +1863,12 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
     constexpr uint32_t kOne = FMT == kKvF16 ? 0x3c00u : 0x3f80u;
     for (int tb = begin; tb < end; tb += 16) {
       const int stage = begin + (tb - begin) / NK * NK;
-      if (stage + NK <= all_hi && stage >= all_lo) continue;
+      if (stage + NK <= all_hi && stage >= all_lo) {
+        bool there = true;
+#pragma unroll
+        for (int i = 0; i < BLK; ++i) there &= kv_page(c, seq, stage + 16 * i) >= 0;
+        if (there) continue;
+      }
       const int page = kv_page(c, seq, tb), key = tb + 8 * hh;
       uint32_t see[4] = {0, 0, 0, 0};
 #pragma unroll
