@@ -305,7 +305,8 @@ template <int FMT, int D, int RUN>
 EOS_DEV void append_run(const KvRowsArgs& a) {
   constexpr int LANES = D / 8, NG = RUN / 8;
   constexpr bool kPlain = FMT == kKvF16 || FMT == kKvBf16;
-  __shared__ uint16_t vt[FMT == kKvTq4 ? 1 : NG * D * 8];
+  __shared__ __align__(16) uint16_t vt[FMT == kKvTq4 ? 8 : NG * D * 8];
+  static_assert(__alignof__(vt) >= 16, "read by 16 bytes");
   __shared__ uint32_t vw[FMT == kKvTq4 ? NG * 8 * LANES : 1];
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, h = blockIdx.y;
@@ -462,6 +463,7 @@ EOS_DEV void read_run(const KvRowsArgs& a) {
   constexpr int kType = FMT == kKvF16 ? kKvRowF16 : kKvRowBf16;
   __shared__ __align__(16) uint16_t vh[kPlain ? NG * 8 * D : 8];
   __shared__ __align__(16) uint8_t vb[kPlain ? 16 : NG * 8 * D];
+  static_assert(__alignof__(vh) >= 16 && __alignof__(vb) >= 8, "read by 16 and 8 bytes");
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, h = blockIdx.y;
   KvRun g;
@@ -678,6 +680,7 @@ EOS_DEV void read_tq4_run(const KvRowsArgs& a) {
   constexpr int KS = D / 32, NT = D / 16, LANES = D / 8, NG = kKvRun / 8;
   constexpr int VS = D + 16;  // bytes between V's rows in LDS: 8 rows on different banks
   __shared__ __align__(16) uint8_t vb[kKvRun * VS];
+  static_assert(__alignof__(vb) >= 8 && VS % 8 == 0, "read by 8 bytes");
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, part = lane >> 4, h = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
