@@ -891,6 +891,9 @@ int eoship_hadamard_tq_release(EosHipRuntime* rt, EosHipHadamardTQ* h, char** er
  *      x^2), index = how many midpoints between codebook magnitudes lie below
  *      |w| / (s sqrt(D)), code = index + 8 where w < 0, stands for
  *      signs * Hd (+-codebook[index]) * s / sqrt(D).
+ *      The rotation is summed in f32: a value nearer to a midpoint, or to zero,
+ *      than that rounds may take the code of either side, and not the same one
+ *      from calls with and without row offsets. Equal calls give equal codes.
  * A scale below 2^-60 is stored as zero; a row with a NaN, an infinity or a
  * scale above 2^40 is stored with a NaN scale and reads as NaN.
  * ------------------------------------------------------------------------ */
