@@ -156,6 +156,11 @@ KV_HD int kv_steps(const KvCacheArgs& c, int b, int group, int window) {
   if (!kv_tile(t, 0, kKvTileRows, group, window, 1)) return 0;
   return (t.hi - t.base + 127) / 128;
 }
+// ... of all its tiles (64 bits: 2^23 steps of a thousand tiles pass 32).
+KV_HD int kv_tiles_of(int group) { return (group + kKvTileRows - 1) / kKvTileRows; }
+KV_HD long long kv_seq_steps(const KvCacheArgs& c, int b, int group, int window) {
+  return (long long)kv_steps(c, b, group, window) * kv_tiles_of(group);
+}
 KV_HD long long kv_share(long long steps, int workgroups) {
   const long long q = (steps + workgroups - 1) / workgroups;
   return q < 2 ? 2 : q;

@@ -1332,12 +1332,11 @@ EOS_DEV void stream_steps(const KvAttnArgs& a, long long* pre) {
   __shared__ long long part[4];
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, per = (c.batch + 255) / 256;
-  const int tiles = (a.group + kKvTileRows - 1) / kKvTileRows;
   long long sum = 0;
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
     if (b < c.batch) {
-      const int n = kv_steps(c, b, a.group, a.window) * tiles;
+      const long long n = kv_seq_steps(c, b, a.group, a.window);
       pre[b] = n;
       sum += n;
     }
@@ -1370,7 +1369,7 @@ EOS_DEV void attn_stream(const KvAttnArgs& a) {
   __shared__ long long pre[kKvStreamBatch + 1];
   const KvCacheArgs& c = a.c;
   stream_steps(a, pre);
-  const int tiles = (a.group + kKvTileRows - 1) / kKvTileRows;
+  const int tiles = kv_tiles_of(a.group);
   const long long total = pre[c.batch], all = total * c.kv_heads;
   const long long share = kv_share(all, a.workgroups), start = share * blockIdx.x;
   const long long end = start + share < all ? start + share : all;
@@ -2106,7 +2105,7 @@ EOS_DEV void attn_stream_join(const KvAttnArgs& a) {
   __shared__ long long pre[kKvStreamBatch + 1];
   const KvCacheArgs& c = a.c;
   const int grp = threadIdx.x / (D / 8), b = blockIdx.x, head = blockIdx.y, h = head / a.group;
-  const int tiles = (a.group + kKvTileRows - 1) / kKvTileRows, r = head % a.group;
+  const int tiles = kv_tiles_of(a.group), r = head % a.group;
   const KvSeq s = kv_seq(c, b);
   flag(c, s.bad);
   stream_steps(a, pre);
