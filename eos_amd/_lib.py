@@ -411,6 +411,9 @@ _SIGNATURES = {
                          C.c_void_p], C.c_int),
     "eoship_kv_check_batch": ([C.POINTER(EosHipKVDesc), C.c_void_p, C.c_int32, C.c_int32,
                                C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p], C.c_int),
+    "eoship_kv_check_batch_window": ([C.POINTER(EosHipKVDesc), C.c_void_p, C.c_int32, C.c_int32,
+                                      C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32,
+                                      C.c_void_p], C.c_int),
     "eoship_kv_bind": ([C.c_void_p, C.POINTER(EosHipKVDesc), C.POINTER(C.c_void_p), C.c_void_p],
                        C.c_int),
     "eoship_kv_release": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),

@@ -214,9 +214,18 @@ int eoship_kv_bytes(const EosHipKVDesc* desc, int64_t* pool_bytes, int64_t* scal
 int eoship_kv_check_batch(const EosHipKVDesc* desc, const int32_t* page_table,
                           int32_t table_stride, int32_t batch, const int32_t* lengths,
                           const int32_t* offsets, int64_t rows, int32_t writes, char** err) {
+  return eoship_kv_check_batch_window(desc, page_table, table_stride, batch, lengths, offsets, rows,
+                                      0, writes, err);
+}
+
+int eoship_kv_check_batch_window(const EosHipKVDesc* desc, const int32_t* page_table,
+                                 int32_t table_stride, int32_t batch, const int32_t* lengths,
+                                 const int32_t* offsets, int64_t rows, int32_t window,
+                                 int32_t writes, char** err) {
   const char* what = "eoship_kv_check_batch";
   return guarded(what, err, [&]() -> int {
     if (check_desc(desc, what, err) != 0) return 1;
+    if (window < 0) return set_err(err, "%s: window must not be negative, got %d", what, window);
     if (batch < 0 || rows < 0 || rows > INT32_MAX)
       return set_err(err, "%s: batch and rows must be in 0..2^31-1", what);
     if (batch == 0 || rows == 0) return 0;
@@ -245,7 +254,9 @@ int eoship_kv_check_batch(const EosHipKVDesc* desc, const int32_t* page_table,
       if (s.bad & kKvBadLength)
         return set_err(err, "%s: sequence %d: length %d outside 0..%lld of its table row", what, b,
                        lengths[b], (long long)table_stride * desc->page_tokens);
-      for (int i = 0; i << c.page_shift < s.keys; ++i)
+      // (the first row's window reaches furthest back)
+      const int from = window == 0 ? 0 : s.n == 0 ? s.keys : (int)std::max(0LL, (long long)s.len - s.n - window + 1);
+      for (int i = from >> c.page_shift; from < s.keys && i << c.page_shift < s.keys; ++i)
         if (kv_page(c, b, i << c.page_shift) < 0)
           return set_err(err, "%s: sequence %d: page %d of its table row is %d, not in 0..%lld", what,
                          b, i, page_table[(size_t)b * table_stride + i], (long long)desc->pages - 1);

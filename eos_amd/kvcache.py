@@ -44,9 +44,12 @@ def kv_bytes(fmt: str, kv_heads: int, head_dim: int, page_tokens: int, pages: in
 
 
 def check_batch(fmt: str, kv_heads: int, head_dim: int, page_tokens: int, pages: int, page_table,
-                lengths, offsets=None, rows: int | None = None, writes: bool = False) -> None:
+                lengths, offsets=None, rows: int | None = None, writes: bool = False,
+                window: int = 0) -> None:
     """Checks a batch's host arrays (page ids, lengths, offsets; with
-    ``writes`` also that no page is written twice) before they are uploaded."""
+    ``writes`` also that no page is written twice) before they are uploaded.
+    With a ``window``, attention's own, pages in front of every row's window may
+    be gone; 1 asks for the pages of the rows themselves only."""
     table = np.ascontiguousarray(page_table, np.int32)
     if table.ndim != 2:
         raise ValueError("page_table must be [batch, pages]")
@@ -62,10 +65,10 @@ def check_batch(fmt: str, kv_heads: int, head_dim: int, page_tokens: int, pages:
     if rows is None:
         rows = batch if off is None else int(off[-1])
     d = _desc(fmt, kv_heads, head_dim, page_tokens, pages)
-    _lib.call("eoship_kv_check_batch", C.byref(d), table.ctypes.data_as(C.c_void_p),
+    _lib.call("eoship_kv_check_batch_window", C.byref(d), table.ctypes.data_as(C.c_void_p),
               C.c_int32(table.shape[1]), C.c_int32(batch), lens.ctypes.data_as(C.c_void_p),
               off.ctypes.data_as(C.c_void_p) if off is not None else None, C.c_int64(rows),
-              C.c_int32(int(writes)))
+              C.c_int32(int(window)), C.c_int32(int(writes)))
 
 
 def _address(buf):

@@ -942,6 +942,14 @@ int eoship_kv_bytes(const EosHipKVDesc* desc, int64_t* pool_bytes, int64_t* scal
 int eoship_kv_check_batch(const EosHipKVDesc* desc, const int32_t* page_table,
                           int32_t table_stride, int32_t batch, const int32_t* lengths,
                           const int32_t* offsets, int64_t rows, int32_t writes, char** err);
+/* The same where attention takes a window: page ids in front of every row's
+ * window are not looked at, as the kernels do not (0: no window, as above; 1:
+ * the pages that an append or read of the rows needs). A sequence without rows
+ * then needs no page. */
+int eoship_kv_check_batch_window(const EosHipKVDesc* desc, const int32_t* page_table,
+                                 int32_t table_stride, int32_t batch, const int32_t* lengths,
+                                 const int32_t* offsets, int64_t rows, int32_t window,
+                                 int32_t writes, char** err);
 /* Binds a cache for one runtime. The pools stay the caller's and have to
  * outlive the handle; a second runtime binds them again. */
 int eoship_kv_bind(EosHipRuntime* rt, const EosHipKVDesc* desc, EosHipKVCache** out, char** err);
