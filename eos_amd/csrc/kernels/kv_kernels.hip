@@ -930,7 +930,11 @@ EOS_DEV void attn_segment(const KvAttnArgs& a, KvTile t, int h, int begin, int e
   const KvCacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // The same in every lane, as the compiler cannot see.
+  // The same in every lane, as the compiler cannot see. Results depend on it: with
+  // the loop's bounds in vector registers its body stood under a divergent
+  // condition, and a build gave the weights and a fragment of V overlapping
+  // registers, both live (f16, width 128). A host test looks for such operands in
+  // the built kernels.
   h = __builtin_amdgcn_readfirstlane(h);
   begin = __builtin_amdgcn_readfirstlane(begin);
   end = __builtin_amdgcn_readfirstlane(end);

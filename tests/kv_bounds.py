@@ -28,45 +28,53 @@ def attention(plan, q, heads, dtype, scale, window=0):
     lse = np.full((plan.rows, heads), -np.inf)
     tol, ltol = np.zeros_like(out), np.zeros_like(lse)
     for b in range(len(plan.n)):
-        k, v = plan.sequence(b, vals[0]), plan.sequence(b, vals[1])
+        pos = int(plan.lengths[b]) - int(plan.n[b]) + np.arange(plan.n[b])
+        at = int(plan.offsets[b]) + np.nonzero(pos >= 0)[0]
+        pos = pos[pos >= 0]
+        if not len(pos):
+            continue
+        key = np.arange(int(plan.lengths[b]))
+        see = key <= pos[:, None]
+        if window:
+            see &= key > pos[:, None] - window
+        n = see.sum(1)
+        k, v = (plan.sequence(b, x).copy() for x in vals)
+        k[:, ~see.any(0)] = v[:, ~see.any(0)] = 0.0          # no row's: whatever stands there
         ka, va = np.abs((k * sg) @ back), np.abs((v * sg) @ back)
-        for i in range(plan.n[b]):
-            pos = int(plan.lengths[b]) - int(plan.n[b]) + i
-            if pos < 0:
-                continue
-            lo = max(0, pos - window + 1) if window else 0
-            row, n = int(plan.offsets[b]) + i, pos + 1 - lo
-            for j in range(heads):
-                h = j // group
-                kh, vh, vah = k[h, lo:pos + 1], v[h, lo:pos + 1], va[h, lo:pos + 1]
-                s = (kh @ q[row, j]) * scale
-                top = s.max()
-                p = np.exp(s - top)
-                tot = p.sum()
-                out[row, j] = (p @ vh) / tot
-                lse[row, j] = top + np.log(tot)
-                qa = np.abs((q[row, j] * sg) @ back)
-                # A score: the query's rounding (its second term's smallest step,
-                # 2^-25 of its largest), 2 d f32 additions and a few factors; the
-                # exponential's argument is rounded in f32 beside the reference, which
-                # lies within 64 + 41 of the scores (the exponent of a V scale).
-                small = 2.0 ** -25 * qa.max() * ka[h, lo:pos + 1].sum(-1) * abs(scale) if tq4 else 0.0
-                ds = (uq + (2 * d + 8) * U["f32"]) * ((ka[h, lo:pos + 1] @ qa) * abs(scale)) + small
-                ds = ds + 8 * U["f32"] * (np.abs(s) + np.abs(top) + (110 if quant else 2))
-                # Weight by weight: its score's error, its rounding, f32 sums.
-                rel = up + 2 * (ds + ds.max()) + (n + 64) * 2 * U["f32"]
-                e = ((p * rel) @ vah) / tot
-                if pool.fmt != "bf16":
-                    # operands below the f16 steps, times the largest value one stands for
-                    if quant:
-                        one = p * vah.max(-1)
-                        if tq4:  # (a row may lack the largest magnitude)
-                            one = p * np.sqrt((vah ** 2).mean(-1)) * 4.0
-                        e = e + 2.0 ** -31 * n * one.max() / tot
-                    else:
-                        e = e + 2.0 ** -31 * vah.sum(0) * p.max() / tot
-                if tq4:  # rotated back: every coordinate has a share of each error
-                    e = np.full(d, np.sqrt((e * e).sum()))
-                tol[row, j] = U[dtype] * (np.abs(out[row, j]) + e) + e + (2.0 ** -25 if dtype == "f16" else 0)
-                ltol[row, j] = 2 * ds.max() + (n + 64) * 2 * U["f32"] + 4 * U["f32"] * (abs(lse[row, j]) + 110)
+        for j in range(heads):
+            h = j // group
+            x = np.where(see, (q[at, j] @ k[h].T) * scale, -np.inf)
+            top = x.max(1, keepdims=True)
+            p = np.exp(x - top)
+            tot = p.sum(1, keepdims=True)
+            got = (p @ v[h]) / tot
+            out[at, j], lse[at, j] = got, top[:, 0] + np.log(tot[:, 0])
+            qa = np.abs((q[at, j] * sg) @ back)
+            # A score: the query's rounding (its second term's smallest step, 2^-25
+            # of its largest), 2 d f32 additions and a few factors; the exponential's
+            # argument is rounded in f32 beside the reference, which lies within 64 +
+            # 41 of the scores (the exponent of a V scale).
+            ds = (uq + (2 * d + 8) * U["f32"]) * ((qa @ ka[h].T) * abs(scale))
+            if tq4:
+                ds += 2.0 ** -25 * qa.max(1, keepdims=True) * ka[h].sum(-1) * abs(scale)
+            far = np.where(see, np.abs(x), 0)
+            ds += 8 * U["f32"] * (far + np.abs(top) + (110 if quant else 2))
+            ds = np.where(see, ds, 0)
+            most = ds.max(1, keepdims=True)
+            # Weight by weight: its score's error, its rounding, f32 sums.
+            rel = up + 2 * (ds + most) + (n[:, None] + 64) * 2 * U["f32"]
+            e = ((p * rel) @ va[h]) / tot
+            if pool.fmt != "bf16":
+                # operands below the f16 steps, times the largest value one stands for
+                if quant:
+                    big = va[h].max(-1)
+                    if tq4:  # (a row may lack the largest magnitude)
+                        big = np.sqrt((va[h] ** 2).mean(-1)) * 4.0
+                    e += 2.0 ** -31 * n[:, None] * (p * big).max(1, keepdims=True) / tot
+                else:
+                    e += 2.0 ** -31 * (see @ va[h]) / tot
+            if tq4:  # rotated back: every coordinate has a share of each error
+                e = np.repeat(np.sqrt((e * e).sum(1, keepdims=True)), d, 1)
+            tol[at, j] = U[dtype] * (np.abs(got) + e) + e + (2.0 ** -25 if dtype == "f16" else 0)
+            ltol[at, j] = 2 * most[:, 0] + (n + 64) * 2 * U["f32"] + 4 * U["f32"] * (np.abs(lse[at, j]) + 110)
     return out, lse, tol, ltol
