@@ -45,6 +45,10 @@ struct Runtime {
   hipEvent_t timer[kTimerSlots];
 
   int function(const char* name, hipFunction_t* out, char** err);
+  // The key-value cache's code object, loaded by the first cache that is bound:
+  // creating a runtime takes 9 ms, with it 14.
+  hipModule_t kv_module = nullptr;
+  int load_kv(char** err);
   // Launches builtin kernel `name` whose single by-value argument is *args.
   // `label` names the launch in profiles (defaults to the kernel name).
   int launch(const char* name, dim3 grid, dim3 block, size_t lds, void* args, char** err,

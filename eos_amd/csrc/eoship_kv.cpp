@@ -288,6 +288,7 @@ int eoship_kv_bind(EosHipRuntime* rt, const EosHipKVDesc* desc, EosHipKVCache** 
       return set_err(err, "%s: %s needs 16-byte aligned scale pools", what, kFormats[desc->format]);
     if (rt == nullptr || out == nullptr) return set_err(err, "%s: NULL argument", what);
     OnDevice on(rt->device);
+    if (rt->load_kv(err) != 0) return 1;
     auto* kv = new EosHipKVCache();
     kv->rt = rt;
     kv->d = *desc;

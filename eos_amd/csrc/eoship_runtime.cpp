@@ -75,6 +75,18 @@ int Runtime::function(const char* name, hipFunction_t* out, char** err) {
   return 0;
 }
 
+int Runtime::load_kv(char** err) {
+  if (kv_module != nullptr) return 0;
+  hipModule_t m = nullptr;
+  const hipError_t e = eoship_kv_co_end > eoship_kv_co_begin
+                           ? hipModuleLoadData(&m, eoship_kv_co_begin)
+                           : hipErrorInvalidImage;
+  if (e != hipSuccess) return hip_err(err, "hipModuleLoadData(key-value cache code object)", e);
+  builtin.push_back(m);
+  kv_module = m;
+  return 0;
+}
+
 int Runtime::launch(const char* name, dim3 grid, dim3 block, size_t lds, void* args,
                     char** err, const char* label) {
   hipFunction_t f = nullptr;
@@ -230,11 +242,10 @@ int eoship_runtime_create(int device, EosHipRuntime** out, char** err) {
     delete rt;
     return hip_err(err, "hipStreamCreateWithFlags", e);
   }
-  const unsigned char* images[5][2] = {{eoship_tq_co_begin, eoship_tq_co_end},
+  const unsigned char* images[4][2] = {{eoship_tq_co_begin, eoship_tq_co_end},
                                        {eoship_tqe_co_begin, eoship_tqe_co_end},
                                        {eoship_enc_co_begin, eoship_enc_co_end},
-                                       {eoship_ret_co_begin, eoship_ret_co_end},
-                                       {eoship_kv_co_begin, eoship_kv_co_end}};
+                                       {eoship_ret_co_begin, eoship_ret_co_end}};
   for (auto& im : images) {
     hipModule_t m = nullptr;
     e = im[1] > im[0] ? hipModuleLoadData(&m, im[0]) : hipErrorInvalidImage;

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kv_reference as ref
-from eos_amd.runtime import DeviceBuffer
+from eos_amd.runtime import DeviceBuffer, Runtime
 from test_kv_cache_gpu import FORMATS, World, _case, _io, put_rows
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +149,26 @@ def test_a_row_is_the_same_by_either_form(rt, fmt, io, d):
         values.append([o.download(np.uint32, (n, d)) for o in out])
     for a, b in zip(*values):
         np.testing.assert_array_equal(a, b)
+
+
+def test_caches_of_one_runtime_and_of_several():
+    """The kernels are loaded with a runtime's first cache: two caches of one
+    runtime, one bound after the first is gone, and two runtimes at once."""
+    _case("kernels loaded with the first cache")
+    runtimes = [Runtime(0), Runtime(0)]
+    try:
+        for r in (runtimes[0], runtimes[0], runtimes[1], runtimes[0]):
+            worlds = [_step(r, fmt, 64, 2, 16, seed=7) for fmt in ("f16", "tq4")]
+            for w in worlds:
+                w.fill()
+                out = [DeviceBuffer(r, w.plan.rows * 128 * 4) for _ in range(2)]
+                w.cache.read(w.batch, *out, "f32")
+                assert w.cache.status() == 0
+                k = out[0].download(np.float32, (w.plan.rows, 128)).reshape(-1, 2, 64)
+                for row, _, _, page, slot in w.plan.slots():
+                    want = w.pool.values()[0][page, :, slot]
+                    assert np.abs(k[row] - want).max() <= 2.0 ** -18 * np.abs(want).max()
+                w.cache.release()
+    finally:
+        for r in runtimes:
+            r.close()
