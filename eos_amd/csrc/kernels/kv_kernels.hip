@@ -1665,11 +1665,13 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
     const uint8_t* src = a.q + ((size_t)(t.s.row0 + qrow) * a.q_stride +
                                 (size_t)(h * a.group + (real ? rr % a.group : 0)) * D) * 2;
     const uint32_t neg = a.scale < 0.0f ? 0x80008000u : 0u;
+    // (a factor of zero takes the query itself: the scores' own is never zero)
+    const uint32_t keep = a.scale != 0.0f ? ~0u : 0u;
     if constexpr (!kQuant) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         q[s] = real ? *reinterpret_cast<const v4u*>(src + (s * 16 + hh * 8) * 2) : v4u{0, 0, 0, 0};
-        q[s] ^= v4u{neg, neg, neg, neg};
+        q[s] = (q[s] ^ v4u{neg, neg, neg, neg}) & v4u{keep, keep, keep, keep};
       }
     } else {
       float x[KS][8];
@@ -1708,6 +1710,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
       float down = __builtin_amdgcn_ldexpf(1.0f, -ex);
       qs = __builtin_amdgcn_ldexpf(qs, ex);
       if (neg != 0) down = -down;
+      if (keep == 0) down = 0.0f;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll

@@ -93,3 +93,21 @@ def test_small_weights_of_large_values(rt, form):
     assert want.min() > 2.0 ** -8 and tol.max() < 2.0 ** -11, (want.min(), tol.max())
     assert (np.abs(out - want) <= tol).all(), (float(out.min()), float(want.min()))
     assert (np.abs(lse - wl) <= ltol).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("fmt", ["bf16", "q8", "tq4"])
+def test_a_factor_of_zero_levels_any_scores(rt, fmt, form):
+    """scale 0: equal weights, however large the products q . k are."""
+    _case(f"scale 0 {fmt} {form}")
+
+    def rows(x):
+        x[0] = np.where(np.arange(x.shape[1]) % 2, 2.0 ** 38, -2.0 ** 38)[:, None, None]
+        x[1] = np.where(np.arange(x.shape[1]) % 2, 1.0, 3.0)[:, None, None]
+    w, heads = _world(rt, fmt, form, 90, 1, rows)
+    q = np.full((w.plan.rows, heads, 64), 2.0 ** 80, np.float32)
+    q64, out, lse = _attend(w, heads, "bf16", scale=0.0, q=q)
+    want, wl, _, _ = kv_bounds.attention(w.plan, q64, heads, "bf16", 0.0)
+    # equal weights: the output's rounding, the weights' and f32 sums
+    assert (np.abs(out - want) <= 3 * (2.0 ** -8 + 2.0 ** -8 + 200 * 2.0 ** -24)).all(), (out.min(), out.max())
+    assert (np.abs(lse - wl) <= 2.0 ** -16).all()
