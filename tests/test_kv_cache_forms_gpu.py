@@ -172,3 +172,49 @@ def test_caches_of_one_runtime_and_of_several():
     finally:
         for r in runtimes:
             r.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_prompts_then_tokens_are_stored_as_given(rt, fmt):
+    """Prompts by row ranges, then tokens one a sequence into the same pages and
+    half-filled groups: what the cache holds is every row's own."""
+    _case(f"stored prompt and tokens {fmt}")
+    kvh, d, p, io = 2, 64, 16, _io(fmt)
+    prompt, steps = np.array([21, 9]), 20
+    total = prompt + steps
+    w = World(rt, fmt, kvh, d, p, total, np.array([1, 1]), seed=12, spare=1)
+    given = np.zeros((2, w.pool.pages, p, kvh, d), np.float32)      # K and V by page and slot
+    there = np.zeros((w.pool.pages, p), bool)
+
+    def call(lengths, n):
+        plan = ref.Plan(w.pool, total, n, 12)
+        plan.lengths = np.asarray(lengths, np.int32)
+        np.testing.assert_array_equal(plan.table, w.plan.table)
+        bits = [ref.to_rows(w.rng.normal(size=(plan.rows, kvh * d)).astype(np.float32) * 2, io) for _ in "kv"]
+        w.cache.append(w.on_device(plan), *(DeviceBuffer.from_array(rt, b) for b in bits), io)
+        for row, _, _, page, slot in plan.slots():
+            assert not there[page, slot]
+            there[page, slot] = True
+            for a, b in zip(given, bits):
+                a[page, slot] = ref.from_rows(b[row], io).reshape(kvh, d)
+    call(prompt, prompt)
+    for i in range(1, steps + 1):
+        call(prompt + i, np.array([1, 1]))
+    assert w.cache.status() == 0 and there.sum() == total.sum()
+    got = w.pools()
+    page, slot = np.nonzero(there)
+    if fmt != "tq4":
+        for name, a in zip("kv", given):
+            put_rows(w.pool, name, a[page, slot], list(zip(page, slot)))
+        for name, a in w.pool.arrays().items():
+            np.testing.assert_array_equal(got[name], a, err_msg=name)
+        return
+    for name in got:
+        setattr(w.pool, name, got[name])
+    k, v, ks, vs = w.pool.views()
+    for codes, scales, a in ((k.swapaxes(1, 2)[page, slot], ks, given[0]),
+                             (v.swapaxes(-1, -2).reshape(w.pool.pages, kvh, p, d).swapaxes(1, 2)[page, slot], vs,
+                              given[1])):
+        want, s, near = w.pool.quantize(a[page, slot])
+        assert (near | (codes == want)).all()
+        assert (np.abs(scales.swapaxes(1, 2)[page, slot] - s) <= 2 * ref.U["f32"] * s).all()

@@ -4,7 +4,6 @@ import numpy as np
 import pytest
 
 import kv_bounds
-import kv_reference as ref
 from test_kv_cache_gpu import World, _attend, _case, _io
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +84,26 @@ def test_zero_rows_keep_their_weight_beside_large_ones(rt, fmt, zeros, rows, wid
     want, wl, tol, ltol = kv_bounds.attention(w.plan, q64, heads, "bf16", 64 ** -0.5)
     assert (np.abs(out - want) <= tol).all(), float((np.abs(out - want) / np.maximum(tol, 1e-30)).max())
     assert (np.abs(lse - wl) <= ltol).all(), float(np.abs(lse - wl).max())
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "q8", "tq4"])
+@pytest.mark.parametrize("rows,wide", [(1, False), (8, False), (64, True)])
+def test_values_that_grow_and_shrink(rt, fmt, rows, wide):
+    """Scores that rise, V rows that swell and shrink by 2^12: a row's bound is
+    what its own weights times values leave."""
+    _case(f"growing {fmt} rows={rows} wide={wide}")
+    n, heads = 600, 6
+    w = World(rt, fmt, 1, 64, 16, np.array([n]), np.array([rows]), seed=8, shuffle=False,
+              stride=200 if wide else None)
+
+    def values(r):
+        ramp = np.linspace(0, 1, r.shape[1], dtype=np.float32)[:, None, None]
+        r[0] = r[0] * 0.3 + ramp * 6
+        r[1] *= np.float32(2) ** np.rint(12 * np.sin(9 * ramp))
+        return r
+    w.fill(values)
+    q = np.ones((rows, heads, 64), np.float32) * np.array([1.0, -1.0, 0.01, 0.3, -0.3, 0.0], np.float32)[:, None]
+    q64, out, lse = _attend(w, heads, "bf16" if fmt == "bf16" else "f16", q=q)
+    want, wl, tol, ltol = kv_bounds.attention(w.plan, q64, heads, "bf16" if fmt == "bf16" else "f16", 64 ** -0.5)
+    assert (np.abs(out - want) <= tol).all(), float((np.abs(out - want) / tol).max())
+    assert (np.abs(lse - wl) <= ltol).all()
