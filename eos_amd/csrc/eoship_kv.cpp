@@ -41,7 +41,9 @@ namespace {
 // 71, 128 rows 133 / 128.
 constexpr int kPromptFrom[] = {8, 8, 96, 384};
 // ... and not while the 16-row workgroups are on the CUs at once over so few
-// keys (4 prompts of 256, 8 heads of 64: 10 / 17).
+// keys (4 prompts of 256, 8 heads of 64: 10 / 17). Here and for the equal shares
+// below, keys are those that the page table has room for: lengths are on the
+// device, so short sequences under a wide table take the kernels of long ones.
 constexpr int kPromptKeys = 1024;
 
 const char* const kFormats[] = {"f16", "bf16", "q8", "tq4"};

@@ -204,8 +204,11 @@ EOS_DEV v4f mfma16(v4u a, v4u b, v4f c) {
 // whose entries are signs: the parity of i & j % 4, t % 2 & j / 4, g' & g and
 // t / 2 & s for output (t, g', i) and input (s, g, j). So there are two fragments,
 // for even and odd t, and the rest is a sign of x. Products by +-1 are exact,
-// sums f32. (32,768 tokens x 8 heads x 128 appended and 24,576 read alone: 85
-// and 55 us; by butterflies between lanes 106 and 62.)
+// sums f32. (32,768 tokens x 8 heads x 128 appended, the same ones again: 88 us,
+// by butterflies between lanes 106; 24,576 read, other pages each time: 56 and 62.)
+// One row a sequence stays with the butterflies: 16 rows of 8 heads of 128 take
+// 5.3 us, on the matrix cores 6.8, of 256 5.2 and 11.8. Either adds in f32, in an
+// order of its own: a value next to a threshold may take another code.
 template <int FMT, int D>
 EOS_DEV void rotate16(const v4u (&x)[D / 32], v4f (&y)[D / 16]) {
   constexpr uint32_t kOne = FMT == kKvBf16 ? 0x3f80u : 0x3c00u;
@@ -300,7 +303,8 @@ EOS_DEV void find_blocks(const KvCacheArgs& c, const KvRun& g, int b, int h, lon
 // another writer. Bound by the rows' bytes and the latency of three dependent
 // loads (numbers, page ids, rows), which runs of 32 positions share among four
 // groups: 8 x 1,021 ragged rows of 12 heads of 64 in q8 appended and read back,
-// 20 us, by single groups 23.
+// 20 us, by single groups 23. 32,768 rows of 8 heads of 128 appended and read: f16
+// 65 and 59 us, 4.1 and 4.5 TB/s, q8 69 and 59.
 template <int FMT, int D, int RUN>
 EOS_DEV void append_run(const KvRowsArgs& a) {
   constexpr int LANES = D / 8, NG = RUN / 8;
@@ -909,11 +913,13 @@ EOS_DEV void finish_row(const KvAttnArgs& a, const KvSeq& s, int r, int h, int l
 // = lane / 16, query lane % 16) are the 8 consecutive summands that its
 // operand of the second product holds: nothing crosses lanes between the two.
 // K's rows are taken in the order 8 (r / 4) + 4 j + r % 4 for that. Weights are
-// rounded to the operand's 16 bits, sums and statistics are f32. Bound by the
-// cache's bytes in 16 and 8 bits (one sequence of 131,072 tokens of q8, 32
-// heads on 8 of 128: 48 us, 5.8 TB/s; 32 ragged ones in bf16: 66 us, 4.4 TB/s);
-// in 4 bits by the vector unit, with 440 instructions for 32 keys of 128, half
-// of them the codes' expansion (64 sequences, 0.6 GB: 165 us, 3.7 TB/s).
+// rounded to 16 bits, the type that V has or is expanded to, since a matrix
+// instruction takes both operands in one; sums and statistics are f32. Bound by
+// the cache's bytes in 16 and 8 bits (one sequence of 131,072 tokens of q8, 32
+// heads on 8 of 128: 61 us with the join, 4.5 TB/s, read again from the
+// memory-side cache 52; 32 ragged ones in bf16: 67 us, 4.3 TB/s); in 4 bits by
+// the vector unit, with 440 instructions for 32 keys of 128, half of them the
+// codes' expansion (64 sequences, 0.6 GB: 166 us, 3.7 TB/s).
 // The whole of the rows' keys goes to the output, else the sums go to place
 // `at` of the parts.
 template <int FMT, int D>
@@ -1453,10 +1459,11 @@ EOS_DEV void expand(const KvTables& t, v4u x, v4u (&out)[16 / bits_of(FMT)]) {
 // One workgroup: 128 query rows of a head group, 32 a wavefront, against a
 // split of their keys, 64 (where registers allow, else 32) at a time through
 // two LDS stages that hold K and V as 16-bit operands; 16-bit formats are
-// loaded straight into them. Products as in attn_segment, on 32 x 32 tiles: scores K q^T, outputs V^T p^T, so a lane (query lane % 32, half lane
-// / 32) holds the scores of keys 16 k + 8 half .. + 7, its operand of the
-// second product; K's rows are read with bits 2 and 3 exchanged for that.
-// Two prompts of 8,192 rows in bf16, 32 heads on 8 of 128: 1.33 ms, 0.83
+// loaded straight into them. Products as in attn_segment, on 32 x 32 tiles:
+// scores K q^T, outputs V^T p^T, so a lane (query lane % 32, half lane / 32) holds
+// the scores of keys 16 k + 8 half .. + 7, its operand of the second product; K's
+// rows are read with bits 2 and 3 exchanged for that.
+// Two prompts of 8,192 rows in bf16, 32 heads on 8 of 128: 1.34 ms, 0.82
 // PFLOP/s. Bound by issue and latency at two wavefronts a SIMD: the matrix
 // unit is busy for a third of the time, without the loads it took 1.01 ms,
 // without the exponentials 1.30. 256 rows a workgroup: 1.29 to 1.43 ms.
@@ -1658,7 +1665,7 @@ EOS_DEV void attn_prompt(const KvAttnArgs& a) {
     load_v(0, begin, pid2, ok0);
   }
 
-  // The query as the second operand (see attn_split).
+  // The query as the second operand (see attn_segment).
   v4u q[KS], q2[kTwo ? KS : 1];
   float qs = fabsf(a.scale);
   {

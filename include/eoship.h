@@ -970,7 +970,10 @@ int eoship_kv_read_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBa
  * before) included: out = softmax(scale q K^T) V over positions p' <= p, with
  * window > 0 also p' > p - window. dtype as in append; out likewise. d_lse
  * ([rows][heads], may be NULL): the logarithm of the weights' sum. A row with
- * no key gives 0 and -inf. Uses the runtime's workspace. Enqueued. */
+ * no key gives 0 and -inf. Scores and sums are f32; a weight (q8, tq4: times its
+ * V scale) is rounded to f16, in a bf16 cache to bf16, before it meets V. What a
+ * row does not attend has no part in its roundings. Uses the runtime's
+ * workspace. Enqueued. */
 int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHipKVBatch* batch,
                                const void* d_q, int64_t q_stride, int32_t heads, int32_t dtype,
                                float scale, int32_t window, void* d_out, int64_t out_stride,
