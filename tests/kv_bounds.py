@@ -70,9 +70,14 @@ def attention(plan, q, heads, dtype, scale, window=0):
                     big = va[h].max(-1)
                     if tq4:  # (a row may lack the largest magnitude)
                         big = np.sqrt((va[h] ** 2).mean(-1)) * 4.0
+                    # (the reference counts a scale as 2^-64 at least: its exponent is
+                    # taken upwards, codes go to 127)
+                    big = np.maximum(big, 2.0 ** (-63 + 7))
                     e += 2.0 ** -31 * n[:, None] * (p * big).max(1, keepdims=True) / tot
                 else:
                     e += 2.0 ** -31 * (see @ va[h]) / tot
+            # weights, and products, below f32's range
+            e += 2.0 ** -125 * ((see @ va[h]) / tot + 1)
             if tq4:  # rotated back: every coordinate has a share of each error
                 e = np.repeat(np.sqrt((e * e).sum(1, keepdims=True)), d, 1)
             tol[at, j] = U[dtype] * (np.abs(got) + e) + e + (2.0 ** -25 if dtype == "f16" else 0)
