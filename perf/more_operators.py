@@ -284,6 +284,7 @@ def _bind(s):
     dev = s["dev"] = {n: _Dev(t) for n, t in s.items() if isinstance(t, torch.Tensor)}
     if kind == "linear":
         from eos_amd.microscale import MXLinear
+        torch.cuda.synchronize()  # the layer is laid out on the runtime's own stream
         s["layer"] = MXLinear(_rt, dev["w"], dev["w_scales"], case["n"], case["k"],
                               bias=dev.get("bias"))
     elif kind == "rotary":
