@@ -239,6 +239,41 @@ class EosHipKVBatch(C.Structure):
     ]
 
 
+class EosHipRotaryDesc(C.Structure):
+    _fields_ = [
+        ("head_dim", C.c_int32),
+        ("rotary_dim", C.c_int32),
+        ("layout", C.c_int32),
+        ("factor", C.c_float),
+        ("frequencies", C.c_void_p),
+    ]
+
+
+class EosHipKVPagerDesc(C.Structure):
+    _fields_ = [
+        ("slots", C.c_int32),
+        ("table_stride", C.c_int32),
+        ("page_tokens", C.c_int32),
+        ("pages", C.c_int64),
+        ("d_page_table", C.c_void_p),
+        ("d_lengths", C.c_void_p),
+        ("d_free", C.c_void_p),
+        ("d_free_count", C.c_void_p),
+    ]
+
+
+class EosHipKVPlan(C.Structure):
+    _fields_ = [
+        ("d_slots", C.c_void_p),
+        ("d_page_table", C.c_void_p),
+        ("d_lengths", C.c_void_p),
+        ("d_offsets", C.c_void_p),
+        ("d_positions", C.c_void_p),
+        ("d_slot_map", C.c_void_p),
+        ("rows", C.c_int64),
+    ]
+
+
 class EosHipHadamardSpec(C.Structure):
     _fields_ = [
         ("channels", C.c_int32),
@@ -426,6 +461,34 @@ _SIGNATURES = {
                                     C.c_int64, C.c_int32, C.c_int32, C.c_float, C.c_int32,
                                     C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p], C.c_int),
     "eoship_kv_status": ([C.c_void_p, C.c_void_p, C.POINTER(C.c_int32), C.c_void_p], C.c_int),
+    "eoship_rotary_bind": ([C.c_void_p, C.POINTER(EosHipRotaryDesc), C.POINTER(C.c_void_p),
+                            C.c_void_p], C.c_int),
+    "eoship_rotary_release": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_rotary_device": ([C.c_void_p, C.c_void_p, C.POINTER(EosHipKVBatch), C.c_void_p,
+                              C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int32,
+                              C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
+                              C.c_int64, C.c_void_p], C.c_int),
+    "eoship_kv_pager_bind": ([C.c_void_p, C.POINTER(EosHipKVPagerDesc), C.POINTER(C.c_void_p),
+                              C.c_void_p], C.c_int),
+    "eoship_kv_pager_release": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_kv_pager_reset_device": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_kv_pager_extend_device": ([C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.POINTER(EosHipKVPlan), C.c_void_p], C.c_int),
+    "eoship_kv_pager_trim_device": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_kv_pager_status": ([C.c_void_p, C.c_void_p, C.POINTER(C.c_int32), C.c_void_p],
+                               C.c_int),
+    "eoship_mx_bytes": ([C.c_int64, C.c_int32, C.POINTER(C.c_int64), C.POINTER(C.c_int64),
+                         C.c_void_p], C.c_int),
+    "eoship_mx_quantize_device": ([C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64,
+                                   C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_mx_dequantize_device": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
+                                     C.c_void_p, C.c_int64, C.c_int32, C.c_void_p], C.c_int),
+    "eoship_mx_bind": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+                        C.POINTER(C.c_void_p), C.c_void_p], C.c_int),
+    "eoship_mx_release": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "eoship_mx_linear_device": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
+                                 C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32,
+                                 C.c_void_p], C.c_int),
     "eoship_tq_ip_encode_device": ([C.c_void_p, C.POINTER(EosHipTQIPSpec), C.c_void_p, C.c_int64,
                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
                                    C.c_int),

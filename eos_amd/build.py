@@ -36,6 +36,8 @@ DEVICE_SOURCES = [
     ("enc", os.path.join(CSRC, "kernels", "enc_kernels.hip")),
     ("ret", os.path.join(CSRC, "kernels", "ret_kernels.hip")),
     ("kv", os.path.join(CSRC, "kernels", "kv_kernels.hip")),
+    ("mx", os.path.join(CSRC, "kernels", "mx_kernels.hip")),
+    ("step", os.path.join(CSRC, "kernels", "step_kernels.hip")),
 ]
 # Extra flags per code object. The encoder kernels are built without the
 # mixed-precision FMA instructions (v_fma_mix*): the compiler folds some
@@ -64,6 +66,9 @@ HOST_SOURCES = [
     os.path.join(CSRC, "eoship_mll.cpp"),
     os.path.join(CSRC, "eoship_retrieval.cpp"),
     os.path.join(CSRC, "eoship_kv.cpp"),
+    os.path.join(CSRC, "eoship_mx.cpp"),
+    os.path.join(CSRC, "eoship_rotary.cpp"),
+    os.path.join(CSRC, "eoship_pager.cpp"),
 ]
 
 # Packed-FP32 instructions are disabled for every device build.

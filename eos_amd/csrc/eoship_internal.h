@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <exception>
 #include <map>
 #include <string>
 #include <unordered_map>
@@ -45,10 +46,11 @@ struct Runtime {
   hipEvent_t timer[kTimerSlots];
 
   int function(const char* name, hipFunction_t* out, char** err);
-  // The key-value cache's code object, loaded by the first cache that is bound:
-  // creating a runtime takes 9 ms, with it 14.
-  hipModule_t kv_module = nullptr;
-  int load_kv(char** err);
+  // Code objects that a runtime's first call of their kind loads: creating a
+  // runtime takes 9 ms, with the key-value cache's 14.
+  enum Extra { kKv, kMx, kStep, kExtras };
+  hipModule_t extra[kExtras] = {};
+  int load(Extra which, char** err);
   // Launches builtin kernel `name` whose single by-value argument is *args.
   // `label` names the launch in profiles (defaults to the kernel name).
   int launch(const char* name, dim3 grid, dim3 block, size_t lds, void* args, char** err,
@@ -88,6 +90,32 @@ struct Runtime {
     return hipMemcpy(dst, src, bytes, kind);
   }
 };
+
+// Makes a runtime's device current for the length of a call.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    if (hipGetDevice(&was_) != hipSuccess) was_ = device;
+    if (was_ != device) (void)hipSetDevice(device);
+    now_ = device;
+  }
+  ~OnDevice() {
+    if (was_ != now_) (void)hipSetDevice(was_);
+  }
+
+ private:
+  int was_ = 0, now_ = 0;
+};
+
+// Runs a call's body: no exception (host memory may run out) leaves a C entry.
+template <class F>
+int guarded(const char* what, char** err, F body) {
+  try {
+    return body();
+  } catch (const std::exception& e) {
+    return set_err(err, "%s: %s", what, e.what());
+  }
+}
 
 // Two-stage rerank on a caller-chosen scratch buffer of at least
 // q * c * 4 bytes (the candidates' f32 scores between its two kernels).

@@ -8,14 +8,15 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
-#include <exception>
 #include <string>
 #include <vector>
 
 #include "eoship_internal.h"
 #include "kernels/kv_index.h"
 
+using eoship::guarded;
 using eoship::hip_err;
+using eoship::OnDevice;
 using eoship::set_err;
 
 struct EosHipKVCache {
@@ -51,32 +52,6 @@ const char* const kFormats[] = {"f16", "bf16", "q8", "tq4"};
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int bits_of(int format) { return format == kKvQ8 ? 8 : format == kKvTq4 ? 4 : 16; }
-
-// Makes a runtime's device current for the length of a call.
-class OnDevice {
- public:
-  explicit OnDevice(int device) {
-    if (hipGetDevice(&was_) != hipSuccess) was_ = device;
-    if (was_ != device) (void)hipSetDevice(device);
-    now_ = device;
-  }
-  ~OnDevice() {
-    if (was_ != now_) (void)hipSetDevice(was_);
-  }
-
- private:
-  int was_ = 0, now_ = 0;
-};
-
-// Runs a call's body: no exception (host memory may run out) leaves a C entry.
-template <class F>
-int guarded(const char* what, char** err, F body) {
-  try {
-    return body();
-  } catch (const std::exception& e) {
-    return set_err(err, "%s: %s", what, e.what());
-  }
-}
 
 // The f16 bits of a float that f16 holds exactly and normally, or 0.
 uint16_t exact_f16(float f) {
@@ -290,7 +265,7 @@ int eoship_kv_bind(EosHipRuntime* rt, const EosHipKVDesc* desc, EosHipKVCache** 
       return set_err(err, "%s: %s needs 16-byte aligned scale pools", what, kFormats[desc->format]);
     if (rt == nullptr || out == nullptr) return set_err(err, "%s: NULL argument", what);
     OnDevice on(rt->device);
-    if (rt->load_kv(err) != 0) return 1;
+    if (rt->load(eoship::Runtime::kKv, err) != 0) return 1;
     auto* kv = new EosHipKVCache();
     kv->rt = rt;
     kv->d = *desc;

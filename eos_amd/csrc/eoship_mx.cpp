@@ -1,0 +1,258 @@
+// Microscaled 4-bit half of the eoship C ABI: rows quantised and taken back,
+// and linear layers over weights held in that form. Beside the q8 encoder's
+// matrix products (runtime/backend/tensor_ops.go:938-2208 on the host), the
+// form that the matrix units of gfx950 multiply directly.
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "eoship_internal.h"
+#include "kernels/mx_args.h"
+
+using eoship::guarded;
+using eoship::hip_err;
+using eoship::OnDevice;
+using eoship::set_err;
+
+struct EosHipMX {
+  EosHipRuntime* rt = nullptr;
+  int n = 0, k = 0;
+  MxLaid w{};
+  const float* bias = nullptr;
+  void* mem = nullptr;  // codes, scales, bias
+  ~EosHipMX() {
+    if (mem != nullptr) hipFree(mem);
+  }
+};
+
+namespace {
+
+constexpr int kMost = 1 << 24;  // values of a row, outputs of a layer
+
+const char* const kTypes[] = {"f16", "bf16", "f32", "codes"};
+
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+int size_of(int type) { return type == kMxF32 ? 4 : 2; }
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+MxLaid laid(long long rows, int k) {
+  MxLaid m{};
+  m.rows = rows;
+  m.blocks = ceil_div(k, kMxBlock);
+  m.steps = ceil_div(k, kMxStep);
+  m.quads = ceil_div(m.steps, 4);
+  return m;
+}
+size_t tiles(const MxLaid& m) { return (size_t)((m.rows + kMxTile - 1) / kMxTile); }
+size_t code_bytes(const MxLaid& m) { return tiles(m) * m.steps * kMxTileBytes; }
+size_t scale_bytes(const MxLaid& m) { return tiles(m) * m.quads * kMxScaleBytes; }
+void place(MxLaid* m, void* mem) {
+  m->codes = static_cast<uint8_t*>(mem);
+  m->scales = m->codes + code_bytes(*m);
+}
+
+int check_shape(int64_t rows, int32_t k, const char* what, char** err) {
+  if (rows < 0 || rows > INT32_MAX)
+    return set_err(err, "%s: rows must be in 0..2^31-1, got %lld", what, (long long)rows);
+  if (k < 1 || k > kMost) return set_err(err, "%s: k must be in 1..2^24, got %d", what, k);
+  return 0;
+}
+
+int check_type(int32_t type, int most, const char* what, char** err) {
+  if (type < 0 || type > most)
+    return set_err(err, "%s: dtype must be 0 (f16), 1 (bf16)%s, got %d", what,
+                   most == kMxF32 ? " or 2 (f32)" : ", 2 (f32) or 3 (mxfp4)", type);
+  return 0;
+}
+
+int check_rows(const void* p, int64_t stride, int64_t width, const char* name, const char* what,
+               char** err) {
+  if (p == nullptr) return set_err(err, "%s: %s is NULL", what, name);
+  if (!aligned(p)) return set_err(err, "%s: %s is not 16-byte aligned", what, name);
+  if (stride < width || stride % 8 != 0 || stride > 1LL << 40)
+    return set_err(err,
+                   "%s: the row stride of %s must be a multiple of 8 and at least %lld (at most "
+                   "2^40), got %lld",
+                   what, name, (long long)width, (long long)stride);
+  return 0;
+}
+
+int check_codes(const void* codes, const void* scales, const char* what, char** err) {
+  if (codes == nullptr || scales == nullptr)
+    return set_err(err, "%s: NULL codes or scales", what);
+  if (!aligned(codes)) return set_err(err, "%s: codes are not 16-byte aligned", what);
+  return 0;
+}
+
+int launch(EosHipRuntime* rt, const std::string& name, long long blocks, void* args,
+           const char* what, char** err) {
+  if (blocks * 256 > UINT32_MAX) return set_err(err, "%s: too many rows for one call", what);
+  return rt->launch(name.c_str(), dim3((unsigned)blocks), dim3(256), 0, args, err);
+}
+
+// Rows (or codes) into a laid-out matrix.
+int lay(EosHipRuntime* rt, const MxLaid& to, const void* x, int64_t stride, int type,
+        const void* scales, int k, const char* what, char** err) {
+  MxQuantArgs a{};
+  a.x = static_cast<const uint8_t*>(x);
+  a.xs = static_cast<const uint8_t*>(scales);
+  a.stride = type == kMxCodes ? 0 : stride * size_of(type);
+  a.laid = to;
+  a.rows = to.rows;
+  a.k = k;
+  a.blocks = to.blocks;
+  return launch(rt, std::string("eos_mx_lay_") + kTypes[type], (long long)tiles(to) * to.quads, &a,
+                what, err);
+}
+
+}  // namespace
+
+extern "C" {
+
+int eoship_mx_bytes(int64_t rows, int32_t k, int64_t* code_bytes, int64_t* scale_bytes,
+                    char** err) {
+  if (check_shape(rows, k, "eoship_mx_bytes", err) != 0) return 1;
+  const int64_t blocks = rows * ceil_div(k, kMxBlock);
+  if (code_bytes) *code_bytes = blocks * 16;
+  if (scale_bytes) *scale_bytes = blocks;
+  return 0;
+}
+
+int eoship_mx_quantize_device(EosHipRuntime* rt, const void* d_x, int64_t x_stride, int32_t dtype,
+                              int64_t rows, int32_t k, uint8_t* d_codes, uint8_t* d_scales,
+                              char** err) {
+  const char* what = "eoship_mx_quantize_device";
+  return guarded(what, err, [&]() -> int {
+    if (check_shape(rows, k, what, err) != 0 || check_type(dtype, kMxF32, what, err) != 0) return 1;
+    if (rt == nullptr) return set_err(err, "%s: NULL runtime", what);
+    if (rows == 0) return 0;
+    if (check_rows(d_x, x_stride, k, "x", what, err) != 0 ||
+        check_codes(d_codes, d_scales, what, err) != 0)
+      return 1;
+    OnDevice on(rt->device);
+    if (rt->load(eoship::Runtime::kMx, err) != 0) return 1;
+    MxQuantArgs a{};
+    a.x = static_cast<const uint8_t*>(d_x);
+    a.stride = x_stride * size_of(dtype);
+    a.codes = d_codes;
+    a.scales = d_scales;
+    a.rows = rows;
+    a.k = k;
+    a.blocks = ceil_div(k, kMxBlock);
+    return launch(rt, std::string("eos_mx_quantize_") + kTypes[dtype], (rows * a.blocks + 63) / 64,
+                  &a, what, err);
+  });
+}
+
+int eoship_mx_dequantize_device(EosHipRuntime* rt, const uint8_t* d_codes, const uint8_t* d_scales,
+                                int64_t rows, int32_t k, void* d_out, int64_t out_stride,
+                                int32_t dtype, char** err) {
+  const char* what = "eoship_mx_dequantize_device";
+  return guarded(what, err, [&]() -> int {
+    if (check_shape(rows, k, what, err) != 0 || check_type(dtype, kMxF32, what, err) != 0) return 1;
+    if (rt == nullptr) return set_err(err, "%s: NULL runtime", what);
+    if (rows == 0) return 0;
+    if (check_codes(d_codes, d_scales, what, err) != 0 ||
+        check_rows(d_out, out_stride, k, "out", what, err) != 0)
+      return 1;
+    OnDevice on(rt->device);
+    if (rt->load(eoship::Runtime::kMx, err) != 0) return 1;
+    MxDequantArgs a{};
+    a.codes = d_codes;
+    a.scales = d_scales;
+    a.out = static_cast<uint8_t*>(d_out);
+    a.stride = out_stride * size_of(dtype);
+    a.rows = rows;
+    a.k = k;
+    a.blocks = ceil_div(k, kMxBlock);
+    return launch(rt, std::string("eos_mx_dequantize_") + kTypes[dtype],
+                  (rows * a.blocks + 63) / 64, &a, what, err);
+  });
+}
+
+int eoship_mx_bind(EosHipRuntime* rt, const uint8_t* d_codes, const uint8_t* d_scales, int32_t n,
+                   int32_t k, const float* d_bias, EosHipMX** out, char** err) {
+  const char* what = "eoship_mx_bind";
+  return guarded(what, err, [&]() -> int {
+    if (out != nullptr) *out = nullptr;
+    if (n < 1 || n > kMost) return set_err(err, "%s: n must be in 1..2^24, got %d", what, n);
+    if (check_shape(n, k, what, err) != 0 || check_codes(d_codes, d_scales, what, err) != 0)
+      return 1;
+    if (((uintptr_t)d_bias & 3) != 0) return set_err(err, "%s: bias is not 4-byte aligned", what);
+    if (rt == nullptr || out == nullptr) return set_err(err, "%s: NULL argument", what);
+    OnDevice on(rt->device);
+    if (rt->load(eoship::Runtime::kMx, err) != 0) return 1;
+    auto* mx = new EosHipMX();
+    mx->rt = rt;
+    mx->n = n;
+    mx->k = k;
+    mx->w = laid(n, k);
+    const size_t held = code_bytes(mx->w) + scale_bytes(mx->w);
+    int rc = rt->alloc(held + (d_bias != nullptr ? (size_t)n * 4 : 0), &mx->mem, err);
+    if (rc == 0) {
+      place(&mx->w, mx->mem);
+      rc = lay(rt, mx->w, d_codes, 0, kMxCodes, d_scales, k, what, err);
+    }
+    if (rc == 0 && d_bias != nullptr) {
+      float* b = reinterpret_cast<float*>(static_cast<char*>(mx->mem) + held);
+      const hipError_t e = rt->copy_async(b, d_bias, (size_t)n * 4, hipMemcpyDeviceToDevice);
+      if (e != hipSuccess) rc = hip_err(err, what, e);
+      mx->bias = b;
+    }
+    // Done with the caller's memory when the call returns.
+    if (rc == 0) rc = rt->sync(err);
+    if (rc != 0) {
+      delete mx;
+      return rc;
+    }
+    *out = mx;
+    return 0;
+  });
+}
+
+int eoship_mx_release(EosHipRuntime* rt, EosHipMX* mx, char** err) {
+  if (mx == nullptr) return 0;
+  if (rt == nullptr || mx->rt != rt) return set_err(err, "eoship_mx_release: wrong runtime");
+  OnDevice on(rt->device);
+  if (rt->sync(err) != 0) return 1;
+  delete mx;
+  return 0;
+}
+
+int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, int64_t x_stride,
+                            int32_t dtype, const uint8_t* d_x_scales, int64_t rows, void* d_out,
+                            int64_t out_stride, int32_t out_dtype, char** err) {
+  const char* what = "eoship_mx_linear_device";
+  return guarded(what, err, [&]() -> int {
+    if (rt == nullptr || mx == nullptr) return set_err(err, "%s: NULL argument", what);
+    if (mx->rt != rt) return set_err(err, "%s: the layer is bound to another runtime", what);
+    if (check_shape(rows, mx->k, what, err) != 0 || check_type(dtype, kMxCodes, what, err) != 0 ||
+        check_type(out_dtype, kMxF32, what, err) != 0)
+      return 1;
+    if (rows == 0) return 0;
+    if (dtype == kMxCodes ? check_codes(d_x, d_x_scales, what, err) != 0
+                          : check_rows(d_x, x_stride, mx->k, "x", what, err) != 0)
+      return 1;
+    if (check_rows(d_out, out_stride, mx->n, "out", what, err) != 0) return 1;
+    OnDevice on(rt->device);
+    MxLinearArgs a{};
+    a.w = mx->w;
+    a.x = laid(rows, mx->k);
+    a.bias = mx->bias;
+    a.out = static_cast<uint8_t*>(d_out);
+    a.out_stride = out_stride * size_of(out_dtype);
+    a.rows = rows;
+    a.n = mx->n;
+    a.k = mx->k;
+    void* ws = nullptr;
+    if (rt->workspace(code_bytes(a.x) + scale_bytes(a.x), &ws, err) != 0) return 1;
+    place(&a.x, ws);
+    if (lay(rt, a.x, d_x, x_stride, dtype, d_x_scales, mx->k, what, err) != 0) return 1;
+    a.tiles_m = (int)((rows + 63) / 64);
+    a.tiles_n = ceil_div(mx->n, 64);
+    return launch(rt, std::string("eos_mx_linear_") + kTypes[out_dtype],
+                  (long long)a.tiles_m * a.tiles_n, &a, what, err);
+  });
+}
+
+}  // extern "C"

@@ -31,6 +31,10 @@ extern const unsigned char eoship_ret_co_begin[];
 extern const unsigned char eoship_ret_co_end[];
 extern const unsigned char eoship_kv_co_begin[];
 extern const unsigned char eoship_kv_co_end[];
+extern const unsigned char eoship_mx_co_begin[];
+extern const unsigned char eoship_mx_co_end[];
+extern const unsigned char eoship_step_co_begin[];
+extern const unsigned char eoship_step_co_end[];
 }
 
 namespace eoship {
@@ -75,15 +79,23 @@ int Runtime::function(const char* name, hipFunction_t* out, char** err) {
   return 0;
 }
 
-int Runtime::load_kv(char** err) {
-  if (kv_module != nullptr) return 0;
+int Runtime::load(Extra which, char** err) {
+  if (extra[which] != nullptr) return 0;
+  static const struct {
+    const unsigned char *begin, *end;
+    const char* name;
+  } images[kExtras] = {
+      {eoship_kv_co_begin, eoship_kv_co_end, "key-value cache"},
+      {eoship_mx_co_begin, eoship_mx_co_end, "microscaled 4-bit"},
+      {eoship_step_co_begin, eoship_step_co_end, "decoding step"},
+  };
+  const auto& im = images[which];
   hipModule_t m = nullptr;
-  const hipError_t e = eoship_kv_co_end > eoship_kv_co_begin
-                           ? hipModuleLoadData(&m, eoship_kv_co_begin)
-                           : hipErrorInvalidImage;
-  if (e != hipSuccess) return hip_err(err, "hipModuleLoadData(key-value cache code object)", e);
+  const hipError_t e = im.end > im.begin ? hipModuleLoadData(&m, im.begin) : hipErrorInvalidImage;
+  if (e != hipSuccess)
+    return hip_err(err, (std::string("hipModuleLoadData(") + im.name + " code object)").c_str(), e);
   builtin.push_back(m);
-  kv_module = m;
+  extra[which] = m;
   return 0;
 }
 

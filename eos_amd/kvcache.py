@@ -205,3 +205,116 @@ class KVCache:
         st = C.c_int32()
         _lib.call("eoship_kv_status", self.rt.handle, self.handle, C.byref(st))
         return st.value
+
+
+class KVPlan:
+    """Device arrays for what :meth:`KVPager.extend` leaves: the batch of the
+    slots with new tokens (slots, lengths i32 [slots], offsets i32 [slots + 1],
+    page_table i32 [slots, table_stride] or None) and its rows (positions i32,
+    slot_map i64 [rows], either None)."""
+
+    def __init__(self, slots, page_table, lengths, offsets, positions=None, slot_map=None,
+                 rows: int = 0):
+        self.slots, self.page_table, self.lengths = slots, page_table, lengths
+        self.offsets, self.positions, self.slot_map = offsets, positions, slot_map
+        self.rows = int(rows)
+        for buf, size in ((positions, 4), (slot_map, 8)):
+            if buf is not None and buf.nbytes < size * self.rows:
+                raise ValueError("a plan's row array is smaller than its rows")
+        self.c = _lib.EosHipKVPlan(_address(slots), _address(page_table), _address(lengths),
+                                   _address(offsets), _address(positions), _address(slot_map),
+                                   self.rows)
+        self._fits = None  # (slots, table_stride) of the pager it was checked for
+
+    def _check(self, slots: int, stride: int) -> None:
+        if self._fits == (slots, stride):
+            return
+        for buf, need in ((self.slots, slots), (self.lengths, slots), (self.offsets, slots + 1),
+                          (self.page_table, slots * stride)):
+            if buf is not None and buf.nbytes < 4 * need:
+                raise ValueError("a plan's array is smaller than the pager's slots")
+        self._fits = (slots, stride)
+
+    def batch(self, table_stride: int, batch: int, rows: int | None = None) -> KVBatch:
+        """The batch of ``batch`` sequences and ``rows`` rows (None: one each)."""
+        return KVBatch(self.page_table, table_stride, batch, self.lengths,
+                       None if rows is None else self.offsets, rows)
+
+
+class KVPager:
+    """The pages of a cache that a server's requests hold, on the device: slots
+    with a length and a row of page ids each, and a stack of free pages. Arrays
+    that are not given are its own, and then all pages are free."""
+
+    def __init__(self, rt: Runtime, slots: int, table_stride: int, page_tokens: int, pages: int,
+                 page_table=None, lengths=None, free=None, free_count=None):
+        self.rt = rt
+        self.handle = C.c_void_p()
+        self.slots, self.table_stride = int(slots), int(table_stride)
+        self.page_tokens, self.pages = int(page_tokens), int(pages)
+        given = (page_table, lengths, free, free_count)
+        if any(b is None for b in given) != all(b is None for b in given):
+            raise ValueError("page_table, lengths, free and free_count are given together")
+        self._own = []
+        bufs = []
+        for buf, n in zip(given, (self.slots * self.table_stride, self.slots, self.pages, 1)):
+            if buf is None:
+                buf = DeviceBuffer(rt, 4 * max(n, 1))
+                self._own.append(buf)
+            if buf.nbytes < 4 * n:
+                raise ValueError("a pager's array is smaller than its slots or pages")
+            bufs.append(buf)
+        self.page_table, self.lengths, self.free, self.free_count = bufs
+        d = _lib.EosHipKVPagerDesc(self.slots, self.table_stride, self.page_tokens, self.pages,
+                                   *(_address(b) for b in bufs))
+        _lib.call("eoship_kv_pager_bind", rt.handle, C.byref(d), C.byref(self.handle))
+        if self._own:
+            self.reset()
+
+    def release(self) -> None:
+        if self.handle and self.rt.handle:
+            _lib.call("eoship_kv_pager_release", self.rt.handle, self.handle)
+            for b in self._own:
+                b.free()
+        self.handle, self._own = C.c_void_p(), []
+
+    def __del__(self):
+        try:
+            self.release()
+        except Exception:
+            pass
+
+    def reset(self) -> None:
+        """All slots empty, all pages free."""
+        _lib.call("eoship_kv_pager_reset_device", self.rt.handle, self.handle)
+
+    def plan(self, rows: int, page_table: bool = True, lists: bool = True) -> KVPlan:
+        """A plan with arrays of its own for up to ``rows`` rows a step."""
+        buf = lambda n: DeviceBuffer(self.rt, max(n, 16))  # noqa: E731
+        return KVPlan(buf(4 * self.slots),
+                      buf(4 * self.slots * self.table_stride) if page_table else None,
+                      buf(4 * self.slots), buf(4 * (self.slots + 1)),
+                      buf(4 * rows) if lists else None, buf(8 * rows) if lists else None, rows)
+
+    def extend(self, new, plan: KVPlan) -> None:
+        """Adds ``new`` i32 [slots] tokens to the slots and leaves the batch of
+        those with any in ``plan``."""
+        if new.nbytes < 4 * self.slots:
+            raise ValueError("new is smaller than [slots]")
+        plan._check(self.slots, self.table_stride)
+        _lib.call("eoship_kv_pager_extend_device", self.rt.handle, self.handle, new.ptr,
+                  C.byref(plan.c))
+
+    def trim(self, keep) -> None:
+        """Cuts slots down to ``keep`` i32 [slots] tokens (negative: as it is)."""
+        if keep.nbytes < 4 * self.slots:
+            raise ValueError("keep is smaller than [slots]")
+        _lib.call("eoship_kv_pager_trim_device", self.rt.handle, self.handle, keep.ptr)
+
+    def status(self) -> int:
+        """0 where every request of the calls since the last look was met (bit
+        0: too few free pages, 1: a table row too short, 2: a number out of
+        range); waits."""
+        st = C.c_int32()
+        _lib.call("eoship_kv_pager_status", self.rt.handle, self.handle, C.byref(st))
+        return st.value

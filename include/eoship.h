@@ -984,6 +984,151 @@ int eoship_kv_attention_device(EosHipRuntime* rt, EosHipKVCache* kv, const EosHi
  * if masked; nothing outside the pools and rows is touched. */
 int eoship_kv_status(EosHipRuntime* rt, EosHipKVCache* kv, int32_t* status, char** err);
 
+/* ------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (MXFP4): rows quantised and taken back,
+ * and linear layers over weights held so. The matrix units of gfx950 multiply
+ * the format as it lies, at twice their 8-bit rate.
+ *
+ * A row of k values is ceil(k / 32) blocks of 32 consecutive values (zeros
+ * behind the last). A block's scale is 2^e, held as the byte e + 127, with
+ * e = floor(log2(max |x|)) - 2 in -127..127 (a block of zeros: -127); its codes
+ * are sign and magnitude, 0 .5 1 1.5 2 3 4 6: x / 2^e rounded to the nearest,
+ * ties to the even code, beyond 6 to 6. A block with an infinity or a NaN has
+ * scale byte 255 and stands for NaN.
+ *   codes   [rows][ceil(k / 32)][16]  element 2 i of a block in byte i's low half
+ *   scales  [rows][ceil(k / 32)]
+ * Types: 0 f16, 1 bf16, 2 f32, where stated 3 (such codes). Rows of types 0..2
+ * are 16-byte aligned and lie a stride (in elements, a multiple of 8) apart;
+ * codes are 16-byte aligned and without gaps. k is in 1..2^24.
+ * ------------------------------------------------------------------------ */
+
+/* Bytes of the codes and of the scales of rows of k values. */
+int eoship_mx_bytes(int64_t rows, int32_t k, int64_t* code_bytes, int64_t* scale_bytes,
+                    char** err);
+/* Rows x [rows][k] into codes and scales. Enqueued (no wait). */
+int eoship_mx_quantize_device(EosHipRuntime* rt, const void* d_x, int64_t x_stride, int32_t dtype,
+                              int64_t rows, int32_t k, uint8_t* d_codes, uint8_t* d_scales,
+                              char** err);
+/* The values that codes and scales stand for, rounded once to out's type;
+ * what lies between out's rows stays. Enqueued. */
+int eoship_mx_dequantize_device(EosHipRuntime* rt, const uint8_t* d_codes, const uint8_t* d_scales,
+                                int64_t rows, int32_t k, void* d_out, int64_t out_stride,
+                                int32_t dtype, char** err);
+
+typedef struct EosHipMX EosHipMX;
+
+/* Binds a linear layer for one runtime: weights of n rows of k values as codes
+ * and scales, and a bias f32 [n] or NULL. They are laid out anew on the device
+ * and not needed once the call has returned (it waits). n is in 1..2^24. */
+int eoship_mx_bind(EosHipRuntime* rt, const uint8_t* d_codes, const uint8_t* d_scales, int32_t n,
+                   int32_t k, const float* d_bias, EosHipMX** out, char** err);
+int eoship_mx_release(EosHipRuntime* rt, EosHipMX* mx, char** err);
+/* out [rows][n] = Q(x) W^T + bias: x's rows are quantised within the call
+ * (types 0..2), or are codes (3: d_x_scales are their scales, x_stride is not
+ * looked at). Products are exact, sums f32, rounded once to out's type. A row
+ * with a block that stands for NaN gives NaN; what lies between out's rows
+ * stays; out and x do not overlap. Uses the runtime's workspace. Enqueued. */
+int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, int64_t x_stride,
+                            int32_t dtype, const uint8_t* d_x_scales, int64_t rows, void* d_out,
+                            int64_t out_stride, int32_t out_dtype, char** err);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions of queries and keys: in each head, two values (x, y) of
+ * frequency f at position p become c (x cos pf - y sin pf), c (x sin pf + y
+ * cos pf). The reference turns whole rows by pairs (ropeRows,
+ * runtime/backend/tensor_ops.go:1936-1965).
+ * ------------------------------------------------------------------------ */
+
+typedef struct {
+  int32_t head_dim;     /* D: a multiple of 8, 8..1024 */
+  int32_t rotary_dim;   /* R: even, 2..D; values from R on are left as they are */
+  int32_t layout;       /* 0: pairs (2 i, 2 i + 1); 1: halves (i, i + R / 2) */
+  float factor;         /* c, finite (1, or what a stretched context takes) */
+  const double* frequencies;  /* host [R / 2], radians a position, at most 64 */
+} EosHipRotaryDesc;
+
+typedef struct EosHipRotary EosHipRotary;
+
+/* Binds frequencies for one runtime (the host array is not kept). */
+int eoship_rotary_bind(EosHipRuntime* rt, const EosHipRotaryDesc* desc, EosHipRotary** out,
+                       char** err);
+int eoship_rotary_release(EosHipRuntime* rt, EosHipRotary* rot, char** err);
+/* Turns rows of queries [rows][heads][D] and of keys [rows][kv_heads][D]
+ * (dtype 0 f16, 1 bf16, 2 f32; 16-byte aligned, strides in elements, multiples
+ * of 8; heads or kv_heads 0: none) by their positions: those of a cache's
+ * batch (its page table is not looked at, rows is the batch's), or
+ * d_positions i32 [rows] with batch NULL. Rows of a negative position and
+ * rows of no sequence are not written. Angles are taken from f64 products,
+ * sums are f32, rounded once. inverse nonzero: by -p f, which is also the
+ * gradient of the forward call. In place where an output is its input with the
+ * same stride; otherwise they do not overlap. Enqueued (no wait). */
+int eoship_rotary_device(EosHipRuntime* rt, EosHipRotary* rot, const EosHipKVBatch* batch,
+                         const int32_t* d_positions, int64_t rows, int32_t inverse, int32_t dtype,
+                         const void* d_q, int64_t q_stride, int32_t heads, void* d_q_out,
+                         int64_t q_out_stride, const void* d_k, int64_t k_stride, int32_t kv_heads,
+                         void* d_k_out, int64_t k_out_stride, char** err);
+
+/* ------------------------------------------------------------------------
+ * Page tables of a key-value cache, kept on the device: a server's requests
+ * are slots 0..slots-1, each with a length and the pages that hold it; free
+ * pages are a stack. A step extends some slots, runs on the batch that the
+ * call leaves, and trims what it drops; nothing is planned on the host.
+ * ------------------------------------------------------------------------ */
+
+typedef struct {
+  int32_t slots;          /* 1..4096 */
+  int32_t table_stride;   /* pages of a slot at most, 1..2^26 */
+  int32_t page_tokens;    /* P: the cache's (16, 32, 64, 128 or 256) */
+  int64_t pages;          /* 1..2^31-1 */
+  /* Device memory of the caller, as reset or as earlier calls left it: */
+  int32_t* d_page_table;  /* [slots][table_stride], -1 where a slot holds none */
+  int32_t* d_lengths;     /* [slots] tokens */
+  int32_t* d_free;        /* [pages], the first free_count of them free, the last the top */
+  int32_t* d_free_count;  /* [1] */
+} EosHipKVPagerDesc;
+
+typedef struct EosHipKVPager EosHipKVPager;
+
+/* What an extend leaves for the calls of a step: the batch of the slots that
+ * got rows, in their order. Fields of EosHipKVBatch: d_page_table, d_lengths
+ * and, unless every sequence has one row, d_offsets; batch and rows are the
+ * number of slots with new tokens and their sum. Device memory; what lies
+ * behind the batch and its rows, and table entries behind a sequence's pages,
+ * stay. */
+typedef struct {
+  int32_t* d_slots;       /* [slots] slot of each sequence */
+  int32_t* d_page_table;  /* [slots][table_stride] or NULL */
+  int32_t* d_lengths;     /* [slots] the new rows included; 0: refused */
+  int32_t* d_offsets;     /* [slots + 1] */
+  int32_t* d_positions;   /* [rows] position of each row in its sequence, or NULL */
+  int64_t* d_slot_map;    /* [rows] page * P + place in the page, or NULL */
+  int64_t rows;           /* rows that the arrays hold */
+} EosHipKVPlan;
+
+/* Binds the arrays for one runtime; they stay the caller's. */
+int eoship_kv_pager_bind(EosHipRuntime* rt, const EosHipKVPagerDesc* desc, EosHipKVPager** out,
+                         char** err);
+int eoship_kv_pager_release(EosHipRuntime* rt, EosHipKVPager* pager, char** err);
+/* All slots empty, all pages free (page 0 on top). Enqueued, as the next two. */
+int eoship_kv_pager_reset_device(EosHipRuntime* rt, EosHipKVPager* pager, char** err);
+/* Adds d_new i32 [slots] tokens to the slots (0: not in the batch). New pages
+ * come off the stack slot by slot, page by page. Refused, with nothing of the
+ * slot's changed, are a request beyond its table row, one of whose rows not
+ * all are below plan->rows, and from the first request on that the stack does
+ * not cover all those that need a page. A refused request keeps its rows in
+ * the batch, as padding: length 0, positions and slots -1. */
+int eoship_kv_pager_extend_device(EosHipRuntime* rt, EosHipKVPager* pager, const int32_t* d_new,
+                                  const EosHipKVPlan* plan, char** err);
+/* Cuts slots down to d_keep i32 [slots] tokens (0: the request is over;
+ * negative or not below its length: it stays as it is). Pages go back in
+ * such an order that an extend undone leaves the stack as it was. */
+int eoship_kv_pager_trim_device(EosHipRuntime* rt, EosHipKVPager* pager, const int32_t* d_keep,
+                                char** err);
+/* What calls since the last look found: bit 0 too few free pages, bit 1 a
+ * table row too short, bit 2 a number out of range (new tokens, a length, the
+ * free count, rows). Synchronises and clears it. */
+int eoship_kv_pager_status(EosHipRuntime* rt, EosHipKVPager* pager, int32_t* status, char** err);
+
 #ifdef __cplusplus
 }
 #endif
