@@ -156,7 +156,7 @@ int eoship_kv_pager_extend_device(EosHipRuntime* rt, EosHipKVPager* pager, const
     a.slot_map = plan->d_slot_map;
     a.rows = plan->rows;
     const bool listed = a.positions != nullptr || a.slot_map != nullptr;
-    return rt->launch("eos_pager_extend", dim3(blocks(pager, listed ? a.rows : 0)), dim3(kThreads),
+    return rt->launch(a.slots <= kPagerFew ? "eos_pager_extend_few" : a.slots <= kThreads ? "eos_pager_extend_some" : "eos_pager_extend_many", dim3(blocks(pager, listed ? a.rows : 0)), dim3(kThreads),
                       (4 * (size_t)a.slots + 1) * 4, &a, err);
   });
 }
@@ -172,7 +172,7 @@ int eoship_kv_pager_trim_device(EosHipRuntime* rt, EosHipKVPager* pager, const i
     OnDevice on(rt->device);
     PagerArgs a = args(pager);
     a.ask = d_keep;
-    return rt->launch("eos_pager_trim", dim3(blocks(pager, 0)), dim3(kThreads),
+    return rt->launch(a.slots <= kPagerFew ? "eos_pager_trim_few" : a.slots <= kThreads ? "eos_pager_trim_some" : "eos_pager_trim_many", dim3(blocks(pager, 0)), dim3(kThreads),
                       3 * (size_t)a.slots * 4, &a, err);
   });
 }

@@ -29,7 +29,10 @@ struct RotArgs {
 // Status bits of a pager.
 enum { kPagerNoPages = 1, kPagerNoRoom = 2, kPagerBadNumber = 4 };
 constexpr int kPagerSlots = 4096;    // slots that every workgroup sums up
-constexpr int kPagerSegment = 1024;  // table entries that a wavefront moves at a time
+constexpr int kPagerFew = 64;       // ... and every wavefront
+constexpr int kPagerShort = 4;      // rows of a request that one thread writes
+constexpr int kPagerUnit = 256;    // rows that a wavefront takes at a time
+constexpr int kPagerEntries = 256;  // table entries that it does
 
 // state[0] status bits, state[1] workgroups that are done
 struct PagerArgs {

@@ -188,29 +188,52 @@ EOS_DEV void rotate(const RotArgs& a) {
 
 // --------------------------------------------------------------- page tables
 
-constexpr int kThreads = 1024;
-constexpr int kEach = kPagerSlots / kThreads;  // slots of a thread
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
 
-// Sum over the threads in front of this one, and of all.
+// A barrier that LDS accesses are complete at, stores to memory not.
+EOS_DEV void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <int CTRL, int ROWS>
+EOS_DEV long long from_lane(long long x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, true);
+  return (long long)hi << 32 | (uint32_t)lo;
+}
+// Sum of a wavefront's lanes up to and with this one, by the vector unit's own
+// lane moves (a shuffle goes through LDS: a fifth as fast here).
+EOS_DEV long long upto_lane(long long x) {
+  x += from_lane<0x111, 0xf>(x);  // rows of 16 shifted by 1, 2, 4, 8
+  x += from_lane<0x112, 0xf>(x);
+  x += from_lane<0x114, 0xf>(x);
+  x += from_lane<0x118, 0xf>(x);
+  x += from_lane<0x142, 0xa>(x);  // a row's last to the next row, the second's to the last two
+  return x + from_lane<0x143, 0xc>(x);
+}
+EOS_DEV long long of_lane(long long x, int lane) {
+  return (long long)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+// The sum of the threads in front of this one, and of all; where FEW, every
+// wavefront has the same numbers and needs no other.
+template <bool FEW>
 EOS_DEV long long before(long long x, long long* sums, long long& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-  long long upto = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const long long y = __shfl_up(upto, d);
-    if (lane >= d) upto += y;
+  const long long in = upto_lane(x);
+  long long at = in - x;
+  total = of_lane(in, 63);
+  if constexpr (!FEW) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    lds_barrier();
+    if (lane == 0) sums[wave] = total;
+    lds_barrier();
+    const long long all = upto_lane(lane < kWaves ? sums[lane] : 0);
+    if (wave > 0) at += of_lane(all, wave - 1);
+    total = of_lane(all, kWaves - 1);
   }
-  __syncthreads();
-  if (lane == 63) sums[wave] = upto;
-  __syncthreads();
-  long long base = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) base += sums[w];
-    total += sums[w];
-  }
-  return base + upto - x;
+  return at;
 }
 
 EOS_DEV long long room_of(const PagerArgs& a) {
@@ -228,157 +251,216 @@ EOS_DEV int free_pages(const PagerArgs& a, int& bad) {
 }
 
 // True in every thread of the workgroup that is done last: all others have
-// read the state that it is about to write.
+// read the state that it is about to write. (Nothing that they wrote is read:
+// their loads have returned, for what they loaded has been used.)
 EOS_DEV bool last_one(const PagerArgs& a, int* flag) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    *flag = atomicAdd(&a.state[1], 1) == (int)gridDim.x - 1;
-  }
+  lds_barrier();
+  if (gridDim.x == 1) return true;
+  if (threadIdx.x == 0)
+    *flag = __hip_atomic_fetch_add(&a.state[1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+            (int)gridDim.x - 1;
   __syncthreads();
   return *flag != 0;
 }
 
-// Every workgroup sums the requests of all slots up by itself (16 bytes a slot
-// from the L2, no second launch), keeps the batch's ranges in LDS and fills its
-// share of rows and table entries; the last one brings lengths and stack up to date.
+// Every workgroup sums the requests of all slots up by itself, E a thread (8 bytes
+// a slot from the L2, no second launch); where there are FEW, 64 at most, every
+// wavefront does, without a barrier. The rows of a short request its thread
+// writes; for the others and for the table entries, which the workgroups share,
+// the batch's ranges are left in LDS. The last one that is done brings lengths
+// and stack up to date. What these kernels wait for is a chain of loads and, each
+// instruction running once, the instructions: hence loops, not unrolled ones.
+template <bool FEW, int E>
 EOS_DEV void extend(const PagerArgs& a) {
   extern __shared__ int lds[];
-  __shared__ long long sums[kThreads / 64];
-  __shared__ int flag;
+  __shared__ long long sums[kWaves];
+  __shared__ int flag, taken, any_long;
   int* row_of = lds;                 // [batch + 1] first row
   int* len_of = row_of + a.slots + 1;  // [batch] tokens before, -1: refused
   int* page_of = len_of + a.slots;     // [batch] first new page's place below the stack's top
   int* slot_of = page_of + a.slots;    // [batch]
+  const int lane = threadIdx.x & 63, wave_in = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int wave = blockIdx.x * kWaves + wave_in, waves = gridDim.x * kWaves;
+  const int one = (1 << a.page_shift) - 1;
+  if (threadIdx.x == 0) taken = any_long = 0;
+  lds_barrier();
   const long long room = room_of(a);
-  int bad = 0;
-  const int count = free_pages(a, bad);
-  int len[kEach], fresh[kEach], need[kEach];
-  long long mine = 0;  // rows << 13 | requests
+  const int slot0 = (FEW ? lane : (int)threadIdx.x) * E;
+  int bad = 0, len[E], fresh[E], need[E];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int s = threadIdx.x * kEach + i;
+  for (int i = 0; i < E; ++i) {
     len[i] = fresh[i] = 0;
-    if (s < a.slots) {
-      fresh[i] = a.ask[s];
-      len[i] = a.lengths[s];
-      if (fresh[i] < 0) {
-        bad |= kPagerBadNumber;
-        fresh[i] = 0;
-      }
+    if (slot0 + i < a.slots) {
+      fresh[i] = a.ask[slot0 + i];
+      len[i] = a.lengths[slot0 + i];
+    }
+  }
+  const int count = free_pages(a, bad);
+  long long all, mine = 0;  // rows << 13 | requests
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (fresh[i] < 0) {
+      bad |= kPagerBadNumber;
+      fresh[i] = 0;
     }
     mine += fresh[i] > 0 ? ((long long)fresh[i] << 13) + 1 : 0;
   }
-  long long all;
-  long long at = before(mine, sums, all);
-  const int batch = (int)(all & 8191);
-  const long long rows = all >> 13;
+  const long long at0 = before<FEW>(mine, sums, all);
   // A request has room if its table row holds it and its rows are the caller's.
-  long long want = 0, row = at >> 13;
-  bool ok[kEach];
+  long long at = at0;
+  bool ok[E];
+  mine = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
+  for (int i = 0; i < E; ++i) {
     need[i] = 0;
     ok[i] = false;
     if (fresh[i] > 0) {
-      row += fresh[i];
-      if (len[i] < 0 || len[i] > room || row > a.rows) bad |= kPagerBadNumber;
+      at += ((long long)fresh[i] << 13) + 1;
+      if (len[i] < 0 || len[i] > room || (at >> 13) > a.rows) bad |= kPagerBadNumber;
       else if (len[i] + (long long)fresh[i] > room) bad |= kPagerNoRoom;
       else {
         ok[i] = true;
         need[i] = pages_of(len[i] + fresh[i], a.page_shift) - pages_of(len[i], a.page_shift);
+        mine += need[i];
       }
     }
-    want += need[i];
   }
-  long long asked;
-  long long page = before(want, sums, asked);
   // Pages go to slots in order until one asks for more than there are.
-  long long given = 0;
-  int j = (int)(at & 8191);
-  row = at >> 13;
+  long long asked;
+  long long page = before<FEW>(mine, sums, asked);
+  at = at0;
+  int given = 0;
+  bool rows_left = false;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (ok[i] && need[i] > 0 && page + need[i] > count) {
-      ok[i] = false;
-      bad |= kPagerNoPages;
+  for (int i = 0; i < E; ++i) {
+    if (need[i] > 0) {
+      if (page + need[i] > count) {
+        ok[i] = false;
+        bad |= kPagerNoPages;
+      } else {
+        given = (int)page + need[i];
+      }
     }
     if (fresh[i] > 0) {
-      const int s = threadIdx.x * kEach + i;
-      row_of[j] = (int)min(row, a.rows);
-      len_of[j] = ok[i] ? len[i] : -1;
-      page_of[j] = (int)min(page, (long long)count);
-      slot_of[j] = s;
-      if (blockIdx.x == 0) {
-        a.b_slots[j] = s;
-        a.b_lengths[j] = ok[i] ? len[i] + fresh[i] : 0;
-        a.b_offsets[j] = row_of[j];
+      const int s = slot0 + i, j = (int)(at & 8191), r0 = (int)min(at >> 13, a.rows);
+      const int n = (int)min((long long)fresh[i], a.rows - r0);
+      if (!FEW || wave_in == 0) {
+        row_of[j] = r0;
+        len_of[j] = ok[i] ? len[i] : -1;
+        page_of[j] = (int)min(page, (long long)count);
+        slot_of[j] = s;
+        if (blockIdx.x == 0) {
+          a.b_slots[j] = s;
+          a.b_lengths[j] = ok[i] ? len[i] + fresh[i] : 0;
+          a.b_offsets[j] = r0;
+        }
       }
-      row += fresh[i];
-      ++j;
+      rows_left |= n > kPagerShort;
+      if (n <= kPagerShort && (FEW ? wave == waves - 1 : (wave_in * E + i) % (int)gridDim.x == (int)blockIdx.x)) {
+        const int held = pages_of(len[i], a.page_shift);
+#pragma unroll 1
+        for (int c = 0; c < n; ++c) {
+          const int p = len[i] + c, e = p >> a.page_shift;
+          long long place = -1;
+          if (ok[i] && a.slot_map != nullptr) {
+            const int id = e < held ? a.table[(long long)s * a.stride + e]
+                                    : a.free_list[count - 1 - ((int)page + e - held)];
+            place = ((long long)id << a.page_shift) + (p & one);
+          }
+          if (a.positions != nullptr) a.positions[r0 + c] = ok[i] ? p : -1;
+          if (a.slot_map != nullptr) a.slot_map[r0 + c] = place;
+        }
+      }
+      at += ((long long)fresh[i] << 13) + 1;
     }
     page += need[i];
-    if (ok[i] && need[i] > 0) given = page;
   }
+  // The last granted request's end is what the stack has given.
+  const unsigned long long gave = __ballot(given > 0), left = __ballot(rows_left);
+  if (gave != 0) given = __builtin_amdgcn_readlane(given, 63 - __builtin_clzll(gave));
+  if (lane == 0 && gave != 0) atomicMax(&taken, given);
+  if (lane == 0 && left != 0) any_long = 1;
+  const int batch = (int)(all & 8191), upto = (int)min(all >> 13, a.rows);
   if (threadIdx.x == 0) {
-    row_of[batch] = (int)min(rows, a.rows);
-    if (blockIdx.x == 0) a.b_offsets[batch] = row_of[batch];
+    row_of[batch] = upto;
+    if (blockIdx.x == 0) a.b_offsets[batch] = upto;
   }
-  __syncthreads();
-  // Rows: their positions and slots.
-  const int upto = row_of[batch];
-  for (long long r = (long long)blockIdx.x * kThreads + threadIdx.x; r < upto;
-       r += (long long)gridDim.x * kThreads) {
-    int lo = 0, hi = batch - 1;  // the request whose range holds it
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (row_of[mid] <= r) lo = mid;
-      else hi = mid - 1;
-    }
-    int p = -1;
-    long long place = -1;
-    if (len_of[lo] >= 0) {
-      p = len_of[lo] + (int)(r - row_of[lo]);
-      const int i = p >> a.page_shift, held = pages_of(len_of[lo], a.page_shift);
-      const int id = i < held ? a.table[(long long)slot_of[lo] * a.stride + i]
-                              : a.free_list[count - 1 - (page_of[lo] + i - held)];
-      place = ((long long)id << a.page_shift) + (p & ((1 << a.page_shift) - 1));
-    }
-    if (a.positions != nullptr) a.positions[r] = p;
-    if (a.slot_map != nullptr) a.slot_map[r] = place;
-  }
-  // Table rows, by wavefronts: what a slot has, then its new pages.
-  const int segments = (a.stride + kPagerSegment - 1) / kPagerSegment;
-  const long long units = (long long)batch * segments;
-  for (long long u = (long long)blockIdx.x * (kThreads / 64) + threadIdx.x / 64; u < units;
-       u += (long long)gridDim.x * (kThreads / 64)) {
-    const int b = (int)(u / segments), first = (int)(u - (long long)b * segments) * kPagerSegment;
-    if (len_of[b] < 0) continue;
-    const int tokens = len_of[b] + row_of[b + 1] - row_of[b];
-    const int held = pages_of(len_of[b], a.page_shift), end = pages_of(tokens, a.page_shift);
-    int32_t* t = a.table + (long long)slot_of[b] * a.stride;
-    for (int i = first + (threadIdx.x & 63); i < min(end, first + kPagerSegment); i += 64) {
-      int id;
-      if (i < held) {
-        id = t[i];
-      } else {
-        id = a.free_list[count - 1 - (page_of[b] + i - held)];
-        t[i] = id;
+  lds_barrier();
+  // The rows of the others, 256 a wavefront: between the requests that the first
+  // and the last belong to lies each row's.
+  if (any_long != 0 && (a.positions != nullptr || a.slot_map != nullptr))
+    for (long long first = (long long)wave * kPagerUnit; first < upto; first += (long long)waves * kPagerUnit) {
+      const int end = (int)min(first + kPagerUnit, (long long)upto) - 1;
+      int j0 = 0, size = batch;  // 64 probes a turn
+      while (size > 1) {
+        const int step = (size + 63) / 64, probe = j0 + lane * step;
+        const int c = __popcll(__ballot(lane * step < size && row_of[min(probe, batch)] <= (int)first)) - 1;
+        j0 += c * step;
+        size = min(step, size - c * step);
       }
-      if (a.b_table != nullptr) a.b_table[(long long)b * a.stride + i] = id;
+      const int more = __popcll(__ballot(j0 + 1 + lane < batch && row_of[min(j0 + 1 + lane, batch)] <= end));
+      const int j1 = more < 64 ? j0 + more : min(batch - 1, j0 + kPagerUnit);
+      int p[kPagerUnit / 64], id[kPagerUnit / 64];
+      bool set[kPagerUnit / 64];
+#pragma unroll
+      for (int k = 0; k < kPagerUnit / 64; ++k) {
+        const int r = (int)first + k * 64 + lane;
+        p[k] = id[k] = -1;
+        set[k] = false;
+        if (r <= end) {
+          int b = j0, hi = j1;  // the last of them that begins at or before r
+          while (b < hi) {
+            const int mid = (b + hi + 1) / 2;
+            if (row_of[mid] <= r) b = mid;
+            else hi = mid - 1;
+          }
+          const int t = len_of[b];
+          set[k] = row_of[b + 1] - row_of[b] > kPagerShort;
+          if (set[k] && t >= 0) {
+            p[k] = t + (r - row_of[b]);
+            const int i = p[k] >> a.page_shift, held = pages_of(t, a.page_shift);
+            id[k] = i < held ? a.table[(long long)slot_of[b] * a.stride + i]
+                             : a.free_list[count - 1 - (page_of[b] + i - held)];
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kPagerUnit / 64; ++k) {
+        const long long r = first + k * 64 + lane;
+        if (!set[k]) continue;
+        if (a.positions != nullptr) a.positions[r] = p[k];
+        if (a.slot_map != nullptr)
+          a.slot_map[r] = p[k] < 0 ? -1 : ((long long)id[k] << a.page_shift) + (p[k] & one);
+      }
+    }
+  // Table rows: what a slot has, then its new pages; a wavefront a slot and
+  // kPagerEntries of its entries.
+  const int pieces = (a.stride + kPagerEntries - 1) / kPagerEntries;
+  for (int u = wave; u < batch * pieces; u += waves) {
+    const int b = pieces == 1 ? u : u / pieces, first = (u - b * pieces) * kPagerEntries;
+    const int t = len_of[b], held = pages_of(t, a.page_shift);
+    const int end = min(pages_of(t + row_of[b + 1] - row_of[b], a.page_shift), first + kPagerEntries);
+    if (t < 0 || first >= end || (a.b_table == nullptr && held >= end)) continue;
+    int32_t* from = a.table + (long long)slot_of[b] * a.stride;
+    int32_t* to = a.b_table != nullptr ? a.b_table + (long long)b * a.stride : nullptr;
+    const int32_t* top = a.free_list + (count - 1 - page_of[b] + held);
+    int id[kPagerEntries / 64];
+#pragma unroll
+    for (int k = 0; k < kPagerEntries / 64; ++k) {
+      const int i = first + k * 64 + lane;
+      if (i < end) id[k] = *(i < held ? from + i : top - i);
+    }
+#pragma unroll
+    for (int k = 0; k < kPagerEntries / 64; ++k) {
+      const int i = first + k * 64 + lane;
+      if (i < end && i >= held) from[i] = id[k];
+      if (i < end && to != nullptr) to[i] = id[k];
     }
   }
   if (blockIdx.x == 0 && bad != 0) atomicOr(&a.state[0], bad);
   if (!last_one(a, &flag)) return;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i)
-    if (ok[i]) a.lengths[threadIdx.x * kEach + i] = len[i] + fresh[i];
-  // The last granted request's end is what the stack has given.
-  __shared__ int taken;
-  if (threadIdx.x == 0) taken = 0;
-  __syncthreads();
-  if (given > 0) atomicMax(&taken, (int)given);
-  __syncthreads();
+  for (int j = threadIdx.x; j < batch; j += kThreads)
+    if (len_of[j] >= 0) a.lengths[slot_of[j]] = len_of[j] + row_of[j + 1] - row_of[j];
   if (threadIdx.x == 0) {
     *a.free_count = count - taken;
     a.state[1] = 0;
@@ -387,66 +469,85 @@ EOS_DEV void extend(const PagerArgs& a) {
 
 // Pages behind the tokens to keep go back onto the stack, the last slot's last
 // page first: extends undone leave it as it was.
+template <bool FEW, int E>
 EOS_DEV void trim(const PagerArgs& a) {
   extern __shared__ int lds[];
-  __shared__ long long sums[kThreads / 64];
+  __shared__ long long sums[kWaves];
   __shared__ int flag;
   int* page_of = lds;                // [slots] pages in front of a slot's
   int* gone_of = page_of + a.slots;  // [slots] its pages
-  int* left_of = gone_of + a.slots;  // [slots] pages that stay
+  int* keep_of = gone_of + a.slots;  // [slots] tokens that stay, -1: as they are
+  const int lane = threadIdx.x & 63, wave_in = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int wave = blockIdx.x * kWaves + wave_in, waves = gridDim.x * kWaves;
   const long long room = room_of(a);
-  int bad = 0;
-  const int count = free_pages(a, bad);
-  int keep[kEach], gone[kEach];
-  long long mine = 0;
+  const int slot0 = (FEW ? lane : (int)threadIdx.x) * E;
+  int bad = 0, len[E], keep[E], gone[E];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int s = threadIdx.x * kEach + i;
+  for (int i = 0; i < E; ++i) {
+    len[i] = 0;
     keep[i] = -1;
+    if (slot0 + i < a.slots) {
+      len[i] = a.lengths[slot0 + i];
+      keep[i] = a.ask[slot0 + i];
+    }
+  }
+  const int count = free_pages(a, bad);
+  long long all, mine = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
     gone[i] = 0;
-    if (s < a.slots) {
-      const int len = a.lengths[s], k = a.ask[s];
-      if (len < 0 || len > room) {
-        bad |= kPagerBadNumber;
-      } else if (k >= 0 && k < len) {
-        keep[i] = k;
-        left_of[s] = pages_of(k, a.page_shift);
-        gone[i] = pages_of(len, a.page_shift) - left_of[s];
-      }
-      gone_of[s] = gone[i];
+    if (len[i] < 0 || len[i] > room) {
+      bad |= kPagerBadNumber;
+      keep[i] = -1;
+    } else if (keep[i] >= len[i]) {
+      keep[i] = -1;
+    } else if (keep[i] >= 0) {
+      gone[i] = pages_of(len[i], a.page_shift) - pages_of(keep[i], a.page_shift);
     }
     mine += gone[i];
   }
-  long long total;
-  long long at = before(mine, sums, total);
+  long long at = before<FEW>(mine, sums, all);
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int s = threadIdx.x * kEach + i;
-    if (s < a.slots) page_of[s] = (int)min(at, (long long)INT32_MAX);
+  for (int i = 0; i < E; ++i) {
+    const int s = slot0 + i;
+    if (s < a.slots && (!FEW || wave_in == 0)) {
+      page_of[s] = (int)min(at, (long long)INT32_MAX);
+      gone_of[s] = gone[i];
+      keep_of[s] = keep[i];
+    }
     at += gone[i];
   }
-  if (count + total > a.pages) bad |= kPagerBadNumber;
-  __syncthreads();
-  const int segments = (a.stride + kPagerSegment - 1) / kPagerSegment;
-  const long long units = (long long)a.slots * segments;
-  for (long long u = (long long)blockIdx.x * (kThreads / 64) + threadIdx.x / 64; u < units;
-       u += (long long)gridDim.x * (kThreads / 64)) {
-    const int s = (int)(u / segments), first = (int)(u - (long long)s * segments) * kPagerSegment;
-    if (first >= gone_of[s]) continue;
-    int32_t* t = a.table + (long long)s * a.stride + left_of[s];
-    for (int i = first + (threadIdx.x & 63); i < min(gone_of[s], first + kPagerSegment); i += 64) {
-      const long long to = count + total - 1 - (page_of[s] + (long long)i);
-      if (to >= 0 && to < a.pages) a.free_list[to] = t[i];
-      t[i] = -1;
+  if (count + all > a.pages) bad |= kPagerBadNumber;
+  lds_barrier();
+  if (all > 0) {
+    const int pieces = (a.stride + kPagerEntries - 1) / kPagerEntries;
+    for (int u = wave; u < a.slots * pieces; u += waves) {
+      const int s = pieces == 1 ? u : u / pieces, first = (u - s * pieces) * kPagerEntries;
+      const int end = min(gone_of[s], first + kPagerEntries);
+      if (first >= end) continue;
+      int32_t* from = a.table + (long long)s * a.stride + pages_of(keep_of[s], a.page_shift);
+      const long long top = count + all - 1 - page_of[s];
+      int id[kPagerEntries / 64];
+#pragma unroll
+      for (int k = 0; k < kPagerEntries / 64; ++k) {
+        const int i = first + k * 64 + lane;
+        if (i < end) id[k] = from[i];
+      }
+#pragma unroll
+      for (int k = 0; k < kPagerEntries / 64; ++k) {
+        const int i = first + k * 64 + lane;
+        if (i >= end) continue;
+        if (top - i >= 0 && top - i < a.pages) a.free_list[top - i] = id[k];
+        from[i] = -1;
+      }
     }
   }
   if (blockIdx.x == 0 && bad != 0) atomicOr(&a.state[0], bad);
   if (!last_one(a, &flag)) return;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i)
-    if (keep[i] >= 0) a.lengths[threadIdx.x * kEach + i] = keep[i];
+  for (int s = threadIdx.x; s < a.slots; s += kThreads)
+    if (keep_of[s] >= 0) a.lengths[s] = keep_of[s];
   if (threadIdx.x == 0) {
-    *a.free_count = (int)min(count + total, a.pages);
+    *a.free_count = (int)min(count + all, a.pages);
     a.state[1] = 0;
   }
 }
@@ -470,8 +571,16 @@ ROT_KERNELS(f16, kRotF16)
 ROT_KERNELS(bf16, kRotBf16)
 ROT_KERNELS(f32, kRotF32)
 
-extern "C" __global__ __launch_bounds__(kThreads) void eos_pager_extend(PagerArgs a) { extend(a); }
-extern "C" __global__ __launch_bounds__(kThreads) void eos_pager_trim(PagerArgs a) { trim(a); }
+#define PAGER_KERNELS(NAME, FEW, E)                                                                \
+  extern "C" __global__ __launch_bounds__(kThreads) void eos_pager_extend_##NAME(PagerArgs a) {    \
+    extend<FEW, E>(a);                                                                             \
+  }                                                                                                \
+  extern "C" __global__ __launch_bounds__(kThreads) void eos_pager_trim_##NAME(PagerArgs a) {      \
+    trim<FEW, E>(a);                                                                               \
+  }
+PAGER_KERNELS(few, true, 1)
+PAGER_KERNELS(some, false, 1)
+PAGER_KERNELS(many, false, kPagerSlots / kThreads)
 
 extern "C" __global__ __launch_bounds__(256) void eos_pager_reset(PagerArgs a) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)gridDim.x * 256;
