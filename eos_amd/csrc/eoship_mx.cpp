@@ -29,6 +29,24 @@ namespace {
 
 constexpr int kMost = 1 << 24;  // values of a row, outputs of a layer
 
+// Which kernel takes a layer's rows (256 CUs; us of a call among others, 4,096
+// values, bf16).
+// Up to 16 rows are quantised by the workgroups that multiply them, in one
+// launch (16 rows by 6,144 weights 8.6; laid out first 9.7). A workgroup takes
+// 16 weights, 32 where there are more of those than CUs (1 row by 6,144: 6.4 and
+// 6.1, by 4,096: 5.7 and 5.9), 64 where there are more than twice as many and the
+// rows' quantisation weighs (16 by 16,384: 19.7, 13.7 and 12.8; 1 by 16,384: 10.8,
+// 9.1 and 10.2).
+constexpr int kFewRows = 16;
+// Up to 64 are laid out by a launch before and multiplied in the same way (64 by
+// 2,048 9.1, by tiles of 64 11.9; by 6,144 12.0 and 14.6, by 16,384 16.0 and 16.3).
+constexpr int kSomeRows = 64;
+// More go by tiles of outputs. Tiles of 64 while there are no more than two a CU
+// (512 by 4,096: 17.0, by tiles of 128 18.9; 1,024 by 4,096: 26.0 and 22.0); then
+// of 128, two workgroups a CU, or of 256, one, whose turn takes 4/3 the time of the
+// two's (2,048 by 4,096, a turn each: 32.4 and 39.7; by 16,384, four turns and two:
+// 101 and 89).
+
 const char* const kTypes[] = {"f16", "bf16", "f32", "codes"};
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -39,12 +57,11 @@ MxLaid laid(long long rows, int k) {
   MxLaid m{};
   m.rows = rows;
   m.blocks = ceil_div(k, kMxBlock);
-  m.steps = ceil_div(k, kMxStep);
-  m.quads = ceil_div(m.steps, 4);
+  m.quads = ceil_div(k, kMxQuad);
   return m;
 }
 size_t tiles(const MxLaid& m) { return (size_t)((m.rows + kMxTile - 1) / kMxTile); }
-size_t code_bytes(const MxLaid& m) { return tiles(m) * m.steps * kMxTileBytes; }
+size_t code_bytes(const MxLaid& m) { return tiles(m) * m.quads * kMxTileBytes; }
 size_t scale_bytes(const MxLaid& m) { return tiles(m) * m.quads * kMxScaleBytes; }
 void place(MxLaid* m, void* mem) {
   m->codes = static_cast<uint8_t*>(mem);
@@ -103,6 +120,12 @@ int lay(EosHipRuntime* rt, const MxLaid& to, const void* x, int64_t stride, int 
   a.blocks = to.blocks;
   return launch(rt, std::string("eos_mx_lay_") + kTypes[type], (long long)tiles(to) * to.quads, &a,
                 what, err);
+}
+
+// Few rows by 16 `tiles` rows of weights a workgroup.
+int few(EosHipRuntime* rt, const std::string& kind, int tiles, MxLinearArgs* a, char** err) {
+  const std::string name = "eos_mx_few_" + kind + "_" + std::to_string(tiles);
+  return rt->launch(name.c_str(), dim3((unsigned)ceil_div(a->n, 16 * tiles)), dim3(512), 0, a, err);
 }
 
 }  // namespace
@@ -244,14 +267,31 @@ int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, in
     a.rows = rows;
     a.n = mx->n;
     a.k = mx->k;
+    a.out_type = out_dtype;
+    const int cus = rt->compute_units, n16 = ceil_div(mx->n, 16);
+    if (rows <= kFewRows) {
+      a.rows_x = static_cast<const uint8_t*>(d_x);
+      a.scales_x = d_x_scales;
+      a.x_stride = dtype == kMxCodes ? 0 : x_stride * size_of(dtype);
+      const bool four = dtype != kMxCodes && rows <= 4;
+      const int tiles = n16 <= cus ? 1 : n16 <= 2 * cus || four || dtype == kMxCodes ? 2 : 4;
+      return few(rt, std::string(kTypes[dtype]) + (four ? "_4" : "_16"), tiles, &a, err);
+    }
     void* ws = nullptr;
     if (rt->workspace(code_bytes(a.x) + scale_bytes(a.x), &ws, err) != 0) return 1;
     place(&a.x, ws);
     if (lay(rt, a.x, d_x, x_stride, dtype, d_x_scales, mx->k, what, err) != 0) return 1;
-    a.tiles_m = (int)((rows + 63) / 64);
-    a.tiles_n = ceil_div(mx->n, 64);
-    return launch(rt, std::string("eos_mx_linear_") + kTypes[out_dtype],
-                  (long long)a.tiles_m * a.tiles_n, &a, what, err);
+    if (rows <= kSomeRows)
+      return few(rt, "laid_" + std::to_string((rows + 15) / 16 * 16), n16 <= cus ? 1 : 2, &a, err);
+    const auto count = [&](int t) { return ((rows + t - 1) / t) * ceil_div(mx->n, t); };
+    const auto turns = [&](long long tiles, int at_once) {
+      return (tiles + (long long)at_once * cus - 1) / ((long long)at_once * cus);
+    };
+    const int t = count(64) <= 2 * cus ? 64 : 4 * turns(count(256), 1) > 3 * turns(count(128), 2) ? 128 : 256;
+    a.tiles_m = (int)((rows + t - 1) / t);
+    a.tiles_n = ceil_div(mx->n, t);
+    return launch(rt, "eos_mx_product_" + std::to_string(t), (long long)a.tiles_m * a.tiles_n, &a,
+                  what, err);
   });
 }
 

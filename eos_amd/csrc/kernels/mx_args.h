@@ -9,23 +9,22 @@
 enum { kMxF16 = 0, kMxBf16 = 1, kMxF32 = 2, kMxCodes = 3 };
 
 constexpr int kMxBlock = 32;      // values of a scale
-constexpr int kMxStep = 128;      // values of K a matrix instruction takes
-constexpr int kMxTile = 16;       // rows of a laid-out tile
-constexpr int kMxTileBytes = 1024;  // a tile's codes of a step: 64 lanes of 16 bytes
-constexpr int kMxScaleBytes = 256;  // a tile's scales of four steps: 64 lanes of 4 bytes
+constexpr int kMxQuad = 256;      // values of K that are laid out together
+constexpr int kMxTile = 32;       // rows that are laid out together
+constexpr int kMxTileBytes = 4096;  // codes of both
+constexpr int kMxScaleBytes = 256;  // and scales
 
-// Rows in the order that matrix instructions read them. Tile t (16 rows) and
-// step s (128 values) are 1024 bytes at (t * steps + s) * 1024: lane l holds
-// block 4 s + l / 16 of row 16 t + l % 16. Its scales are byte s % 4 of the
-// lanes' words at (t * quads + s / 4) * 256. Rows and blocks that the matrix
-// lacks are zero.
+// Rows in the order that matrix instructions read them. Tile t (32 rows) and
+// quad q (four steps of 64 values) are 4096 bytes at (t * quads + q) * 4096:
+// step s's 1024 hold, 16 bytes a lane, block 8 q + 2 s + l / 32 of row
+// 32 t + l % 32. Their scales are byte s of the lanes' words at (t * quads + q)
+// * 256. Rows and blocks that the matrix lacks are zero.
 struct MxLaid {
   uint8_t* codes;
   uint8_t* scales;
   long long rows;
   int blocks;      // ceil(k / 32)
-  int steps;       // ceil(k / 128)
-  int quads;       // ceil(steps / 4)
+  int quads;       // ceil(k / 256)
 };
 
 struct MxQuantArgs {
@@ -49,12 +48,15 @@ struct MxDequantArgs {
 };
 
 struct MxLinearArgs {
-  MxLaid x, w;
-  const float* bias;   // [n] or NULL
+  MxLaid x, w;           // x where its rows are laid out
+  const uint8_t* rows_x;   // and where they are not: rows, or codes
+  const uint8_t* scales_x;
+  long long x_stride;    // bytes
+  const float* bias;     // [n] or NULL
   uint8_t* out;
   long long out_stride;  // bytes
   long long rows;
-  int n, k;
+  int n, k, out_type;
   int tiles_m, tiles_n;  // workgroup tiles
 };
 
