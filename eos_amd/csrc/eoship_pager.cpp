@@ -4,6 +4,7 @@
 // 1428-1431); the reference plans its buffers on the host.
 #include <algorithm>
 #include <cstdint>
+#include <string>
 
 #include "eoship_internal.h"
 #include "kernels/step_args.h"
@@ -69,11 +70,17 @@ PagerArgs args(const EosHipKVPager* p) {
   return a;
 }
 
-// Workgroups for so many table entries and rows: a few of either a thread, on
-// every CU at most.
-unsigned blocks(const EosHipKVPager* p, long long rows) {
-  const long long work = std::max((long long)p->d.slots * p->d.table_stride, rows);
-  return (unsigned)std::max(1LL, std::min<long long>(p->rt->compute_units, work / (2 * kThreads)));
+// Every wavefront sums up to 64 slots up by itself, a workgroup 1,024, a slot a
+// thread, or 4,096. Workgroups: two table entries or rows a thread, on every CU at
+// most (extend and trim, 64 slots of 128 pages: 1 workgroup 6.7 + 2.7 us, 4 5.4 +
+// 3.1; 4,096 slots of 512: 128 25.0 + 9.1, 256 19.4 + 9.7, 512 26.0 + 12.4).
+int launch(EosHipRuntime* rt, const EosHipKVPager* p, const char* op, long long rows, size_t lds,
+           PagerArgs* a, char** err) {
+  const std::string name = std::string("eos_pager_") + op +
+                           (a->slots <= kPagerFew ? "_few" : a->slots <= kThreads ? "_some" : "_many");
+  const long long work = std::max((long long)a->slots * a->stride, rows);
+  const long long blocks = std::max(1LL, std::min<long long>(rt->compute_units, work / (2 * kThreads)));
+  return rt->launch(name.c_str(), dim3((unsigned)blocks), dim3(kThreads), lds, a, err);
 }
 
 }  // namespace
@@ -145,6 +152,10 @@ int eoship_kv_pager_extend_device(EosHipRuntime* rt, EosHipKVPager* pager, const
         !aligned(plan->d_offsets, 4) || !aligned(plan->d_page_table, 4) ||
         !aligned(plan->d_positions, 4) || !aligned(plan->d_slot_map, 8))
       return set_err(err, "%s: arrays must be aligned to their elements", what);
+    const EosHipKVPagerDesc& d = pager->d;
+    if (plan->d_page_table == d.d_page_table || plan->d_lengths == d.d_lengths ||
+        plan->d_slots == d.d_lengths || plan->d_offsets == d.d_lengths)
+      return set_err(err, "%s: a plan's arrays are not the pager's own", what);
     OnDevice on(rt->device);
     PagerArgs a = args(pager);
     a.ask = d_new;
@@ -156,8 +167,7 @@ int eoship_kv_pager_extend_device(EosHipRuntime* rt, EosHipKVPager* pager, const
     a.slot_map = plan->d_slot_map;
     a.rows = plan->rows;
     const bool listed = a.positions != nullptr || a.slot_map != nullptr;
-    return rt->launch(a.slots <= kPagerFew ? "eos_pager_extend_few" : a.slots <= kThreads ? "eos_pager_extend_some" : "eos_pager_extend_many", dim3(blocks(pager, listed ? a.rows : 0)), dim3(kThreads),
-                      (4 * (size_t)a.slots + 1) * 4, &a, err);
+    return launch(rt, pager, "extend", listed ? a.rows : 0, (4 * (size_t)a.slots + 1) * 4, &a, err);
   });
 }
 
@@ -172,8 +182,7 @@ int eoship_kv_pager_trim_device(EosHipRuntime* rt, EosHipKVPager* pager, const i
     OnDevice on(rt->device);
     PagerArgs a = args(pager);
     a.ask = d_keep;
-    return rt->launch(a.slots <= kPagerFew ? "eos_pager_trim_few" : a.slots <= kThreads ? "eos_pager_trim_some" : "eos_pager_trim_many", dim3(blocks(pager, 0)), dim3(kThreads),
-                      3 * (size_t)a.slots * 4, &a, err);
+    return launch(rt, pager, "trim", 0, 3 * (size_t)a.slots * 4, &a, err);
   });
 }
 

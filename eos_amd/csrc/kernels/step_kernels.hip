@@ -120,68 +120,89 @@ EOS_DEV void rotate(const RotArgs& a) {
   }
   __syncthreads();
   const int lane = threadIdx.x & ((1 << a.lanes_shift) - 1);
-  const int heads = a.heads + a.kv_heads, step = 256 >> a.lanes_shift;
-  for (int r = 0; r < a.each; ++r) {
-    if (pos[r] < 0) continue;
-    const v2f* turns = cs + r * half;
-    for (int h = threadIdx.x >> a.lanes_shift; h < heads; h += step) {
-      const bool key = h >= a.heads;
-      const long long row = row0 + r;
-      const long long at = (long long)(key ? h - a.heads : h) * a.head_dim * size_of(T);
-      const uint8_t* x = (key ? a.k + row * a.k_stride : a.q + row * a.q_stride) + at;
-      uint8_t* y = (key ? a.k_out + row * a.k_out_stride : a.q_out + row * a.q_out_stride) + at;
-      if constexpr (WIDE && LAYOUT == kRotHalves) {
-        if (lane < half / 8) {
-          float u[8], v[8];
-          load8<T>(x + lane * 8 * size_of(T), u);
-          load8<T>(x + (half + lane * 8) * size_of(T), v);
+  const int heads = a.heads + a.kv_heads, step = 256 >> a.lanes_shift, all = a.each * heads;
+  // A head of a row: where it stands and goes, and its row's turns.
+  const auto head = [&](int i, const uint8_t*& x, uint8_t*& y, int& r) {
+    r = a.each == 1 ? 0 : i / heads;
+    const int h = i - r * heads;
+    const bool key = h >= a.heads;
+    const long long row = row0 + r, at = (long long)(key ? h - a.heads : h) * a.head_dim * size_of(T);
+    x = (key ? a.k + row * a.k_stride : a.q + row * a.q_stride) + at;
+    y = (key ? a.k_out + row * a.k_out_stride : a.q_out + row * a.q_out_stride) + at;
+  };
+  if constexpr (WIDE) {
+    // The lane's eight values, of halves also the eight that they turn with. Pairs:
+    // four heads' loads are in flight (9,000 ragged rows of 40 heads of 128, a
+    // quarter turned: 48 -> 41 us, 4.5 TB/s), halves have two already (16,384 rows of
+    // 64 heads: 100 us, 5.4 TB/s; with four heads' 107).
+    constexpr bool kHalves = LAYOUT == kRotHalves;
+    constexpr int kHeads = kHalves ? 1 : 4;
+    const int turning = kHalves ? half / 8 : a.rotary_dim / 8;  // lanes
+    const bool turns = lane < turning;
+    const int at0 = (turns || !kHalves ? lane * 8 : a.rotary_dim + (lane - turning) * 8) * size_of(T);
+    const bool any = at0 < a.head_dim * size_of(T);
+    const v2f* my = cs + (kHalves ? lane * 8 : lane * 4);
+    for (int i0 = threadIdx.x >> a.lanes_shift; i0 < all; i0 += kHeads * step) {
+      float u[kHeads][8], v[kHeads][kHalves ? 8 : 1];
+      uint8_t* y[kHeads];
+      int r[kHeads];
+      bool live[kHeads];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const v2f t = turns[lane * 8 + i];
-            const float p = u[i] * t[0] - v[i] * t[1];
-            v[i] = u[i] * t[1] + v[i] * t[0];
-            u[i] = p;
-          }
-          store8<T>(y + lane * 8 * size_of(T), u);
-          store8<T>(y + (half + lane * 8) * size_of(T), v);
-        } else {
-          const int i = a.rotary_dim + (lane - half / 8) * 8;
-          if (i < a.head_dim && x != y) {
-            float u[8];
-            load8<T>(x + i * size_of(T), u);
-            store8<T>(y + i * size_of(T), u);
-          }
+      for (int c = 0; c < kHeads; ++c) {
+        live[c] = false;
+        if (i0 + c * step >= all) continue;
+        const uint8_t* x;
+        head(i0 + c * step, x, y[c], r[c]);
+        live[c] = any && pos[r[c]] >= 0 && (turns || x != y[c]);
+        if (!live[c]) continue;
+        load8<T>(x + at0, u[c]);
+        if constexpr (kHalves) {
+          if (turns) load8<T>(x + at0 + half * size_of(T), v[c]);
         }
-      } else if constexpr (WIDE) {
-        const int i = lane * 8;
-        if (i < a.rotary_dim) {
-          float u[8];
-          load8<T>(x + i * size_of(T), u);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const v2f t = turns[lane * 4 + j];
-            const float p = u[2 * j] * t[0] - u[2 * j + 1] * t[1];
-            u[2 * j + 1] = u[2 * j] * t[1] + u[2 * j + 1] * t[0];
-            u[2 * j] = p;
-          }
-          store8<T>(y + i * size_of(T), u);
-        } else if (i < a.head_dim && x != y) {
-          float u[8];
-          load8<T>(x + i * size_of(T), u);
-          store8<T>(y + i * size_of(T), u);
-        }
-      } else {
-        for (int i = lane; i < half; i += 1 << a.lanes_shift) {
-          const int i0 = LAYOUT == kRotPairs ? 2 * i : i, i1 = LAYOUT == kRotPairs ? 2 * i + 1 : i + half;
-          const v2f t = turns[i];
-          const float u = load1<T>(x, i0), v = load1<T>(x, i1);
-          store1<T>(y, i0, u * t[0] - v * t[1]);
-          store1<T>(y, i1, u * t[1] + v * t[0]);
-        }
-        if (x != y)
-          for (int i = a.rotary_dim + lane; i < a.head_dim; i += 1 << a.lanes_shift)
-            store1<T>(y, i, load1<T>(x, i));
       }
+#pragma unroll
+      for (int c = 0; c < kHeads; ++c) {
+        if (!live[c]) continue;
+        const v2f* t = my + r[c] * half;
+        if constexpr (kHalves) {
+          if (turns) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float p = u[c][i] * t[i][0] - v[c][i] * t[i][1];
+              v[c][i] = u[c][i] * t[i][1] + v[c][i] * t[i][0];
+              u[c][i] = p;
+            }
+            store8<T>(y[c] + at0 + half * size_of(T), v[c]);
+          }
+        } else if (turns) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = u[c][2 * i] * t[i][0] - u[c][2 * i + 1] * t[i][1];
+            u[c][2 * i + 1] = u[c][2 * i] * t[i][1] + u[c][2 * i + 1] * t[i][0];
+            u[c][2 * i] = p;
+          }
+        }
+        store8<T>(y[c] + at0, u[c]);
+      }
+    }
+  } else {
+    for (int i0 = threadIdx.x >> a.lanes_shift; i0 < all; i0 += step) {
+      const uint8_t* x;
+      uint8_t* y;
+      int r;
+      head(i0, x, y, r);
+      if (pos[r] < 0) continue;
+      const v2f* turns = cs + r * half;
+      for (int i = lane; i < half; i += 1 << a.lanes_shift) {
+        const int i0 = LAYOUT == kRotPairs ? 2 * i : i, i1 = LAYOUT == kRotPairs ? 2 * i + 1 : i + half;
+        const v2f t = turns[i];
+        const float u = load1<T>(x, i0), v = load1<T>(x, i1);
+        store1<T>(y, i0, u * t[0] - v * t[1]);
+        store1<T>(y, i1, u * t[1] + v * t[0]);
+      }
+      if (x != y)
+        for (int i = a.rotary_dim + lane; i < a.head_dim; i += 1 << a.lanes_shift)
+          store1<T>(y, i, load1<T>(x, i));
     }
   }
 }

@@ -98,14 +98,11 @@ class Rotary:
         except Exception:
             pass
 
-    def _rows(self, rows, heads, size, *bufs):
-        width, out = heads * self.head_dim, []
-        for buf, stride in bufs:
-            stride = width if stride is None else int(stride)
-            if rows and buf.nbytes < ((rows - 1) * stride + width) * size:
-                raise ValueError("a row buffer is smaller than its rows")
-            out += [buf.ptr, stride]
-        return out
+    def _rows(self, buf, rows: int, width: int, size: int, stride) -> int:
+        stride = width if stride is None else int(stride)
+        if rows and buf.nbytes < ((rows - 1) * stride + width) * size:
+            raise ValueError("a row buffer is smaller than its rows")
+        return stride
 
     def apply(self, where, dtype: str, q=None, heads: int = 0, k=None, kv_heads: int = 0,
               q_out=None, k_out=None, q_stride: int | None = None, k_stride: int | None = None,
@@ -125,16 +122,24 @@ class Rotary:
             if positions.nbytes < 4 * rows:
                 raise ValueError("positions are fewer than rows")
             batch, positions = None, positions.ptr
-        heads, kv_heads = int(heads) if q is not None else 0, int(kv_heads) if k is not None else 0
-        args = []
-        for x, n, xs, y, ys in ((q, heads, q_stride, q_out, q_out_stride),
-                                (k, kv_heads, k_stride, k_out, k_out_stride)):
-            if n == 0:
-                args += [None, 0, 0, None, 0]
-                continue
-            if y is None:
-                y, ys = x, xs
-            xp, xs, yp, ys = self._rows(rows, n, size, (x, xs), (y, ys))
-            args += [xp, xs, n, yp, ys]
+        qp = qop = kp = kop = None
+        qs = qos = ks = kos = 0
+        if q is None:
+            heads = 0
+        else:
+            qs = self._rows(q, rows, heads * self.head_dim, size, q_stride)
+            qop, qos = q.ptr, qs
+            if q_out is not None:
+                qop, qos = q_out.ptr, self._rows(q_out, rows, heads * self.head_dim, size, q_out_stride)
+            qp = q.ptr
+        if k is None:
+            kv_heads = 0
+        else:
+            ks = self._rows(k, rows, kv_heads * self.head_dim, size, k_stride)
+            kop, kos = k.ptr, ks
+            if k_out is not None:
+                kop, kos = k_out.ptr, self._rows(k_out, rows, kv_heads * self.head_dim, size, k_out_stride)
+            kp = k.ptr
         _lib.call("eoship_rotary_device", self.rt.handle, self.handle, batch, positions, rows,
-                  int(bool(inverse)), DTYPES[dtype], *args)
+                  1 if inverse else 0, DTYPES[dtype], qp, qs, heads, qop, qos, kp, ks, kv_heads, kop,
+                  kos)

@@ -1005,7 +1005,8 @@ int eoship_kv_status(EosHipRuntime* rt, EosHipKVCache* kv, int32_t* status, char
 /* Bytes of the codes and of the scales of rows of k values. */
 int eoship_mx_bytes(int64_t rows, int32_t k, int64_t* code_bytes, int64_t* scale_bytes,
                     char** err);
-/* Rows x [rows][k] into codes and scales. Enqueued (no wait). */
+/* Rows x [rows][k] into codes and scales, which do not overlap x. Enqueued (no
+ * wait). */
 int eoship_mx_quantize_device(EosHipRuntime* rt, const void* d_x, int64_t x_stride, int32_t dtype,
                               int64_t rows, int32_t k, uint8_t* d_codes, uint8_t* d_scales,
                               char** err);
@@ -1025,9 +1026,9 @@ int eoship_mx_bind(EosHipRuntime* rt, const uint8_t* d_codes, const uint8_t* d_s
 int eoship_mx_release(EosHipRuntime* rt, EosHipMX* mx, char** err);
 /* out [rows][n] = Q(x) W^T + bias: x's rows are quantised within the call
  * (types 0..2), or are codes (3: d_x_scales are their scales, x_stride is not
- * looked at). Products are exact, sums f32, rounded once to out's type. A row
- * with a block that stands for NaN gives NaN; what lies between out's rows
- * stays; out and x do not overlap. Uses the runtime's workspace. Enqueued. */
+ * looked at). Products are exact, sums f32 (those below 2^-126 may count as
+ * zero), rounded once to out's type. A row with a block that stands for NaN gives
+ * NaN; what lies between out's rows stays; out and x do not overlap. Uses the runtime's workspace. Enqueued. */
 int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, int64_t x_stride,
                             int32_t dtype, const uint8_t* d_x_scales, int64_t rows, void* d_out,
                             int64_t out_stride, int32_t out_dtype, char** err);
@@ -1094,7 +1095,7 @@ typedef struct EosHipKVPager EosHipKVPager;
  * and, unless every sequence has one row, d_offsets; batch and rows are the
  * number of slots with new tokens and their sum. Device memory; what lies
  * behind the batch and its rows, and table entries behind a sequence's pages,
- * stay. */
+ * stay. The arrays overlap neither each other nor the pager's. */
 typedef struct {
   int32_t* d_slots;       /* [slots] slot of each sequence */
   int32_t* d_page_table;  /* [slots][table_stride] or NULL */
