@@ -100,12 +100,12 @@ int eoship_kv_pager_bind(EosHipRuntime* rt, const EosHipKVPagerDesc* desc, EosHi
     p->rt = rt;
     p->d = *desc;
     while ((1 << p->page_shift) < desc->page_tokens) ++p->page_shift;
-    if (rt->alloc(16, &p->mem, err) != 0) {
+    if (rt->alloc(kPagerState * 4, &p->mem, err) != 0) {
       delete p;
       return 1;
     }
-    const int32_t zero[4] = {};
-    const hipError_t e = rt->copy_sync(p->mem, zero, 16, hipMemcpyHostToDevice);
+    const int32_t zero[kPagerState] = {};
+    const hipError_t e = rt->copy_sync(p->mem, zero, sizeof(zero), hipMemcpyHostToDevice);
     if (e != hipSuccess) {
       delete p;
       return hip_err(err, "hipMemcpy(pager state)", e);

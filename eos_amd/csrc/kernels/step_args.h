@@ -34,7 +34,9 @@ constexpr int kPagerShort = 4;      // rows of a request that one thread writes
 constexpr int kPagerUnit = 256;    // rows that a wavefront takes at a time
 constexpr int kPagerEntries = 256;  // table entries that it does
 
-// state[0] status bits, state[1] workgroups that are done
+constexpr int kPagerLine = 32;      // words of a cache line
+constexpr int kPagerState = 10 * kPagerLine;  // status; workgroups done, of eight groups
+
 struct PagerArgs {
   int32_t* table;     // [slots][stride]
   int32_t* lengths;   // [slots]
