@@ -290,8 +290,8 @@ int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, in
     const int t = count(64) <= 2 * cus ? 64 : 4 * turns(count(256), 1) > 3 * turns(count(128), 2) ? 128 : 256;
     a.tiles_m = (int)((rows + t - 1) / t);
     a.tiles_n = ceil_div(mx->n, t);
-    return launch(rt, "eos_mx_product_" + std::to_string(t), (long long)a.tiles_m * a.tiles_n, &a,
-                  what, err);
+    return launch(rt, "eos_mx_product_" + std::to_string(t) + "_" + kTypes[out_dtype],
+                  (long long)a.tiles_m * a.tiles_n, &a, what, err);
   });
 }
 

@@ -131,7 +131,8 @@ EOS_DEV uint32_t quarter(const Eight<T>& e, uint32_t& byte) {
 // ------------------------------------------------------------ quantised rows
 
 // Four lanes a block, eight values a lane: every load and store of a wavefront
-// is of consecutive bytes.
+// is of consecutive bytes. Bound by them: 16,384 rows of 4,096 bf16 in 35 us and
+// back in 31, 170 MB each (4.9 and 5.5 TB/s; a copy reaches 4.7 to 5.2).
 template <int T>
 EOS_DEV void quantize(const MxQuantArgs& a) {
   const long long first = (long long)blockIdx.x * 64;  // blocks of all rows in order
@@ -151,6 +152,7 @@ EOS_DEV void quantize(const MxQuantArgs& a) {
 }
 
 // The same into laid-out tiles: a workgroup a tile and quad, a wavefront a step.
+// 8,192 rows of 8,192 bf16: 38 us, 4.5 TB/s; of a small call 2, its latency.
 template <int T>
 EOS_DEV void lay(const MxQuantArgs& a) {
   const MxLaid& o = a.laid;
@@ -309,55 +311,50 @@ EOS_DEV void place(const MxLinearArgs& a, int& bm, int& bn) {
   bm = (int)(group * 8 + in - bn * high);
 }
 
-// A wavefront's MF x NF tiles of outputs from row m0 and output n0 on: through
-// its part of LDS 32 rows at a time, so that a store writes whole lines. (One
-// wavefront a SIMD issues an instruction every four cycles or five: what counts
-// is how many these are.)
+// A wavefront's NF tiles of outputs of 32 rows from row m0 and output n0 on: through
+// its part of LDS, so that a store writes whole lines. (One wavefront a SIMD
+// issues an instruction every four cycles or five: what counts is how many these
+// are.)
 template <int T, int MF, int NF>
-EOS_DEV void put(const MxLinearArgs& a, const v16f (&acc)[NF][MF], void* mine, long long m0, int n0) {
+EOS_DEV void put(const MxLinearArgs& a, const v16f (&acc)[NF][MF], int j, uint8_t* mine, long long m0,
+                 int n0) {
   constexpr int kSize = size_of(T), kEach = 16 / kSize;       // outputs of a store
   constexpr int kRow = NF * 32 * kSize + 16;                  // bytes of a row in LDS
   constexpr int kLanes = NF * 32 / kEach, kRows = 64 / kLanes;  // lanes of a row, rows of a store
   const int lane = threadIdx.x & 63;
-  uint8_t* to = static_cast<uint8_t*>(mine) + lane % 32 * kRow + lane / 32 * 4 * kSize;
-  const uint8_t* from = static_cast<uint8_t*>(mine) + lane / kLanes * kRow + lane % kLanes * 16;
+  uint8_t* to = mine + lane % 32 * kRow + lane / 32 * 4 * kSize;
+#pragma unroll
+  for (int i = 0; i < NF; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const v4f y = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      store4(to + (i * 32 + 8 * g) * kSize, T, y, 4);
+    }
+  __builtin_amdgcn_wave_barrier();
+  const uint8_t* from = mine + lane / kLanes * kRow + lane % kLanes * 16;
   const int n = n0 + lane % kLanes * kEach;
-  uint8_t* out = a.out + (m0 + lane / kLanes) * a.out_stride + (long long)n * kSize;
-#pragma unroll
-  for (int j = 0; j < MF; ++j) {
-#pragma unroll
-    for (int i = 0; i < NF; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const v4f y = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        store4(to + (i * 32 + 8 * g) * kSize, T, y, 4);
-      }
-    __builtin_amdgcn_wave_barrier();
-    if (m0 + j * 32 + 32 <= a.rows && n0 + NF * 32 <= a.n) {
-      uint8_t* p = out + j * 32 * a.out_stride;
+  uint8_t* p = a.out + (m0 + lane / kLanes) * a.out_stride + (long long)n * kSize;
+  if (m0 + 32 <= a.rows && n0 + NF * 32 <= a.n) {
 #pragma unroll 4
-      for (int r = 0; r < 32 / kRows; ++r, p += kRows * a.out_stride)
-        *reinterpret_cast<v4u*>(p) = *reinterpret_cast<const v4u*>(from + r * kRows * kRow);
-    } else if (n < a.n) {
+    for (int r = 0; r < 32; r += kRows, p += kRows * a.out_stride)
+      *reinterpret_cast<v4u*>(p) = *reinterpret_cast<const v4u*>(from + r * kRow);
+  } else if (n < a.n) {
 #pragma unroll 1
-      for (int r = 0; r < 32; r += kRows) {
-        if (m0 + j * 32 + lane / kLanes + r >= a.rows) break;
-        uint8_t* p = out + (j * 32 + r) * a.out_stride;
-        if (n + kEach <= a.n) {
-          *reinterpret_cast<v4u*>(p) = *reinterpret_cast<const v4u*>(from + r * kRow);
-          continue;
-        }
+    for (int r = 0; r < 32 && m0 + lane / kLanes + r < a.rows; r += kRows, p += kRows * a.out_stride) {
+      if (n + kEach <= a.n) {
+        *reinterpret_cast<v4u*>(p) = *reinterpret_cast<const v4u*>(from + r * kRow);
+        continue;
+      }
 #pragma unroll 1
-        for (int i = 0; n + i < a.n; ++i) {
-          if constexpr (T == kMxF32)
-            reinterpret_cast<uint32_t*>(p)[i] = reinterpret_cast<const uint32_t*>(from + r * kRow)[i];
-          else
-            reinterpret_cast<uint16_t*>(p)[i] = reinterpret_cast<const uint16_t*>(from + r * kRow)[i];
-        }
+      for (int i = 0; n + i < a.n; ++i) {
+        if constexpr (T == kMxF32)
+          reinterpret_cast<uint32_t*>(p)[i] = reinterpret_cast<const uint32_t*>(from + r * kRow)[i];
+        else
+          reinterpret_cast<uint16_t*>(p)[i] = reinterpret_cast<const uint16_t*>(from + r * kRow)[i];
       }
     }
-    __builtin_amdgcn_wave_barrier();
   }
+  __builtin_amdgcn_wave_barrier();
 }
 
 typedef __amdgpu_buffer_rsrc_t Buffer;
@@ -381,6 +378,13 @@ EOS_DEV uint32_t load4(Buffer b, int lane_offset, int offset) {
 // the store of a register for the next quad and its load for the one after,
 // which so has a quad's time to arrive. The barrier stands where all of a
 // quad's reads have been issued and its stores are long done.
+//
+// Tiles of 32 x 32 x 64: on values as they come these reach 6.5 PFLOP/s of the
+// card, 16 x 16 x 128 5.6 (on zeros 9.5 and 6.9: it is the power that they draw).
+// MF = NF = 4: a wavefront's 128 x 128 outputs read 16 KB of LDS for 128 values of
+// K, half of what 64 x 64 read for as many products. 8,192^3: 263 us, 4.2 PFLOP/s
+// (3.4 in the compiler's order); on zeros 202, so 1.8 us a quad against 1.3 is
+// power, and 7 us of each of four turns are the first loads and the stores.
 template <int MF, int NF>
 struct Product {
   static constexpr int TM = 2 * MF, TN = 2 * NF, TILES = TM + TN, SLOTS = MF + NF;
@@ -424,7 +428,7 @@ struct Product {
   }
 };
 
-template <int MF, int NF>
+template <int T, int MF, int NF>
 EOS_DEV void product(const MxLinearArgs& a) {
   typedef Product<MF, NF> P;
   constexpr int TM = P::TM, TN = P::TN, TILES = P::TILES;
@@ -486,10 +490,9 @@ EOS_DEV void product(const MxLinearArgs& a) {
   lds_barrier();
   const long long m0 = (long long)(bm * TM + wm) * kMxTile;
   const int n0 = (bn * TN + wn) * kMxTile;
-  void* mine = lds[0] + wave * (sizeof(lds) / 64);
-  if (a.out_type == kMxF32) put<kMxF32, MF, NF>(a, p.acc, mine, m0, n0);
-  else if (a.out_type == kMxF16) put<kMxF16, MF, NF>(a, p.acc, mine, m0, n0);
-  else put<kMxBf16, MF, NF>(a, p.acc, mine, m0, n0);
+  uint8_t* mine = reinterpret_cast<uint8_t*>(lds) + wave * (sizeof(lds) / 4);
+#pragma unroll
+  for (int j = 0; j < MF; ++j) put<T, MF, NF>(a, p.acc, j, mine, m0 + j * 32, n0);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -585,7 +588,9 @@ EOS_DEV void quantize_rows(const MxLinearArgs& a, Rows16<U>& to, int first) {
 // Up to 16 MT rows of x (16, where they are not laid out) by 16 NT rows of w a
 // workgroup: its eight wavefronts take 128 values of K in turn, U at a time, so
 // that the weights, read once, arrive in long runs; their sums meet in LDS, in
-// the wavefronts' order.
+// the wavefronts' order. Bound by the weights: 16,384 x 16,384 by one row in 26
+// us, 5.5 TB/s; 48 rows by 4,096 x 16,384 8.4, 4.5 TB/s; one by 4,096 x 6,144 4.4,
+// a chain of launch, loads, sums.
 template <int X, bool FOUR, int MT, int NT, int U>
 EOS_DEV void few(const MxLinearArgs& a) {
   constexpr bool kRows = X < kMxCodes;
@@ -680,13 +685,17 @@ MX_KERNELS(bf16, kMxBf16)
 MX_KERNELS(f32, kMxF32)
 extern "C" __global__ __launch_bounds__(256) void eos_mx_lay_codes(MxQuantArgs a) { lay<kMxCodes>(a); }
 
-#define MX_PRODUCT(SIZE, MF, NF, WAVES)                                                        \
-  extern "C" __global__ __launch_bounds__(256, WAVES) void eos_mx_product_##SIZE(MxLinearArgs a) { \
-    product<MF, NF>(a);                                                                         \
+#define MX_PRODUCT(NAME, T, MF, NF, WAVES)                                                         \
+  extern "C" __global__ __launch_bounds__(256, WAVES) void eos_mx_product_##NAME(MxLinearArgs a) { \
+    product<T, MF, NF>(a);                                                                         \
   }
-MX_PRODUCT(64, 1, 1, 2)
-MX_PRODUCT(128, 2, 2, 2)
-MX_PRODUCT(256, 4, 4, 1)
+#define MX_PRODUCTS(TYPE, T)          \
+  MX_PRODUCT(64_##TYPE, T, 1, 1, 2)   \
+  MX_PRODUCT(128_##TYPE, T, 2, 2, 2)  \
+  MX_PRODUCT(256_##TYPE, T, 4, 4, 1)
+MX_PRODUCTS(f16, kMxF16)
+MX_PRODUCTS(bf16, kMxBf16)
+MX_PRODUCTS(f32, kMxF32)
 
 #define MX_FEW(NAME, X, FOUR, MT, NT, U)                                                       \
   extern "C" __global__ __launch_bounds__(512) void eos_mx_few_##NAME##_##NT(MxLinearArgs a) { \

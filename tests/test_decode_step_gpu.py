@@ -121,7 +121,7 @@ def test_every_kernel_is_reached(rt):
     """Each variant by a call that takes it."""
     types = ("f16", "bf16", "f32")
     names = [f"eos_mx_{op}_{t}" for op in ("quantize", "dequantize", "lay") for t in types]
-    names += ["eos_mx_lay_codes"] + [f"eos_mx_product_{t}" for t in (64, 128, 256)]
+    names += ["eos_mx_lay_codes"] + [f"eos_mx_product_{n}_{t}" for n in (64, 128, 256) for t in types]
     names += [f"eos_mx_few_{t}_4_{n}" for t in types for n in (1, 2)]
     names += [f"eos_mx_few_{t}_16_{n}" for t in types for n in (1, 2, 4)]
     names += [f"eos_mx_few_codes_16_{n}" for n in (1, 2)]
@@ -151,9 +151,10 @@ def test_every_kernel_is_reached(rt):
                 w.apply(big, rows, "mxfp4", big.view(48 << 20, 48 << 20), "f16",
                         out_stride=32 * cus + 8, x_scales=big)
         small = layer(64, 32)
-        small.apply(big, 65, "f16", big.view(48 << 20, 48 << 20), "f16")
-        small.apply(big, 64 * 2 * cus + 1, "f16", big.view(48 << 20, 48 << 20), "f16")
-        widths[1].apply(big, 4096, "f16", big.view(16 << 20, 80 << 20), "f16")
+        for t in types:
+            small.apply(big, 65, "f16", big.view(48 << 20, 48 << 20), t)
+            small.apply(big, 64 * 2 * cus + 1, "f16", big.view(48 << 20, 48 << 20), t)
+            widths[1].apply(big, 4096, "f16", big.view(16 << 20, 80 << 20), t)
 
     rt.profile(True)
     rt.profile_reset()
