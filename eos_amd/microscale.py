@@ -36,7 +36,7 @@ def _stride(buf, rows: int, width: int, dtype: str, stride, name: str) -> int:
 
 
 def _held(codes, scales, rows: int, k: int) -> None:
-    blocks = int(rows) * -(-int(k) // 32)
+    blocks = rows * -(-k // 32)
     if codes.nbytes < 16 * blocks or scales.nbytes < blocks:
         raise ValueError("codes or scales are smaller than their rows")
 
@@ -45,6 +45,7 @@ def quantize(rt: Runtime, x, rows: int, k: int, dtype: str, codes, scales,
              x_stride: int | None = None) -> None:
     """Rows x [rows, k] into codes u8 [rows, ceil(k / 32), 16] and scales u8
     [rows, ceil(k / 32)]."""
+    rows, k = int(rows), int(k)
     stride = _stride(x, rows, k, dtype, x_stride, "x")
     _held(codes, scales, rows, k)
     _lib.call("eoship_mx_quantize_device", rt.handle, x.ptr, stride, DTYPES[dtype], rows, k,
@@ -54,6 +55,7 @@ def quantize(rt: Runtime, x, rows: int, k: int, dtype: str, codes, scales,
 def dequantize(rt: Runtime, codes, scales, rows: int, k: int, out, dtype: str,
                out_stride: int | None = None) -> None:
     """The values that codes and scales stand for into rows out [rows, k]."""
+    rows, k = int(rows), int(k)
     stride = _stride(out, rows, k, dtype, out_stride, "out")
     _held(codes, scales, rows, k)
     _lib.call("eoship_mx_dequantize_device", rt.handle, codes.ptr, scales.ptr, rows, k, out.ptr,
@@ -68,7 +70,7 @@ class MXLinear:
     def __init__(self, rt: Runtime, codes, scales, n: int, k: int, bias=None):
         self.rt, self.n, self.k = rt, int(n), int(k)
         self.handle = C.c_void_p()
-        _held(codes, scales, n, k)
+        _held(codes, scales, self.n, self.k)
         if bias is not None and bias.nbytes < 4 * self.n:
             raise ValueError("bias is smaller than [n]")
         _lib.call("eoship_mx_bind", rt.handle, codes.ptr, scales.ptr, self.n, self.k,
@@ -101,6 +103,7 @@ class MXLinear:
         """out [rows, n] = Q(x) W^T + bias for rows x [rows, k] of ``dtype``
         (quantised within the call), or for codes x with ``x_scales``
         (``dtype`` "mxfp4"). ``out_dtype`` None: x's."""
+        rows = int(rows)
         if dtype == "mxfp4":
             if x_scales is None:
                 raise ValueError("x_scales is needed with codes")

@@ -114,11 +114,11 @@ class Rotary:
         ``k_out`` in place. ``inverse``: back again, the gradient's direction."""
         if dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}, got {dtype!r}")
-        size = 4 if dtype == "f32" else 2
+        size, heads, kv_heads = 4 if dtype == "f32" else 2, int(heads), int(kv_heads)
         if isinstance(where, KVBatch):
             batch, positions, rows = C.byref(where.c), None, where.rows
         else:
-            positions, rows = where
+            positions, rows = where[0], int(where[1])
             if positions.nbytes < 4 * rows:
                 raise ValueError("positions are fewer than rows")
             batch, positions = None, positions.ptr

@@ -117,6 +117,49 @@ def test_steps_from_lengths_to_outputs(rt, layout, rotary_dim):
     step([1, 1, 1, 0, 1, 1, 1, 1, 1], True)
 
 
+@pytest.mark.parametrize("one_each", [True, False])
+def test_a_refused_request_is_padding(rt, one_each):
+    """Requests that the pages do not cover: no row of theirs is turned, stored
+    or attended, and nothing of the others' changes."""
+    rng = np.random.default_rng(1)
+    pager = KVPager(rt, 4, 3, PAGE, 3)
+    cache = KVCache(rt, "bf16", KVH, D, PAGE, 3)
+    plan = pager.plan(64)
+    rotary = Rotary(rt, D, frequencies(D)[0])
+    i32 = lambda a: DeviceBuffer.from_array(rt, np.asarray(a, np.int32))  # noqa: E731
+    width = (HEADS + 2 * KVH) * D
+    pager.extend(i32([16, 15, 0, 0]), plan)  # a page each, one left
+    x = mx.to_bits(rng.normal(size=(31, width)), "bf16")
+    qkv = DeviceBuffer.from_array(rt, x)
+    part = lambda b, a: b.view(a * D * 2, b.nbytes - a * D * 2)  # noqa: E731
+    b = plan.batch(3, 2, 31)
+    cache.append(b, part(qkv, HEADS), part(qkv, HEADS + KVH), "bf16", width, width)
+    new = [1, 1, 1, 1] if one_each else [2, 1, 17, 3]
+    rows = sum(new)
+    pager.extend(i32(new), plan)             # the first takes it, the third and fourth wait
+    assert pager.status() == 1
+    assert plan.lengths.download(np.int32, (4,)).tolist() == [16 + new[0], 16, 0, 0]
+    x = mx.to_bits(rng.normal(size=(rows, width)), "bf16")
+    qkv = DeviceBuffer.from_array(rt, x)
+    b = plan.batch(3, 4, None if one_each else rows)
+    before = [p.download(np.uint16, (p.nbytes // 2,)) for p in (cache.k, cache.v)]
+    live = new[0] + new[1]
+    for where in (b, (plan.positions, rows)):
+        rotary.apply(where, "bf16", qkv, HEADS, part(qkv, HEADS), KVH, q_stride=width, k_stride=width)
+        got = qkv.download(np.uint16, x.shape)
+        np.testing.assert_array_equal(got[live:], x[live:])
+        assert (got[:live, :HEADS * D] != x[:live, :HEADS * D]).any(1).all()
+    cache.append(b, part(qkv, HEADS), part(qkv, HEADS + KVH), "bf16", width, width)
+    after = [p.download(np.uint16, (p.nbytes // 2,)) for p in (cache.k, cache.v)]
+    for p, q in zip(before, after):
+        assert (p != q).sum() <= live * KVH * D
+    out = DeviceBuffer.from_array(rt, np.full((rows, HEADS * D), 0x4141, np.uint16))
+    cache.attend(b, qkv, HEADS, out, "bf16", q_stride=width)
+    got = out.download(np.uint16, (rows, HEADS * D))
+    assert (got[live:] == 0).all() and (got[:live] != 0).any(1).all()
+    assert cache.status() == 0
+
+
 def test_every_kernel_is_reached(rt):
     """Each variant by a call that takes it."""
     types = ("f16", "bf16", "f32")

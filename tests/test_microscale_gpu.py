@@ -245,6 +245,70 @@ def test_linear_scales_at_their_ends(rt, rows):
     assert (got[0] == 0).all()
 
 
+def _filled(rt, nbytes, byte):
+    from eos_amd import _lib
+    buf = DeviceBuffer(rt, nbytes)
+    _lib.call("eoship_memset", rt.handle, buf.ptr, byte, nbytes)
+    return buf
+
+
+@pytest.mark.parametrize("rows", [1, 20, 65])
+def test_weights_beyond_four_gigabytes(rt, rows):
+    """131,077 weights rows of 65,536 ones, some rows others; sums of whole numbers."""
+    _case(f"large weights {rows}")
+    n, k = 131077, 65536
+    codes, scales = _filled(rt, n * k // 2, 0x22), _filled(rt, n * k // 32, 127)  # 1.0, 1.0
+    want = np.full(n, float(k))
+    for i, (byte, value) in {0: (0x44, 2.0), 77777: (0xAA, -1.0), 131071: (0x11, 0.5),
+                             131072: (0x22, 1.0), n - 1: (0x66, 4.0)}.items():
+        codes.view(i * k // 2, k // 2).upload(np.full(k // 2, byte, np.uint8))
+        want[i] = value * k
+    layer = MXLinear(rt, codes, scales, n, k)
+    codes.free()
+    scales.free()
+    x = np.ones((rows, k), np.float16)
+    x[rows // 2] = -1.5
+    out = DeviceBuffer(rt, rows * (n + 3) * 4)
+    layer.apply(DeviceBuffer.from_array(rt, x), rows, "f16", out, "f32", out_stride=n + 3)
+    got = out.download(np.float32, (rows, n + 3))[:, :n]
+    for r in range(rows):
+        np.testing.assert_array_equal(got[r], want * float(x[r, 0]))
+    layer.release()
+
+
+def test_rows_beyond_four_gigabytes(rt):
+    """2^21 + 35 rows of 4,096 codes; their last rows differ."""
+    _case("large rows")
+    rows, k, n = (1 << 21) + 35, 4096, 8
+    x, xs = _filled(rt, rows * k // 2, 0x22), _filled(rt, rows * k // 32, 127)
+    want = np.full(rows, float(k))
+    for i, (byte, value) in {5: (0x44, 2.0), 1 << 20: (0xAA, -1.0), rows - 35: (0x11, 0.5),
+                             rows - 1: (0x66, 4.0)}.items():
+        x.view(i * k // 2, k // 2).upload(np.full(k // 2, byte, np.uint8))
+        want[i] = value * k
+    w = np.ones((n, k))
+    w[3] = 0.0
+    c, s = ref.quantize(w)
+    layer = MXLinear(rt, DeviceBuffer.from_array(rt, c), DeviceBuffer.from_array(rt, s), n, k)
+    out = DeviceBuffer(rt, rows * n * 4)
+    layer.apply(x, rows, "mxfp4", out, "f32", x_scales=xs)
+    got = out.download(np.float32, (rows, n))
+    for j in range(n):
+        np.testing.assert_array_equal(got[:, j], want * (j != 3))
+    back = DeviceBuffer(rt, rows * k * 2)  # 17 GB: offsets of rows beyond 32 bits
+    microscale.dequantize(rt, x, xs, rows, k, back, "bf16")
+    again, ags = _filled(rt, rows * k // 2, 0), _filled(rt, rows * k // 32, 0)
+    microscale.quantize(rt, back, rows, k, "bf16", again, ags)
+    for i in (0, 5, 1 << 20, rows - 35, rows - 2, rows - 1):
+        got = back.view(i * k * 2, k * 2).download(np.uint16, (k,))
+        np.testing.assert_array_equal(ref.from_bits(got, "bf16"), want[i] / k)
+        c = again.view(i * k // 2, k // 2).download(np.uint8, (1, k // 2))
+        s = ags.view(i * k // 32, k // 32).download(np.uint8, (1, k // 32))
+        np.testing.assert_array_equal(ref.values(c, s, k)[0], want[i] / k)
+    for b in (x, xs, out, back, again, ags):
+        b.free()
+
+
 def test_linear_of_no_rows_and_after_the_weights_are_gone(rt):
     rng = np.random.default_rng(4)
     w = rng.normal(size=(33, 70)).astype(np.float32)
