@@ -43,9 +43,9 @@ constexpr int kFewRows = 16;
 constexpr int kSomeRows = 64;
 // More go by tiles of outputs. Tiles of 64 while there are no more than two a CU
 // (512 by 4,096: 17.0, by tiles of 128 18.9; 1,024 by 4,096: 26.0 and 22.0); then
-// of 128, two workgroups a CU, or of 256, one, whose turn takes 4/3 the time of the
+// of 128, two workgroups a CU, or of 256, one, whose turn takes 3/2 the time of the
 // two's (2,048 by 4,096, a turn each: 32.4 and 39.7; by 16,384, four turns and two:
-// 101 and 89).
+// 101 and 82).
 
 const char* const kTypes[] = {"f16", "bf16", "f32", "codes"};
 
@@ -287,7 +287,7 @@ int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, in
     const auto turns = [&](long long tiles, int at_once) {
       return (tiles + (long long)at_once * cus - 1) / ((long long)at_once * cus);
     };
-    const int t = count(64) <= 2 * cus ? 64 : 4 * turns(count(256), 1) > 3 * turns(count(128), 2) ? 128 : 256;
+    const int t = count(64) <= 2 * cus ? 64 : 3 * turns(count(256), 1) > 2 * turns(count(128), 2) ? 128 : 256;
     a.tiles_m = (int)((rows + t - 1) / t);
     a.tiles_n = ceil_div(mx->n, t);
     return launch(rt, "eos_mx_product_" + std::to_string(t) + "_" + kTypes[out_dtype],

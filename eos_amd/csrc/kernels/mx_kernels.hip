@@ -370,26 +370,50 @@ EOS_DEV uint32_t load4(Buffer b, int lane_offset, int offset) {
   return __builtin_amdgcn_raw_buffer_load_b32(b, lane_offset, offset, 0);
 }
 
+// 16 bytes a lane from memory straight into LDS: lane i's at lds + 16 i. loads_wait
+// and a barrier stand before their first use. Written out because the compiler,
+// which cannot tell the two buffers apart, would wait for the builtin's before
+// every read of the other.
+EOS_DEV void load_lds16(v4u memory, int lane_offset, int offset, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(lds), "v"(lane_offset), "s"(memory), "s"(offset)
+      : "memory", "m0");
+}
+EOS_DEV void loads_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+EOS_DEV v4u descriptor(const uint8_t* p) {
+  const uint64_t u = (uint64_t)(uintptr_t)p;
+  return v4u{(uint32_t)u, (uint32_t)(u >> 32), 0xffffffffu, 0x00027000u};
+}
+
 // 2 x 2 wavefronts, each MF x NF tiles of 32 x 32 outputs. Quads of K go from
-// memory through registers into one of two LDS buffers while the other is
-// multiplied. The order of the instructions is the one written: between any two
-// matrix instructions of a step stand a read of an operand of the next step
-// (the quad's last step: of the next quad's first), in the first two steps also
-// the store of a register for the next quad and its load for the one after,
-// which so has a quad's time to arrive. The barrier stands where all of a
-// quad's reads have been issued and its stores are long done.
+// memory into one of two LDS buffers while the other is multiplied. The order of
+// the instructions is the one written: between any two matrix instructions of a
+// step stand a read of an operand of the next step (the quad's last step: of the
+// next quad's first) and a load.
+// DIRECT: loads straight into LDS, in the quad's first step and the one before it,
+// for which the barrier of the quad before has made room; they have two steps to
+// arrive. Otherwise through registers, which are stored in the first two steps and
+// at once loaded again, a quad ahead; a load that comes back so takes 29 clocks of
+// the matrix unit's. The 256 tile's steps are long enough for the former (8,192^3
+// 263 -> 230 us), those of 64 and 128 not (512 by 4,096 x 4,096 from HBM 13.7 us
+// direct, 12.3 through registers; 1,024 17.1 and 15.1).
 //
 // Tiles of 32 x 32 x 64: on values as they come these reach 6.5 PFLOP/s of the
 // card, 16 x 16 x 128 5.6 (on zeros 9.5 and 6.9: it is the power that they draw).
 // MF = NF = 4: a wavefront's 128 x 128 outputs read 16 KB of LDS for 128 values of
-// K, half of what 64 x 64 read for as many products. 8,192^3: 263 us, 4.2 PFLOP/s
-// (3.4 in the compiler's order). A quad is 2,770 clocks, 2,048 of them matrix
-// instructions, 470 where loads come back; the clock is 2.4 GHz for one workgroup,
-// 1.5 when all multiply (2.2 on zeros): power. 7 us of each of four turns are the
-// first loads and the stores.
+// K, half of what 64 x 64 read for as many products. 8,192^3: 230 us, 4.8 PFLOP/s
+// (298 in the compiler's order). A quad is 2,480 clocks, 2,048 of them matrix
+// instructions; the clock is 2.4 GHz for one workgroup, 1.45 when all multiply (2.2
+// on zeros): power. 7 us of each of four turns are the first loads and the stores.
 template <int MF, int NF>
 struct Product {
   static constexpr int TM = 2 * MF, TN = 2 * NF, TILES = TM + TN, SLOTS = MF + NF;
+  static constexpr bool DIRECT = MF * NF >= 16;
+  v4u lds_x, lds_w;  // descriptors of the codes
   Buffer codes_x, codes_w, scales_x, scales_w;
   int at[TILES], scale_at[SLOTS];  // offsets of tiles (x, then w), of the wavefront's scales
   v4u stage[TILES];
@@ -397,8 +421,20 @@ struct Product {
   uint32_t sc[SLOTS], next[SLOTS];  // scales of x, then w
   v16f acc[NF][MF];
 
+  // Direct scales that have arrived: their registers are taken here, where all
+  // loads are waited for, or the compiler would wait at their use, for later loads
+  // too.
+  EOS_DEV void scales_here() {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) asm volatile("" : "+v"(next[i]));
+  }
+  // The thread's 16 bytes of tile i of quad q to a register, or to the buffer whose
+  // part for the wavefront begins at `lds`.
   EOS_DEV void fetch(int i, int q) {
     stage[i] = load16(i < TM ? codes_x : codes_w, threadIdx.x * 16, at[i] + q * kMxTileBytes);
+  }
+  EOS_DEV void fetch_lds(int i, int q, uint32_t lds) {
+    load_lds16(i < TM ? lds_x : lds_w, threadIdx.x * 16, at[i] + q * kMxTileBytes, lds + i * kMxTileBytes);
   }
   EOS_DEV void fetch_scales(int i, int q) {
     next[i] = load4(i < MF ? scales_x : scales_w, (threadIdx.x & 63) * 4,
@@ -410,14 +446,18 @@ struct Product {
     else if (k <= MF) xv[to][k - 1] = x[(k - 1) * 256 + step * 64];
     else wv[to][k - MF] = w[(k - MF) * 256 + step * 64];
   }
-  // x, w: where the next step's operands are read, from its step `step`.
+  // x, w: where the next step's operands are read, from its step `step`; to: the
+  // buffer that is loaded or stored.
   template <int S>
-  EOS_DEV void step(const v4u* x, const v4u* w, int step, v4u* to, int q, int last) {
+  EOS_DEV void step(const v4u* x, const v4u* w, int step, v4u* to, uint32_t to_lds, int q, int last) {
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
       read((S + 1) & 1, k, x, w, step);
-      if constexpr (S < 2) {
-        to[(S * SLOTS + k) * 256] = stage[S * SLOTS + k];
+      if constexpr (DIRECT) {
+        if constexpr (S == 3) fetch_lds(k, min(q + 2, last), to_lds);
+        if constexpr (S == 0) fetch_lds(SLOTS + k, min(q + 1, last), to_lds);
+      } else if constexpr (S < 2) {
+        to[(S * SLOTS + k) * 256 + threadIdx.x] = stage[S * SLOTS + k];
         fetch(S * SLOTS + k, min(q + 2, last));
       }
       if constexpr (S == 0) fetch_scales(k, min(q + 1, last));
@@ -443,8 +483,12 @@ EOS_DEV void product(const MxLinearArgs& a) {
   const int last_m = (int)((a.rows - 1) / kMxTile) - bm * TM, last_n = (a.n - 1) / kMxTile - bn * TN;
   const int quads = a.w.quads, last = quads - 1;
   P p;
-  p.codes_x = buffer(a.x.codes + (long long)bm * TM * quads * kMxTileBytes);
-  p.codes_w = buffer(a.w.codes + (long long)bn * TN * quads * kMxTileBytes);
+  const uint8_t* codes_x = a.x.codes + (long long)bm * TM * quads * kMxTileBytes;
+  const uint8_t* codes_w = a.w.codes + (long long)bn * TN * quads * kMxTileBytes;
+  p.lds_x = descriptor(codes_x);
+  p.lds_w = descriptor(codes_w);
+  p.codes_x = buffer(codes_x);
+  p.codes_w = buffer(codes_w);
   p.scales_x = buffer(a.x.scales + (long long)bm * TM * quads * kMxScaleBytes);
   p.scales_w = buffer(a.w.scales + (long long)bn * TN * quads * kMxScaleBytes);
 #pragma unroll
@@ -464,31 +508,49 @@ EOS_DEV void product(const MxLinearArgs& a) {
 #pragma unroll
     for (int j = 0; j < MF; ++j) p.acc[i][j] = b;
   }
+  // (a wavefront's part of a tile: 1024 bytes)
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds[0] + wave * 1024;
+  constexpr uint32_t kBuffer = sizeof(lds[0]);
 #pragma unroll
   for (int i = 0; i < MF + NF; ++i) p.fetch_scales(i, 0);
+  if constexpr (P::DIRECT) {
 #pragma unroll
-  for (int i = 0; i < TILES; ++i) p.fetch(i, 0);
+    for (int i = 0; i < TILES; ++i) p.fetch_lds(i, 0, lds0);
+    loads_wait();
+    p.scales_here();
+#pragma unroll
+    for (int i = 0; i < TILES / 2; ++i) p.fetch_lds(i, min(1, last), lds0 + kBuffer);
+  } else {
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) p.fetch(i, 0);
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+      lds[0][i * 256 + threadIdx.x] = p.stage[i];
+      p.fetch(i, min(1, last));
+    }
+  }
 #pragma unroll
   for (int i = 0; i < MF + NF; ++i) p.sc[i] = p.next[i];
-#pragma unroll
-  for (int i = 0; i < TILES; ++i) {
-    lds[0][i * 256 + threadIdx.x] = p.stage[i];
-    p.fetch(i, min(1, last));
-  }
   lds_barrier();
   const int x0 = wm * 256 + lane, w0 = (TM + wn) * 256 + lane;
 #pragma unroll
   for (int k = 0; k < MF + NF; ++k) p.read(0, k, lds[0] + x0, lds[0] + w0, 0);
   for (int q = 0; q < quads; ++q) {
     v4u *now = lds[q & 1], *then = lds[(q + 1) & 1];
-    p.template step<0>(now + x0, now + w0, 1, then + threadIdx.x, q, last);
-    p.template step<1>(now + x0, now + w0, 2, then + threadIdx.x, q, last);
-    p.template step<2>(now + x0, now + w0, 3, nullptr, q, last);
+    const uint32_t lds_now = lds0 + (q & 1) * kBuffer, lds_then = lds0 + ((q + 1) & 1) * kBuffer;
+    p.template step<0>(now + x0, now + w0, 1, then, lds_then, q, last);
+    p.template step<1>(now + x0, now + w0, 2, then, 0, q, last);
+    p.template step<2>(now + x0, now + w0, 3, nullptr, 0, q, last);
+    if constexpr (P::DIRECT) {
+      loads_wait();
+      p.scales_here();
+    }
     lds_barrier();
-    p.template step<3>(then + x0, then + w0, 0, nullptr, q, last);
+    p.template step<3>(then + x0, then + w0, 0, nullptr, lds_now, q, last);
 #pragma unroll
     for (int i = 0; i < MF + NF; ++i) p.sc[i] = p.next[i];
   }
+  if constexpr (P::DIRECT) loads_wait();  // the outputs take the buffers' place
   lds_barrier();
   const long long m0 = (long long)(bm * TM + wm) * kMxTile;
   const int n0 = (bn * TN + wn) * kMxTile;
