@@ -12,6 +12,10 @@ e = floor(log2(largest magnitude)) - 2 in -127..127; an element is x / 2^e
 rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code)
 and their negatives, saturating; codes [rows][16 blocks] bytes, element 2 i in
 the low half of byte i; scales [rows][blocks] bytes.
+
+The package's calls are enqueued on its runtime's own stream, which torch's
+streams do not wait for: whoever reads the outputs of `run`, or drops a state
+whose memory torch may then hand out again, synchronises the device first.
 """
 import math
 
@@ -282,9 +286,9 @@ def _bind(s):
         _rt = Runtime(0)
     case, kind = s["case"], s["case"]["kind"]
     dev = s["dev"] = {n: _Dev(t) for n, t in s.items() if isinstance(t, torch.Tensor)}
+    torch.cuda.synchronize()  # the runtime's own stream does not wait for torch's
     if kind == "linear":
         from eos_amd.microscale import MXLinear
-        torch.cuda.synchronize()  # the layer is laid out on the runtime's own stream
         s["layer"] = MXLinear(_rt, dev["w"], dev["w_scales"], case["n"], case["k"],
                               bias=dev.get("bias"))
     elif kind == "rotary":
