@@ -8,10 +8,15 @@
 
 #include "eoship_internal.h"
 #include "kernels/mx_args.h"
+#include "row_ranges.h"
 
+using eoship::bytes_of;
 using eoship::guarded;
 using eoship::hip_err;
 using eoship::OnDevice;
+using eoship::Rows;
+using eoship::rows_meet;
+using eoship::rows_of;
 using eoship::set_err;
 
 struct EosHipMX {
@@ -257,6 +262,14 @@ int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, in
                           : check_rows(d_x, x_stride, mx->k, "x", what, err) != 0)
       return 1;
     if (check_rows(d_out, out_stride, mx->n, "out", what, err) != 0) return 1;
+    const int64_t blocks = rows * ceil_div(mx->k, kMxBlock), size = size_of(out_dtype);
+    const Rows out = rows_of(d_out, rows, out_stride * size, mx->n * size);
+    const Rows in = dtype == kMxCodes
+                        ? bytes_of(d_x, blocks * 16)
+                        : rows_of(d_x, rows, x_stride * size_of(dtype), (int64_t)mx->k * size_of(dtype));
+    if (rows_meet(out, in)) return set_err(err, "%s: out overlaps x", what);
+    if (dtype == kMxCodes && rows_meet(out, bytes_of(d_x_scales, blocks)))
+      return set_err(err, "%s: out overlaps x's scales", what);
     OnDevice on(rt->device);
     MxLinearArgs a{};
     a.w = mx->w;

@@ -1028,7 +1028,9 @@ int eoship_mx_release(EosHipRuntime* rt, EosHipMX* mx, char** err);
  * (types 0..2), or are codes (3: d_x_scales are their scales, x_stride is not
  * looked at). Products are exact, sums f32 (those below 2^-126 may count as
  * zero), rounded once to out's type. A row with a block that stands for NaN gives
- * NaN; what lies between out's rows stays; out and x do not overlap. Uses the runtime's workspace. Enqueued. */
+ * NaN; what lies between out's rows stays. Rows of out that share memory with
+ * those of x or its scales are refused (columns of one array do not). Uses the
+ * runtime's workspace. Enqueued. */
 int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, int64_t x_stride,
                             int32_t dtype, const uint8_t* d_x_scales, int64_t rows, void* d_out,
                             int64_t out_stride, int32_t out_dtype, char** err);
