@@ -157,6 +157,12 @@ int eoship_mx_quantize_device(EosHipRuntime* rt, const void* d_x, int64_t x_stri
     if (check_rows(d_x, x_stride, k, "x", what, err) != 0 ||
         check_codes(d_codes, d_scales, what, err) != 0)
       return 1;
+    const int64_t blocks = rows * ceil_div(k, kMxBlock);
+    const Rows x = rows_of(d_x, rows, x_stride * size_of(dtype), (int64_t)k * size_of(dtype));
+    const Rows codes = bytes_of(d_codes, blocks * 16), scales = bytes_of(d_scales, blocks);
+    if (rows_meet(x, codes) || rows_meet(x, scales))
+      return set_err(err, "%s: codes or scales overlap x", what);
+    if (rows_meet(codes, scales)) return set_err(err, "%s: scales overlap codes", what);
     OnDevice on(rt->device);
     if (rt->load(eoship::Runtime::kMx, err) != 0) return 1;
     MxQuantArgs a{};
@@ -183,6 +189,10 @@ int eoship_mx_dequantize_device(EosHipRuntime* rt, const uint8_t* d_codes, const
     if (check_codes(d_codes, d_scales, what, err) != 0 ||
         check_rows(d_out, out_stride, k, "out", what, err) != 0)
       return 1;
+    const int64_t blocks = rows * ceil_div(k, kMxBlock);
+    const Rows out = rows_of(d_out, rows, out_stride * size_of(dtype), (int64_t)k * size_of(dtype));
+    if (rows_meet(out, bytes_of(d_codes, blocks * 16)) || rows_meet(out, bytes_of(d_scales, blocks)))
+      return set_err(err, "%s: out overlaps codes or scales", what);
     OnDevice on(rt->device);
     if (rt->load(eoship::Runtime::kMx, err) != 0) return 1;
     MxDequantArgs a{};

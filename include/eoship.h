@@ -1005,13 +1005,14 @@ int eoship_kv_status(EosHipRuntime* rt, EosHipKVCache* kv, int32_t* status, char
 /* Bytes of the codes and of the scales of rows of k values. */
 int eoship_mx_bytes(int64_t rows, int32_t k, int64_t* code_bytes, int64_t* scale_bytes,
                     char** err);
-/* Rows x [rows][k] into codes and scales, which do not overlap x. Enqueued (no
- * wait). */
+/* Rows x [rows][k] into codes and scales. Those that share memory with x's rows
+ * or each other are refused. Enqueued (no wait). */
 int eoship_mx_quantize_device(EosHipRuntime* rt, const void* d_x, int64_t x_stride, int32_t dtype,
                               int64_t rows, int32_t k, uint8_t* d_codes, uint8_t* d_scales,
                               char** err);
 /* The values that codes and scales stand for, rounded once to out's type;
- * what lies between out's rows stays. Enqueued. */
+ * what lies between out's rows stays. Rows of out that share memory with codes
+ * or scales are refused. Enqueued. */
 int eoship_mx_dequantize_device(EosHipRuntime* rt, const uint8_t* d_codes, const uint8_t* d_scales,
                                 int64_t rows, int32_t k, void* d_out, int64_t out_stride,
                                 int32_t dtype, char** err);

@@ -50,6 +50,30 @@ def linear_overlap():
     assert rows > 64 and stub.stub_launches(b"eos_mx_product_64_bf16") == 4
 
 
+def rows_overlap():
+    """Codes, scales and values in each other's place."""
+    rt = Runtime(0)
+    buf = DeviceBuffer(rt, 1 << 16)
+    part = lambda at: buf.view(at, buf.nbytes - at)  # noqa: E731
+    rows, k = 20, 96  # x 192 bytes a row, codes 48, scales 3
+    x, c, s = rows * 192, rows * 48, rows * 3
+    q = lambda *a, **kw: microscale.quantize(rt, *a, **kw)  # noqa: E731
+    q(buf, rows, k, "bf16", part(x), part(x + c))
+    q(part(c + 64), rows, k, "bf16", buf, part(c))
+    refused("codes or scales overlap x", q, buf, rows, k, "bf16", part(x - 16), part(1 << 15))
+    refused("codes or scales overlap x", q, part(16), rows, k, "bf16", part(1 << 15), part(16 + x - 1))
+    refused("scales overlap codes", q, buf, rows, k, "bf16", part(1 << 15), part((1 << 15) + c - 1))
+    # behind a row's values
+    q(buf, 1, k, "bf16", part(256), part(192), x_stride=96)
+    d = lambda *a, **kw: microscale.dequantize(rt, *a, **kw)  # noqa: E731
+    d(buf, part(c), rows, k, part(c + 64), "bf16")
+    d(part(x), part(x + c), rows, k, buf, "bf16")
+    refused("out overlaps codes or scales", d, buf, part(1 << 15), rows, k, part(c - 16), "f32")
+    refused("out overlaps codes or scales", d, part(1 << 15), buf, rows, k, part(s - s % 16), "f16")
+    refused("out overlaps codes or scales", d, part(16), part(1 << 15), rows, k, buf, "f16", out_stride=104)
+    assert stub.stub_launches(b"eos_mx_quantize_bf16") == 3
+
+
 if __name__ == "__main__":
     globals()[sys.argv[2]]()
     print("OK")
