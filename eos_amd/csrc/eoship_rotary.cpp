@@ -10,10 +10,15 @@
 
 #include "eoship_internal.h"
 #include "kernels/step_args.h"
+#include "row_ranges.h"
 
+using eoship::bytes_of;
 using eoship::guarded;
 using eoship::hip_err;
 using eoship::OnDevice;
+using eoship::Rows;
+using eoship::rows_meet;
+using eoship::rows_of;
 using eoship::set_err;
 
 struct EosHipRotary {
@@ -147,8 +152,24 @@ int eoship_rotary_device(EosHipRuntime* rt, EosHipRotary* rot, const EosHipKVBat
     if ((heads > 0 && d_q == d_q_out && q_stride != q_out_stride) ||
         (kv_heads > 0 && d_k == d_k_out && k_stride != k_out_stride))
       return set_err(err, "%s: rows turned in place keep their stride", what);
-    OnDevice on(rt->device);
     const int size = dtype == kRotF32 ? 4 : 2;
+    const auto rows_at = [&](const void* p, int64_t stride, int n) {
+      return rows_of(p, n > 0 ? a.rows : 0, stride * size, n * d * size);
+    };
+    const Rows q = rows_at(d_q, q_stride, heads), q_out = rows_at(d_q_out, q_out_stride, heads);
+    const Rows k = rows_at(d_k, k_stride, kv_heads), k_out = rows_at(d_k_out, k_out_stride, kv_heads);
+    if (d_q != d_q_out && rows_meet(q_out, q)) return set_err(err, "%s: q_out overlaps q", what);
+    if (d_k != d_k_out && rows_meet(k_out, k)) return set_err(err, "%s: k_out overlaps k", what);
+    if (d_k != d_k_out && rows_meet(q_out, k)) return set_err(err, "%s: q_out overlaps k", what);
+    if (d_q != d_q_out && rows_meet(k_out, q)) return set_err(err, "%s: k_out overlaps q", what);
+    if (rows_meet(q_out, k_out)) return set_err(err, "%s: q_out overlaps k_out", what);
+    const Rows read[] = {bytes_of(d_positions, d_positions != nullptr ? 4 * a.rows : 0),
+                         bytes_of(a.lengths, a.lengths != nullptr ? 4LL * a.batch : 0),
+                         bytes_of(a.offsets, a.offsets != nullptr ? 4LL * a.batch + 4 : 0)};
+    for (const Rows& r : read)
+      if (rows_meet(q_out, r) || rows_meet(k_out, r))
+        return set_err(err, "%s: an output overlaps positions, lengths or offsets", what);
+    OnDevice on(rt->device);
     a.q = static_cast<const uint8_t*>(d_q);
     a.k = static_cast<const uint8_t*>(d_k);
     a.q_out = static_cast<uint8_t*>(d_q_out);

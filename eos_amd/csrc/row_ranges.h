@@ -33,6 +33,11 @@ inline __int128 first_within(__int128 a, __int128 m, __int128 l, __int128 r) {
 inline bool rows_meet(const Rows& a, const Rows& b) {
   if (a.count < 1 || b.count < 1 || a.width < 1 || b.width < 1) return false;
   if (a.end() <= (__int128)b.at || b.end() <= (__int128)a.at) return false;
+  if (a.stride == b.stride && a.count > 1 && b.count > 1) {
+    // columns of one array: all rows stand alike
+    const int64_t c = ((int64_t)(a.at - b.at) + a.width - 1) % a.stride;
+    return (c < 0 ? c + a.stride : c) <= a.width + b.width - 2;
+  }
   // a's rows from i0 to i1 reach into the bytes that b's first row to its last
   // span. There one shares a byte with a row of b if, counted from b's first, its
   // last byte stands less than both widths behind a multiple of b's stride.

@@ -1065,7 +1065,9 @@ int eoship_rotary_release(EosHipRuntime* rt, EosHipRotary* rot, char** err);
  * rows of no sequence are not written. Angles are taken from f64 products,
  * sums are f32, rounded once. inverse nonzero: by -p f, which is also the
  * gradient of the forward call. In place where an output is its input with the
- * same stride; otherwise they do not overlap. Enqueued (no wait). */
+ * same stride. Rows of an output that otherwise share memory with rows of q, k or
+ * the other output, or with positions, lengths or offsets, are refused (columns of
+ * one array do not). Enqueued (no wait). */
 int eoship_rotary_device(EosHipRuntime* rt, EosHipRotary* rot, const EosHipKVBatch* batch,
                          const int32_t* d_positions, int64_t rows, int32_t inverse, int32_t dtype,
                          const void* d_q, int64_t q_stride, int32_t heads, void* d_q_out,

@@ -10,9 +10,13 @@ stub.stub_launches.argtypes = [C.c_char_p]
 stub.stub_launches.restype = C.c_long
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
+import numpy as np  # noqa: E402
+
 from eos_amd import microscale  # noqa: E402
 from eos_amd._lib import EosHipError  # noqa: E402
+from eos_amd.kvcache import KVBatch  # noqa: E402
 from eos_amd.microscale import MXLinear  # noqa: E402
+from eos_amd.rotary import Rotary  # noqa: E402
 from eos_amd.runtime import DeviceBuffer, Runtime  # noqa: E402
 
 
@@ -72,6 +76,41 @@ def rows_overlap():
     refused("out overlaps codes or scales", d, part(1 << 15), buf, rows, k, part(s - s % 16), "f16")
     refused("out overlaps codes or scales", d, part(16), part(1 << 15), rows, k, buf, "f16", out_stride=104)
     assert stub.stub_launches(b"eos_mx_quantize_bf16") == 3
+
+
+def rotary_overlap():
+    """Turned rows in the place of others, or of their positions."""
+    rt = Runtime(0)
+    d, rows = 64, 10
+    rot = Rotary(rt, d, np.ones(d // 2))
+    buf, pos = DeviceBuffer(rt, 1 << 18), DeviceBuffer(rt, 4 * rows)
+    part = lambda at: buf.view(at, buf.nbytes - at)  # noqa: E731
+    where = (pos, rows)
+    far = part(1 << 17)
+
+    def turn(q=None, k=None, q_out=None, k_out=None, stride=6 * d, at=where, **kw):
+        rot.apply(at, "bf16", q, 4 if q else 0, k, 2 if k else 0, q_out, k_out, stride, stride, **kw)
+
+    packed = dict(q=buf, k=part(4 * d * 2))  # q | k, two bytes a value
+    turn(**packed)
+    turn(**packed, q_out=far, k_out=part((1 << 17) + 4 * d * 2), q_out_stride=6 * d, k_out_stride=6 * d)
+    turn(**packed, q_out=far)                                # the keys stay where they are
+    turn(**packed, k_out=far)
+    turn(q=buf, k=far, q_out=part(6 * d * 2 * rows))
+    refused("q_out overlaps k", turn, q=buf, k=part(4 * d * 2 - 16))
+    refused("q_out overlaps k", turn, q=buf, k=buf)
+    refused("q_out overlaps q", turn, q=buf, q_out=part(16), q_out_stride=6 * d)
+    refused("q_out overlaps q", turn, q=far, q_out=part((1 << 17) - 4 * d * 2 * rows + 16))
+    refused("k_out overlaps k", turn, k=buf, k_out=part(6 * d * 2), k_out_stride=8 * d)
+    refused("k_out overlaps q", turn, q=buf, k=far, q_out=part(1 << 16), k_out=part(2 * d * 2), k_out_stride=6 * d)
+    refused("q_out overlaps k_out", turn, q=buf, k=part(4 * d * 2), q_out=far, k_out=far)
+    refused("an output overlaps positions", turn, q=buf, at=(part(6 * d * 2 * 9 + 4 * d * 2 - 16), rows))
+    turn(q=buf, at=(part(6 * d * 2 * 9 + 4 * d * 2), rows))
+    i32 = DeviceBuffer(rt, 4096)
+    turn(q=buf, at=KVBatch(None, 0, rows, i32))
+    refused("an output overlaps positions", turn, q=buf, at=KVBatch(None, 0, rows, buf))
+    refused("an output overlaps positions", turn, k=buf, at=KVBatch(None, 0, 3, i32, buf, rows))
+    assert stub.stub_launches(b"eos_rot_halves_bf16") == 7
 
 
 if __name__ == "__main__":
