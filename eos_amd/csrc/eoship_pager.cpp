@@ -56,6 +56,22 @@ int check(const EosHipRuntime* rt, const EosHipKVPager* pager, const char* what,
   return 0;
 }
 
+// An array's bytes, none where it is not given.
+struct Span {
+  uintptr_t at, end;
+  Span(const void* p, int64_t bytes) : at((uintptr_t)p), end((uintptr_t)p + (p != nullptr ? bytes : 0)) {}
+};
+// (an empty one meets none)
+bool meet(const Span& a, const Span& b) { return std::max(a.at, b.at) < std::min(a.end, b.end); }
+
+// A pager's arrays.
+struct Arrays {
+  Span table, free, lengths, count;
+  explicit Arrays(const EosHipKVPagerDesc& d)
+      : table(d.d_page_table, 4LL * d.slots * d.table_stride), free(d.d_free, 4 * d.pages),
+        lengths(d.d_lengths, 4LL * d.slots), count(d.d_free_count, 4) {}
+};
+
 PagerArgs args(const EosHipKVPager* p) {
   PagerArgs a{};
   a.table = p->d.d_page_table;
@@ -94,6 +110,10 @@ int eoship_kv_pager_bind(EosHipRuntime* rt, const EosHipKVPagerDesc* desc, EosHi
     if (out != nullptr) *out = nullptr;
     if (check_desc(desc, what, err) != 0) return 1;
     if (rt == nullptr || out == nullptr) return set_err(err, "%s: NULL argument", what);
+    const Arrays own(*desc);
+    if (meet(own.table, own.free) || meet(own.table, own.lengths) || meet(own.table, own.count) ||
+        meet(own.free, own.lengths) || meet(own.free, own.count) || meet(own.lengths, own.count))
+      return set_err(err, "%s: arrays overlap", what);
     OnDevice on(rt->device);
     if (rt->load(eoship::Runtime::kStep, err) != 0) return 1;
     auto* p = new EosHipKVPager();
@@ -153,9 +173,26 @@ int eoship_kv_pager_extend_device(EosHipRuntime* rt, EosHipKVPager* pager, const
         !aligned(plan->d_positions, 4) || !aligned(plan->d_slot_map, 8))
       return set_err(err, "%s: arrays must be aligned to their elements", what);
     const EosHipKVPagerDesc& d = pager->d;
-    if (plan->d_page_table == d.d_page_table || plan->d_lengths == d.d_lengths ||
-        plan->d_slots == d.d_lengths || plan->d_offsets == d.d_lengths)
-      return set_err(err, "%s: a plan's arrays are not the pager's own", what);
+    const Arrays own(d);
+    const int64_t slots = 4LL * d.slots;
+    const Span put[] = {{plan->d_slots, slots},
+                        {plan->d_page_table, slots * d.table_stride},
+                        {plan->d_lengths, slots},
+                        {plan->d_offsets, slots + 4},
+                        {plan->d_positions, 4 * plan->rows},
+                        {plan->d_slot_map, 8 * plan->rows}};
+    const Span ask(d_new, slots);
+    bool one = false, asked = false;
+    for (int i = 0; i < 6; ++i) {
+      for (int j = 0; j < i; ++j) one |= meet(put[i], put[j]);
+      one |= meet(put[i], own.table) | meet(put[i], own.free) | meet(put[i], own.lengths) |
+             meet(put[i], own.count);
+      asked |= meet(put[i], ask);
+    }
+    if (one) return set_err(err, "%s: a plan's arrays overlap each other or the pager's", what);
+    if (asked) return set_err(err, "%s: new overlaps a plan's arrays", what);
+    // (lengths and the count are written when all workgroups have read theirs)
+    if (meet(ask, own.table)) return set_err(err, "%s: new overlaps the page table", what);
     OnDevice on(rt->device);
     PagerArgs a = args(pager);
     a.ask = d_new;
@@ -179,6 +216,10 @@ int eoship_kv_pager_trim_device(EosHipRuntime* rt, EosHipKVPager* pager, const i
     if (d_keep == nullptr) return set_err(err, "%s: NULL argument", what);
     if (!aligned(d_keep, 4))
       return set_err(err, "%s: arrays must be aligned to their elements", what);
+    const Arrays own(pager->d);
+    const Span ask(d_keep, 4LL * pager->d.slots);
+    if (meet(ask, own.table) || meet(ask, own.free))
+      return set_err(err, "%s: keep overlaps the page table or the free pages", what);
     OnDevice on(rt->device);
     PagerArgs a = args(pager);
     a.ask = d_keep;

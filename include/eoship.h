@@ -1100,7 +1100,7 @@ typedef struct EosHipKVPager EosHipKVPager;
  * and, unless every sequence has one row, d_offsets; batch and rows are the
  * number of slots with new tokens and their sum. Device memory; what lies
  * behind the batch and its rows, and table entries behind a sequence's pages,
- * stay. The arrays overlap neither each other nor the pager's. */
+ * stay. Arrays that overlap each other or the pager's are refused. */
 typedef struct {
   int32_t* d_slots;       /* [slots] slot of each sequence */
   int32_t* d_page_table;  /* [slots][table_stride] or NULL */
@@ -1111,7 +1111,8 @@ typedef struct {
   int64_t rows;           /* rows that the arrays hold */
 } EosHipKVPlan;
 
-/* Binds the arrays for one runtime; they stay the caller's. */
+/* Binds the arrays for one runtime; they stay the caller's. Arrays that overlap
+ * are refused. */
 int eoship_kv_pager_bind(EosHipRuntime* rt, const EosHipKVPagerDesc* desc, EosHipKVPager** out,
                          char** err);
 int eoship_kv_pager_release(EosHipRuntime* rt, EosHipKVPager* pager, char** err);
@@ -1122,12 +1123,14 @@ int eoship_kv_pager_reset_device(EosHipRuntime* rt, EosHipKVPager* pager, char**
  * slot's changed, are a request beyond its table row, one of whose rows not
  * all are below plan->rows, and from the first request on that the stack does
  * not cover all those that need a page. A refused request keeps its rows in
- * the batch, as padding: length 0, positions and slots -1. */
+ * the batch, as padding: length 0, positions and slots -1. d_new overlaps neither
+ * the plan's arrays nor the page table. */
 int eoship_kv_pager_extend_device(EosHipRuntime* rt, EosHipKVPager* pager, const int32_t* d_new,
                                   const EosHipKVPlan* plan, char** err);
 /* Cuts slots down to d_keep i32 [slots] tokens (0: the request is over;
  * negative or not below its length: it stays as it is). Pages go back in
- * such an order that an extend undone leaves the stack as it was. */
+ * such an order that an extend undone leaves the stack as it was. d_keep overlaps
+ * neither the page table nor the free pages. */
 int eoship_kv_pager_trim_device(EosHipRuntime* rt, EosHipKVPager* pager, const int32_t* d_keep,
                                 char** err);
 /* What calls since the last look found: bit 0 too few free pages, bit 1 a

@@ -14,7 +14,7 @@ import numpy as np  # noqa: E402
 
 from eos_amd import microscale  # noqa: E402
 from eos_amd._lib import EosHipError  # noqa: E402
-from eos_amd.kvcache import KVBatch  # noqa: E402
+from eos_amd.kvcache import KVBatch, KVPager, KVPlan  # noqa: E402
 from eos_amd.microscale import MXLinear  # noqa: E402
 from eos_amd.rotary import Rotary  # noqa: E402
 from eos_amd.runtime import DeviceBuffer, Runtime  # noqa: E402
@@ -111,6 +111,66 @@ def rotary_overlap():
     refused("an output overlaps positions", turn, q=buf, at=KVBatch(None, 0, rows, buf))
     refused("an output overlaps positions", turn, k=buf, at=KVBatch(None, 0, 3, i32, buf, rows))
     assert stub.stub_launches(b"eos_rot_halves_bf16") == 7
+
+
+def pager_overlap():
+    """A pager's arrays, a plan's and a call's in each other's place, by a byte of
+    their last element or whole."""
+    rt = Runtime(0)
+    slots, stride, pages, rows = 6, 5, 40, 32
+    size = dict(page_table=4 * slots * stride, lengths=4 * slots, free=4 * pages, free_count=4)
+    plan_size = dict(slots=4 * slots, page_table=4 * slots * stride, lengths=4 * slots,
+                     offsets=4 * slots + 4, positions=4 * rows, slot_map=8 * rows)
+    buf = DeviceBuffer(rt, 1 << 16)
+    at = {}  # every array's place, one behind the other
+
+    def place(names, sizes, first):
+        for n in names:
+            first = -(-first // 8) * 8
+            at[n] = buf.view(first, sizes[n.split(".")[-1]])
+            first += sizes[n.split(".")[-1]]
+        return first
+
+    end = place([f"own.{n}" for n in size], size, 0)
+    end = place([f"plan.{n}" for n in plan_size], plan_size, end)
+    new = buf.view(-(-end // 8) * 8, 4 * slots)
+    own = {n: at[f"own.{n}"] for n in size}
+    pager = KVPager(rt, slots, stride, 16, pages, **own)
+
+    def plan(**kw):
+        return KVPlan(**({n: at[f"plan.{n}"] for n in plan_size} | dict(rows=rows) | kw))
+
+    pager.extend(new, plan())
+    pager.extend(new, plan(page_table=None, positions=None, slot_map=None))
+    pager.extend(own["lengths"], plan())  # read before they are written
+    pager.trim(own["lengths"])
+    pager.trim(new)
+    n = 0
+    for name in plan_size:
+        first = at[f"plan.{name}"].ptr.value
+        others = [(w, a) for w, a in at.items() if w != f"plan.{name}"]
+        for where, other in others:
+            for put in (other.ptr.value, other.ptr.value + other.nbytes - 8, other.ptr.value - plan_size[name] + 8):
+                put -= buf.ptr.value + (put - buf.ptr.value) % 8
+                if put < 0 or put + buf.ptr.value == first:
+                    continue
+                # (a place may also meet a third array; that is refused as well)
+                moved = buf.view(put, plan_size[name])
+                refused("a plan's arrays overlap", pager.extend, new, plan(**{name: moved}))
+                n += 1
+        refused("new overlaps", pager.extend, buf.view(first - buf.ptr.value, 4 * slots), plan())
+    assert n > 100
+    for name, what in (("page_table", "new overlaps"),):
+        refused(what, pager.extend, buf.view(own[name].ptr.value - buf.ptr.value + 8, 4 * slots), plan())
+    for name in ("page_table", "free"):
+        refused("keep overlaps", pager.trim, buf.view(own[name].ptr.value - buf.ptr.value + 8, 4 * slots))
+    for a in size:
+        for b in size:
+            if a != b and size[a] <= size[b]:
+                refused("arrays overlap", KVPager, rt, slots, stride, 16, pages,
+                        **(own | {a: buf.view(own[b].ptr.value - buf.ptr.value + size[b] - size[a], size[a])}))
+    # without lists their sizes do not count
+    pager.extend(new, plan(positions=None, slot_map=None, rows=1 << 30))
 
 
 if __name__ == "__main__":

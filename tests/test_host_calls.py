@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
-CASES = ["linear_overlap", "rows_overlap", "rotary_overlap"]
+CASES = ["linear_overlap", "rows_overlap", "rotary_overlap", "pager_overlap"]
 
 
 @pytest.fixture(scope="module")
