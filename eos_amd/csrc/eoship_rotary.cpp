@@ -142,6 +142,8 @@ int eoship_rotary_device(EosHipRuntime* rt, EosHipRotary* rot, const EosHipKVBat
     if (a.rows < 0 || a.rows > INT32_MAX)
       return set_err(err, "%s: rows must be in 0..2^31-1, got %lld", what, (long long)a.rows);
     if (a.rows == 0) return 0;
+    if ((((uintptr_t)d_positions | (uintptr_t)a.lengths | (uintptr_t)a.offsets) & 3) != 0)
+      return set_err(err, "%s: positions, lengths and offsets must be 4-byte aligned", what);
     const int64_t d = rot->head_dim;
     if (heads > 0 && (check_rows(d_q, q_stride, heads * d, "q", what, err) != 0 ||
                       check_rows(d_q_out, q_out_stride, heads * d, "q_out", what, err) != 0))

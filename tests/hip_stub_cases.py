@@ -173,6 +173,20 @@ def pager_overlap():
     pager.extend(new, plan(positions=None, slot_map=None, rows=1 << 30))
 
 
+def rotary_alignment():
+    """Positions, lengths and offsets are read as words: wherever else they stand,
+    a scalar load takes others."""
+    rt = Runtime(0)
+    rot = Rotary(rt, 64, np.ones(32))
+    buf, i32 = DeviceBuffer(rt, 1 << 16), DeviceBuffer(rt, 4096)
+    for at in (1, 2, 3):
+        odd = i32.view(at, 2048)
+        refused("4-byte aligned", rot.apply, (odd, 3), "f16", buf, 1)
+        refused("4-byte aligned", rot.apply, KVBatch(None, 0, 3, odd), "f16", buf, 1)
+        refused("4-byte aligned", rot.apply, KVBatch(None, 0, 3, i32, odd, 3), "f16", buf, 1)
+    rot.apply((i32.view(4, 2048), 3), "f16", buf, 1)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[2]]()
     print("OK")

@@ -10,7 +10,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
-CASES = ["linear_overlap", "rows_overlap", "rotary_overlap", "pager_overlap"]
+CASES = ["linear_overlap", "rows_overlap", "rotary_overlap", "pager_overlap",
+         "rotary_alignment"]
 
 
 @pytest.fixture(scope="module")
