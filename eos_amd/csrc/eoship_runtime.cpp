@@ -160,6 +160,7 @@ int Runtime::take_event(hipEvent_t* ev, char** err) {
 int Runtime::alloc(size_t bytes, void** p, char** err) {
   *p = nullptr;
   if (bytes == 0) return 0;
+  OnDevice on(device);
   hipError_t e = hipMalloc(p, bytes);
   if (e != hipSuccess) return hip_err(err, "hipMalloc", e);
   return 0;

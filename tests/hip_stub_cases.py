@@ -14,7 +14,7 @@ import numpy as np  # noqa: E402
 
 from eos_amd import microscale  # noqa: E402
 from eos_amd._lib import EosHipError  # noqa: E402
-from eos_amd.kvcache import KVBatch, KVPager, KVPlan  # noqa: E402
+from eos_amd.kvcache import KVBatch, KVCache, KVPager, KVPlan  # noqa: E402
 from eos_amd.microscale import MXLinear  # noqa: E402
 from eos_amd.rotary import Rotary  # noqa: E402
 from eos_amd.runtime import DeviceBuffer, Runtime  # noqa: E402
@@ -185,6 +185,32 @@ def rotary_alignment():
         refused("4-byte aligned", rot.apply, KVBatch(None, 0, 3, odd), "f16", buf, 1)
         refused("4-byte aligned", rot.apply, KVBatch(None, 0, 3, i32, odd, 3), "f16", buf, 1)
     rot.apply((i32.view(4, 2048), 3), "f16", buf, 1)
+
+
+def another_current_device():
+    """A runtime's memory is its own device's, whichever the program made current,
+    and that one stays current."""
+    near, far = Runtime(0), Runtime(1)
+    for rt, device in ((near, 0), (far, 1)):
+        for current in (0, 1):
+            stub.stub_set_device(current)
+            own = lambda b: stub.stub_device_of(b.ptr) == device  # noqa: E731
+            buf = DeviceBuffer(rt, 4096)
+            assert own(buf) and stub.stub_device() == current
+            layer = MXLinear.from_rows(rt, buf, 16, 32, "f32")
+            layer.apply(buf, 20, "f16", DeviceBuffer(rt, 4096), "f16")
+            pager = KVPager(rt, 3, 2, 16, 9)
+            plan = pager.plan(8)
+            assert all(map(own, (pager.page_table, pager.free, plan.slots, plan.slot_map)))
+            pager.extend(DeviceBuffer(rt, 12), plan)
+            pager.trim(DeviceBuffer(rt, 12))
+            assert pager.status() == 0
+            cache = KVCache(rt, "q8", 1, 32, 16, 2)
+            assert own(cache.k) and own(cache.v_scale)
+            Rotary(rt, 32, np.ones(16)).apply((buf, 3), "f16", DeviceBuffer(rt, 256), 1)
+            for x in (layer, pager, cache):
+                x.release()
+            assert stub.stub_device() == current
 
 
 if __name__ == "__main__":

@@ -11,7 +11,7 @@ ROOT = os.path.dirname(HERE)
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 CASES = ["linear_overlap", "rows_overlap", "rotary_overlap", "pager_overlap",
-         "rotary_alignment"]
+         "rotary_alignment", "another_current_device"]
 
 
 @pytest.fixture(scope="module")
