@@ -33,6 +33,7 @@ struct EosHipMX {
 namespace {
 
 constexpr int kMost = 1 << 24;  // values of a row, outputs of a layer
+constexpr long long kGroups = (1 << 24) - 1;  // workgroups of 256 threads in a launch
 
 // Which kernel takes a layer's rows (256 CUs; us of a call among others, 4,096
 // values, bf16).
@@ -80,6 +81,18 @@ int check_shape(int64_t rows, int32_t k, const char* what, char** err) {
   return 0;
 }
 
+int check_blocks(int64_t rows, int32_t k, const char* what, char** err) {
+  if (rows * ceil_div(k, kMxBlock) <= 64 * kGroups) return 0;
+  return set_err(err, "%s: %lld rows of %d values are more than 2^30 - 64 blocks", what,
+                 (long long)rows, k);
+}
+
+int check_tiles(int64_t rows, int32_t k, const char* what, char** err) {
+  if ((rows + kMxTile - 1) / kMxTile * ceil_div(k, kMxQuad) <= kGroups) return 0;
+  return set_err(err, "%s: %lld rows of %d values are more than 2^24 - 1 tiles of 32 rows by 256",
+                 what, (long long)rows, k);
+}
+
 int check_type(int32_t type, int most, const char* what, char** err) {
   if (type < 0 || type > most)
     return set_err(err, "%s: dtype must be 0 (f16), 1 (bf16)%s, got %d", what,
@@ -108,7 +121,7 @@ int check_codes(const void* codes, const void* scales, const char* what, char** 
 
 int launch(EosHipRuntime* rt, const std::string& name, long long blocks, void* args,
            const char* what, char** err) {
-  if (blocks * 256 > UINT32_MAX) return set_err(err, "%s: too many rows for one call", what);
+  if (blocks > kGroups) return set_err(err, "%s: too many outputs for one call", what);
   return rt->launch(name.c_str(), dim3((unsigned)blocks), dim3(256), 0, args, err);
 }
 
@@ -151,7 +164,9 @@ int eoship_mx_quantize_device(EosHipRuntime* rt, const void* d_x, int64_t x_stri
                               char** err) {
   const char* what = "eoship_mx_quantize_device";
   return guarded(what, err, [&]() -> int {
-    if (check_shape(rows, k, what, err) != 0 || check_type(dtype, kMxF32, what, err) != 0) return 1;
+    if (check_shape(rows, k, what, err) != 0 || check_type(dtype, kMxF32, what, err) != 0 ||
+        check_blocks(rows, k, what, err) != 0)
+      return 1;
     if (rt == nullptr) return set_err(err, "%s: NULL runtime", what);
     if (rows == 0) return 0;
     if (check_rows(d_x, x_stride, k, "x", what, err) != 0 ||
@@ -183,7 +198,9 @@ int eoship_mx_dequantize_device(EosHipRuntime* rt, const uint8_t* d_codes, const
                                 int32_t dtype, char** err) {
   const char* what = "eoship_mx_dequantize_device";
   return guarded(what, err, [&]() -> int {
-    if (check_shape(rows, k, what, err) != 0 || check_type(dtype, kMxF32, what, err) != 0) return 1;
+    if (check_shape(rows, k, what, err) != 0 || check_type(dtype, kMxF32, what, err) != 0 ||
+        check_blocks(rows, k, what, err) != 0)
+      return 1;
     if (rt == nullptr) return set_err(err, "%s: NULL runtime", what);
     if (rows == 0) return 0;
     if (check_codes(d_codes, d_scales, what, err) != 0 ||
@@ -214,7 +231,8 @@ int eoship_mx_bind(EosHipRuntime* rt, const uint8_t* d_codes, const uint8_t* d_s
   return guarded(what, err, [&]() -> int {
     if (out != nullptr) *out = nullptr;
     if (n < 1 || n > kMost) return set_err(err, "%s: n must be in 1..2^24, got %d", what, n);
-    if (check_shape(n, k, what, err) != 0 || check_codes(d_codes, d_scales, what, err) != 0)
+    if (check_shape(n, k, what, err) != 0 || check_tiles(n, k, what, err) != 0 ||
+        check_codes(d_codes, d_scales, what, err) != 0)
       return 1;
     if (((uintptr_t)d_bias & 3) != 0) return set_err(err, "%s: bias is not 4-byte aligned", what);
     if (rt == nullptr || out == nullptr) return set_err(err, "%s: NULL argument", what);
@@ -264,7 +282,8 @@ int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, in
   return guarded(what, err, [&]() -> int {
     if (rt == nullptr || mx == nullptr) return set_err(err, "%s: NULL argument", what);
     if (mx->rt != rt) return set_err(err, "%s: the layer is bound to another runtime", what);
-    if (check_shape(rows, mx->k, what, err) != 0 || check_type(dtype, kMxCodes, what, err) != 0 ||
+    if (check_shape(rows, mx->k, what, err) != 0 || check_tiles(rows, mx->k, what, err) != 0 ||
+        check_type(dtype, kMxCodes, what, err) != 0 ||
         check_type(out_dtype, kMxF32, what, err) != 0)
       return 1;
     if (rows == 0) return 0;

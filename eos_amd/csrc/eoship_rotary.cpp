@@ -199,8 +199,10 @@ int eoship_rotary_device(EosHipRuntime* rt, EosHipRotary* rot, const EosHipKVBat
     // where there are not rows enough for every CU.
     const long long most = std::max(1, std::min(kRotAngles / half, kRotRows));
     a.each = (int)std::max(1LL, std::min(most, a.rows / (4 * rt->compute_units)));
-    const long long blocks = (a.rows + a.each - 1) / a.each;
-    if (blocks * 256 > UINT32_MAX) return set_err(err, "%s: too many rows for one call", what);
+    const long long blocks = (a.rows + a.each - 1) / a.each, groups = (1 << 24) - 1;
+    if (blocks > groups)
+      return set_err(err, "%s: %lld rows are more than %lld rows of one call", what,
+                     (long long)a.rows, groups * most);
     const std::string name = std::string(rot->layout == kRotHalves ? "eos_rot_halves_" : "eos_rot_pairs_") +
                              (wide ? "" : "odd_") + kTypes[dtype];
     return rt->launch(name.c_str(), dim3((unsigned)blocks), dim3(256), 0, &a, err);

@@ -999,7 +999,9 @@ int eoship_kv_status(EosHipRuntime* rt, EosHipKVCache* kv, int32_t* status, char
  *   scales  [rows][ceil(k / 32)]
  * Types: 0 f16, 1 bf16, 2 f32, where stated 3 (such codes). Rows of types 0..2
  * are 16-byte aligned and lie a stride (in elements, a multiple of 8) apart;
- * codes are 16-byte aligned and without gaps. k is in 1..2^24.
+ * codes are 16-byte aligned and without gaps. k is in 1..2^24; a call quantises or
+ * takes back up to 2^30 - 64 blocks, and a layer's weights, or the rows that it is
+ * applied to, are up to 2^24 - 1 tiles of 32 rows by 256 values.
  * ------------------------------------------------------------------------ */
 
 /* Bytes of the codes and of the scales of rows of k values. */
@@ -1059,7 +1061,8 @@ int eoship_rotary_bind(EosHipRuntime* rt, const EosHipRotaryDesc* desc, EosHipRo
 int eoship_rotary_release(EosHipRuntime* rt, EosHipRotary* rot, char** err);
 /* Turns rows of queries [rows][heads][D] and of keys [rows][kv_heads][D]
  * (dtype 0 f16, 1 bf16, 2 f32; 16-byte aligned, strides in elements, multiples
- * of 8; heads or kv_heads 0: none) by their positions: those of a cache's
+ * of 8; heads or kv_heads 0: none; up to 2^24 - 1 rows, four times as many where R
+ * is up to 128, 16 where it is up to 32) by their positions: those of a cache's
  * batch (its page table is not looked at, rows is the batch's), or
  * d_positions i32 [rows] with batch NULL. Rows of a negative position and
  * rows of no sequence are not written. Angles are taken from f64 products,

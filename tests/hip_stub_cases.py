@@ -12,7 +12,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 import numpy as np  # noqa: E402
 
-from eos_amd import microscale  # noqa: E402
+from eos_amd import _lib, microscale  # noqa: E402
 from eos_amd._lib import EosHipError  # noqa: E402
 from eos_amd.kvcache import KVBatch, KVCache, KVPager, KVPlan  # noqa: E402
 from eos_amd.microscale import MXLinear  # noqa: E402
@@ -211,6 +211,41 @@ def another_current_device():
             for x in (layer, pager, cache):
                 x.release()
             assert stub.stub_device() == current
+
+
+def largest_calls():
+    """The most that a call takes is what its documentation says, and more is
+    refused by that name before anything is enqueued."""
+    rt = Runtime(0)
+    near, far = C.c_void_p(1 << 20), C.c_void_p(1 << 60)
+    quant = lambda rows, k: _lib.call(  # noqa: E731
+        "eoship_mx_quantize_device", rt.handle, near, -(-k // 8) * 8, 1, rows, k, far, 1 << 61)
+    back = lambda rows, k: _lib.call(  # noqa: E731
+        "eoship_mx_dequantize_device", rt.handle, far, 1 << 61, rows, k, near, -(-k // 8) * 8, 1)
+    for rows, k in ((2 ** 30 - 64, 32), (2 ** 30 - 64, 1), (2 ** 29 - 32, 64), (2 ** 11 - 1, 2 ** 24)):
+        quant(rows, k)
+        back(rows, k)
+    for rows, k in ((2 ** 30 - 63, 32), (2 ** 29 - 31, 33), (2 ** 11, 2 ** 24), (2 ** 31 - 1, 1)):
+        refused("more than 2^30 - 64 blocks", quant, rows, k)
+        refused("more than 2^30 - 64 blocks", back, rows, k)
+    handle = C.c_void_p()
+    bind = lambda n, k: _lib.call(  # noqa: E731
+        "eoship_mx_bind", rt.handle, near, far, n, k, None, C.byref(handle))
+    refused("more than 2^24 - 1 tiles of 32 rows by 256", bind, 2 ** 13, 2 ** 24)
+    refused("more than 2^24 - 1 tiles of 32 rows by 256", bind, 2 ** 24, 2 ** 13)
+    layer = MXLinear(rt, DeviceBuffer(rt, 16 * 16), DeviceBuffer(rt, 16), 16, 32)
+    apply = lambda rows: _lib.call(  # noqa: E731
+        "eoship_mx_linear_device", rt.handle, layer.handle, near, 32, 1, None, rows, far, 16, 1)
+    refused("more than 2^24 - 1 tiles of 32 rows by 256", apply, 2 ** 29)
+    d = 1024
+    turn = lambda rot, rows: _lib.call(  # noqa: E731
+        "eoship_rotary_device", rt.handle, rot.handle, None, far, rows, 0, 1, near, d, 1, near, d,
+        None, 0, 0, None, 0)
+    for half, each in ((512, 1), (256, 1), (64, 4), (48, 5), (4, 16)):
+        rot = Rotary(rt, d, np.ones(half))
+        most = min((2 ** 24 - 1) * each, 2 ** 31 - 1)
+        turn(rot, most)
+        refused(f"more than {most} rows", turn, rot, most + 1)
 
 
 if __name__ == "__main__":

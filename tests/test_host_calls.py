@@ -11,7 +11,8 @@ ROOT = os.path.dirname(HERE)
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 CASES = ["linear_overlap", "rows_overlap", "rotary_overlap", "pager_overlap",
-         "rotary_alignment", "another_current_device"]
+         "rotary_alignment", "another_current_device",
+         "largest_calls"]
 
 
 @pytest.fixture(scope="module")
