@@ -36,22 +36,25 @@ constexpr int kMost = 1 << 24;  // values of a row, outputs of a layer
 constexpr long long kGroups = (1 << 24) - 1;  // workgroups of 256 threads in a launch
 
 // Which kernel takes a layer's rows (256 CUs; us of a call among others, 4,096
-// values, bf16).
+// values, bf16, weights from HBM).
 // Up to 16 rows are quantised by the workgroups that multiply them, in one
-// launch (16 rows by 6,144 weights 8.6; laid out first 9.7). A workgroup takes
-// 16 weights, 32 where there are more of those than CUs (1 row by 6,144: 6.4 and
-// 6.1, by 4,096: 5.7 and 5.9), 64 where there are more than twice as many and the
-// rows' quantisation weighs (16 by 16,384: 19.7, 13.7 and 12.8; 1 by 16,384: 10.8,
-// 9.1 and 10.2).
+// launch (16 rows by 6,144 weights 8.6, by 16,384 12.7; laid out first 10.2 and
+// 13.1). A workgroup takes 16 weights, 32 where there are more of those than CUs
+// (1 row by 6,144: 6.1 and 5.8, 16 rows 12.1 and 8.6; by 4,096: 5.4 and 5.4, 7.8
+// and 7.9), 64 where there are more than twice as many and the rows' quantisation
+// weighs (16 by 16,384: 20.5, 15.5 and 12.7; by 6,144 with 64 10.3).
 constexpr int kFewRows = 16;
 // Up to 64 are laid out by a launch before and multiplied in the same way (64 by
-// 2,048 9.1, by tiles of 64 11.9; by 6,144 12.0 and 14.6, by 16,384 16.0 and 16.3).
+// 2,048 9.1, by tiles of 64 12.0; by 6,144 12.0 and 14.7, by 16,384 16.0 and 15.9).
 constexpr int kSomeRows = 64;
 // More go by tiles of outputs. Tiles of 64 while there are no more than two a CU
-// (512 by 4,096: 17.0, by tiles of 128 18.9; 1,024 by 4,096: 26.0 and 22.0); then
+// (512 by 4,096: 17.0, by tiles of 128 18.9; 1,024 by 4,096: 26.4 and 22.0); then
 // of 128, two workgroups a CU, or of 256, one, whose turn takes 3/2 the time of the
-// two's (2,048 by 4,096, a turn each: 32.4 and 39.7; by 16,384, four turns and two:
-// 101 and 82).
+// two's or more (2,048 rows; a turn each, by 4,096: 32.4 and 38.6; two turns and
+// one, by 8,192: 54.7 and 44.7; four and two, by 16,384: 102 and 83). At three
+// turns and two, where both predict the same, those of 128: their last turn is
+// shorter where it is not full (by 10,240: 65.5 and 74.1; full, by 12,288: 76.8 and
+// 76.4).
 
 const char* const kTypes[] = {"f16", "bf16", "f32", "codes"};
 
@@ -329,7 +332,7 @@ int eoship_mx_linear_device(EosHipRuntime* rt, EosHipMX* mx, const void* d_x, in
     const auto turns = [&](long long tiles, int at_once) {
       return (tiles + (long long)at_once * cus - 1) / ((long long)at_once * cus);
     };
-    const int t = count(64) <= 2 * cus ? 64 : 3 * turns(count(256), 1) > 2 * turns(count(128), 2) ? 128 : 256;
+    const int t = count(64) <= 2 * cus ? 64 : 3 * turns(count(256), 1) >= 2 * turns(count(128), 2) ? 128 : 256;
     a.tiles_m = (int)((rows + t - 1) / t);
     a.tiles_n = ceil_div(mx->n, t);
     return launch(rt, "eos_mx_product_" + std::to_string(t) + "_" + kTypes[out_dtype],

@@ -95,9 +95,11 @@ def test_tiles(rt, tile, rows, n, k, out):
 
 
 @pytest.mark.parametrize("tile,rows,n,k,out", [(128, 70001, 300, 40, "f16"), (128, 70001, 300, 700, "f32"),
-                                               (256, 200, 70001, 40, "f32"), (256, 200, 70001, 700, "bf16")])
+                                               (256, 200, 65501, 40, "f32"), (256, 200, 65501, 700, "bf16"),
+                                               (128, 2048, 10240, 256, "bf16")])
 def test_tiles_along_one_axis(rt, tile, rows, n, k, out):
-    """One column of tiles, or a row: how they are dealt to the XCDs."""
+    """One column of tiles, or a row: how they are dealt to the XCDs; three turns of
+    tiles of 128 where two of 256 would do."""
     _run(rt, np.random.default_rng(k), f"eos_mx_product_{tile}_{out}", rows, n, k, "bf16", out, True)
 
 
