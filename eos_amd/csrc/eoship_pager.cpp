@@ -88,8 +88,9 @@ PagerArgs args(const EosHipKVPager* p) {
 
 // Every wavefront sums up to 64 slots up by itself, a workgroup 1,024, a slot a
 // thread, or 4,096. Workgroups: two table entries or rows a thread, on every CU at
-// most (extend and trim, 64 slots of 128 pages: 1 workgroup 6.7 + 2.7 us, 4 5.4 +
-// 3.1; 4,096 slots of 512: 128 25.0 + 9.1, 256 19.4 + 9.7, 512 26.0 + 12.4).
+// most (extend and trim, 64 slots of 128 pages: 1 workgroup 6.6 + 4.0 us, 4 5.2 +
+// 3.8, 64 4.9 + 3.9, 256 6.8 + 5.6; 4,096 slots of 512: 64 38.7 + 9.6, 128 25.3 +
+// 8.6, 256 18.5 + 7.6, 512 24.8 + 9.3).
 int launch(EosHipRuntime* rt, const EosHipKVPager* p, const char* op, long long rows, size_t lds,
            PagerArgs* a, char** err) {
   const std::string name = std::string("eos_pager_") + op +

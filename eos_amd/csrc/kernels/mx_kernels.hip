@@ -152,7 +152,7 @@ EOS_DEV void quantize(const MxQuantArgs& a) {
 }
 
 // The same into laid-out tiles: a workgroup a tile and quad, a wavefront a step.
-// 8,192 rows of 8,192 bf16: 38 us, 4.5 TB/s; of a small call 2, its latency.
+// 8,192 rows of 8,192 bf16: 39 us, 4.4 TB/s; of a small call 3, its latency.
 template <int T>
 EOS_DEV void lay(const MxQuantArgs& a) {
   const MxLaid& o = a.laid;
@@ -399,14 +399,15 @@ EOS_DEV v4u descriptor(const uint8_t* p) {
 // arrive. Otherwise through registers, which are stored in the first two steps and
 // at once loaded again, a quad ahead; a load that comes back so takes 29 clocks of
 // the matrix unit's. The 256 tile's steps are long enough for the former (8,192^3
-// 263 -> 230 us), those of 64 and 128 not (512 by 4,096 x 4,096 from HBM 13.7 us
+// through registers in the compiler's order 298 us, in the written one 263, straight
+// into LDS 230), those of 64 and 128 not (512 by 4,096 x 4,096 from HBM 13.7 us
 // direct, 12.3 through registers; 1,024 17.1 and 15.1).
 //
 // Tiles of 32 x 32 x 64: on values as they come these reach 6.5 PFLOP/s of the
 // card, 16 x 16 x 128 5.6 (on zeros 9.5 and 6.9: it is the power that they draw).
 // MF = NF = 4: a wavefront's 128 x 128 outputs read 16 KB of LDS for 128 values of
-// K, half of what 64 x 64 read for as many products. 8,192^3: 230 us, 4.8 PFLOP/s
-// (298 in the compiler's order). A quad is 2,480 clocks, 2,048 of them matrix
+// K, half of what 64 x 64 read for as many products. 8,192^3: 230 to 241 us by the
+// card, 4.6 to 4.8 PFLOP/s. A quad is 2,480 clocks, 2,048 of them matrix
 // instructions; the clock is 2.4 GHz for one workgroup, 1.45 when all multiply (2.2
 // on zeros): power. 7 us of each of four turns are the first loads and the stores.
 template <int MF, int NF>
@@ -596,7 +597,7 @@ struct Rows16 {
 // Up to four rows a row at a time, eight values a lane as they lie in memory;
 // more of them a block a lane, four rows at a time, which loads parts of lines
 // but takes 0.6 of the instructions (16,384 values by 4,096 weights: one row 9.2
-// us against 11.8; 4,096 by 6,144: 16 rows 9.2 against 8.2).
+// us against 11.8; 4,096 by 6,144: 16 rows 9.2 against 8.2; from HBM).
 template <int X, bool FOUR, int U>
 EOS_DEV void quantize_rows(const MxLinearArgs& a, Rows16<U>& to, int first) {
   static_assert(U == 4, "64 lanes take four times 16 lanes' or 16 blocks");
@@ -653,8 +654,9 @@ EOS_DEV void quantize_rows(const MxLinearArgs& a, Rows16<U>& to, int first) {
 // workgroup: its eight wavefronts take 128 values of K in turn, U at a time, so
 // that the weights, read once, arrive in long runs; their sums meet in LDS, in
 // the wavefronts' order. Bound by the weights: 16,384 x 16,384 by one row in 26
-// us, 5.5 TB/s; 48 rows by 4,096 x 16,384 8.4, 4.5 TB/s; one by 4,096 x 6,144 4.4,
-// a chain of launch, loads, sums.
+// us, 5.5 TB/s; 48 rows by 4,096 x 16,384 11.1 from HBM, 8.6 (4.4 TB/s) where the
+// weights are still on the chip; one by 4,096 x 6,144 5.5 and 4.4, a chain of launch,
+// loads, sums. 16 rows by it 8.2; as codes, without their quantisation, 6.0.
 template <int X, bool FOUR, int MT, int NT, int U>
 EOS_DEV void few(const MxLinearArgs& a) {
   constexpr bool kRows = X < kMxCodes;

@@ -133,8 +133,8 @@ EOS_DEV void rotate(const RotArgs& a) {
   if constexpr (WIDE) {
     // The lane's eight values, of halves also the eight that they turn with. Pairs:
     // four heads' loads are in flight (9,000 ragged rows of 40 heads of 128, a
-    // quarter turned: 48 -> 41 us, 4.5 TB/s), halves have two already (16,384 rows of
-    // 64 heads: 100 us, 5.4 TB/s; with four heads' 107).
+    // quarter turned: 48 -> 42 us, 4.3 TB/s), halves have two already (16,384 rows of
+    // 64 heads: 101 us, 5.3 TB/s; with four heads' 107).
     constexpr bool kHalves = LAYOUT == kRotHalves;
     constexpr int kHeads = kHalves ? 1 : 4;
     const int turning = kHalves ? half / 8 : a.rotary_dim / 8;  // lanes
@@ -186,6 +186,10 @@ EOS_DEV void rotate(const RotArgs& a) {
       }
     }
   } else {
+    // Halves or pairs that do not begin at such: a value at a time (16,384 rows of 40
+    // heads of 128 bf16 in place: 122 of the head turned in 128 us by halves and 114
+    // by pairs, all of it eight at a time in 67 and 71; one row a sequence takes as
+    // long either way).
     for (int i0 = threadIdx.x >> a.lanes_shift; i0 < all; i0 += step) {
       const uint8_t* x;
       uint8_t* y;
@@ -302,8 +306,9 @@ EOS_DEV bool last_one(const PagerArgs& a, int* flag) {
 // the batch's ranges are left in LDS. The last one that is done brings lengths
 // and stack up to date. What these kernels wait for is a chain of loads and, each
 // instruction running once, the instructions: hence loops, not unrolled ones. A
-// token for each of 64 slots of 8,000: 8.3 -> 5.4 us, trimmed again 5.7 -> 3.1;
-// 1.6 million rows for 4,096 slots 34.6 -> 18.8 and 13.1 -> 8.1 (0.6 TB/s).
+// token for each of 64 slots of 8,000: 8.3 -> 5.8 us, trimmed again 5.7 -> 3.3;
+// 1.9 million rows for 4,096 slots 34.6 -> 18.9 (27 MB, 1.4 TB/s) and 13.1 -> 8.1
+// (1.5 MB: loads, a scan and the count of workgroups, one behind the other).
 template <bool FEW, int E>
 EOS_DEV void extend(const PagerArgs& a) {
   extern __shared__ int lds[];
